@@ -169,6 +169,60 @@ int b2_sync(b2_handle* h);
  * stays usable. No reference counterpart (the reference's machine has no device waits, base2.py:102-114). */
 int b2_check_wait(b2_handle* h, void* stream);
 
+/* ---- the key/value store held in 4 bits --------------------------------------------------------------------------
+ * 67 bytes a position and head of 64 dims, where the engine's 16-bit store takes 396. A store stands by itself (any
+ * layer of any integer machine may use one); the engine's own streams are held this way with "store_bits" 4
+ * (b2_set_scalar). Numbers are whole, at the stream's scale 2^-16; rnd(x, s) is x 2^-s to nearest, halves up.
+ *   write   magnitudes are kept below 2^47. A key head row: for each half of 32 dims t = the bit length of its largest
+ *           magnitude, s = min(max(t - 3, 0), 44), and at least the larger half's s less 3; codes c = rnd(x, s) kept in
+ *           [-8, 7]. A value head row: the same with one shift over the 64.
+ *   read    c 2^s.
+ *   attend  (base2.py:85-100 over the held keys and values) q15 = rnd(q, u), u = max(bit length - 14, 0); the score of
+ *           key k = c 2^s is q15 . k 2^u over 8 at 2^-10, rounded (and held below 2^30); start = the largest;
+ *           a = arrival[start - score], 0 past the table; Z = sum a; w = rnd(a, 1 + M - s), s the value's shift and M
+ *           the largest of the visible keys'; out = power(sum w c, 65536 (M + 1) - log2fix(Z)). Every sum is exact, so
+ *           the result does not depend on the order or on how a call is split.
+ * Streams: stream i's rows are cu[i] .. cu[i + 1] - 1 of the call's rows (cu [n_streams + 1]; NULL: one row a stream,
+ * rows = n_streams), its first row at position pos[i]; max_rows is a bound on a stream's rows (1 with cu = NULL). Rows
+ * that no stream has are neither read nor written. cu, pos, first, k, v, q, out are DEVICE pointers; row r's head h is
+ * at r * ld + 64 h (ld in elements, at least 64 n_head). Work is queued on `stream`; nothing is allocated, copied to
+ * the host or kept between calls, so calls may be captured into a graph, and calls that do not write what another one
+ * reads or writes may run at once. A stream whose rows do not fit the call or whose positions pass the context is
+ * skipped and flagged: b2_store_sync reports it (B2_ERR_ARG, B2_ERR_CTX). */
+typedef struct b2_store b2_store;
+typedef struct {
+    int32_t n_slots;    /* streams, 1 .. 65535 */
+    int32_t n_layer;    /* 1 .. 1024 */
+    int32_t n_head;     /* heads of 64 dims, 1 .. 1024 */
+    int32_t max_ctx;    /* positions of a stream, 1 .. 65536 */
+} b2_store_config;
+
+/* A store on `device`, every position standing for zeros. arrival [n_arrival] (entries in [0, 2^24], the first at least
+ * 1), log2 and exp2 [65536]: the machine's tables (base2_convert.py:50-59), HOST pointers. After an error *out, where it
+ * is not NULL, holds the message (b2_store_last_error) and is to be destroyed. */
+int b2_store_create(const b2_store_config* cfg, int device, const int64_t* arrival, int64_t n_arrival, const int64_t* log2,
+                    const int64_t* exp2, b2_store** out);
+
+/* Put rows into the store (the key/value append; base2.py:93 with 4 bits for to16's 16). */
+int b2_store_write(b2_store* s, int32_t layer, const int64_t* k, int64_t ldk, const int64_t* v, int64_t ldv, const int32_t* cu,
+                   const int32_t* pos, int32_t n_streams, int32_t rows, int32_t max_rows, void* stream);
+
+/* The values that the held codes stand for: k, v [rows][n_head][64] (either may be NULL). */
+int b2_store_read(b2_store* s, int32_t layer, const int32_t* cu, const int32_t* pos, int32_t n_streams, int32_t rows,
+                  int32_t max_rows, int64_t* k, int64_t* v, void* stream);
+
+/* The arrival of rows over the store: out [rows][n_head][64]. A row at position p sees positions lo .. p, lo = the
+ * largest of 0, first[i] (optional, [n_streams]) and p - window + 1 (window 0: none); with none left its out is zeros.
+ * The row's own key and value have to be in the store (b2_store_write before it). */
+int b2_store_attend(b2_store* s, int32_t layer, const int64_t* q, int64_t ldq, const int32_t* cu, const int32_t* pos,
+                    const int32_t* first, int32_t n_streams, int32_t rows, int32_t max_rows, int32_t window, int64_t* out,
+                    void* stream);
+
+/* Wait for queued work and report what the device checks flagged since the last call. */
+int b2_store_sync(b2_store* s);
+const char* b2_store_last_error(const b2_store* s);
+void b2_store_destroy(b2_store* s);
+
 const char* b2_last_error(const b2_handle* h);
 void b2_destroy(b2_handle* h);
 int b2_abi_version(void);

@@ -13,6 +13,7 @@ enum : uint32_t {
     DERR_VOVF = 4u,      // a V value outside int32 (the value store holds int32)
     DERR_INDEX = 8u,     // an arrival-table index below -len (where base2.py raises IndexError)
     DERR_TIMEOUT = 16u,  // a bounded wait in a tensor-core kernel gave up (the results of that call are void)
+    DERR_ROWS = 64u,     // a row table (the streams' first rows) that does not fit the call
     DERR_RANGE = 32u,    // a value where the reference raises: an exact power outside int64, a turn input past 2^31
 };
 

@@ -1,0 +1,139 @@
+// b2_store.cuh -- the key/value store held in 4 bits: its layout on the device, its arithmetic and the launches that
+// write rows into it, read them back and run the arrival over it (b2_store.cu; the C ABI's b2_store_* and the engine's
+// "store_bits" 4).
+//
+// Per (slot, layer, head) the positions are contiguous (stride ctx, a multiple of 32):
+//   k  [pos][32 bytes]  64 codes, two per byte (the lower dimension in the low digits). The two halves' words lie in
+//                       turn: word 2j is dims 8j .. 8j + 7, word 2j + 1 dims 32 + 8j .., so that one 8-byte load holds
+//                       the same place of both halves
+//   ks [pos][2]         the halves' shifts
+//   v  [pos][32 bytes]  64 codes, word j is dims 8j .. 8j + 7
+//   vs [pos]            the value's shift
+// 67 bytes a position and head; the 16-bit store (struct KV) takes 396.
+#pragma once
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "b2_epi.cuh"
+
+namespace b2 {
+
+struct Store4 {
+    uint8_t* k;
+    int8_t* ks;
+    uint8_t* v;
+    int8_t* vs;
+    int L, H, ctx;     // ctx: the positions' stride
+    int lim;           // positions a stream may hold
+};
+
+// a call's rows: stream i gives rows cu[i] .. cu[i + 1] - 1 (cu == nullptr: row i), its first at position pos[i]
+struct StoreRows {
+    const int32_t* cu;
+    const int32_t* pos;
+    int n_streams, rows, max_rows;
+};
+
+struct StoreAttend {
+    Store4 st;
+    StoreRows rw;
+    int layer;
+    const int64_t* q;      // row r's head h at q + r * ldq + 64 h
+    int64_t ldq;
+    const int32_t* first;  // optional [n_streams]: the first position that a stream still sees
+    int window;            // 0, or how many positions a row sees (its own the last)
+    const int32_t* ARR;
+    int alen;
+    const int32_t* LOG2;
+    const int32_t* EXP2;
+    int64_t* out;          // [rows][H][64]
+    uint64_t* or_out;      // optional [rows]: OR of |out| per row (the next bank's to16 shift)
+    uint32_t* err;
+};
+
+// how the launches below are made: on `stream`, as programmatic dependent launches where pdl is set
+struct StoreLaunch {
+    cudaStream_t stream;
+    bool pdl;
+};
+
+cudaError_t store_write(const Store4& st, const StoreRows& rw, int layer, const int64_t* k, int64_t ldk, const int64_t* v,
+                        int64_t ldv, uint32_t* err, StoreLaunch how);
+cudaError_t store_read(const Store4& st, const StoreRows& rw, int layer, int64_t* k, int64_t* v, uint32_t* err, StoreLaunch how);
+cudaError_t store_attend(const StoreAttend& a, StoreLaunch how);
+
+constexpr int64_t STORE_TOP = 1ll << 47;          // magnitudes are held below this
+constexpr int32_t STORE_LIM = (1 << 30) - 1;      // scores are held between -STORE_LIM and STORE_LIM
+constexpr int STORE_MAX_SHIFT = 44;               // 2^47 in 4 bits
+constexpr int STORE_MAX_CTX = 65536;              // 255 x 128 x 65,536 < 2^31: the tensor cores' sums stay in 32 bits
+constexpr int32_t STORE_MAX_ARR = 1 << 24;        // the arrival table's largest entry (the converter's ARR[0])
+constexpr int STORE_W_SHIFT = 1;                  // a weight is the table's entry halved: its top byte stays below 129
+
+// the store's arrays, zeroed (every position stands for zeros until it is written); alloc(void**, bytes) gives a status
+template <class A>
+int store_alloc(Store4& st, int n_slots, int L, int H, int max_ctx, A alloc) {
+    st.L = L;
+    st.H = H;
+    st.lim = max_ctx;
+    st.ctx = (max_ctx + 31) / 32 * 32;
+    const size_t n = (size_t)n_slots * L * H * st.ctx;
+    void *k, *ks, *v, *vs;
+    int rc;
+    if ((rc = alloc(&k, n * 32)) || (rc = alloc(&ks, n * 2)) || (rc = alloc(&v, n * 32)) || (rc = alloc(&vs, n))) return rc;
+    st.k = (uint8_t*)k;
+    st.ks = (int8_t*)ks;
+    st.v = (uint8_t*)v;
+    st.vs = (int8_t*)vs;
+    if (cudaMemset(k, 0, n * 32) != cudaSuccess || cudaMemset(ks, 0, n * 2) != cudaSuccess ||
+        cudaMemset(v, 0, n * 32) != cudaSuccess || cudaMemset(vs, 0, n) != cudaSuccess)
+        return 2;   // B2_ERR_CUDA
+    return 0;
+}
+
+#ifdef __CUDACC__
+// x 2^-s to nearest, halves up, s >= 0: with no carry past the word (base2.py:18-22 wherever that does not overflow)
+B2_DEV int32_t rnd32(int32_t x, int s) { return s > 0 ? ((x >> (s - 1)) + 1) >> 1 : x; }
+B2_DEV int64_t rnd64(int64_t x, int s) { return s > 0 ? ((x >> (s - 1)) + 1) >> 1 : x; }
+B2_DEV int64_t store_clamp(int64_t x) { return x < -STORE_TOP ? -STORE_TOP : (x > STORE_TOP - 1 ? STORE_TOP - 1 : x); }
+B2_DEV int store_code(int64_t x, int s) {
+    const int64_t c = rnd64(x, s);
+    return c < -8 ? -8 : (c > 7 ? 7 : (int)c);
+}
+// where the key codes of dims 2i, 2i + 1 lie in their 32 bytes (i = 0 .. 31), and back
+B2_DEV int key_byte(int i) { return ((i & 12) << 1) | ((i & 16) >> 2) | (i & 3); }
+B2_DEV int key_pair(int m) { return ((m & 4) << 2) | ((m & 24) >> 1) | (m & 3); }
+
+// the score: dot 2^-r rounded (r = 28 - u - S), held between -STORE_LIM and STORE_LIM; |dot| <= 2^26
+B2_DEV int32_t store_score(int32_t dot, int r) {
+    if (r >= 0) return rnd32(dot, r);
+    const int up = -r < 31 ? -r : 31;
+    const int32_t lim = STORE_LIM >> up;
+    if (dot > lim) return STORE_LIM;
+    if (dot < -lim) return -STORE_LIM;
+    return (int32_t)((uint32_t)dot << (up & 31));
+}
+
+// the rows of stream s; false: nothing to do (no rows, or an inconsistent table, which is flagged)
+struct StoreRun { int r0, n, p0; };
+B2_DEV bool store_run(const StoreRows& w, int s, int lim, StoreRun& run, uint32_t* err) {
+    const int r0 = w.cu ? w.cu[s] : s, r1 = w.cu ? w.cu[s + 1] : s + 1;
+    run.r0 = r0;
+    run.n = 0;
+    run.p0 = 0;
+    if (r0 < 0 || r1 < r0 || r1 > w.rows || r1 - r0 > w.max_rows) {
+        set_err(err, DERR_ROWS);
+        return false;
+    }
+    if (r1 == r0) return false;
+    const int p0 = w.pos[s];
+    if (p0 < 0 || p0 > lim - (r1 - r0)) {
+        set_err(err, DERR_POS);
+        return false;
+    }
+    run.n = r1 - r0;
+    run.p0 = p0;
+    return true;
+}
+#endif
+
+}  // namespace b2

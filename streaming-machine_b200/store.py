@@ -1,0 +1,152 @@
+"""The key/value store held in 4 bits, over the C ABI's b2_store_*: rows written into it, read back, and the arrival
+(attention) over it.
+
+    from streaming_machine_b200 import convert, store
+    st = store.Store(convert.tables(), n_streams=64, max_ctx=1024, n_head=12)
+    st.write(k, v, pos)              # one new position per stream: k, v [64, 12, 64] int64, pos [64] int32
+    y = st.attend(q, pos)            # [64, 12, 64] int64: what each row takes from its stream's positions 0 .. pos
+    k4, v4 = st.read(pos)            # the values that the store holds for those positions
+
+Numbers are whole, at the stream's scale 2^-16; include/base2.h has the formulas. A prompt pass gives many rows per
+stream: stream i's are rows cu[i] .. cu[i + 1] - 1, its first at position pos[i], none with more than max_rows.
+Tensors are CUDA tensors of the store's device; calls queue their work on the current stream, allocate nothing but what
+they return and copy nothing to the host, so that they may be captured into a graph.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import numpy as np
+
+from .engine import B2Error, StoreConfig, _torch, lib
+
+HEAD = 64
+
+
+class Store:
+    """A 4-bit key/value store of `n_streams` streams of up to `max_ctx` positions, with `n_head` heads of 64 dims in each
+    of `n_layer` layers; every position stands for zeros until it is written. M: the machine's tables ("arrival", "log2",
+    "exp2", as convert.tables() or a converted model holds them)."""
+
+    def __init__(self, M: dict, n_streams: int, max_ctx: int, n_head: int, n_layer: int = 1, device: int = 0):
+        self.torch = _torch()
+        self.device = self.torch.device("cuda", device)
+        self.n_streams, self.max_ctx, self.n_head, self.n_layer = n_streams, max_ctx, n_head, n_layer
+        t = [np.ascontiguousarray(M[k], dtype=np.int64) for k in ("arrival", "log2", "exp2")]
+        if t[1].size != 65536 or t[2].size != 65536:
+            raise ValueError("the log2 and exp2 tables have 65,536 entries")
+        h = ctypes.c_void_p()
+        cfg = StoreConfig(n_streams, n_layer, n_head, max_ctx)
+        rc = lib().b2_store_create(ctypes.byref(cfg), device, t[0].ctypes.data, t[0].size, t[1].ctypes.data, t[2].ctypes.data,
+                                   ctypes.byref(h))
+        self.h = h if h.value else None
+        if rc:
+            msg = lib().b2_store_last_error(self.h).decode() if self.h else f"b2_store_create failed ({n_streams} streams, " \
+                f"{n_layer} layers, {n_head} heads, context {max_ctx}, device {device})"
+            self.close()
+            raise B2Error(rc, msg)
+
+    # ---- plumbing ---------------------------------------------------------------------------------------------
+    def _call(self, fn: str, *args):
+        if not self.h:
+            raise ValueError("the store is closed")
+        rc = getattr(lib(), fn)(self.h, *args)
+        if rc:
+            raise B2Error(rc, lib().b2_store_last_error(self.h).decode())
+
+    def _stream(self):
+        return ctypes.c_void_p(self.torch.cuda.current_stream(self.device).cuda_stream)
+
+    def _rows(self, x, name: str):
+        """(pointer, row stride) of int64 rows [rows, n_head, 64] or [rows, n_head * 64]; only the rows may be strided."""
+        self._on_device(x, name, self.torch.int64)
+        d = self.n_head * HEAD
+        ok = (x.dim() == 2 and x.shape[1] == d and (x.stride(1) == 1)) or \
+            (x.dim() == 3 and x.shape[1:] == (self.n_head, HEAD) and x.stride(2) == 1 and
+             (self.n_head == 1 or x.stride(1) == HEAD))
+        if not ok:
+            raise ValueError(f"{name}: rows of [{self.n_head}, {HEAD}] (or {d}) values, one behind the other, got shape "
+                             f"{tuple(x.shape)}, strides {x.stride()}")
+        if x.shape[0] > 1 and x.stride(0) < d:
+            raise ValueError(f"{name}: the rows overlap (stride {x.stride(0)}, rows of {d})")
+        return x.data_ptr(), max(x.stride(0), d)
+
+    def _on_device(self, x, name: str, dtype):
+        if not isinstance(x, self.torch.Tensor) or x.device != self.device or x.dtype != dtype:
+            what = f"{x.dtype} on {x.device}" if isinstance(x, self.torch.Tensor) else type(x).__name__
+            raise ValueError(f"{name}: a {dtype} tensor on {self.device}, got {what}")
+
+    def _i32(self, x, name: str, n: int | None = None):
+        self._on_device(x, name, self.torch.int32)
+        if x.dim() != 1 or not x.is_contiguous() or (n is not None and x.shape[0] != n):
+            raise ValueError(f"{name}: {'n' if n is None else n} int32 values in a row, got shape {tuple(x.shape)}")
+        return x.data_ptr()
+
+    def _table(self, pos, cu, rows: int, max_rows):
+        """The row table's arguments: cu, pos, n_streams, rows, max_rows."""
+        p = self._i32(pos, "pos")
+        n = pos.shape[0]
+        if cu is None:
+            if rows != n or max_rows not in (None, 1):
+                raise ValueError(f"without cu every stream gives one row: {rows} rows, {n} positions, max_rows {max_rows}")
+            return None, p, n, rows, 1
+        if max_rows is None:
+            raise ValueError("max_rows (the most rows a stream gives) goes with cu")
+        return self._i32(cu, "cu", n + 1), p, n, rows, max_rows
+
+    def _out(self, out, rows: int, name: str):
+        shape = (rows, self.n_head, HEAD)
+        if out is None:
+            return self.torch.empty(shape, dtype=self.torch.int64, device=self.device)
+        self._on_device(out, name, self.torch.int64)
+        if tuple(out.shape) != shape or not out.is_contiguous():
+            raise ValueError(f"{name}: a contiguous {shape}, got shape {tuple(out.shape)}, strides {out.stride()}")
+        return out
+
+    # ---- the operators ----------------------------------------------------------------------------------------
+    def write(self, k, v, pos, cu=None, max_rows: int | None = None, layer: int = 0):
+        """Hold rows k, v (int64 [rows, n_head, 64], or rows of n_head * 64; rows may be strided, as slices of a qkv row
+        are) at their streams' positions."""
+        (pk, ldk), (pv, ldv) = self._rows(k, "k"), self._rows(v, "v")
+        if k.shape[0] != v.shape[0]:
+            raise ValueError(f"{k.shape[0]} rows of keys, {v.shape[0]} of values")
+        self._call("b2_store_write", layer, pk, ldk, pv, ldv, *self._table(pos, cu, k.shape[0], max_rows), self._stream())
+
+    def read(self, pos, cu=None, max_rows: int | None = None, rows: int | None = None, layer: int = 0, out=None):
+        """(k, v), int64 [rows, n_head, 64]: the values that the store holds at the rows' positions. rows: how many there
+        are (with cu; its last entry). out: two tensors to fill instead of new ones. Rows that no stream has keep what
+        `out` held."""
+        if rows is None:
+            if cu is not None:
+                raise ValueError("rows (cu's last entry) goes with cu")
+            rows = pos.shape[0]
+        k, v = (self._out(o, rows, n) for o, n in zip(out if out is not None else (None, None), ("out k", "out v")))
+        self._call("b2_store_read", layer, *self._table(pos, cu, rows, max_rows), k.data_ptr(), v.data_ptr(), self._stream())
+        return k, v
+
+    def attend(self, q, pos, cu=None, max_rows: int | None = None, window: int = 0, first=None, layer: int = 0, out=None):
+        """The arrival of rows q (int64 [rows, n_head, 64], or rows of n_head * 64, strided or not) over the held keys and
+        values: int64 [rows, n_head, 64]. A row at position p sees the positions from the largest of 0, first[stream] (if
+        given) and p - window + 1 (if window > 0) to p; one that sees none gets zeros."""
+        pq, ldq = self._rows(q, "q")
+        out = self._out(out, q.shape[0], "out")
+        cu, p, n, rows, most = self._table(pos, cu, q.shape[0], max_rows)
+        f = self._i32(first, "first", n) if first is not None else None
+        self._call("b2_store_attend", layer, pq, ldq, cu, p, f, n, rows, most, window, out.data_ptr(), self._stream())
+        return out
+
+    def sync(self):
+        """Wait for the device and raise what its checks flagged (rows that do not fit the call, a position past the
+        context): the streams concerned were skipped."""
+        self._call("b2_store_sync")
+
+    def close(self):
+        if getattr(self, "h", None):
+            lib().b2_store_destroy(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass

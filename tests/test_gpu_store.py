@@ -1,0 +1,301 @@
+"""The 4-bit key/value store on the GPU against the formulas in plain Python (store_reference.py), bit for bit: every
+result is a whole number, so the tolerance is zero."""
+import numpy as np
+import pytest
+
+import store_reference as ref
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def T():
+    from streaming_machine_b200 import convert
+    return convert.tables()
+
+
+def make(T, streams, ctx, heads, layers=1):
+    from streaming_machine_b200 import store
+    return store.Store(T, n_streams=streams, max_ctx=ctx, n_head=heads, n_layer=layers), ref.Store(T, heads)
+
+
+def values(rng, rows, heads, size):
+    """Normal values of standard deviation 2^16 size; some channels 8 times larger, some rows of one sign or all zero."""
+    x = rng.standard_normal((rows, heads, 64)) * 65536 * size
+    x[..., rng.random(64) < 0.06] *= 8
+    x *= 2.0 ** rng.integers(-6, 3, (rows, heads, 1))
+    x[rng.random((rows, heads)) < 0.03] = 0
+    return np.round(x).astype(np.int64)
+
+
+def dev(a, dtype=None):
+    import torch
+    return torch.as_tensor(np.ascontiguousarray(a, dtype=dtype)).cuda()
+
+
+def i32(a):
+    return dev(a, np.int32)
+
+
+def run(T, rng, heads, held, rows, window=0, first=None, size=1.5, layers=1, layer=0):
+    """Streams that hold held[i] positions take rows[i] more: written, read back and attended, all against the reference."""
+    n = len(held)
+    st, pl = make(T, n, max(h + r for h, r in zip(held, rows)), heads, layers)
+    try:
+        for lens, pos in ((held, [0] * n), (rows, held)):
+            if not sum(lens):
+                continue
+            cu = np.concatenate([[0], np.cumsum(lens)])
+            k, v = values(rng, sum(lens), heads, 1.0), values(rng, sum(lens), heads, 0.3)
+            st.write(dev(k), dev(v), i32(pos), cu=i32(cu), max_rows=max(lens), layer=layer)
+            pl.write(k, v, pos, cu, layer)
+        q = values(rng, sum(rows), heads, size)
+        got = st.attend(dev(q), i32(held), cu=i32(cu), max_rows=max(rows), window=window, layer=layer,
+                        first=None if first is None else i32(first)).cpu().numpy()
+        back = [t.cpu().numpy() for t in st.read(i32(held), cu=i32(cu), max_rows=max(rows), rows=sum(rows), layer=layer)]
+        st.sync()
+        for b, w in zip(back, pl.read(held, cu, layer)):
+            assert np.array_equal(b, w)
+        assert np.array_equal(got, pl.attend(q, held, cu, window, first, layer))
+    finally:
+        st.close()
+
+
+@pytest.mark.parametrize("held", [0, 1, 2, 7, 15, 16, 31, 32, 33, 63, 64, 127, 300])
+def test_one_row(T, held):
+    run(T, np.random.default_rng(held), 2, [held, 0, held // 2], [1, 1, 1])
+
+
+@pytest.mark.parametrize("rows", [[1, 2, 5], [16, 17, 15], [33, 1, 64], [0, 40, 3], [65, 0, 0]])
+def test_many_rows(T, rows):
+    run(T, np.random.default_rng(sum(rows)), 2, [0, 9, 70], rows)
+
+
+@pytest.mark.parametrize("heads", [1, 3, 5])
+def test_head_counts(T, heads):
+    run(T, np.random.default_rng(heads), heads, [20, 3], [1, 4])
+
+
+@pytest.mark.parametrize("window", [1, 2, 16, 33, 1000])
+@pytest.mark.parametrize("rows", [[1, 1, 1], [20, 3, 1]])
+def test_windows(T, window, rows):
+    run(T, np.random.default_rng(window), 1, [90, 32, 5], rows, window=window)
+
+
+def test_dropped_beginnings_and_empty_rows(T):
+    """first below, inside and past a stream's rows: the second stream's rows see nothing, the third's first two do not,
+    and a negative first is none."""
+    run(T, np.random.default_rng(3), 2, [50, 50, 10, 5], [3, 3, 4, 1], first=[17, 53, 12, -7])
+    run(T, np.random.default_rng(4), 2, [50, 40], [1, 1], first=[51, 40], window=9)
+
+
+@pytest.mark.parametrize("size", [2.0 ** -16, 0.01, 40.0, 2.0 ** 20, 2.0 ** 40])
+def test_query_sizes(T, size):
+    """Scores from zeros to ones that are held at their limit (and weights from all alike to a single one)."""
+    run(T, np.random.default_rng(5), 1, [40], [2], size=size)
+
+
+def test_extremes(T):
+    """The largest magnitudes, +-2^63 and around 2^47 among them, and rows of zeros: nothing wraps."""
+    rng = np.random.default_rng(6)
+    big = np.array([-2 ** 63, 2 ** 63 - 1, -2 ** 47, 2 ** 47 - 1, 2 ** 47, -2 ** 47 - 1, 2 ** 46, 7, -8, 0, 1, 2 ** 31], dtype=np.int64)
+    st, pl = make(T, 3, 24, 2)
+    n = 24
+    pick = lambda rows, p: np.where(rng.random((rows, 2, 64)) < p, rng.choice(big, (rows, 2, 64)), rng.integers(-9, 9, (rows, 2, 64)))  # noqa: E731
+    k, v = pick(3 * n, 0.1), pick(3 * n, 0.05)
+    k[5], v[9], k[30:34], v[40:44] = 0, 0, 2 ** 47 - 1, -2 ** 63
+    cu, pos = [0, n, 2 * n, 3 * n], [0, 0, 0]
+    st.write(dev(k), dev(v), i32(pos), cu=i32(cu), max_rows=n)
+    pl.write(k, v, pos, cu)
+    for b, w in zip(st.read(i32(pos), cu=i32(cu), max_rows=n, rows=3 * n), pl.read(pos, cu)):
+        assert np.array_equal(b.cpu().numpy(), w)
+    for p in (0.0, 0.02, 0.5, 1.0):
+        q = pick(3 * n, p)
+        assert np.array_equal(st.attend(dev(q), i32(pos), cu=i32(cu), max_rows=n).cpu().numpy(), pl.attend(q, pos, cu))
+        # single rows at the last position too
+        q1, p1 = q[:3], [n - 1] * 3
+        assert np.array_equal(st.attend(dev(q1), i32(p1)).cpu().numpy(), pl.attend(q1, p1))
+    st.sync()
+    st.close()
+
+
+def test_other_tables(T):
+    """A table whose entries are equal, one that ends at once and one that starts at 1."""
+    rng = np.random.default_rng(7)
+    for arr in (np.full(3000, 1 << 24), np.array([1]), np.array([1, 0, 1, 5, 7]), np.array([1 << 24, 255, 1, 0, 3])):
+        T2 = dict(T, arrival=arr.astype(np.int64))
+        run(T2, rng, 1, [30, 2], [1, 1])
+        run(T2, rng, 1, [30, 2], [20, 3])
+
+
+def test_layers_and_slots_are_apart(T):
+    """What one (slot, layer) holds does not show in another; a stream written again from position 0 starts anew."""
+    rng = np.random.default_rng(8)
+    st, pl = make(T, 3, 40, 2, layers=3)
+    for layer in (2, 0, 1, 0):
+        lens = [int(t) for t in rng.integers(1, 30, 3)]
+        cu = np.concatenate([[0], np.cumsum(lens)])
+        k, v = values(rng, cu[-1], 2, 1.0), values(rng, cu[-1], 2, 0.3)
+        st.write(dev(k), dev(v), i32([0, 3, 1]), cu=i32(cu), max_rows=30, layer=layer)
+        pl.write(k, v, [0, 3, 1], cu, layer)
+    for layer in range(3):
+        q = values(rng, 3, 2, 1.5)
+        assert np.array_equal(st.attend(dev(q), i32([30, 32, 30]), layer=layer).cpu().numpy(), pl.attend(q, [30, 32, 30], layer=layer))
+        cu = [0, 40, 80, 120]
+        for b, w in zip(st.read(i32([0, 0, 0]), cu=i32(cu), max_rows=40, rows=120, layer=layer), pl.read([0, 0, 0], cu, layer)):
+            assert np.array_equal(b.cpu().numpy(), w)
+    st.sync()
+    st.close()
+
+
+@pytest.mark.parametrize("off", [0, 1])
+def test_strided_rows_and_rows_left_alone(T, off):
+    """Keys, values and queries as slices of a qkv row (also at an odd element), outputs with rows that no stream has: those
+    stay as they were, in the call's outputs and in the store."""
+    import torch
+    rng = np.random.default_rng(9)
+    H, d = 2, 128
+    st, pl = make(T, 3, 50, H)
+    cu, pos, rows = [0, 4, 4, 9], [2, 0, 0], 12
+    qkv = torch.zeros(rows, 3 * d + 5 + off, dtype=torch.int64, device="cuda")
+    x = values(rng, rows, 3 * H, 1.0).reshape(rows, 3 * d)
+    qkv[:, off:off + 3 * d] = dev(x)
+    part = [qkv[:, off + i * d:off + (i + 1) * d] for i in range(3)]
+    st.write(part[1], part[2], i32(pos), cu=i32(cu), max_rows=6)
+    host = [x[:, i * d:(i + 1) * d].reshape(rows, H, 64) for i in range(3)]
+    pl.write(host[1], host[2], pos, cu)
+    outs = [torch.full((rows, H, 64), -77, dtype=torch.int64, device="cuda") for _ in range(3)]
+    got = st.attend(part[0], i32(pos), cu=i32(cu), max_rows=6, out=outs[0])
+    assert got is outs[0]
+    st.read(i32(pos), cu=i32(cu), max_rows=6, rows=rows, out=outs[1:])
+    want = [pl.attend(host[0], pos, cu), *pl.read(pos, cu)]
+    for o, w in zip(outs, want):
+        o = o.cpu().numpy()
+        assert np.array_equal(o[:9], w) and (o[9:] == -77).all()
+    every = st.read(i32([0, 0, 0]), cu=i32([0, 50, 100, 150]), max_rows=50, rows=150)
+    for b, w in zip(every, pl.read([0, 0, 0], [0, 50, 100, 150])):
+        assert np.array_equal(b.cpu().numpy(), w)
+    st.sync()
+    st.close()
+
+
+def test_bad_rows_are_flagged_and_skipped(T):
+    """Each device check by itself: the stream concerned is left out, the others are done, and sync() reports it once."""
+    import torch
+    from streaming_machine_b200 import engine
+    rng = np.random.default_rng(10)
+    st, pl = make(T, 3, 16, 1)
+    k, v, q = (values(rng, 6, 1, 1.0) for _ in range(3))
+    good = [0, 2, 4, 6]
+    st.write(dev(k), dev(v), i32([0, 0, 0]), cu=i32(good), max_rows=2)
+    pl.write(k, v, [0, 0, 0], good)
+    want = pl.attend(q, [0, 0, 0], good)
+    k2, v2 = values(rng, 6, 1, 1.0), values(rng, 6, 1, 1.0)
+    #       cu, pos, the code, the streams left out
+    bad = [([0, 2, 1, 6], [0, 0, 0], 1, (1, 2)), ([0, 2, 4, 7], [0, 0, 0], 1, (2,)), ([-1, 2, 4, 6], [0, 0, 0], 1, (0,)),
+           ([0, 2, 4, 6], [15, 0, 0], 4, (0,)), ([0, 2, 4, 6], [0, -1, 0], 4, (1,)), ([0, 2, 4, 6], [0, 0, 2 ** 31 - 1], 4, (2,)),
+           ([0, 2, 4, 2 ** 31 - 1], [0, 0, 0], 1, (2,)), ([-2 ** 31, 2, 4, 6], [0, 0, 0], 1, (0,))]
+    for cu, pos, code, left in bad:
+        out = torch.full((6, 1, 64), -5, dtype=torch.int64, device="cuda")
+        st.attend(dev(q), i32(pos), cu=i32(cu), max_rows=2, out=out)
+        with pytest.raises(engine.B2Error) as ex:
+            st.sync()
+        assert ex.value.code == code
+        st.sync()                                          # reported once
+        out = out.cpu().numpy()
+        for s in range(3):
+            rows = slice(2 * s, 2 * s + 2)
+            assert (out[rows] == -5).all() if s in left else np.array_equal(out[rows], want[rows])
+        # a write of the same table leaves those streams as they were (the others get what they already hold)
+        kk, vv = k.copy(), v.copy()
+        for s in left:
+            kk[2 * s:2 * s + 2], vv[2 * s:2 * s + 2] = k2[2 * s:2 * s + 2], v2[2 * s:2 * s + 2]
+        st.write(dev(kk), dev(vv), i32(pos), cu=i32(cu), max_rows=2)
+        with pytest.raises(engine.B2Error):
+            st.sync()
+        for b, w in zip(st.read(i32([0, 0, 0]), cu=i32(good), max_rows=2, rows=6), pl.read([0, 0, 0], good)):
+            assert np.array_equal(b.cpu().numpy(), w)
+    st.sync()
+    st.close()
+
+
+def test_refusals(T):
+    """What the host refuses: nothing is launched, the store stays usable."""
+    import torch
+    from streaming_machine_b200 import engine, store
+    with pytest.raises(engine.B2Error) as ex:
+        store.Store(dict(T, arrival=np.array([1 << 25])), 1, 16, 1)
+    assert ex.value.code == 5 and "arrival" in str(ex.value)
+    with pytest.raises(engine.B2Error) as ex:
+        store.Store(dict(T, arrival=np.array([0, 5])), 1, 16, 1)
+    assert ex.value.code == 5
+    with pytest.raises(engine.B2Error) as ex:
+        store.Store(T, 1, 65537, 1)
+    assert ex.value.code == 1
+    with pytest.raises(engine.B2Error) as ex:
+        store.Store(T, 65535, 65536, 1024, n_layer=1024)     # far past the device's memory
+    assert ex.value.code == 3
+    st, _ = make(T, 2, 16, 1, layers=2)
+    x = torch.zeros(2, 1, 64, dtype=torch.int64, device="cuda")
+    pos = i32([0, 0])
+    for call in (lambda: st.write(x, x, pos, layer=2), lambda: st.write(x, x, pos, layer=-1),
+                 lambda: st.attend(x, pos, window=-1), lambda: st.write(x[:1].expand(3, 1, 64).contiguous(), x[:1].expand(3, 1, 64).contiguous(), i32([0, 0, 0])),
+                 lambda: st.attend(x, pos, cu=i32([0, 1, 2]), max_rows=17), lambda: st.attend(x, pos, cu=i32([0, 1, 2]), max_rows=0),
+                 lambda: st.attend(x, i32([]), cu=i32([0]), max_rows=1)):
+        with pytest.raises(engine.B2Error) as ex:
+            call()
+        assert ex.value.code == 1
+    for call in (lambda: st.write(x.cpu(), x, pos), lambda: st.write(x, x[:1], pos), lambda: st.attend(x.float(), pos),
+                 lambda: st.attend(x, pos.long()), lambda: st.attend(x, pos, first=i32([0])), lambda: st.attend(x, pos, out=x[:1])):
+        with pytest.raises(ValueError):
+            call()
+    empty = torch.zeros(0, 1, 64, dtype=torch.int64, device="cuda")   # nothing to do is no error
+    st.write(empty, empty, pos, cu=i32([0, 0, 0]), max_rows=0)
+    assert st.attend(empty, pos, cu=i32([0, 0, 0]), max_rows=0).shape == (0, 1, 64)
+    assert st.attend(empty, i32([])).shape == (0, 1, 64)
+    st.sync()
+    st.close()
+    with pytest.raises(ValueError):
+        st.attend(x, pos)
+
+
+def test_captured_and_on_another_stream(T):
+    """write and attend captured into two graphs on one store and replayed with other inputs and positions, then the same
+    on a side stream: each the plain calls' results."""
+    import torch
+    rng = np.random.default_rng(11)
+    H = 2
+    st, pl = make(T, 4, 64, H)
+    pos = i32([0, 5, 0, 9])
+    k, v, q = (dev(values(rng, 4, H, 1.0)) for _ in range(3))
+    out = torch.zeros(4, H, 64, dtype=torch.int64, device="cuda")
+    st.write(k, v, pos)
+    st.attend(q, pos, out=out)                               # the first calls load the kernels
+    torch.cuda.synchronize()
+    graphs = []
+    side = torch.cuda.Stream()
+    for step in (lambda: st.write(k, v, pos), lambda: st.attend(q, pos, out=out)):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            step()
+        graphs.append(g)
+    pl.write(k.cpu().numpy(), v.cpu().numpy(), [0, 5, 0, 9])
+    at = np.array([0, 5, 0, 9])
+    for t in range(3):
+        at = at + 1
+        pos.copy_(i32(at))
+        for x in (k, v, q):
+            x.copy_(dev(values(rng, 4, H, 1.0)))
+        pl.write(k.cpu().numpy(), v.cpu().numpy(), at)
+        if t < 2:
+            for g in graphs:
+                g.replay()
+        else:
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                st.write(k, v, pos)
+                st.attend(q, pos, out=out)
+            side.synchronize()
+        assert np.array_equal(out.cpu().numpy(), pl.attend(q.cpu().numpy(), at))
+    st.sync()
+    st.close()

@@ -1,0 +1,101 @@
+"""The 4-bit store on the CPU: the formulas' own bounds, the layout's permutation, and every refusal that is made before
+anything is launched."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+import store_reference as ref
+
+RNG = np.random.default_rng(41)
+
+
+@pytest.mark.parametrize("bits", [0, 1, 3, 4, 5, 17, 31, 46, 47, 48, 60, 62])
+def test_held_values_are_near(bits):
+    """A held value is off by at most half a step 2^s, or by a whole one where the code 8 does not exist (its 4 bits
+    reach 7): |x| < 2^t, s = t - 3, so x 2^-s < 8 rounds to at most 8, which is held as 7, a step away at most."""
+    for _ in range(20):
+        x = np.array([int(RNG.integers(-(1 << 62), 1 << 62)) >> (62 - bits) if bits else 0 for _ in range(64)], dtype=np.int64)
+        for held, read, shifts in ((ref.hold_key(x), ref.read_key, 2), (ref.hold_value(x), ref.read_value, 1)):
+            c, s = held
+            assert all(-8 <= t <= 7 for t in c)
+            step = np.repeat([1 << t for t in s], 32) if shifts == 2 else np.full(64, 1 << s)
+            off = np.abs(ref.clamp(x) - read(held))
+            assert (2 * off <= step * (1 + (np.array(c) == 7))).all()
+            if np.abs(x).max() <= 7:          # a bit length of 3: no shift, and every value is its own code
+                assert (off == 0).all()
+
+
+def test_halves_stay_within_three_digits():
+    x = np.zeros(64, np.int64)
+    x[3], x[40] = 1 << 30, 5
+    _, s = ref.hold_key(x)
+    assert s == [28, 25]
+    x[3] = 9
+    assert ref.hold_key(x)[1] == [1, 0]
+
+
+def _bare(n_head=3):
+    """A Store whose checks run without a GPU: the host logic alone (nothing is launched by a call that is refused)."""
+    from streaming_machine_b200 import store
+    st = object.__new__(store.Store)
+    st.torch, st.device, st.n_head, st.n_streams, st.max_ctx, st.n_layer, st.h = torch, torch.device("cpu"), n_head, 4, 64, 1, None
+    return st
+
+
+def test_rows_are_refused():
+    st = _bare()
+    good = torch.zeros(5, 3, 64, dtype=torch.int64)
+    assert st._rows(good, "k")[1] == 192
+    qkv = torch.zeros(5, 9 * 64, dtype=torch.int64)
+    p, ld = st._rows(qkv[:, 192:384], "k")
+    assert ld == 576 and p == qkv.data_ptr() + 192 * 8
+    assert st._rows(qkv[:, 192:384].unflatten(1, (3, 64)), "k")[1] == 576
+    for bad in (good.to(torch.int32), good.float(), good[:, :2], good.transpose(0, 1), good[..., ::2], good[:, :, :32],
+                torch.zeros(5, 3, 128, dtype=torch.int64)[..., ::2], good.view(15, 64), torch.zeros(1, 192, dtype=torch.int64).expand(5, 192),
+                np.zeros((5, 3, 64), np.int64)):
+        with pytest.raises(ValueError):
+            st._rows(bad, "k")
+
+
+def test_tables_are_refused():
+    st = _bare()
+    pos = torch.zeros(4, dtype=torch.int32)
+    cu = torch.zeros(5, dtype=torch.int32)
+    assert st._table(pos, None, 4, None)[2:] == (4, 4, 1)
+    assert st._table(pos, cu, 9, 3)[2:] == (4, 9, 3)
+    for args in ((pos, None, 5, None), (pos, None, 4, 2), (pos, cu, 9, None), (pos, cu[:4], 9, 3), (pos.long(), None, 4, None),
+                 (pos[::2], None, 2, None), (pos[None], None, 1, None)):
+        with pytest.raises(ValueError):
+            st._table(*args)
+    with pytest.raises(ValueError):
+        st._out(torch.zeros(4, 3, 32, dtype=torch.int64), 4, "out")
+    with pytest.raises(ValueError):
+        st._out(torch.zeros(4, 3, 128, dtype=torch.int64)[..., :64], 4, "out")
+    with pytest.raises(ValueError):
+        st.read(pos, cu=cu, max_rows=3)                       # rows goes with cu
+    with pytest.raises(ValueError):
+        st.attend(torch.zeros(4, 3, 64, dtype=torch.int64), pos)   # a closed store
+
+
+def test_create_refuses_before_it_touches_a_device():
+    from streaming_machine_b200 import engine
+    L = engine.lib()
+    t = np.ones(65536, np.int64)
+    h = ctypes.c_void_p()
+
+    def create(cfg, arr=t, n=100, log2=t, exp2=t):
+        ptr = [a.ctypes.data if a is not None else None for a in (arr, log2, exp2)]
+        return L.b2_store_create(ctypes.byref(engine.StoreConfig(*cfg)), 0, ptr[0], n, ptr[1], ptr[2], ctypes.byref(h))
+    for cfg in ((0, 1, 1, 1), (65536, 1, 1, 1), (1, 0, 1, 1), (1, 1025, 1, 1), (1, 1, 0, 1), (1, 1, 1025, 1), (1, 1, 1, 0),
+                (1, 1, 1, 65537), (-1, 1, 1, 1)):
+        assert create(cfg) == 1 and not h.value
+    for kw in (dict(arr=None), dict(log2=None), dict(exp2=None), dict(n=0), dict(n=-5), dict(n=(1 << 20) + 1)):
+        assert create((1, 1, 1, 1), **kw) == 1 and not h.value
+    for f, args in (("b2_store_write", (0, None, 0, None, 0, None, None, 0, 0, 0, None)),
+                    ("b2_store_read", (0, None, None, 0, 0, 0, None, None, None)),
+                    ("b2_store_attend", (0, None, 0, None, None, None, 0, 0, 0, 0, None, None)), ("b2_store_sync", ())):
+        assert getattr(L, f)(None, *args) == 1
+    assert L.b2_store_last_error(None) == b"null store"
+    L.b2_store_destroy(None)
