@@ -4,12 +4,14 @@
 #include <stdio.h>
 #include <string.h>
 
+#include <algorithm>
 #include <exception>
 #include <new>
 #include <string>
 #include <vector>
 
 #include "../../include/base2.h"
+#include "b2_ptx.cuh"
 #include "b2_store.cuh"
 
 namespace b2 {
@@ -95,104 +97,271 @@ __global__ void __launch_bounds__(SW_WARPS * 32) k_store_read(Store4 st, StoreRo
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// the arrival, one CTA of 8 warps per (row, head): a warp takes a key at a time, two dims a lane.
-//   pass 1  every visible key's score: the largest; the largest value shift
-//   pass 2  the scores again, a = ARR[start - score], Z = sum a, num = sum rnd(a, 1 + M - vs) c
+// the arrival of few rows a stream (a decode step), one CTA of SF_WARPS warps per (row, head), or a cluster of CS sharing
+// its keys. The integer table softmax needs the largest score before any weight (a = ARR[start - score] does not factor),
+// so the keys are read once for the scores, which stay in shared memory, and the values once after it:
+//   pass 1  32 keys a warp: their codes as the A rows of m16n8k32 (16 c: the digits stay in a byte's upper half, no sign
+//           to extend), the query's two bytes as B columns, so the two products of a key meet in one lane; scores into
+//           shared memory, the largest score and value shift by warp maxima
+//   pass 2  a = ARR[start - score], Z += a, the weight's three bytes into three planes of shared memory
+//   pass 3  num: the planes as the A rows, the values' codes as B (4 keys x 8 dims of nibbles turned by byte permutes)
 // ---------------------------------------------------------------------------------------------------------------------
-constexpr int SA_WARPS = 8;
+constexpr int SF_WARPS = 4;
+constexpr int SF_BYTES = 8;      // shared memory a key: 4 score, 3 planes, 1 value shift
 
-B2_DEV int32_t key_dot(const Store4& st, size_t e, int lane, int q0, int q1, int& S) {
-    const int c = (int)(int8_t)st.k[e * 32 + key_byte(lane)];
-    const int lo = (int)((uint32_t)c << 28) >> 28, hi = c >> 4;
-    const int s0 = st.ks[e * 2], s1 = st.ks[e * 2 + 1];
-    S = max(s0, s1);
-    const int up = (lane < 16 ? s0 : s1) - S + 3;
-    return __reduce_add_sync(0xffffffffu, (lo * q0 + hi * q1) << up);
+B2_DEV void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+B2_DEV void mma_u8s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// eight 4-bit codes of a word as signed bytes 16 c: the even dims' and the odd dims'
+B2_DEV uint32_t even16(uint32_t w) { return (w << 4) & 0xF0F0F0F0u; }
+B2_DEV uint32_t odd16(uint32_t w) { return w & 0xF0F0F0F0u; }
+
+// the same score from 16 dot (what the tensor cores give of 16 c): r16 = 32 - u - S
+B2_DEV int32_t score16(int32_t dot16, int r16) { return r16 >= 4 ? rnd32(dot16, r16) : store_score(dot16 >> 4, r16 - 4); }
+
+// four words (one of each of four keys, eight dims each) -> byte b of all four in r[b] (dims 2b and 2b + 1)
+B2_DEV void turn4(const uint32_t* w, uint32_t (&r)[4]) {
+    const uint32_t t0 = __byte_perm(w[0], w[1], 0x5140), t1 = __byte_perm(w[2], w[3], 0x5140);
+    const uint32_t t2 = __byte_perm(w[0], w[1], 0x7362), t3 = __byte_perm(w[2], w[3], 0x7362);
+    r[0] = __byte_perm(t0, t1, 0x5410);
+    r[1] = __byte_perm(t0, t1, 0x7632);
+    r[2] = __byte_perm(t2, t3, 0x5410);
+    r[3] = __byte_perm(t2, t3, 0x7632);
 }
 
-__global__ void __launch_bounds__(SA_WARPS * 32) k_store_attend(StoreAttend a) {
-    griddep_wait();
-    griddep_launch();
-    const int i = blockIdx.x, h = blockIdx.y, s = blockIdx.z;
-    const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
-    __shared__ int64_t s_num[SA_WARPS][64], s_z[SA_WARPS];
-    __shared__ int32_t s_max[SA_WARPS], s_shift[SA_WARPS];
-    StoreRun run;
-    if (!store_run(a.rw, s, a.st.lim, run, a.err) || i >= run.n) return;
-    const int H = a.st.H, row = run.r0 + i, p = run.p0 + i;
-    int lo = a.window > 0 ? max(0, p - a.window + 1) : 0;
-    if (a.first) lo = max(lo, a.first[s]);
-    int64_t* out = a.out + ((size_t)row * H + h) * 64;
-    if (lo > p) {
-        if (threadIdx.x < 64) out[threadIdx.x] = 0;
-        return;
-    }
-    const int64_t* q = a.q + (size_t)row * a.ldq + h * 64 + 2 * lane;
-    const int64_t x0 = store_clamp(q[0]), x1 = store_clamp(q[1]);
+// a row's 64 query values at 15 bits, as two signed bytes q15 = 256 hi + lo, in a lane's pair (dims 2 lane, 2 lane + 1):
+// bytes hi, lo of the first, hi, lo of the second. Returns the row's shift u. Every lane of the warp takes part.
+B2_DEV int query_bytes(const int64_t* q, bool wide, int lane, uint32_t& word) {
+    int64_t x0, x1;
+    load_pair(q + 2 * lane, wide, x0, x1);
+    x0 = store_clamp(x0);
+    x1 = store_clamp(x1);
     const uint64_t m0 = mag(x0), m1 = mag(x1);
     const int u = max((int)__reduce_max_sync(0xffffffffu, (uint32_t)bitlen_u(m0 > m1 ? m0 : m1)) - 14, 0);
-    const int q0 = (int)rnd64(x0, u), q1 = (int)rnd64(x1, u);
-    const size_t base = kv_index(s, a.layer, h, 0, a.st.L, H, a.st.ctx);
-    int32_t start = -STORE_LIM - 1;
-    int M = 0, S;
-    for (int j = lo + wid; j <= p; j += SA_WARPS) {
-        const int32_t dot = key_dot(a.st, base + j, lane, q0, q1, S);
-        start = max(start, store_score(dot, 28 - u - S));
-        M = max(M, (int)a.st.vs[base + j]);
+    const int a = (int)rnd64(x0, u), b = (int)rnd64(x1, u);
+    word = (uint32_t)(((a + 128) >> 8) & 255) | (uint32_t)(a & 255) << 8 | (uint32_t)(((b + 128) >> 8) & 255) << 16 |
+           (uint32_t)(b & 255) << 24;
+    return u;
+}
+
+template <int CS>
+__global__ void __launch_bounds__(SF_WARPS * 32) k_store_attend_few(StoreAttend a, int chunk, int wide) {
+    griddep_wait();
+    griddep_launch();
+    extern __shared__ __align__(16) uint8_t sm[];
+    int32_t* const SC = reinterpret_cast<int32_t*>(sm);              // [chunk]
+    uint8_t* const WP = sm + (size_t)chunk * 4;                      // [3][chunk]
+    int8_t* const VS = reinterpret_cast<int8_t*>(sm + (size_t)chunk * 7);   // [chunk]
+    __shared__ int32_t s_max[SF_WARPS], s_shift[SF_WARPS], s_acc[SF_WARPS][3][64];
+    __shared__ int64_t s_z[SF_WARPS], s_num[65];
+    __shared__ int2 s_own;                                           // CS > 1: this CTA's largest score and shift
+    const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, g = lane >> 2, j = lane & 3;
+    const int H = a.st.H, h = blockIdx.y, s = blockIdx.z, i = CS > 1 ? blockIdx.x / CS : blockIdx.x;
+    const int rank = CS > 1 ? (int)cluster_rank() : 0;
+    StoreRun run;
+    if (!store_run(a.rw, s, a.st.lim, run, a.err) || i >= run.n) return;   // the same for a whole cluster
+    const int row = run.r0 + i, p = run.p0 + i;
+    int lo = a.window > 0 ? max(0, p - a.window + 1) : 0;
+    if (a.first) lo = max(lo, a.first[s]);
+    int64_t* const out = a.out + ((size_t)row * H + h) * 64;
+    if (lo > p) {
+        if (rank == 0 && threadIdx.x < 64) out[threadIdx.x] = 0;
+        return;
     }
+    // blocks of 32 positions; this CTA's are b0 .. b0 + nb - 1
+    const int first_block = lo >> 5, blocks = (p >> 5) - first_block + 1;
+    const int per = CS > 1 ? (blocks + CS - 1) / CS : blocks;
+    const int b0 = first_block + rank * per, nb = max(0, min(per, blocks - rank * per));
+    const size_t base = kv_index(s, a.layer, h, 0, a.st.L, H, a.st.ctx) + (size_t)b0 * 32;
+    const uint8_t* const K = a.st.k + base * 32;
+    const uint8_t* const V = a.st.v + base * 32;
+    const int8_t* const KS = a.st.ks + base * 2;
+    const int from = lo - b0 * 32, to = p - b0 * 32;                 // visible: from <= local key <= to
+
+    uint32_t word, q0[2], q1[2];                                     // B operands of the two halves
+    const int u = query_bytes(a.q + (size_t)row * a.ldq + h * 64, wide, lane, word);
+    {
+        const uint32_t pick = (g & 1) ? 0x5151u : 0x4040u;           // odd columns the low bytes
+#pragma unroll
+        for (int x = 0; x < 2; x++) {
+            uint32_t w[4];
+#pragma unroll
+            for (int b = 0; b < 4; b++) w[b] = __shfl_sync(0xffffffffu, word, 16 * x + 4 * j + b);
+            const uint32_t e01 = __byte_perm(w[0], w[1], pick & 0xFF), e23 = __byte_perm(w[2], w[3], pick & 0xFF);
+            const uint32_t o01 = __byte_perm(w[0], w[1], (pick & 0xFF) + 0x22), o23 = __byte_perm(w[2], w[3], (pick & 0xFF) + 0x22);
+            q0[x] = __byte_perm(e01, e23, 0x5410);
+            q1[x] = __byte_perm(o01, o23, 0x5410);
+        }
+    }
+    int32_t start = -STORE_LIM - 1;
+    int M = 0;
+    for (int b = wid; b < nb; b += SF_WARPS) {
+        const int key = b * 32 + 16 * (j >> 1) + 8 * (j & 1) + g;    // the key whose score this lane finishes
+        uint2 w[4];
+#pragma unroll
+        for (int t = 0; t < 4; t++) w[t] = *reinterpret_cast<const uint2*>(K + (size_t)(b * 32 + 8 * t + g) * 32 + 8 * j);
+        const int ksw = *reinterpret_cast<const uint16_t*>(KS + (size_t)key * 2);
+        const int vs = a.st.vs[base + key];
+        int d[2][2][4] = {};                                         // [block of 16][half]
+#pragma unroll
+        for (int m = 0; m < 2; m++) {
+            mma_s8(d[m][0], even16(w[2 * m].x), even16(w[2 * m + 1].x), odd16(w[2 * m].x), odd16(w[2 * m + 1].x), q0[0], q1[0]);
+            mma_s8(d[m][1], even16(w[2 * m].y), even16(w[2 * m + 1].y), odd16(w[2 * m].y), odd16(w[2 * m + 1].y), q0[1], q1[1]);
+        }
+        int dot[2];
+#pragma unroll
+        for (int x = 0; x < 2; x++) {
+            const int hi = (j & 2) ? ((j & 1) ? d[1][x][2] : d[1][x][0]) : ((j & 1) ? d[0][x][2] : d[0][x][0]);
+            const int lw = (j & 2) ? ((j & 1) ? d[1][x][3] : d[1][x][1]) : ((j & 1) ? d[0][x][3] : d[0][x][1]);
+            dot[x] = 256 * hi + lw;
+        }
+        const int s0 = (int8_t)(ksw & 255), s1 = (int8_t)(ksw >> 8), S = max(s0, s1);
+        const int32_t sc = score16((dot[0] << (s0 - S + 3)) + (dot[1] << (s1 - S + 3)), 32 - u - S);
+        SC[key] = sc;
+        VS[key] = (int8_t)vs;
+        if (key >= from && key <= to) {
+            start = max(start, sc);
+            M = max(M, vs);
+        }
+    }
+    start = __reduce_max_sync(0xffffffffu, start);
+    M = __reduce_max_sync(0xffffffffu, M);
     if (lane == 0) { s_max[wid] = start; s_shift[wid] = M; }
     __syncthreads();
-    for (int k = 0; k < SA_WARPS; k++) {
+#pragma unroll
+    for (int k = 0; k < SF_WARPS; k++) {
         start = max(start, s_max[k]);
         M = max(M, s_shift[k]);
     }
-    int64_t n0 = 0, n1 = 0, z = 0;
-    for (int j = lo + wid; j <= p; j += SA_WARPS) {
-        const int32_t dot = key_dot(a.st, base + j, lane, q0, q1, S);
-        const int32_t d = start - store_score(dot, 28 - u - S);
-        if (d >= a.alen) continue;
-        const int32_t w = __ldg(a.ARR + d);
-        z += w;
-        const int64_t wr = rnd32(w, min(STORE_W_SHIFT + M - a.st.vs[base + j], 26));
-        const int c = (int)(int8_t)a.st.v[(base + j) * 32 + lane];
-        n0 += wr * ((int)((uint32_t)c << 28) >> 28);
-        n1 += wr * (c >> 4);
+    if (CS > 1) {
+        if (threadIdx.x == 0) s_own = make_int2(start, M);
+        cluster_sync();
+#pragma unroll
+        for (int k = 0; k < CS; k++) {
+            const int64_t o = ld_dsmem(mapa(saddr(&s_own), (uint32_t)k));
+            start = max(start, (int32_t)o);
+            M = max(M, (int)(o >> 32));
+        }
     }
-    s_num[wid][2 * lane] = n0;
-    s_num[wid][2 * lane + 1] = n1;
+    // ---- weights: four keys a thread
+    int64_t z = 0;
+    for (int k = threadIdx.x * 4; k < nb * 32; k += SF_WARPS * 128) {
+        const int4 sc = *reinterpret_cast<const int4*>(SC + k);
+        const uint32_t v4 = *reinterpret_cast<const uint32_t*>(VS + k);
+        const int scs[4] = {sc.x, sc.y, sc.z, sc.w};
+        uint32_t w[4];
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            const int d = start - scs[t];
+            const bool seen = k + t >= from && k + t <= to && d < a.alen;
+            const int av = seen ? __ldg(a.ARR + d) : 0;
+            z += av;
+            w[t] = seen ? (uint32_t)rnd32(av, min(STORE_W_SHIFT + M - (int)(int8_t)(v4 >> (8 * t)), 26)) : 0u;
+        }
+        uint32_t r[4];
+        turn4(w, r);
+#pragma unroll
+        for (int b = 0; b < 3; b++) *reinterpret_cast<uint32_t*>(WP + (size_t)b * chunk + k) = r[b];
+    }
+    z = warp_sum64(z);
     if (lane == 0) s_z[wid] = z;
     __syncthreads();
-    if (wid) return;
-    n0 = n1 = z = 0;
-    for (int k = 0; k < SA_WARPS; k++) {
-        n0 += s_num[k][2 * lane];
-        n1 += s_num[k][2 * lane + 1];
-        z += s_z[k];
+    // ---- values: a lane takes word g (dims 8g .. 8g + 7) of keys 8j .. 8j + 7 of a block of 32
+    int acc[8][4] = {};
+    for (int b = wid; b < nb; b += SF_WARPS) {
+        uint32_t w[8];
+#pragma unroll
+        for (int t = 0; t < 8; t++) w[t] = *reinterpret_cast<const uint32_t*>(V + (size_t)(b * 32 + 8 * j + t) * 32 + 4 * g);
+        uint2 p8 = make_uint2(0, 0);
+        if (g < 3) p8 = *reinterpret_cast<const uint2*>(WP + (size_t)g * chunk + b * 32 + 8 * j);
+        uint32_t r0[4], r1[4];
+        turn4(w, r0);
+        turn4(w + 4, r1);
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            mma_u8s8(acc[2 * t], p8.x, 0, p8.y, 0, even16(r0[t]), even16(r1[t]));
+            mma_u8s8(acc[2 * t + 1], p8.x, 0, p8.y, 0, odd16(r0[t]), odd16(r1[t]));
+        }
     }
-    const int64_t F = 65536ll * (M + STORE_W_SHIFT) - log2fix(z, a.LOG2);
-    const int64_t y0 = power(n0, F, a.EXP2), y1 = power(n1, F, a.EXP2);
-    out[2 * lane] = y0;
-    out[2 * lane + 1] = y1;
-    if (a.or_out) {
-        const uint64_t o = warp_or64(mag(y0) | mag(y1));
-        if (lane == 0) atomicOr((unsigned long long*)&a.or_out[row], (unsigned long long)o);
+    // row g of the tiles is plane g; columns 2j, 2j + 1 of tile t are dims 16j + t and 16j + 8 + t
+    if (g < 3) {
+#pragma unroll
+        for (int t = 0; t < 8; t++) {
+            s_acc[wid][g][16 * j + t] = acc[t][0];
+            s_acc[wid][g][16 * j + 8 + t] = acc[t][1];
+        }
     }
+    __syncthreads();
+    int64_t num = 0;
+    if (threadIdx.x < 64) {
+#pragma unroll
+        for (int b = 0; b < 3; b++) {
+            int t = 0;
+#pragma unroll
+            for (int k = 0; k < SF_WARPS; k++) t += s_acc[k][b][threadIdx.x];
+            num += (int64_t)t << (8 * b);
+        }
+        z = 0;
+#pragma unroll
+        for (int k = 0; k < SF_WARPS; k++) z += s_z[k];
+    }
+    if (CS > 1) {
+        if (threadIdx.x < 64) {
+            s_num[threadIdx.x] = num;
+            if (threadIdx.x == 0) s_num[64] = z;
+        }
+        cluster_sync();
+        if (rank == 0 && threadIdx.x < 64) {
+            num = z = 0;
+#pragma unroll
+            for (int k = 0; k < CS; k++) {
+                num += ld_dsmem(mapa(saddr(&s_num[threadIdx.x]), (uint32_t)k));
+                z += ld_dsmem(mapa(saddr(&s_num[64]), (uint32_t)k));
+            }
+        }
+    }
+    if (rank == 0 && threadIdx.x < 64) {
+        const int64_t F = 65536ll * (M + STORE_W_SHIFT) - log2fix(z, a.LOG2);
+        const int64_t y = power(num >> 4, F, a.EXP2);                // the tiles hold 16 c
+        out[threadIdx.x] = y;
+        if (a.or_out) {
+            const uint64_t o = warp_or64(mag(y));
+            if (lane == 0) atomicOr((unsigned long long*)&a.or_out[row], (unsigned long long)o);
+        }
+    }
+    if (CS > 1) cluster_sync();                                      // rank 0 has read the others' sums
 }
 
 // ---- launches -------------------------------------------------------------------------------------------------------
 namespace {
 template <typename... KArgs, typename... Args>
-cudaError_t store_launch(StoreLaunch how, void (*kernel)(KArgs...), dim3 grid, int threads, size_t smem, Args... args) {
+cudaError_t store_launch(StoreLaunch how, void (*kernel)(KArgs...), dim3 grid, int threads, size_t smem, int cluster, Args... args) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = how.stream;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchAttribute at[2];
+    int n = 0;
+    if (cluster > 1) {
+        at[n].id = cudaLaunchAttributeClusterDimension;
+        at[n].val.clusterDim.x = cluster;
+        at[n].val.clusterDim.y = 1;
+        at[n++].val.clusterDim.z = 1;
+    }
+    if (how.pdl) {
+        at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[n++].val.programmaticStreamSerializationAllowed = 1;
+    }
     cfg.attrs = at;
-    cfg.numAttrs = how.pdl ? 1 : 0;
+    cfg.numAttrs = n;
     return cudaLaunchKernelEx(&cfg, kernel, ((KArgs)args)...);
 }
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
@@ -203,20 +372,44 @@ cudaError_t store_write(const Store4& st, const StoreRows& rw, int layer, const 
     if (rw.n_streams == 0 || rw.rows == 0) return cudaSuccess;
     const int wide = aligned16(k) && aligned16(v) && ldk % 2 == 0 && ldv % 2 == 0;
     const dim3 grid((unsigned)(((int64_t)rw.max_rows * 2 * st.H + SW_WARPS - 1) / SW_WARPS), rw.n_streams);
-    return store_launch(how, k_store_write, grid, SW_WARPS * 32, 0, st, rw, layer, k, ldk, v, ldv, wide, err);
+    return store_launch(how, k_store_write, grid, SW_WARPS * 32, 0, 1, st, rw, layer, k, ldk, v, ldv, wide, err);
 }
 
 cudaError_t store_read(const Store4& st, const StoreRows& rw, int layer, int64_t* k, int64_t* v, uint32_t* err, StoreLaunch how) {
     if (rw.n_streams == 0 || rw.rows == 0) return cudaSuccess;
     const int wide = aligned16(k) && aligned16(v);
     const dim3 grid((unsigned)(((int64_t)rw.max_rows * 2 * st.H + SW_WARPS - 1) / SW_WARPS), rw.n_streams);
-    return store_launch(how, k_store_read, grid, SW_WARPS * 32, 0, st, rw, layer, k, v, wide, err);
+    return store_launch(how, k_store_read, grid, SW_WARPS * 32, 0, 1, st, rw, layer, k, v, wide, err);
+}
+
+constexpr int SF_MOST_KEYS = 8192;   // of a CTA: 64 KB of shared memory
+
+cudaError_t store_init() {
+    cudaError_t e = cudaFuncSetAttribute(k_store_attend_few<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, SF_MOST_KEYS * SF_BYTES);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(k_store_attend_few<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, SF_MOST_KEYS * SF_BYTES);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(k_store_attend_few<4>, cudaFuncAttributeMaxDynamicSharedMemorySize, SF_MOST_KEYS * SF_BYTES);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(k_store_attend_few<8>, cudaFuncAttributeMaxDynamicSharedMemorySize, SF_MOST_KEYS * SF_BYTES);
+    return e;
 }
 
 cudaError_t store_attend(const StoreAttend& a, StoreLaunch how) {
     if (a.rw.n_streams == 0 || a.rw.rows == 0) return cudaSuccess;
-    const dim3 grid(a.rw.max_rows, a.st.H, a.rw.n_streams);
-    return store_launch(how, k_store_attend, grid, SA_WARPS * 32, 0, a);
+    const int wide = aligned16(a.q) && a.ldq % 2 == 0;
+    // blocks of 32 positions that a row may see
+    int blocks = (a.st.lim + 31) / 32;
+    if (a.window > 0 && a.window < a.st.lim) blocks = std::min(blocks, (a.window + 30) / 32 + 1);
+    const int64_t units = (int64_t)a.rw.n_streams * a.rw.max_rows * a.st.H;
+    int cs = 1;
+    while (cs < 8 && ((units * cs < how.sms * 2 && blocks >= cs * 8) || blocks * 32 > cs * SF_MOST_KEYS)) cs *= 2;
+    const int chunk = (blocks + cs - 1) / cs * 32;
+    const dim3 grid(a.rw.max_rows * cs, a.st.H, a.rw.n_streams);
+    const size_t smem = (size_t)chunk * SF_BYTES;
+    switch (cs) {
+        case 1: return store_launch(how, k_store_attend_few<1>, grid, SF_WARPS * 32, smem, 1, a, chunk, wide);
+        case 2: return store_launch(how, k_store_attend_few<2>, grid, SF_WARPS * 32, smem, 2, a, chunk, wide);
+        case 4: return store_launch(how, k_store_attend_few<4>, grid, SF_WARPS * 32, smem, 4, a, chunk, wide);
+        default: return store_launch(how, k_store_attend_few<8>, grid, SF_WARPS * 32, smem, 8, a, chunk, wide);
+    }
 }
 
 }  // namespace b2
@@ -232,7 +425,7 @@ struct b2_store {
     std::string err;
     Store4 st{};
     int32_t *ARR = nullptr, *LOG2 = nullptr, *EXP2 = nullptr;
-    int alen = 0;
+    int alen = 0, sms = 148;
     uint32_t* d_err = nullptr;
     std::vector<void*> allocs;
 };
@@ -282,44 +475,47 @@ int salloc(b2_store* h, T** p, size_t n) {
     return B2_OK;
 }
 
-int upload32(b2_store* h, int32_t** dst, const int64_t* src, int64_t n, int64_t lo, int64_t hi, const char* name) {
-    std::vector<int32_t> t((size_t)n);
+int table32(b2_store* h, std::vector<int32_t>& t, const int64_t* src, int64_t n, int64_t lo, int64_t hi, const char* name) {
     for (int64_t i = 0; i < n; i++) {
         if (src[i] < lo || src[i] > hi)
             return sfail(h, B2_ERR_VALUE, "b2_store_create: %s[%lld] = %lld outside [%lld, %lld]", name, (long long)i,
                          (long long)src[i], (long long)lo, (long long)hi);
-        t[(size_t)i] = (int32_t)src[i];
+        t.push_back((int32_t)src[i]);
     }
-    const int rc = salloc(h, dst, (size_t)n);
-    if (rc) return rc;
-    SCK(cudaMemcpy(*dst, t.data(), sizeof(int32_t) * n, cudaMemcpyHostToDevice));
     return B2_OK;
 }
 
 void store_release(b2_store* h) {
     for (void* p : h->allocs) cudaFree(p);
     h->allocs.clear();
+    h->d_err = nullptr;
 }
 
 int store_build(b2_store* h, const int64_t* arrival, int64_t n_arrival, const int64_t* log2, const int64_t* exp2) {
     const b2_store_config& c = h->cfg;
-    int rc;
+    SCK(store_init());
+    SCK(cudaDeviceGetAttribute(&h->sms, cudaDevAttrMultiProcessorCount, h->device));
     if (arrival[0] < 1) return sfail(h, B2_ERR_VALUE, "b2_store_create: arrival[0] = %lld (at least 1)", (long long)arrival[0]);
-    if ((rc = upload32(h, &h->ARR, arrival, n_arrival, 0, STORE_MAX_ARR, "arrival")) ||
-        (rc = upload32(h, &h->LOG2, log2, 65536, 0, 65536, "log2")) ||
-        (rc = upload32(h, &h->EXP2, exp2, 65536, 65536, 131072, "exp2")))
+    // one piece for the error words and the tables, one for the store
+    std::vector<int32_t> t(4, 0);
+    t.reserve(4 + 2 * 65536 + (size_t)n_arrival);
+    int rc;
+    if ((rc = table32(h, t, log2, 65536, 0, 65536, "log2")) || (rc = table32(h, t, exp2, 65536, 65536, 131072, "exp2")) ||
+        (rc = table32(h, t, arrival, n_arrival, 0, STORE_MAX_ARR, "arrival")))
         return rc;
-    h->alen = (int)n_arrival;
-    if ((rc = store_alloc(h->st, c.n_slots, c.n_layer, c.n_head, c.max_ctx, [&](void** p, size_t n) {
-             uint8_t* q = nullptr;
-             const int r = salloc(h, &q, n);
-             *p = q;
-             return r;
-         })))
-        return rc;
-    if ((rc = salloc(h, &h->d_err, 4))) return rc;
-    SCK(cudaMemset(h->d_err, 0, 4 * sizeof(uint32_t)));
+    int32_t* d = nullptr;
+    uint8_t* mem = nullptr;
+    const size_t bytes = store_layout(h->st, c.n_slots, c.n_layer, c.n_head, c.max_ctx, nullptr);
+    if ((rc = salloc(h, &mem, bytes)) || (rc = salloc(h, &d, t.size()))) return rc;
+    store_layout(h->st, c.n_slots, c.n_layer, c.n_head, c.max_ctx, mem);
+    SCK(cudaMemset(mem, 0, bytes));
+    SCK(cudaMemcpy(d, t.data(), sizeof(int32_t) * t.size(), cudaMemcpyHostToDevice));
     SCK(cudaDeviceSynchronize());
+    h->LOG2 = d + 4;
+    h->EXP2 = h->LOG2 + 65536;
+    h->ARR = h->EXP2 + 65536;
+    h->alen = (int)n_arrival;
+    h->d_err = (uint32_t*)d;
     return B2_OK;
 }
 
@@ -392,7 +588,7 @@ int b2_store_write(b2_store* h, int32_t layer, const int64_t* k, int64_t ldk, co
         OnDevice on(h->device);
         SCK(on.e);
         SCK(store_write(h->st, StoreRows{cu, pos, n_streams, rows, max_rows}, layer, k, ldk, v, ldv, h->d_err,
-                        StoreLaunch{(cudaStream_t)stream, false}));
+                        StoreLaunch{(cudaStream_t)stream, false, h->sms}));
         return (int)B2_OK;
     });
 }
@@ -407,7 +603,7 @@ int b2_store_read(b2_store* h, int32_t layer, const int32_t* cu, const int32_t* 
         OnDevice on(h->device);
         SCK(on.e);
         SCK(store_read(h->st, StoreRows{cu, pos, n_streams, rows, max_rows}, layer, k, v, h->d_err,
-                       StoreLaunch{(cudaStream_t)stream, false}));
+                       StoreLaunch{(cudaStream_t)stream, false, h->sms}));
         return (int)B2_OK;
     });
 }
@@ -426,7 +622,7 @@ int b2_store_attend(b2_store* h, int32_t layer, const int64_t* q, int64_t ldq, c
         SCK(on.e);
         StoreAttend a{h->st, StoreRows{cu, pos, n_streams, rows, max_rows}, layer, q, ldq, first, window, h->ARR, h->alen,
                       h->LOG2, h->EXP2, out, nullptr, h->d_err};
-        SCK(store_attend(a, StoreLaunch{(cudaStream_t)stream, false}));
+        SCK(store_attend(a, StoreLaunch{(cudaStream_t)stream, false, h->sms}));
         return (int)B2_OK;
     });
 }

@@ -55,7 +55,10 @@ struct StoreAttend {
 struct StoreLaunch {
     cudaStream_t stream;
     bool pdl;
+    int sms;           // the device's SM count
 };
+
+cudaError_t store_init();   // once per device (current), before the first launch there
 
 cudaError_t store_write(const Store4& st, const StoreRows& rw, int layer, const int64_t* k, int64_t ldk, const int64_t* v,
                         int64_t ldv, uint32_t* err, StoreLaunch how);
@@ -69,25 +72,18 @@ constexpr int STORE_MAX_CTX = 65536;              // 255 x 128 x 65,536 < 2^31: 
 constexpr int32_t STORE_MAX_ARR = 1 << 24;        // the arrival table's largest entry (the converter's ARR[0])
 constexpr int STORE_W_SHIFT = 1;                  // a weight is the table's entry halved: its top byte stays below 129
 
-// the store's arrays, zeroed (every position stands for zeros until it is written); alloc(void**, bytes) gives a status
-template <class A>
-int store_alloc(Store4& st, int n_slots, int L, int H, int max_ctx, A alloc) {
+// the store's arrays in one piece of memory: its size, and the pointers into it
+inline size_t store_layout(Store4& st, int n_slots, int L, int H, int max_ctx, void* at) {
     st.L = L;
     st.H = H;
     st.lim = max_ctx;
     st.ctx = (max_ctx + 31) / 32 * 32;
-    const size_t n = (size_t)n_slots * L * H * st.ctx;
-    void *k, *ks, *v, *vs;
-    int rc;
-    if ((rc = alloc(&k, n * 32)) || (rc = alloc(&ks, n * 2)) || (rc = alloc(&v, n * 32)) || (rc = alloc(&vs, n))) return rc;
-    st.k = (uint8_t*)k;
-    st.ks = (int8_t*)ks;
-    st.v = (uint8_t*)v;
-    st.vs = (int8_t*)vs;
-    if (cudaMemset(k, 0, n * 32) != cudaSuccess || cudaMemset(ks, 0, n * 2) != cudaSuccess ||
-        cudaMemset(v, 0, n * 32) != cudaSuccess || cudaMemset(vs, 0, n) != cudaSuccess)
-        return 2;   // B2_ERR_CUDA
-    return 0;
+    const size_t n = (size_t)n_slots * L * H * st.ctx;     // a multiple of 32: every array starts on 32 bytes
+    st.k = (uint8_t*)at;
+    st.v = st.k + n * 32;
+    st.ks = (int8_t*)(st.v + n * 32);
+    st.vs = st.ks + n * 2;
+    return n * 67;
 }
 
 #ifdef __CUDACC__

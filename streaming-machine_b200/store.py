@@ -29,9 +29,8 @@ class Store:
     "exp2", as convert.tables() or a converted model holds them)."""
 
     def __init__(self, M: dict, n_streams: int, max_ctx: int, n_head: int, n_layer: int = 1, device: int = 0):
-        self.torch = _torch()
-        self.device = self.torch.device("cuda", device)
-        self.n_streams, self.max_ctx, self.n_head, self.n_layer = n_streams, max_ctx, n_head, n_layer
+        self.h = None
+        self._host(_torch(), "cuda", device, n_streams, max_ctx, n_head, n_layer)
         t = [np.ascontiguousarray(M[k], dtype=np.int64) for k in ("arrival", "log2", "exp2")]
         if t[1].size != 65536 or t[2].size != 65536:
             raise ValueError("the log2 and exp2 tables have 65,536 entries")
@@ -46,60 +45,67 @@ class Store:
             self.close()
             raise B2Error(rc, msg)
 
-    # ---- plumbing ---------------------------------------------------------------------------------------------
-    def _call(self, fn: str, *args):
+    def _host(self, torch, kind: str, device: int, n_streams: int, max_ctx: int, n_head: int, n_layer: int):
+        """The host side's own state (no device work)."""
+        self.torch, self.device = torch, torch.device(kind, device if kind == "cuda" else None)
+        self.n_streams, self.max_ctx, self.n_head, self.n_layer = n_streams, max_ctx, n_head, n_layer
+        self._i64, self._i32 = torch.int64, torch.int32
+        self._row, self._flat, self._unit = (n_head, HEAD), (n_head * HEAD,), (HEAD, 1)
+        self._stream, self._index = torch._C._cuda_getCurrentRawStream if kind == "cuda" else (lambda i: None), device
+        L = lib()
+        self._write, self._read, self._attend = L.b2_store_write, L.b2_store_read, L.b2_store_attend
+
+    # ---- plumbing (a decode step calls these for every layer: the usual case is settled by a few comparisons) ----
+    def _call(self, fn, *args):
         if not self.h:
             raise ValueError("the store is closed")
-        rc = getattr(lib(), fn)(self.h, *args)
+        rc = fn(self.h, *args, self._stream(self._index))
         if rc:
             raise B2Error(rc, lib().b2_store_last_error(self.h).decode())
 
-    def _stream(self):
-        return ctypes.c_void_p(self.torch.cuda.current_stream(self.device).cuda_stream)
-
     def _rows(self, x, name: str):
         """(pointer, row stride) of int64 rows [rows, n_head, 64] or [rows, n_head * 64]; only the rows may be strided."""
-        self._on_device(x, name, self.torch.int64)
+        self._on_device(x, name, self._i64)
+        shape, st = x.shape, x.stride()
         d = self.n_head * HEAD
-        ok = (x.dim() == 2 and x.shape[1] == d and (x.stride(1) == 1)) or \
-            (x.dim() == 3 and x.shape[1:] == (self.n_head, HEAD) and x.stride(2) == 1 and
-             (self.n_head == 1 or x.stride(1) == HEAD))
-        if not ok:
-            raise ValueError(f"{name}: rows of [{self.n_head}, {HEAD}] (or {d}) values, one behind the other, got shape "
-                             f"{tuple(x.shape)}, strides {x.stride()}")
-        if x.shape[0] > 1 and x.stride(0) < d:
-            raise ValueError(f"{name}: the rows overlap (stride {x.stride(0)}, rows of {d})")
-        return x.data_ptr(), max(x.stride(0), d)
+        if shape[1:] == self._row and (st[1:] == self._unit or (self.n_head == 1 and st[2] == 1)) or \
+                shape[1:] == self._flat and st[1] == 1:
+            if st[0] >= d:
+                return x.data_ptr(), st[0]
+            if shape[0] <= 1:                                    # a single row's stride says nothing
+                return x.data_ptr(), d
+        raise ValueError(f"{name}: rows of [{self.n_head}, {HEAD}] (or {d}) values, one behind the other and apart, got shape "
+                         f"{tuple(shape)}, strides {st}")
 
     def _on_device(self, x, name: str, dtype):
-        if not isinstance(x, self.torch.Tensor) or x.device != self.device or x.dtype != dtype:
+        if not isinstance(x, self.torch.Tensor) or x.dtype is not dtype or x.device != self.device:
             what = f"{x.dtype} on {x.device}" if isinstance(x, self.torch.Tensor) else type(x).__name__
             raise ValueError(f"{name}: a {dtype} tensor on {self.device}, got {what}")
 
-    def _i32(self, x, name: str, n: int | None = None):
-        self._on_device(x, name, self.torch.int32)
-        if x.dim() != 1 or not x.is_contiguous() or (n is not None and x.shape[0] != n):
-            raise ValueError(f"{name}: {'n' if n is None else n} int32 values in a row, got shape {tuple(x.shape)}")
+    def _ints(self, x, name: str, n: int):
+        self._on_device(x, name, self._i32)
+        if x.shape != (n,) or (n > 1 and x.stride() != (1,)):
+            raise ValueError(f"{name}: {n} int32 values in a row, got shape {tuple(x.shape)}, strides {x.stride()}")
         return x.data_ptr()
 
     def _table(self, pos, cu, rows: int, max_rows):
         """The row table's arguments: cu, pos, n_streams, rows, max_rows."""
-        p = self._i32(pos, "pos")
-        n = pos.shape[0]
+        n = len(pos) if isinstance(pos, self.torch.Tensor) and pos.dim() == 1 else -1
+        p = self._ints(pos, "pos", n)
         if cu is None:
             if rows != n or max_rows not in (None, 1):
                 raise ValueError(f"without cu every stream gives one row: {rows} rows, {n} positions, max_rows {max_rows}")
             return None, p, n, rows, 1
         if max_rows is None:
             raise ValueError("max_rows (the most rows a stream gives) goes with cu")
-        return self._i32(cu, "cu", n + 1), p, n, rows, max_rows
+        return self._ints(cu, "cu", n + 1), p, n, rows, max_rows
 
     def _out(self, out, rows: int, name: str):
-        shape = (rows, self.n_head, HEAD)
+        shape = (rows, *self._row)
         if out is None:
-            return self.torch.empty(shape, dtype=self.torch.int64, device=self.device)
-        self._on_device(out, name, self.torch.int64)
-        if tuple(out.shape) != shape or not out.is_contiguous():
+            return self.torch.empty(shape, dtype=self._i64, device=self.device)
+        self._on_device(out, name, self._i64)
+        if out.shape != shape or not out.is_contiguous():
             raise ValueError(f"{name}: a contiguous {shape}, got shape {tuple(out.shape)}, strides {out.stride()}")
         return out
 
@@ -110,7 +116,7 @@ class Store:
         (pk, ldk), (pv, ldv) = self._rows(k, "k"), self._rows(v, "v")
         if k.shape[0] != v.shape[0]:
             raise ValueError(f"{k.shape[0]} rows of keys, {v.shape[0]} of values")
-        self._call("b2_store_write", layer, pk, ldk, pv, ldv, *self._table(pos, cu, k.shape[0], max_rows), self._stream())
+        self._call(self._write, layer, pk, ldk, pv, ldv, *self._table(pos, cu, k.shape[0], max_rows))
 
     def read(self, pos, cu=None, max_rows: int | None = None, rows: int | None = None, layer: int = 0, out=None):
         """(k, v), int64 [rows, n_head, 64]: the values that the store holds at the rows' positions. rows: how many there
@@ -119,9 +125,9 @@ class Store:
         if rows is None:
             if cu is not None:
                 raise ValueError("rows (cu's last entry) goes with cu")
-            rows = pos.shape[0]
+            rows = len(pos)
         k, v = (self._out(o, rows, n) for o, n in zip(out if out is not None else (None, None), ("out k", "out v")))
-        self._call("b2_store_read", layer, *self._table(pos, cu, rows, max_rows), k.data_ptr(), v.data_ptr(), self._stream())
+        self._call(self._read, layer, *self._table(pos, cu, rows, max_rows), k.data_ptr(), v.data_ptr())
         return k, v
 
     def attend(self, q, pos, cu=None, max_rows: int | None = None, window: int = 0, first=None, layer: int = 0, out=None):
@@ -131,14 +137,18 @@ class Store:
         pq, ldq = self._rows(q, "q")
         out = self._out(out, q.shape[0], "out")
         cu, p, n, rows, most = self._table(pos, cu, q.shape[0], max_rows)
-        f = self._i32(first, "first", n) if first is not None else None
-        self._call("b2_store_attend", layer, pq, ldq, cu, p, f, n, rows, most, window, out.data_ptr(), self._stream())
+        f = self._ints(first, "first", n) if first is not None else None
+        self._call(self._attend, layer, pq, ldq, cu, p, f, n, rows, most, window, out.data_ptr())
         return out
 
     def sync(self):
         """Wait for the device and raise what its checks flagged (rows that do not fit the call, a position past the
         context): the streams concerned were skipped."""
-        self._call("b2_store_sync")
+        if not self.h:
+            raise ValueError("the store is closed")
+        rc = lib().b2_store_sync(self.h)
+        if rc:
+            raise B2Error(rc, lib().b2_store_last_error(self.h).decode())
 
     def close(self):
         if getattr(self, "h", None):

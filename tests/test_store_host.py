@@ -40,7 +40,8 @@ def _bare(n_head=3):
     """A Store whose checks run without a GPU: the host logic alone (nothing is launched by a call that is refused)."""
     from streaming_machine_b200 import store
     st = object.__new__(store.Store)
-    st.torch, st.device, st.n_head, st.n_streams, st.max_ctx, st.n_layer, st.h = torch, torch.device("cpu"), n_head, 4, 64, 1, None
+    st.h = None
+    st._host(torch, "cpu", 0, 4, 64, n_head, 1)
     return st
 
 
@@ -75,8 +76,10 @@ def test_tables_are_refused():
         st._out(torch.zeros(4, 3, 128, dtype=torch.int64)[..., :64], 4, "out")
     with pytest.raises(ValueError):
         st.read(pos, cu=cu, max_rows=3)                       # rows goes with cu
-    with pytest.raises(ValueError):
-        st.attend(torch.zeros(4, 3, 64, dtype=torch.int64), pos)   # a closed store
+    x = torch.zeros(4, 3, 64, dtype=torch.int64)
+    for call in (lambda: st.attend(x, pos), lambda: st.write(x, x, pos), lambda: st.read(pos), st.sync):
+        with pytest.raises(ValueError, match="closed"):
+            call()
 
 
 def test_create_refuses_before_it_touches_a_device():
