@@ -197,8 +197,8 @@ typedef struct {
     int32_t max_ctx;    /* positions of a stream, 1 .. 65536 */
 } b2_store_config;
 
-/* A store on `device`, every position standing for zeros. arrival [n_arrival] (entries in [0, 2^24], the first at least
- * 1), log2 and exp2 [65536]: the machine's tables (base2_convert.py:50-59), HOST pointers. After an error *out, where it
+/* A store on `device`, every position standing for zeros. arrival [n_arrival] (1 .. 32768 entries in [0, 2^24], the first
+ * at least 1), log2 and exp2 [65536]: the machine's tables (base2_convert.py:50-59), HOST pointers. After an error *out, where it
  * is not NULL, holds the message (b2_store_last_error) and is to be destroyed. */
 int b2_store_create(const b2_store_config* cfg, int device, const int64_t* arrival, int64_t n_arrival, const int64_t* log2,
                     const int64_t* exp2, b2_store** out);

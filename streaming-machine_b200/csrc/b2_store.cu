@@ -339,6 +339,390 @@ __global__ void __launch_bounds__(SF_WARPS * 32) k_store_attend_few(StoreAttend 
     if (CS > 1) cluster_sync();                                      // rank 0 has read the others' sums
 }
 
+// ---------------------------------------------------------------------------------------------------------------------
+// the arrival of many rows a stream (a prompt pass): a CTA of 8 warps takes 16 QG consecutive rows of one head, 16 to a
+// warp, and 8 / QG warps share a group's keys. Tiles of 128 keys (and values) are brought into shared memory once for all
+// the CTA's rows, as signed bytes in the order of the tensor cores' B operands (c 2^(s - S + 3) for keys, 16 c for values).
+//   pass 1  every score (m16n8k32, the query's two bytes one after the other), the rows' largest and largest value shift
+//   pass 2  the scores again (cheaper than keeping 4 bytes a pair), a = ARR[start - score] from a copy of the table in
+//           shared memory (a gather from L1 takes a line a lane), the weight's three bytes as the A operands of
+//           num += w c: a lane's score of tile t lies where its A operand wants it when k is taken in the order below
+// CTAs are persistent so that the table is copied once an SM, the longest rows first.
+// ---------------------------------------------------------------------------------------------------------------------
+constexpr int SM_TILE = 128;
+constexpr int SM_THREADS = 256;
+struct SmTile {
+    uint4 k[SM_TILE / 8][32];            // [8 keys][lane (g, j)]: key g, dims of word j of both halves, even and odd
+    uint4 v[SM_TILE / 32][2][2][32];     // [32 keys][b0, b1][tiles 0-3, 4-7][lane]
+    int32_t kr[SM_TILE];                 // 27 - S: a score's shift less one is kr - u
+    int32_t vs[SM_TILE];
+};
+
+// bytes c 2^up of the word's even (or, shifted down, odd) codes; up = 0 .. 3: c + 8 moves up, 8 2^up comes off again
+B2_DEV uint32_t codes_up(uint32_t w, int up, uint32_t less) {
+    return ((((w & 0x0F0F0F0Fu) ^ 0x08080808u) << up) + less) ^ 0x80808080u;
+}
+B2_DEV uint32_t shr_u32(uint32_t x, uint32_t s) {     // 0 for s > 31
+    uint32_t r;
+    asm("shr.u32 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(s));
+    return r;
+}
+
+template <int QG>
+struct SmShared {
+    SmTile tile[2];
+    uint32_t q[16 * QG][33];
+    int32_t u[16 * QG], y[16 * QG], m[16 * QG];
+    unsigned long long z[16 * QG];
+    int32_t umax, slow;
+};
+
+template <int QG>
+__global__ void __launch_bounds__(SM_THREADS, 1) k_store_attend_many(StoreAttend a, int tiles, int wide) {
+    griddep_wait();
+    griddep_launch();
+    extern __shared__ __align__(16) uint8_t sm[];
+    SmShared<QG>& S = *reinterpret_cast<SmShared<QG>*>(sm);
+    int32_t* const TAB = reinterpret_cast<int32_t*>(sm + sizeof(SmShared<QG>));   // [alen + 1], 0 at the end
+    constexpr int KS = 8 / QG, ROWS = 16 * QG, BLOCKS = SM_TILE / 32;
+    const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, g = lane >> 2, j = lane & 3;
+    const int qg = wid % QG, kg = wid / QG;
+    const int H = a.st.H, alen = a.alen;
+    for (int i = tid; i < alen; i += SM_THREADS) TAB[i] = __ldg(a.ARR + i);
+    if (tid == 0) TAB[alen] = 0;
+    const int64_t items = (int64_t)tiles * H * a.rw.n_streams;
+    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+        const int s = (int)(item % a.rw.n_streams);
+        const int h = (int)(item / a.rw.n_streams % H), tile = tiles - 1 - (int)(item / a.rw.n_streams / H);
+        StoreRun run;
+        if (!store_run(a.rw, s, a.st.lim, run, a.err) || tile * ROWS >= run.n) continue;
+        const int i0 = tile * ROWS, nr = min(ROWS, run.n - i0);
+        const int from = a.first ? max(0, a.first[s]) : 0, win = a.window > 0 ? a.window : 0x40000000;
+        const int p_first = run.p0 + i0, p_last = p_first + nr - 1;
+        const int k_lo = max(from, p_first - win + 1);       // the first row sees the earliest position
+        __syncthreads();                                      // the item before is done with shared memory
+        if (k_lo > p_last) {                                  // nothing to see for any row
+            for (int t = tid; t < nr * 64; t += SM_THREADS)
+                a.out[((size_t)(run.r0 + i0 + (t >> 6)) * H + h) * 64 + (t & 63)] = 0;
+            continue;
+        }
+        if (tid == 0) {
+            S.umax = 0;
+            S.slow = 0;
+        }
+        for (int r = tid; r < ROWS; r += SM_THREADS) {
+            S.y[r] = INT32_MIN;
+            S.m[r] = 0;
+            S.z[r] = 0;
+        }
+        __syncthreads();
+        for (int r = wid; r < ROWS; r += 8) {
+            uint32_t word = 0;
+            int u = 0;
+            if (r < nr) u = query_bytes(a.q + (size_t)(run.r0 + i0 + r) * a.ldq + h * 64, wide, lane, word);
+            S.q[r][lane] = word;
+            if (lane == 0) {
+                S.u[r] = u;
+                atomicMax(&S.umax, u);
+            }
+        }
+        __syncthreads();
+        // this lane's rows and their A operands: [plane][half][even row g, even g + 8, odd g, odd g + 8]
+        const int ra = qg * 16 + g, rb = ra + 8;
+        uint32_t q[2][2][4];
+#pragma unroll
+        for (int x = 0; x < 2; x++)
+#pragma unroll
+            for (int y = 0; y < 2; y++) {
+                const uint32_t* w = &S.q[y ? rb : ra][16 * x + 4 * j];
+                const uint32_t t0 = __byte_perm(w[0], w[1], 0x6240), t1 = __byte_perm(w[2], w[3], 0x6240);   // hi: even, even, odd, odd
+                const uint32_t l0 = __byte_perm(w[0], w[1], 0x7351), l1 = __byte_perm(w[2], w[3], 0x7351);   // lo
+                q[0][x][y] = __byte_perm(t0, t1, 0x5410);
+                q[0][x][2 + y] = __byte_perm(t0, t1, 0x7632);
+                q[1][x][y] = __byte_perm(l0, l1, 0x5410);
+                q[1][x][2 + y] = __byte_perm(l0, l1, 0x7632);
+            }
+        const int ua = S.u[ra], ub = S.u[rb], umax = S.umax;
+        const int pa = min(p_first + ra, p_last), pb = min(p_first + rb, p_last);      // rows past the last repeat it
+        const int la = max(from, pa - win + 1), lb = max(from, pb - win + 1);
+        const int w_p0 = min(p_first + qg * 16, p_last), w_p1 = min(p_first + qg * 16 + 15, p_last);
+        const int w_l0 = max(from, w_p0 - win + 1), w_l1 = max(from, w_p1 - win + 1);
+        const int k0 = k_lo & ~31, k1 = (p_last | 31) + 1, nt = (k1 - k0 + SM_TILE - 1) / SM_TILE;
+        const size_t base = kv_index(s, a.layer, h, 0, a.st.L, H, a.st.ctx);
+
+        // ---- a tile on its way: from global memory into registers, then unpacked into shared memory
+        uint2 kw[2];
+        uint32_t vw[4], kss[2];
+        int vsr = 0;
+        auto fetch = [&](int t, bool values) {
+            const int kt = k0 + t * SM_TILE;
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+                const int key = kt + (wid * 2 + x) * 8 + g;
+                if (key < k1) {
+                    kw[x] = *reinterpret_cast<const uint2*>(a.st.k + (base + key) * 32 + 8 * j);
+                    kss[x] = *reinterpret_cast<const uint16_t*>(a.st.ks + (base + key) * 2);
+                }
+            }
+            const int key = kt + tid;
+            if (tid < SM_TILE && key < k1) vsr = a.st.vs[base + key];
+            if (values) {
+                const int vk = kt + (wid >> 1) * 32 + (wid & 1) * 16 + 2 * j;      // keys vk, vk + 1, vk + 8, vk + 9
+                if (vk < k1) {
+#pragma unroll
+                    for (int x = 0; x < 4; x++)
+                        vw[x] = *reinterpret_cast<const uint32_t*>(a.st.v + (base + vk + (x & 1) + 4 * (x & 2)) * 32 + 4 * g);
+                }
+            }
+        };
+        auto put = [&](int t, bool values) {
+            const int kt = k0 + t * SM_TILE;
+            SmTile& T = S.tile[t & 1];
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+                const int kl = (wid * 2 + x) * 8 + g;
+                if (kt + kl < k1) {
+                    const int s0 = (int8_t)(kss[x] & 255), s1 = (int8_t)(kss[x] >> 8), big = max(s0, s1);
+                    const int up0 = s0 - big + 3, up1 = s1 - big + 3;
+                    const uint32_t less0 = 0x80808080u - (0x08080808u << up0), less1 = 0x80808080u - (0x08080808u << up1);
+                    T.k[wid * 2 + x][lane] = make_uint4(codes_up(kw[x].x, up0, less0), codes_up(kw[x].x >> 4, up0, less0),
+                                                        codes_up(kw[x].y, up1, less1), codes_up(kw[x].y >> 4, up1, less1));
+                    if (j == 0) {
+                        T.kr[kl] = 27 - big;
+                        if (27 - big < umax) S.slow = 1;
+                    }
+                }
+            }
+            if (tid < SM_TILE) T.vs[tid] = vsr;
+            if (values && kt + (wid >> 1) * 32 < k1) {
+                uint32_t r[4];
+                turn4(vw, r);
+                uint4* const to = &T.v[wid >> 1][wid & 1][0][lane];
+                to[0] = make_uint4(even16(r[0]), odd16(r[0]), even16(r[1]), odd16(r[1]));
+                to[32] = make_uint4(even16(r[2]), odd16(r[2]), even16(r[3]), odd16(r[3]));
+            }
+        };
+        // twice the rounded score (fast: its digit below the last one kept; slow: shifts up, and the limits) of tile n of
+        // eight keys: rows ra and rb, keys 2j and 2j + 1
+        auto scores = [&](const SmTile& T, int n, bool slow, int (&y)[4]) {
+            const uint4 b = T.k[n][lane];
+            int d[4] = {};
+            mma_s8(d, q[0][0][0], q[0][0][1], q[0][0][2], q[0][0][3], b.x, b.y);
+            mma_s8(d, q[0][1][0], q[0][1][1], q[0][1][2], q[0][1][3], b.z, b.w);
+#pragma unroll
+            for (int x = 0; x < 4; x++) d[x] = (int)((uint32_t)d[x] << 8);
+            mma_s8(d, q[1][0][0], q[1][0][1], q[1][0][2], q[1][0][3], b.x, b.y);
+            mma_s8(d, q[1][1][0], q[1][1][1], q[1][1][2], q[1][1][3], b.z, b.w);
+            const int2 kr = *reinterpret_cast<const int2*>(&T.kr[n * 8 + 2 * j]);
+            if (!slow) {
+                y[0] = d[0] >> (kr.x - ua);
+                y[1] = d[1] >> (kr.y - ua);
+                y[2] = d[2] >> (kr.x - ub);
+                y[3] = d[3] >> (kr.y - ub);
+            } else {
+                y[0] = 2 * store_score(d[0], kr.x - ua + 1);
+                y[1] = 2 * store_score(d[1], kr.y - ua + 1);
+                y[2] = 2 * store_score(d[2], kr.x - ub + 1);
+                y[3] = 2 * store_score(d[3], kr.y - ub + 1);
+            }
+        };
+
+        // ---- pass 1
+        int ya = INT32_MIN, yb = INT32_MIN, ma = 0, mb = 0;
+        fetch(0, false);
+        put(0, false);
+        __syncthreads();
+        for (int t = 0; t < nt; t++) {
+            if (t + 1 < nt) fetch(t + 1, false);
+            const SmTile& T = S.tile[t & 1];
+            const bool slow = S.slow;
+#pragma unroll 1
+            for (int b = kg; b < BLOCKS; b += KS) {
+                const int kb = k0 + t * SM_TILE + b * 32;
+                if (kb > w_p1 || kb + 31 < w_l0) continue;
+                const bool whole = kb + 31 <= w_p0 && kb >= w_l1;
+#pragma unroll
+                for (int n = 0; n < 4; n++) {
+                    int y[4];
+                    scores(T, b * 4 + n, slow, y);
+                    const int2 vs = *reinterpret_cast<const int2*>(&T.vs[b * 32 + n * 8 + 2 * j]);
+                    if (whole) {
+                        ya = max(ya, max(y[0], y[1]));
+                        yb = max(yb, max(y[2], y[3]));
+                        ma = max(ma, max(vs.x, vs.y));
+                        mb = max(mb, max(vs.x, vs.y));
+                    } else {
+                        const int key = kb + n * 8 + 2 * j;
+                        if (key >= la && key <= pa) { ya = max(ya, y[0]); ma = max(ma, vs.x); }
+                        if (key + 1 >= la && key + 1 <= pa) { ya = max(ya, y[1]); ma = max(ma, vs.y); }
+                        if (key >= lb && key <= pb) { yb = max(yb, y[2]); mb = max(mb, vs.x); }
+                        if (key + 1 >= lb && key + 1 <= pb) { yb = max(yb, y[3]); mb = max(mb, vs.y); }
+                    }
+                }
+            }
+            if (t + 1 < nt) {
+                put(t + 1, false);
+                __syncthreads();
+            }
+        }
+#pragma unroll
+        for (int o = 1; o < 4; o <<= 1) {
+            ya = max(ya, __shfl_xor_sync(0xffffffffu, ya, o));
+            yb = max(yb, __shfl_xor_sync(0xffffffffu, yb, o));
+            ma = max(ma, __shfl_xor_sync(0xffffffffu, ma, o));
+            mb = max(mb, __shfl_xor_sync(0xffffffffu, mb, o));
+        }
+        if (j == 0) {
+            atomicMax(&S.y[ra], ya);
+            atomicMax(&S.y[rb], yb);
+            atomicMax(&S.m[ra], ma);
+            atomicMax(&S.m[rb], mb);
+        }
+        fetch(0, true);
+        __syncthreads();
+        put(0, true);
+        // twice the largest score: a digit below the last rounds up with it
+        const uint32_t sa = (uint32_t)(((S.y[ra] >> 1) + (S.y[ra] & 1)) * 2), sb = (uint32_t)(((S.y[rb] >> 1) + (S.y[rb] & 1)) * 2);
+        ma = S.m[ra];
+        mb = S.m[rb];
+        __syncthreads();
+
+        // ---- pass 2
+        int acc[3][8][4];
+#pragma unroll
+        for (int x = 0; x < 3; x++)
+#pragma unroll
+            for (int t = 0; t < 8; t++)
+#pragma unroll
+                for (int c = 0; c < 4; c++) acc[x][t][c] = 0;
+        int64_t za = 0, zb = 0;
+        for (int t = 0; t < nt; t++) {
+            if (t + 1 < nt) fetch(t + 1, true);
+            const SmTile& T = S.tile[t & 1];
+            const bool slow = S.slow;
+#pragma unroll 1
+            for (int b = kg; b < BLOCKS; b += KS) {
+                const int kb = k0 + t * SM_TILE + b * 32;
+                if (kb > w_p1 || kb + 31 < w_l0) continue;
+                const bool whole = kb + 31 <= w_p0 && kb >= w_l1;
+                uint32_t p[3][4];                 // the weights' planes as A operands
+                int32_t s_a = 0, s_b = 0;         // 8 entries of at most 2^24
+#pragma unroll
+                for (int n = 0; n < 4; n += 2) {
+                    uint32_t wa[4], wb[4];
+#pragma unroll
+                    for (int x = 0; x < 2; x++) {
+                        int y[4];
+                        scores(T, b * 4 + n + x, slow, y);
+                        const int2 vs = *reinterpret_cast<const int2*>(&T.vs[b * 32 + (n + x) * 8 + 2 * j]);
+                        // start - score, from twice both: (start2 - y) / 2 rounded down
+                        uint32_t d[4] = {(sa - (uint32_t)y[0]) >> 1, (sa - (uint32_t)y[1]) >> 1, (sb - (uint32_t)y[2]) >> 1,
+                                         (sb - (uint32_t)y[3]) >> 1};
+#pragma unroll
+                        for (int c = 0; c < 4; c++) d[c] = min(d[c], (uint32_t)alen);
+                        if (!whole) {
+                            const int key = kb + (n + x) * 8 + 2 * j;
+                            if (!(key >= la && key <= pa)) d[0] = alen;
+                            if (!(key + 1 >= la && key + 1 <= pa)) d[1] = alen;
+                            if (!(key >= lb && key <= pb)) d[2] = alen;
+                            if (!(key + 1 >= lb && key + 1 <= pb)) d[3] = alen;
+                        }
+                        const int v[4] = {TAB[d[0]], TAB[d[1]], TAB[d[2]], TAB[d[3]]};
+                        s_a += v[0] + v[1];
+                        s_b += v[2] + v[3];
+                        // rnd(a, 1 + M - vs); a key that a row does not see (whose vs may pass M) has a = 0
+                        wa[2 * x] = (shr_u32(v[0], ma - vs.x) + 1) >> 1;
+                        wa[2 * x + 1] = (shr_u32(v[1], ma - vs.y) + 1) >> 1;
+                        wb[2 * x] = (shr_u32(v[2], mb - vs.x) + 1) >> 1;
+                        wb[2 * x + 1] = (shr_u32(v[3], mb - vs.y) + 1) >> 1;
+                    }
+                    uint32_t r[4];
+                    turn4(wa, r);
+                    p[0][n] = r[0];
+                    p[1][n] = r[1];
+                    p[2][n] = r[2];
+                    turn4(wb, r);
+                    p[0][n + 1] = r[0];
+                    p[1][n + 1] = r[1];
+                    p[2][n + 1] = r[2];
+                }
+                za += s_a;
+                zb += s_b;
+#pragma unroll
+                for (int x = 0; x < 2; x++) {
+                    const uint4 b0 = T.v[b][0][x][lane], b1 = T.v[b][1][x][lane];
+                    const uint32_t c0[4] = {b0.x, b0.y, b0.z, b0.w}, c1[4] = {b1.x, b1.y, b1.z, b1.w};
+#pragma unroll
+                    for (int y = 0; y < 4; y++)
+#pragma unroll
+                        for (int z = 0; z < 3; z++)
+                            mma_u8s8(acc[z][4 * x + y], p[z][0], p[z][1], p[z][2], p[z][3], c0[y], c1[y]);
+                }
+            }
+            if (t + 1 < nt) {
+                put(t + 1, true);
+                __syncthreads();
+            }
+        }
+        atomicAdd(&S.z[ra], (unsigned long long)za);
+        atomicAdd(&S.z[rb], (unsigned long long)zb);
+        // the sums of a group's warps: the later ones' into shared memory (in place of the tiles), added by the first
+        int64_t* const part = reinterpret_cast<int64_t*>(S.tile);     // [QG][16 rows][64], a warp's 8 KB in lane order
+        for (int k = 1; k < KS; k++) {
+            __syncthreads();
+            if (kg == k) {
+#pragma unroll
+                for (int t = 0; t < 8; t++)
+#pragma unroll
+                    for (int c = 0; c < 4; c++)
+                        part[(qg * 32 + t * 4 + c) * 32 + lane] =
+                            (int64_t)acc[0][t][c] + ((int64_t)acc[1][t][c] << 8) + ((int64_t)acc[2][t][c] << 16);
+            }
+            __syncthreads();
+            if (kg == 0) {
+#pragma unroll
+                for (int t = 0; t < 8; t++)
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        // back into the planes: the low byte's plane takes what is left of the sum
+                        const int64_t o = part[(qg * 32 + t * 4 + c) * 32 + lane] + acc[0][t][c];
+                        acc[0][t][c] = (int)(o & 0xFFFF);
+                        acc[2][t][c] += (int)(o >> 16);
+                    }
+            }
+        }
+        __syncthreads();
+        if (kg == 0) {
+#pragma unroll
+            for (int y = 0; y < 2; y++) {
+                const int r = y ? rb : ra;
+                const int64_t z = (int64_t)S.z[r];
+                const bool none = (y ? lb > pb : la > pa) || z == 0;
+                const int64_t F = 65536ll * ((y ? mb : ma) + STORE_W_SHIFT) - log2fix(none ? 1 : z, a.LOG2);
+                const int64_t e = __ldg(a.EXP2 + (F & 0xFFFF));
+                const int64_t sh = 16 - (F >> 16);
+                uint64_t any = 0;
+                int64_t* const out = a.out + ((size_t)(run.r0 + i0 + min(r, nr - 1)) * H + h) * 64;
+#pragma unroll
+                for (int c = 0; c < 2; c++)           // columns 2j + c: dims 8 (2j + c) + t
+#pragma unroll
+                    for (int t = 0; t < 8; t++) {
+                        const int x = 2 * y + c;
+                        const int64_t num = ((int64_t)acc[0][t][x] + ((int64_t)acc[1][t][x] << 8) + ((int64_t)acc[2][t][x] << 16)) >> 4;
+                        const int64_t o = none ? 0 : rshift(wmul(num, e), sh);
+                        any |= mag(o);
+                        if (r < nr) out[16 * j + 8 * c + t] = o;
+                    }
+                if (a.or_out) {
+                    any |= __shfl_xor_sync(0xffffffffu, any, 1);
+                    any |= __shfl_xor_sync(0xffffffffu, any, 2);
+                    if (j == 0 && r < nr) atomicOr((unsigned long long*)&a.or_out[run.r0 + i0 + r], (unsigned long long)any);
+                }
+            }
+        }
+    }
+}
+
 // ---- launches -------------------------------------------------------------------------------------------------------
 namespace {
 template <typename... KArgs, typename... Args>
@@ -382,6 +766,8 @@ cudaError_t store_read(const Store4& st, const StoreRows& rw, int layer, int64_t
     return store_launch(how, k_store_read, grid, SW_WARPS * 32, 0, 1, st, rw, layer, k, v, wide, err);
 }
 
+constexpr int SM_FROM_ROWS = 4;
+constexpr int SM_SMEM_MOST = 200 * 1024;
 constexpr int SF_MOST_KEYS = 8192;   // of a CTA: 64 KB of shared memory
 
 cudaError_t store_init() {
@@ -389,12 +775,28 @@ cudaError_t store_init() {
     if (e == cudaSuccess) e = cudaFuncSetAttribute(k_store_attend_few<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, SF_MOST_KEYS * SF_BYTES);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(k_store_attend_few<4>, cudaFuncAttributeMaxDynamicSharedMemorySize, SF_MOST_KEYS * SF_BYTES);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(k_store_attend_few<8>, cudaFuncAttributeMaxDynamicSharedMemorySize, SF_MOST_KEYS * SF_BYTES);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(k_store_attend_many<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, SM_SMEM_MOST);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(k_store_attend_many<4>, cudaFuncAttributeMaxDynamicSharedMemorySize, SM_SMEM_MOST);
     return e;
 }
+
+namespace {
+template <int QG>
+cudaError_t attend_many(const StoreAttend& a, StoreLaunch how, int wide) {
+    const int tiles = (a.rw.max_rows + 16 * QG - 1) / (16 * QG);
+    const int64_t items = (int64_t)tiles * a.st.H * a.rw.n_streams;
+    const size_t smem = sizeof(SmShared<QG>) + (size_t)(a.alen + 1) * 4;
+    return store_launch(how, k_store_attend_many<QG>, dim3((unsigned)std::min<int64_t>(items, how.sms)), SM_THREADS, smem, 1, a,
+                        tiles, wide);
+}
+}  // namespace
 
 cudaError_t store_attend(const StoreAttend& a, StoreLaunch how) {
     if (a.rw.n_streams == 0 || a.rw.rows == 0) return cudaSuccess;
     const int wide = aligned16(a.q) && a.ldq % 2 == 0;
+    if (a.rw.max_rows > SM_FROM_ROWS)
+        return (int64_t)((a.rw.max_rows + 63) / 64) * a.st.H * a.rw.n_streams >= how.sms ? attend_many<4>(a, how, wide)
+                                                                                          : attend_many<2>(a, how, wide);
     // blocks of 32 positions that a row may see
     int blocks = (a.st.lim + 31) / 32;
     if (a.window > 0 && a.window < a.st.lim) blocks = std::min(blocks, (a.window + 30) / 32 + 1);
@@ -557,7 +959,7 @@ int b2_store_create(const b2_store_config* cfg, int device, const int64_t* arriv
                     const int64_t* exp2, b2_store** out) {
     if (!out) return B2_ERR_ARG;
     *out = nullptr;
-    if (!cfg || !arrival || !log2 || !exp2 || n_arrival < 1 || n_arrival > (1 << 20)) return B2_ERR_ARG;
+    if (!cfg || !arrival || !log2 || !exp2 || n_arrival < 1 || n_arrival > STORE_MAX_ALEN) return B2_ERR_ARG;
     if (cfg->n_slots < 1 || cfg->n_slots > 65535 || cfg->n_layer < 1 || cfg->n_layer > 1024 || cfg->n_head < 1 ||
         cfg->n_head > 1024 || cfg->max_ctx < 1 || cfg->max_ctx > STORE_MAX_CTX)
         return B2_ERR_ARG;

@@ -70,6 +70,7 @@ constexpr int32_t STORE_LIM = (1 << 30) - 1;      // scores are held between -ST
 constexpr int STORE_MAX_SHIFT = 44;               // 2^47 in 4 bits
 constexpr int STORE_MAX_CTX = 65536;              // 255 x 128 x 65,536 < 2^31: the tensor cores' sums stay in 32 bits
 constexpr int32_t STORE_MAX_ARR = 1 << 24;        // the arrival table's largest entry (the converter's ARR[0])
+constexpr int STORE_MAX_ALEN = 32768;             // its entries: a copy has to fit shared memory (the converter's has 17,745)
 constexpr int STORE_W_SHIFT = 1;                  // a weight is the table's entry halved: its top byte stays below 129
 
 // the store's arrays in one piece of memory: its size, and the pointers into it

@@ -94,7 +94,7 @@ def test_create_refuses_before_it_touches_a_device():
     for cfg in ((0, 1, 1, 1), (65536, 1, 1, 1), (1, 0, 1, 1), (1, 1025, 1, 1), (1, 1, 0, 1), (1, 1, 1025, 1), (1, 1, 1, 0),
                 (1, 1, 1, 65537), (-1, 1, 1, 1)):
         assert create(cfg) == 1 and not h.value
-    for kw in (dict(arr=None), dict(log2=None), dict(exp2=None), dict(n=0), dict(n=-5), dict(n=(1 << 20) + 1)):
+    for kw in (dict(arr=None), dict(log2=None), dict(exp2=None), dict(n=0), dict(n=-5), dict(n=32769)):
         assert create((1, 1, 1, 1), **kw) == 1 and not h.value
     for f, args in (("b2_store_write", (0, None, 0, None, 0, None, None, 0, 0, 0, None)),
                     ("b2_store_read", (0, None, None, 0, 0, 0, None, None, None)),
