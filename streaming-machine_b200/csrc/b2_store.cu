@@ -8,6 +8,7 @@
 #include <exception>
 #include <new>
 #include <string>
+#include <type_traits>
 #include <vector>
 
 #include "../../include/base2.h"
@@ -119,6 +120,11 @@ B2_DEV void mma_u8s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_
         : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+B2_DEV void mma_s8_first(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+        : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(0));
+}
 // eight 4-bit codes of a word as signed bytes 16 c: the even dims' and the odd dims'
 B2_DEV uint32_t even16(uint32_t w) { return (w << 4) & 0xF0F0F0F0u; }
 B2_DEV uint32_t odd16(uint32_t w) { return w & 0xF0F0F0F0u; }
@@ -136,6 +142,14 @@ B2_DEV void turn4(const uint32_t* w, uint32_t (&r)[4]) {
     r[3] = __byte_perm(t2, t3, 0x7632);
 }
 
+// four weights below 2^24 -> their bytes by place, those of the four weights in a word
+B2_DEV void turn3(const uint32_t* w, uint32_t& b0, uint32_t& b1, uint32_t& b2) {
+    const uint32_t t0 = __byte_perm(w[0], w[1], 0x5140), t1 = __byte_perm(w[2], w[3], 0x5140);
+    b0 = __byte_perm(t0, t1, 0x5410);
+    b1 = __byte_perm(t0, t1, 0x7632);
+    b2 = __byte_perm(__byte_perm(w[0], w[1], 0x0062), __byte_perm(w[2], w[3], 0x0062), 0x5410);
+}
+
 // a row's 64 query values at 15 bits, as two signed bytes q15 = 256 hi + lo, in a lane's pair (dims 2 lane, 2 lane + 1):
 // bytes hi, lo of the first, hi, lo of the second. Returns the row's shift u. Every lane of the warp takes part.
 B2_DEV int query_bytes(const int64_t* q, bool wide, int lane, uint32_t& word) {
@@ -143,11 +157,11 @@ B2_DEV int query_bytes(const int64_t* q, bool wide, int lane, uint32_t& word) {
     load_pair(q + 2 * lane, wide, x0, x1);
     x0 = store_clamp(x0);
     x1 = store_clamp(x1);
-    const uint64_t m0 = mag(x0), m1 = mag(x1);
-    const int u = max((int)__reduce_max_sync(0xffffffffu, (uint32_t)bitlen_u(m0 > m1 ? m0 : m1)) - 14, 0);
+    // the largest magnitude's bit length is that of the magnitudes' OR
+    const int u = max((int)__reduce_max_sync(0xffffffffu, (uint32_t)bitlen_u(mag(x0) | mag(x1))) - 14, 0);
     const int a = (int)rnd64(x0, u), b = (int)rnd64(x1, u);
-    word = (uint32_t)(((a + 128) >> 8) & 255) | (uint32_t)(a & 255) << 8 | (uint32_t)(((b + 128) >> 8) & 255) << 16 |
-           (uint32_t)(b & 255) << 24;
+    // byte 0: a + 128 >> 8, byte 1: a, byte 2: b + 128 >> 8, byte 3: b
+    word = __byte_perm(__byte_perm(a + 128, a, 0x41), __byte_perm(b + 128, b, 0x41), 0x5410);
     return u;
 }
 
@@ -186,7 +200,7 @@ __global__ void __launch_bounds__(SF_WARPS * 32) k_store_attend_few(StoreAttend 
     const int from = lo - b0 * 32, to = p - b0 * 32;                 // visible: from <= local key <= to
 
     uint32_t word, q0[2], q1[2];                                     // B operands of the two halves
-    const int u = query_bytes(a.q + (size_t)row * a.ldq + h * 64, wide, lane, word);
+    const int u = query_bytes(a.q + (size_t)row * a.ldq + h * 64, wide & 1, lane, word);
     {
         const uint32_t pick = (g & 1) ? 0x5151u : 0x4040u;           // odd columns the low bytes
 #pragma unroll
@@ -265,8 +279,8 @@ __global__ void __launch_bounds__(SF_WARPS * 32) k_store_attend_few(StoreAttend 
             z += av;
             w[t] = seen ? (uint32_t)rnd32(av, min(STORE_W_SHIFT + M - (int)(int8_t)(v4 >> (8 * t)), 26)) : 0u;
         }
-        uint32_t r[4];
-        turn4(w, r);
+        uint32_t r[3];
+        turn3(w, r[0], r[1], r[2]);
 #pragma unroll
         for (int b = 0; b < 3; b++) *reinterpret_cast<uint32_t*>(WP + (size_t)b * chunk + k) = r[b];
     }
@@ -340,8 +354,8 @@ __global__ void __launch_bounds__(SF_WARPS * 32) k_store_attend_few(StoreAttend 
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// the arrival of many rows a stream (a prompt pass): a CTA of 8 warps takes 16 QG consecutive rows of one head, 16 to a
-// warp, and 8 / QG warps share a group's keys. Tiles of 128 keys (and values) are brought into shared memory once for all
+// the arrival of many rows a stream (a prompt pass): a CTA of 4 warps takes 16 QG consecutive rows of one head, 16 to a
+// warp, and 4 / QG warps share a group's keys. Tiles of 64 keys (and values) are brought into shared memory once for all
 // the CTA's rows, as signed bytes in the order of the tensor cores' B operands (c 2^(s - S + 3) for keys, 16 c for values).
 //   pass 1  every score (m16n8k32, the query's two bytes one after the other), the rows' largest and largest value shift
 //   pass 2  the scores again (cheaper than keeping 4 bytes a pair), a = ARR[start - score] from a copy of the table in
@@ -349,8 +363,8 @@ __global__ void __launch_bounds__(SF_WARPS * 32) k_store_attend_few(StoreAttend 
 //           num += w c: a lane's score of tile t lies where its A operand wants it when k is taken in the order below
 // CTAs are persistent so that the table is copied once an SM, the longest rows first.
 // ---------------------------------------------------------------------------------------------------------------------
-constexpr int SM_TILE = 128;
-constexpr int SM_THREADS = 256;
+constexpr int SM_TILE = 64;
+constexpr int SM_WARPS = 4, SM_THREADS = SM_WARPS * 32;
 struct SmTile {
     uint4 k[SM_TILE / 8][32];            // [8 keys][lane (g, j)]: key g, dims of word j of both halves, even and odd
     uint4 v[SM_TILE / 32][2][2][32];     // [32 keys][b0, b1][tiles 0-3, 4-7][lane]
@@ -378,22 +392,22 @@ struct SmShared {
 };
 
 template <int QG>
-__global__ void __launch_bounds__(SM_THREADS, 1) k_store_attend_many(StoreAttend a, int tiles, int wide) {
+__global__ void __launch_bounds__(SM_THREADS, 2) k_store_attend_many(StoreAttend a, int tiles, int wide) {
     griddep_wait();
     griddep_launch();
     extern __shared__ __align__(16) uint8_t sm[];
     SmShared<QG>& S = *reinterpret_cast<SmShared<QG>*>(sm);
     int32_t* const TAB = reinterpret_cast<int32_t*>(sm + sizeof(SmShared<QG>));   // [alen + 1], 0 at the end
-    constexpr int KS = 8 / QG, ROWS = 16 * QG, BLOCKS = SM_TILE / 32;
+    constexpr int KS = SM_WARPS / QG, ROWS = 16 * QG, BLOCKS = SM_TILE / 32;
     const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, g = lane >> 2, j = lane & 3;
     const int qg = wid % QG, kg = wid / QG;
     const int H = a.st.H, alen = a.alen;
     for (int i = tid; i < alen; i += SM_THREADS) TAB[i] = __ldg(a.ARR + i);
     if (tid == 0) TAB[alen] = 0;
-    const int64_t items = (int64_t)tiles * H * a.rw.n_streams;
-    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-        const int s = (int)(item % a.rw.n_streams);
-        const int h = (int)(item / a.rw.n_streams % H), tile = tiles - 1 - (int)(item / a.rw.n_streams / H);
+    const uint32_t items = (uint32_t)(tiles * H * a.rw.n_streams);     // below 2^31 (the launch sees to it)
+    for (uint32_t item = blockIdx.x; item < items; item += gridDim.x) {
+        const uint32_t sh = item / a.rw.n_streams;
+        const int s = item - sh * a.rw.n_streams, h = sh % H, tile = tiles - 1 - (int)(sh / H);
         StoreRun run;
         if (!store_run(a.rw, s, a.st.lim, run, a.err) || tile * ROWS >= run.n) continue;
         const int i0 = tile * ROWS, nr = min(ROWS, run.n - i0);
@@ -416,10 +430,10 @@ __global__ void __launch_bounds__(SM_THREADS, 1) k_store_attend_many(StoreAttend
             S.z[r] = 0;
         }
         __syncthreads();
-        for (int r = wid; r < ROWS; r += 8) {
+        for (int r = wid; r < ROWS; r += SM_WARPS) {
             uint32_t word = 0;
             int u = 0;
-            if (r < nr) u = query_bytes(a.q + (size_t)(run.r0 + i0 + r) * a.ldq + h * 64, wide, lane, word);
+            if (r < nr) u = query_bytes(a.q + (size_t)(run.r0 + i0 + r) * a.ldq + h * 64, wide & 1, lane, word);
             S.q[r][lane] = word;
             if (lane == 0) {
                 S.u[r] = u;
@@ -504,67 +518,68 @@ __global__ void __launch_bounds__(SM_THREADS, 1) k_store_attend_many(StoreAttend
         };
         // twice the rounded score (fast: its digit below the last one kept; slow: shifts up, and the limits) of tile n of
         // eight keys: rows ra and rb, keys 2j and 2j + 1
-        auto scores = [&](const SmTile& T, int n, bool slow, int (&y)[4]) {
+        auto scores = [&](const SmTile& T, int n, auto slow, int (&y)[4]) {
             const uint4 b = T.k[n][lane];
-            int d[4] = {};
-            mma_s8(d, q[0][0][0], q[0][0][1], q[0][0][2], q[0][0][3], b.x, b.y);
+            int d[4];
+            mma_s8_first(d, q[0][0][0], q[0][0][1], q[0][0][2], q[0][0][3], b.x, b.y);
             mma_s8(d, q[0][1][0], q[0][1][1], q[0][1][2], q[0][1][3], b.z, b.w);
 #pragma unroll
             for (int x = 0; x < 4; x++) d[x] = (int)((uint32_t)d[x] << 8);
             mma_s8(d, q[1][0][0], q[1][0][1], q[1][0][2], q[1][0][3], b.x, b.y);
             mma_s8(d, q[1][1][0], q[1][1][1], q[1][1][2], q[1][1][3], b.z, b.w);
             const int2 kr = *reinterpret_cast<const int2*>(&T.kr[n * 8 + 2 * j]);
-            if (!slow) {
-                y[0] = d[0] >> (kr.x - ua);
-                y[1] = d[1] >> (kr.y - ua);
-                y[2] = d[2] >> (kr.x - ub);
-                y[3] = d[3] >> (kr.y - ub);
-            } else {
-                y[0] = 2 * store_score(d[0], kr.x - ua + 1);
-                y[1] = 2 * store_score(d[1], kr.y - ua + 1);
-                y[2] = 2 * store_score(d[2], kr.x - ub + 1);
-                y[3] = 2 * store_score(d[3], kr.y - ub + 1);
-            }
+            const int r[4] = {kr.x - ua, kr.y - ua, kr.x - ub, kr.y - ub};
+#pragma unroll
+            for (int x = 0; x < 4; x++) y[x] = decltype(slow)::value ? 2 * store_score(d[x], r[x] + 1) : d[x] >> r[x];
         };
 
         // ---- pass 1
-        int ya = INT32_MIN, yb = INT32_MIN, ma = 0, mb = 0;
-        fetch(0, false);
-        put(0, false);
-        __syncthreads();
-        for (int t = 0; t < nt; t++) {
-            if (t + 1 < nt) fetch(t + 1, false);
-            const SmTile& T = S.tile[t & 1];
-            const bool slow = S.slow;
-#pragma unroll 1
-            for (int b = kg; b < BLOCKS; b += KS) {
-                const int kb = k0 + t * SM_TILE + b * 32;
-                if (kb > w_p1 || kb + 31 < w_l0) continue;
-                const bool whole = kb + 31 <= w_p0 && kb >= w_l1;
+        int ya, yb, ma, mb, mw;
+        auto largest = [&](const SmTile& T, int b, int kb, auto slow, auto whole) {
+            if (decltype(whole)::value) mw = max(mw, T.vs[b * 32 + lane]);
 #pragma unroll
-                for (int n = 0; n < 4; n++) {
-                    int y[4];
-                    scores(T, b * 4 + n, slow, y);
+            for (int n = 0; n < 4; n++) {
+                int y[4];
+                scores(T, b * 4 + n, slow, y);
+                if (decltype(whole)::value) {
+                    ya = max(ya, max(y[0], y[1]));
+                    yb = max(yb, max(y[2], y[3]));
+                } else {
                     const int2 vs = *reinterpret_cast<const int2*>(&T.vs[b * 32 + n * 8 + 2 * j]);
-                    if (whole) {
-                        ya = max(ya, max(y[0], y[1]));
-                        yb = max(yb, max(y[2], y[3]));
-                        ma = max(ma, max(vs.x, vs.y));
-                        mb = max(mb, max(vs.x, vs.y));
-                    } else {
-                        const int key = kb + n * 8 + 2 * j;
-                        if (key >= la && key <= pa) { ya = max(ya, y[0]); ma = max(ma, vs.x); }
-                        if (key + 1 >= la && key + 1 <= pa) { ya = max(ya, y[1]); ma = max(ma, vs.y); }
-                        if (key >= lb && key <= pb) { yb = max(yb, y[2]); mb = max(mb, vs.x); }
-                        if (key + 1 >= lb && key + 1 <= pb) { yb = max(yb, y[3]); mb = max(mb, vs.y); }
-                    }
+                    const int key = kb + n * 8 + 2 * j;
+                    if (key >= la && key <= pa) { ya = max(ya, y[0]); ma = max(ma, vs.x); }
+                    if (key + 1 >= la && key + 1 <= pa) { ya = max(ya, y[1]); ma = max(ma, vs.y); }
+                    if (key >= lb && key <= pb) { yb = max(yb, y[2]); mb = max(mb, vs.x); }
+                    if (key + 1 >= lb && key + 1 <= pb) { yb = max(yb, y[3]); mb = max(mb, vs.y); }
                 }
             }
-            if (t + 1 < nt) {
-                put(t + 1, false);
+        };
+        auto pass1 = [&](auto slow) {
+            ya = yb = INT32_MIN;
+            ma = mb = mw = 0;             // mw: of blocks that all rows see
+            fetch(0, false);
+            put(0, false);
+            __syncthreads();
+            for (int t = 0; t < nt; t++) {
+                if (t + 1 < nt) fetch(t + 1, false);
+                const SmTile& T = S.tile[t & 1];
+#pragma unroll 1
+                for (int b = kg; b < BLOCKS; b += KS) {
+                    const int kb = k0 + t * SM_TILE + b * 32;
+                    if (kb > w_p1 || kb + 31 < w_l0) continue;
+                    if (kb + 31 <= w_p0 && kb >= w_l1) largest(T, b, kb, slow, std::true_type());
+                    else largest(T, b, kb, slow, std::false_type());
+                }
+                if (t + 1 < nt) put(t + 1, false);
                 __syncthreads();
             }
-        }
+        };
+        pass1(std::false_type());
+        const bool slow = S.slow;         // some key's score shifts up (or not down): all again with the general form
+        if (slow) pass1(std::true_type());
+        mw = __reduce_max_sync(0xffffffffu, mw);
+        ma = max(ma, mw);
+        mb = max(mb, mw);
 #pragma unroll
         for (int o = 1; o < 4; o <<= 1) {
             ya = max(ya, __shfl_xor_sync(0xffffffffu, ya, o));
@@ -572,20 +587,24 @@ __global__ void __launch_bounds__(SM_THREADS, 1) k_store_attend_many(StoreAttend
             ma = max(ma, __shfl_xor_sync(0xffffffffu, ma, o));
             mb = max(mb, __shfl_xor_sync(0xffffffffu, mb, o));
         }
-        if (j == 0) {
-            atomicMax(&S.y[ra], ya);
-            atomicMax(&S.y[rb], yb);
-            atomicMax(&S.m[ra], ma);
-            atomicMax(&S.m[rb], mb);
-        }
         fetch(0, true);
-        __syncthreads();
+        if (KS > 1) {
+            if (j == 0) {
+                atomicMax(&S.y[ra], ya);
+                atomicMax(&S.y[rb], yb);
+                atomicMax(&S.m[ra], ma);
+                atomicMax(&S.m[rb], mb);
+            }
+            __syncthreads();
+            ya = S.y[ra];
+            yb = S.y[rb];
+            ma = S.m[ra];
+            mb = S.m[rb];
+        }
         put(0, true);
-        // twice the largest score: a digit below the last rounds up with it
-        const uint32_t sa = (uint32_t)(((S.y[ra] >> 1) + (S.y[ra] & 1)) * 2), sb = (uint32_t)(((S.y[rb] >> 1) + (S.y[rb] & 1)) * 2);
-        ma = S.m[ra];
-        mb = S.m[rb];
         __syncthreads();
+        // twice the largest score: a digit below the last rounds up with it
+        const uint32_t sa = (uint32_t)(((ya >> 1) + (ya & 1)) * 2), sb = (uint32_t)(((yb >> 1) + (yb & 1)) * 2);
 
         // ---- pass 2
         int acc[3][8][4];
@@ -596,128 +615,122 @@ __global__ void __launch_bounds__(SM_THREADS, 1) k_store_attend_many(StoreAttend
 #pragma unroll
                 for (int c = 0; c < 4; c++) acc[x][t][c] = 0;
         int64_t za = 0, zb = 0;
-        for (int t = 0; t < nt; t++) {
-            if (t + 1 < nt) fetch(t + 1, true);
-            const SmTile& T = S.tile[t & 1];
-            const bool slow = S.slow;
-#pragma unroll 1
-            for (int b = kg; b < BLOCKS; b += KS) {
-                const int kb = k0 + t * SM_TILE + b * 32;
-                if (kb > w_p1 || kb + 31 < w_l0) continue;
-                const bool whole = kb + 31 <= w_p0 && kb >= w_l1;
-                uint32_t p[3][4];                 // the weights' planes as A operands
-                int32_t s_a = 0, s_b = 0;         // 8 entries of at most 2^24
+        auto add = [&](const SmTile& T, int b, int kb, auto slow, auto whole) {
+            uint32_t p[3][4];                 // the weights' planes as A operands
+            int32_t s_a = 0, s_b = 0;         // 8 entries of at most 2^24
 #pragma unroll
-                for (int n = 0; n < 4; n += 2) {
-                    uint32_t wa[4], wb[4];
-#pragma unroll
-                    for (int x = 0; x < 2; x++) {
-                        int y[4];
-                        scores(T, b * 4 + n + x, slow, y);
-                        const int2 vs = *reinterpret_cast<const int2*>(&T.vs[b * 32 + (n + x) * 8 + 2 * j]);
-                        // start - score, from twice both: (start2 - y) / 2 rounded down
-                        uint32_t d[4] = {(sa - (uint32_t)y[0]) >> 1, (sa - (uint32_t)y[1]) >> 1, (sb - (uint32_t)y[2]) >> 1,
-                                         (sb - (uint32_t)y[3]) >> 1};
-#pragma unroll
-                        for (int c = 0; c < 4; c++) d[c] = min(d[c], (uint32_t)alen);
-                        if (!whole) {
-                            const int key = kb + (n + x) * 8 + 2 * j;
-                            if (!(key >= la && key <= pa)) d[0] = alen;
-                            if (!(key + 1 >= la && key + 1 <= pa)) d[1] = alen;
-                            if (!(key >= lb && key <= pb)) d[2] = alen;
-                            if (!(key + 1 >= lb && key + 1 <= pb)) d[3] = alen;
-                        }
-                        const int v[4] = {TAB[d[0]], TAB[d[1]], TAB[d[2]], TAB[d[3]]};
-                        s_a += v[0] + v[1];
-                        s_b += v[2] + v[3];
-                        // rnd(a, 1 + M - vs); a key that a row does not see (whose vs may pass M) has a = 0
-                        wa[2 * x] = (shr_u32(v[0], ma - vs.x) + 1) >> 1;
-                        wa[2 * x + 1] = (shr_u32(v[1], ma - vs.y) + 1) >> 1;
-                        wb[2 * x] = (shr_u32(v[2], mb - vs.x) + 1) >> 1;
-                        wb[2 * x + 1] = (shr_u32(v[3], mb - vs.y) + 1) >> 1;
-                    }
-                    uint32_t r[4];
-                    turn4(wa, r);
-                    p[0][n] = r[0];
-                    p[1][n] = r[1];
-                    p[2][n] = r[2];
-                    turn4(wb, r);
-                    p[0][n + 1] = r[0];
-                    p[1][n + 1] = r[1];
-                    p[2][n + 1] = r[2];
-                }
-                za += s_a;
-                zb += s_b;
+            for (int n = 0; n < 4; n += 2) {
+                uint32_t wa[4], wb[4];
 #pragma unroll
                 for (int x = 0; x < 2; x++) {
-                    const uint4 b0 = T.v[b][0][x][lane], b1 = T.v[b][1][x][lane];
-                    const uint32_t c0[4] = {b0.x, b0.y, b0.z, b0.w}, c1[4] = {b1.x, b1.y, b1.z, b1.w};
+                    int y[4];
+                    scores(T, b * 4 + n + x, slow, y);
+                    const int2 vs = *reinterpret_cast<const int2*>(&T.vs[b * 32 + (n + x) * 8 + 2 * j]);
+                    // start - score, from twice both: (start2 - y) / 2 rounded down
+                    uint32_t d[4] = {(sa - (uint32_t)y[0]) >> 1, (sa - (uint32_t)y[1]) >> 1, (sb - (uint32_t)y[2]) >> 1,
+                                     (sb - (uint32_t)y[3]) >> 1};
 #pragma unroll
-                    for (int y = 0; y < 4; y++)
+                    for (int c = 0; c < 4; c++) d[c] = min(d[c], (uint32_t)alen);
+                    if (!decltype(whole)::value) {
+                        const int key = kb + (n + x) * 8 + 2 * j;
+                        if (!(key >= la && key <= pa)) d[0] = alen;
+                        if (!(key + 1 >= la && key + 1 <= pa)) d[1] = alen;
+                        if (!(key >= lb && key <= pb)) d[2] = alen;
+                        if (!(key + 1 >= lb && key + 1 <= pb)) d[3] = alen;
+                    }
+                    const int v[4] = {TAB[d[0]], TAB[d[1]], TAB[d[2]], TAB[d[3]]};
+                    s_a += v[0] + v[1];
+                    s_b += v[2] + v[3];
+                    // rnd(a, 1 + M - vs); a key that a row does not see (whose vs may pass M) has a = 0
+                    wa[2 * x] = (shr_u32(v[0], ma - vs.x) + 1) >> 1;
+                    wa[2 * x + 1] = (shr_u32(v[1], ma - vs.y) + 1) >> 1;
+                    wb[2 * x] = (shr_u32(v[2], mb - vs.x) + 1) >> 1;
+                    wb[2 * x + 1] = (shr_u32(v[3], mb - vs.y) + 1) >> 1;
+                }
+                turn3(wa, p[0][n], p[1][n], p[2][n]);
+                turn3(wb, p[0][n + 1], p[1][n + 1], p[2][n + 1]);
+            }
+            za += s_a;
+            zb += s_b;
 #pragma unroll
-                        for (int z = 0; z < 3; z++)
-                            mma_u8s8(acc[z][4 * x + y], p[z][0], p[z][1], p[z][2], p[z][3], c0[y], c1[y]);
+            for (int x = 0; x < 2; x++) {
+                const uint4 b0 = T.v[b][0][x][lane], b1 = T.v[b][1][x][lane];
+                const uint32_t c0[4] = {b0.x, b0.y, b0.z, b0.w}, c1[4] = {b1.x, b1.y, b1.z, b1.w};
+#pragma unroll
+                for (int y = 0; y < 4; y++)
+#pragma unroll
+                    for (int z = 0; z < 3; z++)
+                        mma_u8s8(acc[z][4 * x + y], p[z][0], p[z][1], p[z][2], p[z][3], c0[y], c1[y]);
+            }
+        };
+        auto pass2 = [&](auto slow) {
+            for (int t = 0; t < nt; t++) {
+                if (t + 1 < nt) fetch(t + 1, true);
+                const SmTile& T = S.tile[t & 1];
+#pragma unroll 1
+                for (int b = kg; b < BLOCKS; b += KS) {
+                    const int kb = k0 + t * SM_TILE + b * 32;
+                    if (kb > w_p1 || kb + 31 < w_l0) continue;
+                    if (kb + 31 <= w_p0 && kb >= w_l1) add(T, b, kb, slow, std::true_type());
+                    else add(T, b, kb, slow, std::false_type());
+                }
+                if (t + 1 < nt) {
+                    put(t + 1, true);
+                    __syncthreads();
                 }
             }
-            if (t + 1 < nt) {
-                put(t + 1, true);
-                __syncthreads();
-            }
-        }
+        };
+        if (slow) pass2(std::true_type());
+        else pass2(std::false_type());
         atomicAdd(&S.z[ra], (unsigned long long)za);
         atomicAdd(&S.z[rb], (unsigned long long)zb);
-        // the sums of a group's warps: the later ones' into shared memory (in place of the tiles), added by the first
-        int64_t* const part = reinterpret_cast<int64_t*>(S.tile);     // [QG][16 rows][64], a warp's 8 KB in lane order
-        for (int k = 1; k < KS; k++) {
+        // a lane's 16 sums of each of its rows; where two warps share a group's keys, each finishes one of the rows
+        int64_t* const part = reinterpret_cast<int64_t*>(S.tile);     // [warp][16][32 lanes]
+        auto sum = [&](int c, int t, int y) {
+            return (int64_t)acc[0][t][2 * y + c] + ((int64_t)acc[1][t][2 * y + c] << 8) + ((int64_t)acc[2][t][2 * y + c] << 16);
+        };
+        __syncthreads();                                              // the tiles are done with, S.z is complete
+        if (KS == 2) {
+#pragma unroll
+            for (int x = 0; x < 16; x++) part[(wid * 16 + x) * 32 + lane] = kg ? sum(x >> 3, x & 7, 0) : sum(x >> 3, x & 7, 1);
             __syncthreads();
-            if (kg == k) {
-#pragma unroll
-                for (int t = 0; t < 8; t++)
-#pragma unroll
-                    for (int c = 0; c < 4; c++)
-                        part[(qg * 32 + t * 4 + c) * 32 + lane] =
-                            (int64_t)acc[0][t][c] + ((int64_t)acc[1][t][c] << 8) + ((int64_t)acc[2][t][c] << 16);
-            }
-            __syncthreads();
-            if (kg == 0) {
-#pragma unroll
-                for (int t = 0; t < 8; t++)
-#pragma unroll
-                    for (int c = 0; c < 4; c++) {
-                        // back into the planes: the low byte's plane takes what is left of the sum
-                        const int64_t o = part[(qg * 32 + t * 4 + c) * 32 + lane] + acc[0][t][c];
-                        acc[0][t][c] = (int)(o & 0xFFFF);
-                        acc[2][t][c] += (int)(o >> 16);
-                    }
-            }
         }
-        __syncthreads();
-        if (kg == 0) {
 #pragma unroll
-            for (int y = 0; y < 2; y++) {
-                const int r = y ? rb : ra;
-                const int64_t z = (int64_t)S.z[r];
-                const bool none = (y ? lb > pb : la > pa) || z == 0;
-                const int64_t F = 65536ll * ((y ? mb : ma) + STORE_W_SHIFT) - log2fix(none ? 1 : z, a.LOG2);
-                const int64_t e = __ldg(a.EXP2 + (F & 0xFFFF));
-                const int64_t sh = 16 - (F >> 16);
-                uint64_t any = 0;
-                int64_t* const out = a.out + ((size_t)(run.r0 + i0 + min(r, nr - 1)) * H + h) * 64;
+        for (int y = 0; y < 2; y++) {
+            if (KS == 2 && y != kg) continue;
+            const int r = y ? rb : ra;
+            const int64_t z = (int64_t)S.z[r];
+            const bool none = (y ? lb > pb : la > pa) || z == 0;
+            const int64_t F = 65536ll * ((y ? mb : ma) + STORE_W_SHIFT) - log2fix(none ? 1 : z, a.LOG2);
+            const int32_t e = none ? 0 : __ldg(a.EXP2 + (F & 0xFFFF));
+            const int64_t sh = 20 - (F >> 16);                        // the tiles hold 16 c: 4 digits more
+            uint64_t any = 0;
+            int64_t* const out = a.out + ((size_t)(run.r0 + i0 + r) * H + h) * 64 + 16 * j;
+            // columns 2j, 2j + 1 of tile t: dims 16j + t, 16j + 8 + t
 #pragma unroll
-                for (int c = 0; c < 2; c++)           // columns 2j + c: dims 8 (2j + c) + t
+            for (int x = 0; x < 16; x += 2) {
+                int64_t o[2];
 #pragma unroll
-                    for (int t = 0; t < 8; t++) {
-                        const int x = 2 * y + c;
-                        const int64_t num = ((int64_t)acc[0][t][x] + ((int64_t)acc[1][t][x] << 8) + ((int64_t)acc[2][t][x] << 16)) >> 4;
-                        const int64_t o = none ? 0 : rshift(wmul(num, e), sh);
-                        any |= mag(o);
-                        if (r < nr) out[16 * j + 8 * c + t] = o;
-                    }
-                if (a.or_out) {
-                    any |= __shfl_xor_sync(0xffffffffu, any, 1);
-                    any |= __shfl_xor_sync(0xffffffffu, any, 2);
-                    if (j == 0 && r < nr) atomicOr((unsigned long long*)&a.or_out[run.r0 + i0 + r], (unsigned long long)any);
+                for (int k = 0; k < 2; k++) {
+                    int64_t num = sum(x >> 3, (x + k) & 7, y);
+                    if (KS == 2) num += part[((wid ^ QG) * 16 + x + k) * 32 + lane];
+                    num *= e;                                          // at most 2^46 2^17
+                    o[k] = sh > 0 ? ((num >> (sh - 1)) + 1) >> 1 : (int64_t)((uint64_t)num << -sh);
+                    any |= mag(o[k]);
                 }
+                if (r < nr) {
+                    if (wide & 2) {
+                        *reinterpret_cast<longlong2*>(out + x) = make_longlong2(o[0], o[1]);
+                    } else {
+                        out[x] = o[0];
+                        out[x + 1] = o[1];
+                    }
+                }
+            }
+            if (a.or_out) {
+                any |= __shfl_xor_sync(0xffffffffu, any, 1);
+                any |= __shfl_xor_sync(0xffffffffu, any, 2);
+                if (j == 0 && r < nr) atomicOr((unsigned long long*)&a.or_out[run.r0 + i0 + r], (unsigned long long)any);
             }
         }
     }
@@ -786,15 +799,15 @@ cudaError_t attend_many(const StoreAttend& a, StoreLaunch how, int wide) {
     const int tiles = (a.rw.max_rows + 16 * QG - 1) / (16 * QG);
     const int64_t items = (int64_t)tiles * a.st.H * a.rw.n_streams;
     const size_t smem = sizeof(SmShared<QG>) + (size_t)(a.alen + 1) * 4;
-    return store_launch(how, k_store_attend_many<QG>, dim3((unsigned)std::min<int64_t>(items, how.sms)), SM_THREADS, smem, 1, a,
+    return store_launch(how, k_store_attend_many<QG>, dim3((unsigned)std::min<int64_t>(items, 2 * how.sms)), SM_THREADS, smem, 1, a,
                         tiles, wide);
 }
 }  // namespace
 
 cudaError_t store_attend(const StoreAttend& a, StoreLaunch how) {
     if (a.rw.n_streams == 0 || a.rw.rows == 0) return cudaSuccess;
-    const int wide = aligned16(a.q) && a.ldq % 2 == 0;
-    if (a.rw.max_rows > SM_FROM_ROWS)
+    const int wide = (aligned16(a.q) && a.ldq % 2 == 0) | aligned16(a.out) << 1;
+    if (a.rw.max_rows > SM_FROM_ROWS && (int64_t)((a.rw.max_rows + 31) / 32) * a.st.H * a.rw.n_streams < INT32_MAX)
         return (int64_t)((a.rw.max_rows + 63) / 64) * a.st.H * a.rw.n_streams >= how.sms ? attend_many<4>(a, how, wide)
                                                                                           : attend_many<2>(a, how, wide);
     // blocks of 32 positions that a row may see
