@@ -354,27 +354,50 @@ __global__ void __launch_bounds__(SF_WARPS * 32) k_store_attend_few(StoreAttend 
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// the arrival of many rows a stream (a prompt pass): a CTA of 4 warps takes 16 QG consecutive rows of one head, 16 to a
-// warp, and 4 / QG warps share a group's keys. Tiles of 64 keys (and values) are brought into shared memory once for all
-// the CTA's rows, as signed bytes in the order of the tensor cores' B operands (c 2^(s - S + 3) for keys, 16 c for values).
+// the arrival of many rows a stream (a prompt pass): a CTA of 8 warps takes 64 consecutive rows of one head, a pair of warps
+// 16 of them; where that gives too few CTAs, a cluster of CS shares the rows' keys. Tiles of 64 keys (and values) are copied
+// into shared memory two ahead (cp.async), then unpacked once for all the rows as signed bytes in the order of the tensor
+// cores' B operands (c 2^(s - S + 3) for keys, 16 c for values); a warp forms the scores of one of a tile's two blocks of 32.
 //   pass 1  every score (m16n8k32, the query's two bytes one after the other), the rows' largest and largest value shift
 //   pass 2  the scores again (cheaper than keeping 4 bytes a pair), a = ARR[start - score] from a copy of the table in
-//           shared memory (a gather from L1 takes a line a lane), the weight's three bytes as the A operands of
-//           num += w c: a lane's score of tile t lies where its A operand wants it when k is taken in the order below
-// CTAs are persistent so that the table is copied once an SM, the longest rows first.
+//           shared memory (a gather from L1 takes a line a lane), the weight's three bytes as A operands (a lane's scores
+//           of a tile lie where its A operand wants them when k is taken in the order below). The two warps of a pair
+//           swap those through shared memory and each adds w c for half of the 64 dims: 48 registers of sums a lane in
+//           place of 96, which lets 16 warps share an SM
+// CTAs are persistent so that the table is copied twice an SM, the longest rows first.
 // ---------------------------------------------------------------------------------------------------------------------
-constexpr int SM_TILE = 64;
-constexpr int SM_WARPS = 4, SM_THREADS = SM_WARPS * 32;
+constexpr int SM_WARPS = 8, SM_THREADS = SM_WARPS * 32, SM_ROWS = 64, SM_KEYS = 64;
+struct SmRaw {
+    uint8_t k[SM_KEYS][32], v[SM_KEYS][32];
+    int8_t ks[SM_KEYS][2], vs[SM_KEYS];
+};
 struct SmTile {
-    uint4 k[SM_TILE / 8][32];            // [8 keys][lane (g, j)]: key g, dims of word j of both halves, even and odd
-    uint4 v[SM_TILE / 32][2][2][32];     // [32 keys][b0, b1][tiles 0-3, 4-7][lane]
-    int32_t kr[SM_TILE];                 // 27 - S: a score's shift less one is kr - u
-    int32_t vs[SM_TILE];
+    uint4 k[SM_KEYS / 8][32];            // [8 keys][lane (g, j)]: key g, dims of word j of both halves, even and odd
+    uint4 v[SM_KEYS / 32][4][32];        // [32 keys][tiles 2b, 2b + 1][lane (g, j)]: dims 8g + 2b, 8g + 2b + 1 of 8 keys
+    int32_t kr[SM_KEYS];                 // 27 - S: a score's shift less one is kr - u
+    int32_t vs[SM_KEYS];
+};
+struct SmShared {
+    SmTile tile[2];
+    SmRaw raw[2];
+    union {
+        uint32_t q[SM_ROWS][33];         // the rows' query bytes, until every lane has its operands
+        uint4 p[SM_WARPS][3][32];        // a block's weights on the way to the pair's other warp
+    };
+    unsigned long long z[SM_ROWS];
+    int2 ym[SM_ROWS];                    // the CTA's largest score (twice) and value shift
+    int32_t u[SM_ROWS], umax, slow;
 };
 
-// bytes c 2^up of the word's even (or, shifted down, odd) codes; up = 0 .. 3: c + 8 moves up, 8 2^up comes off again
-B2_DEV uint32_t codes_up(uint32_t w, int up, uint32_t less) {
+// bytes c 2^up of the word's even and odd codes; up = 0 .. 3: c + 8 moves up, 8 2^up comes off again (less: 128 - 8 2^up)
+B2_DEV uint32_t even_up(uint32_t w, int up, uint32_t less) {
     return ((((w & 0x0F0F0F0Fu) ^ 0x08080808u) << up) + less) ^ 0x80808080u;
+}
+B2_DEV uint32_t odd_up(uint32_t w, int up, uint32_t less) {
+    return ((((w & 0xF0F0F0F0u) ^ 0x80808080u) >> (4 - up)) + less) ^ 0x80808080u;
+}
+B2_DEV void copy16(void* to, const void* from) {      // 16 bytes, asynchronously, past L1
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(saddr(to)), "l"(from) : "memory");
 }
 B2_DEV uint32_t shr_u32(uint32_t x, uint32_t s) {     // 0 for s > 31
     uint32_t r;
@@ -382,32 +405,23 @@ B2_DEV uint32_t shr_u32(uint32_t x, uint32_t s) {     // 0 for s > 31
     return r;
 }
 
-template <int QG>
-struct SmShared {
-    SmTile tile[2];
-    uint32_t q[16 * QG][33];
-    int32_t u[16 * QG], y[16 * QG], m[16 * QG];
-    unsigned long long z[16 * QG];
-    int32_t umax, slow;
-};
-
-template <int QG>
+template <int CS>
 __global__ void __launch_bounds__(SM_THREADS, 2) k_store_attend_many(StoreAttend a, int tiles, int wide) {
     griddep_wait();
     griddep_launch();
     extern __shared__ __align__(16) uint8_t sm[];
-    SmShared<QG>& S = *reinterpret_cast<SmShared<QG>*>(sm);
-    int32_t* const TAB = reinterpret_cast<int32_t*>(sm + sizeof(SmShared<QG>));   // [alen + 1], 0 at the end
-    constexpr int KS = SM_WARPS / QG, ROWS = 16 * QG, BLOCKS = SM_TILE / 32;
+    SmShared& S = *reinterpret_cast<SmShared*>(sm);
+    int32_t* const TAB = reinterpret_cast<int32_t*>(sm + sizeof(SmShared));   // [alen + 1], 0 at the end
+    constexpr int ROWS = SM_ROWS, KEYS = SM_KEYS;
     const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, g = lane >> 2, j = lane & 3;
-    const int qg = wid % QG, kg = wid / QG;
+    const int pair = wid >> 1, blk = wid & 1, rank = CS > 1 ? (int)cluster_rank() : 0;   // blk: the warp's block of a tile
     const int H = a.st.H, alen = a.alen;
     for (int i = tid; i < alen; i += SM_THREADS) TAB[i] = __ldg(a.ARR + i);
     if (tid == 0) TAB[alen] = 0;
     const uint32_t items = (uint32_t)(tiles * H * a.rw.n_streams);     // below 2^31 (the launch sees to it)
-    for (uint32_t item = blockIdx.x; item < items; item += gridDim.x) {
-        const uint32_t sh = item / a.rw.n_streams;
-        const int s = item - sh * a.rw.n_streams, h = sh % H, tile = tiles - 1 - (int)(sh / H);
+    for (uint32_t item = blockIdx.x / CS; item < items; item += gridDim.x / CS) {
+        const uint32_t sh_ = item / a.rw.n_streams;
+        const int s = item - sh_ * a.rw.n_streams, h = sh_ % H, tile = tiles - 1 - (int)(sh_ / H);
         StoreRun run;
         if (!store_run(a.rw, s, a.st.lim, run, a.err) || tile * ROWS >= run.n) continue;
         const int i0 = tile * ROWS, nr = min(ROWS, run.n - i0);
@@ -416,7 +430,7 @@ __global__ void __launch_bounds__(SM_THREADS, 2) k_store_attend_many(StoreAttend
         const int k_lo = max(from, p_first - win + 1);       // the first row sees the earliest position
         __syncthreads();                                      // the item before is done with shared memory
         if (k_lo > p_last) {                                  // nothing to see for any row
-            for (int t = tid; t < nr * 64; t += SM_THREADS)
+            for (int t = rank == 0 ? tid : nr * 64; t < nr * 64; t += SM_THREADS)
                 a.out[((size_t)(run.r0 + i0 + (t >> 6)) * H + h) * 64 + (t & 63)] = 0;
             continue;
         }
@@ -425,11 +439,11 @@ __global__ void __launch_bounds__(SM_THREADS, 2) k_store_attend_many(StoreAttend
             S.slow = 0;
         }
         for (int r = tid; r < ROWS; r += SM_THREADS) {
-            S.y[r] = INT32_MIN;
-            S.m[r] = 0;
+            S.ym[r] = make_int2(INT32_MIN, 0);
             S.z[r] = 0;
         }
         __syncthreads();
+#pragma unroll 2
         for (int r = wid; r < ROWS; r += SM_WARPS) {
             uint32_t word = 0;
             int u = 0;
@@ -442,7 +456,7 @@ __global__ void __launch_bounds__(SM_THREADS, 2) k_store_attend_many(StoreAttend
         }
         __syncthreads();
         // this lane's rows and their A operands: [plane][half][even row g, even g + 8, odd g, odd g + 8]
-        const int ra = qg * 16 + g, rb = ra + 8;
+        const int ra = pair * 16 + g, rb = ra + 8;
         uint32_t q[2][2][4];
 #pragma unroll
         for (int x = 0; x < 2; x++)
@@ -459,61 +473,55 @@ __global__ void __launch_bounds__(SM_THREADS, 2) k_store_attend_many(StoreAttend
         const int ua = S.u[ra], ub = S.u[rb], umax = S.umax;
         const int pa = min(p_first + ra, p_last), pb = min(p_first + rb, p_last);      // rows past the last repeat it
         const int la = max(from, pa - win + 1), lb = max(from, pb - win + 1);
-        const int w_p0 = min(p_first + qg * 16, p_last), w_p1 = min(p_first + qg * 16 + 15, p_last);
+        const int w_p0 = min(p_first + pair * 16, p_last), w_p1 = min(p_first + pair * 16 + 15, p_last);
         const int w_l0 = max(from, w_p0 - win + 1), w_l1 = max(from, w_p1 - win + 1);
-        const int k0 = k_lo & ~31, k1 = (p_last | 31) + 1, nt = (k1 - k0 + SM_TILE - 1) / SM_TILE;
+        const int k0 = k_lo & ~31, k1 = (p_last | 31) + 1, all = (k1 - k0 + KEYS - 1) / KEYS;
+        // this CTA's tiles: t0 .. t1 - 1
+        const int per = CS > 1 ? (all + CS - 1) / CS : all, t0 = rank * per, t1 = min(all, t0 + per);
         const size_t base = kv_index(s, a.layer, h, 0, a.st.L, H, a.st.ctx);
 
-        // ---- a tile on its way: from global memory into registers, then unpacked into shared memory
-        uint2 kw[2];
-        uint32_t vw[4], kss[2];
-        int vsr = 0;
+        // ---- a tile on its way: copied as it is, then unpacked. A warp takes 8 keys, and byte b of the words of 32 values
+        // (dims 8g + 2b, 8g + 2b + 1); positions from k1 on are neither copied nor used
         auto fetch = [&](int t, bool values) {
-            const int kt = k0 + t * SM_TILE;
-#pragma unroll
-            for (int x = 0; x < 2; x++) {
-                const int key = kt + (wid * 2 + x) * 8 + g;
-                if (key < k1) {
-                    kw[x] = *reinterpret_cast<const uint2*>(a.st.k + (base + key) * 32 + 8 * j);
-                    kss[x] = *reinterpret_cast<const uint16_t*>(a.st.ks + (base + key) * 2);
+            const int kt = k0 + t * KEYS;
+            SmRaw& R = S.raw[t & 1];
+            if (t < t1) {
+                const int key = (tid & 127) >> 1, off = (tid & 1) * 16;
+                if (kt + key < k1) {
+                    if (tid < 128) copy16(&R.k[key][off], a.st.k + (base + kt + key) * 32 + off);
+                    else if (values) copy16(&R.v[key][off], a.st.v + (base + kt + key) * 32 + off);
                 }
+                if (tid < 8 && kt + tid * 8 < k1) copy16(&R.ks[tid * 8][0], a.st.ks + (base + kt + tid * 8) * 2);
+                if (tid >= 128 && tid < 132 && kt + (tid - 128) * 16 < k1) copy16(&R.vs[(tid - 128) * 16], a.st.vs + base + kt + (tid - 128) * 16);
             }
-            const int key = kt + tid;
-            if (tid < SM_TILE && key < k1) vsr = a.st.vs[base + key];
-            if (values) {
-                const int vk = kt + (wid >> 1) * 32 + (wid & 1) * 16 + 2 * j;      // keys vk, vk + 1, vk + 8, vk + 9
-                if (vk < k1) {
-#pragma unroll
-                    for (int x = 0; x < 4; x++)
-                        vw[x] = *reinterpret_cast<const uint32_t*>(a.st.v + (base + vk + (x & 1) + 4 * (x & 2)) * 32 + 4 * g);
-                }
-            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
         };
+        auto arrived = [&]() { asm volatile("cp.async.wait_group 0;" ::: "memory"); };   // a barrier makes it everybody's
         auto put = [&](int t, bool values) {
-            const int kt = k0 + t * SM_TILE;
+            const SmRaw& R = S.raw[t & 1];
             SmTile& T = S.tile[t & 1];
-#pragma unroll
-            for (int x = 0; x < 2; x++) {
-                const int kl = (wid * 2 + x) * 8 + g;
-                if (kt + kl < k1) {
-                    const int s0 = (int8_t)(kss[x] & 255), s1 = (int8_t)(kss[x] >> 8), big = max(s0, s1);
-                    const int up0 = s0 - big + 3, up1 = s1 - big + 3;
-                    const uint32_t less0 = 0x80808080u - (0x08080808u << up0), less1 = 0x80808080u - (0x08080808u << up1);
-                    T.k[wid * 2 + x][lane] = make_uint4(codes_up(kw[x].x, up0, less0), codes_up(kw[x].x >> 4, up0, less0),
-                                                        codes_up(kw[x].y, up1, less1), codes_up(kw[x].y >> 4, up1, less1));
-                    if (j == 0) {
-                        T.kr[kl] = 27 - big;
-                        if (27 - big < umax) S.slow = 1;
-                    }
+            {
+                const int kl = wid * 8 + g;
+                const uint2 w = *reinterpret_cast<const uint2*>(&R.k[kl][8 * j]);
+                const int s0 = R.ks[kl][0], s1 = R.ks[kl][1], big = max(s0, s1);
+                const int up0 = s0 - big + 3, up1 = s1 - big + 3;
+                const uint32_t less0 = 0x80808080u - (0x08080808u << up0), less1 = 0x80808080u - (0x08080808u << up1);
+                T.k[wid][lane] = make_uint4(even_up(w.x, up0, less0), odd_up(w.x, up0, less0), even_up(w.y, up1, less1), odd_up(w.y, up1, less1));
+                if (j == 0) {
+                    T.kr[kl] = 27 - big;
+                    if (27 - big < umax && k0 + t * KEYS + kl < k1) S.slow = 1;
                 }
             }
-            if (tid < SM_TILE) T.vs[tid] = vsr;
-            if (values && kt + (wid >> 1) * 32 < k1) {
-                uint32_t r[4];
-                turn4(vw, r);
-                uint4* const to = &T.v[wid >> 1][wid & 1][0][lane];
-                to[0] = make_uint4(even16(r[0]), odd16(r[0]), even16(r[1]), odd16(r[1]));
-                to[32] = make_uint4(even16(r[2]), odd16(r[2]), even16(r[3]), odd16(r[3]));
+            if (tid < KEYS) T.vs[tid] = R.vs[tid];
+            if (values) {
+                // k of an operand's first register: keys 2j, 2j + 1, 8 + 2j, 9 + 2j; of its second: 16 more
+                uint32_t v[2];
+#pragma unroll
+                for (int c = 0; c < 2; c++) {
+                    const uint8_t* r = &R.v[(wid >> 2) * 32 + 16 * c + 2 * j][4 * g + (wid & 3)];
+                    v[c] = __byte_perm(__byte_perm(r[0], r[32], 0x40), __byte_perm(r[256], r[288], 0x40), 0x5410);
+                }
+                T.v[wid >> 2][wid & 3][lane] = make_uint4(even16(v[0]), even16(v[1]), odd16(v[0]), odd16(v[1]));
             }
         };
         // twice the rounded score (fast: its digit below the last one kept; slow: shifts up, and the limits) of tile n of
@@ -535,17 +543,17 @@ __global__ void __launch_bounds__(SM_THREADS, 2) k_store_attend_many(StoreAttend
 
         // ---- pass 1
         int ya, yb, ma, mb, mw;
-        auto largest = [&](const SmTile& T, int b, int kb, auto slow, auto whole) {
-            if (decltype(whole)::value) mw = max(mw, T.vs[b * 32 + lane]);
+        auto largest = [&](const SmTile& T, int kb, auto slow, auto whole) {
+            if (decltype(whole)::value) mw = max(mw, T.vs[blk * 32 + lane]);
 #pragma unroll
             for (int n = 0; n < 4; n++) {
                 int y[4];
-                scores(T, b * 4 + n, slow, y);
+                scores(T, blk * 4 + n, slow, y);
                 if (decltype(whole)::value) {
                     ya = max(ya, max(y[0], y[1]));
                     yb = max(yb, max(y[2], y[3]));
                 } else {
-                    const int2 vs = *reinterpret_cast<const int2*>(&T.vs[b * 32 + n * 8 + 2 * j]);
+                    const int2 vs = *reinterpret_cast<const int2*>(&T.vs[blk * 32 + n * 8 + 2 * j]);
                     const int key = kb + n * 8 + 2 * j;
                     if (key >= la && key <= pa) { ya = max(ya, y[0]); ma = max(ma, vs.x); }
                     if (key + 1 >= la && key + 1 <= pa) { ya = max(ya, y[1]); ma = max(ma, vs.y); }
@@ -554,25 +562,33 @@ __global__ void __launch_bounds__(SM_THREADS, 2) k_store_attend_many(StoreAttend
                 }
             }
         };
+        // a pass over the CTA's tiles: tile t in the works, t + 1 unpacked, t + 2 on its way
+        auto pass = [&](bool values, auto work) {
+            fetch(t0, values);
+            arrived();
+            __syncthreads();
+            fetch(t0 + 1, values);
+            if (t0 < t1) put(t0, values);
+            arrived();
+            __syncthreads();
+            for (int t = t0; t < t1; t++) {
+                fetch(t + 2, values);
+                work(S.tile[t & 1], k0 + t * KEYS);
+                if (t + 1 < t1) put(t + 1, values);
+                arrived();
+                __syncthreads();
+            }
+        };
         auto pass1 = [&](auto slow) {
             ya = yb = INT32_MIN;
             ma = mb = mw = 0;             // mw: of blocks that all rows see
-            fetch(0, false);
-            put(0, false);
-            __syncthreads();
-            for (int t = 0; t < nt; t++) {
-                if (t + 1 < nt) fetch(t + 1, false);
-                const SmTile& T = S.tile[t & 1];
-#pragma unroll 1
-                for (int b = kg; b < BLOCKS; b += KS) {
-                    const int kb = k0 + t * SM_TILE + b * 32;
-                    if (kb > w_p1 || kb + 31 < w_l0) continue;
-                    if (kb + 31 <= w_p0 && kb >= w_l1) largest(T, b, kb, slow, std::true_type());
-                    else largest(T, b, kb, slow, std::false_type());
+            pass(false, [&](const SmTile& T, int kt) {
+                const int kb = kt + blk * 32;
+                if (kb <= w_p1 && kb + 31 >= w_l0) {
+                    if (kb + 31 <= w_p0 && kb >= w_l1) largest(T, kb, slow, std::true_type());
+                    else largest(T, kb, slow, std::false_type());
                 }
-                if (t + 1 < nt) put(t + 1, false);
-                __syncthreads();
-            }
+            });
         };
         pass1(std::false_type());
         const bool slow = S.slow;         // some key's score shifts up (or not down): all again with the general form
@@ -587,35 +603,42 @@ __global__ void __launch_bounds__(SM_THREADS, 2) k_store_attend_many(StoreAttend
             ma = max(ma, __shfl_xor_sync(0xffffffffu, ma, o));
             mb = max(mb, __shfl_xor_sync(0xffffffffu, mb, o));
         }
-        fetch(0, true);
-        if (KS > 1) {
-            if (j == 0) {
-                atomicMax(&S.y[ra], ya);
-                atomicMax(&S.y[rb], yb);
-                atomicMax(&S.m[ra], ma);
-                atomicMax(&S.m[rb], mb);
-            }
-            __syncthreads();
-            ya = S.y[ra];
-            yb = S.y[rb];
-            ma = S.m[ra];
-            mb = S.m[rb];
+        if (j == 0) {
+            atomicMax(&S.ym[ra].x, ya);
+            atomicMax(&S.ym[rb].x, yb);
+            atomicMax(&S.ym[ra].y, ma);
+            atomicMax(&S.ym[rb].y, mb);
         }
-        put(0, true);
-        __syncthreads();
+        if (CS > 1) {
+            cluster_sync();
+#pragma unroll
+            for (int k = 0; k < CS; k++) {
+                const int64_t oa = ld_dsmem(mapa(saddr(&S.ym[ra]), (uint32_t)k)), ob = ld_dsmem(mapa(saddr(&S.ym[rb]), (uint32_t)k));
+                ya = max(ya, (int32_t)oa);
+                yb = max(yb, (int32_t)ob);
+                ma = max(ma, (int)(oa >> 32));
+                mb = max(mb, (int)(ob >> 32));
+            }
+        } else {
+            __syncthreads();
+            ya = S.ym[ra].x;
+            yb = S.ym[rb].x;
+            ma = S.ym[ra].y;
+            mb = S.ym[rb].y;
+        }
         // twice the largest score: a digit below the last rounds up with it
         const uint32_t sa = (uint32_t)(((ya >> 1) + (ya & 1)) * 2), sb = (uint32_t)(((yb >> 1) + (yb & 1)) * 2);
 
         // ---- pass 2
-        int acc[3][8][4];
+        int acc[3][4][4];                     // [plane][tile 4 (wid & 1) + t]
 #pragma unroll
         for (int x = 0; x < 3; x++)
 #pragma unroll
-            for (int t = 0; t < 8; t++)
+            for (int t = 0; t < 4; t++)
 #pragma unroll
                 for (int c = 0; c < 4; c++) acc[x][t][c] = 0;
         int64_t za = 0, zb = 0;
-        auto add = [&](const SmTile& T, int b, int kb, auto slow, auto whole) {
+        auto weights = [&](const SmTile& T, int kb, auto slow, auto whole) {
             uint32_t p[3][4];                 // the weights' planes as A operands
             int32_t s_a = 0, s_b = 0;         // 8 entries of at most 2^24
 #pragma unroll
@@ -624,8 +647,8 @@ __global__ void __launch_bounds__(SM_THREADS, 2) k_store_attend_many(StoreAttend
 #pragma unroll
                 for (int x = 0; x < 2; x++) {
                     int y[4];
-                    scores(T, b * 4 + n + x, slow, y);
-                    const int2 vs = *reinterpret_cast<const int2*>(&T.vs[b * 32 + (n + x) * 8 + 2 * j]);
+                    scores(T, blk * 4 + n + x, slow, y);
+                    const int2 vs = *reinterpret_cast<const int2*>(&T.vs[blk * 32 + (n + x) * 8 + 2 * j]);
                     // start - score, from twice both: (start2 - y) / 2 rounded down
                     uint32_t d[4] = {(sa - (uint32_t)y[0]) >> 1, (sa - (uint32_t)y[1]) >> 1, (sb - (uint32_t)y[2]) >> 1,
                                      (sb - (uint32_t)y[3]) >> 1};
@@ -653,77 +676,85 @@ __global__ void __launch_bounds__(SM_THREADS, 2) k_store_attend_many(StoreAttend
             za += s_a;
             zb += s_b;
 #pragma unroll
-            for (int x = 0; x < 2; x++) {
-                const uint4 b0 = T.v[b][0][x][lane], b1 = T.v[b][1][x][lane];
-                const uint32_t c0[4] = {b0.x, b0.y, b0.z, b0.w}, c1[4] = {b1.x, b1.y, b1.z, b1.w};
+            for (int z = 0; z < 3; z++) S.p[wid][z][lane] = make_uint4(p[z][0], p[z][1], p[z][2], p[z][3]);
+        };
+        // a block's weights times its values, this warp's half of the dims
+        auto add = [&](const SmTile& T, int b) {
+            const uint4* const v = &T.v[b][2 * (wid & 1)][lane];
+            const uint4 v0 = v[0], v1 = v[32];
 #pragma unroll
-                for (int y = 0; y < 4; y++)
-#pragma unroll
-                    for (int z = 0; z < 3; z++)
-                        mma_u8s8(acc[z][4 * x + y], p[z][0], p[z][1], p[z][2], p[z][3], c0[y], c1[y]);
+            for (int z = 0; z < 3; z++) {
+                const uint4 p = S.p[(wid & ~1) + b][z][lane];
+                mma_u8s8(acc[z][0], p.x, p.y, p.z, p.w, v0.x, v0.y);
+                mma_u8s8(acc[z][1], p.x, p.y, p.z, p.w, v0.z, v0.w);
+                mma_u8s8(acc[z][2], p.x, p.y, p.z, p.w, v1.x, v1.y);
+                mma_u8s8(acc[z][3], p.x, p.y, p.z, p.w, v1.z, v1.w);
             }
         };
         auto pass2 = [&](auto slow) {
-            for (int t = 0; t < nt; t++) {
-                if (t + 1 < nt) fetch(t + 1, true);
-                const SmTile& T = S.tile[t & 1];
-#pragma unroll 1
-                for (int b = kg; b < BLOCKS; b += KS) {
-                    const int kb = k0 + t * SM_TILE + b * 32;
-                    if (kb > w_p1 || kb + 31 < w_l0) continue;
-                    if (kb + 31 <= w_p0 && kb >= w_l1) add(T, b, kb, slow, std::true_type());
-                    else add(T, b, kb, slow, std::false_type());
+            pass(true, [&](const SmTile& T, int kt) {
+                const int kb = kt + blk * 32;
+                if (kb <= w_p1 && kb + 31 >= w_l0) {
+                    if (kb + 31 <= w_p0 && kb >= w_l1) weights(T, kb, slow, std::true_type());
+                    else weights(T, kb, slow, std::false_type());
                 }
-                if (t + 1 < nt) {
-                    put(t + 1, true);
-                    __syncthreads();
-                }
-            }
+                const bool b0 = kt <= w_p1 && kt + 31 >= w_l0, b1 = kt + 32 <= w_p1 && kt + 63 >= w_l0;
+                if (b0 || b1) asm volatile("bar.sync %0, 64;" ::"r"(1 + pair) : "memory");   // both warps of the pair
+                if (b0) add(T, 0);
+                if (b1) add(T, 1);
+            });
         };
         if (slow) pass2(std::true_type());
         else pass2(std::false_type());
         atomicAdd(&S.z[ra], (unsigned long long)za);
         atomicAdd(&S.z[rb], (unsigned long long)zb);
-        // a lane's 16 sums of each of its rows; where two warps share a group's keys, each finishes one of the rows
-        int64_t* const part = reinterpret_cast<int64_t*>(S.tile);     // [warp][16][32 lanes]
+        // a lane's 8 sums of each of its rows; a cluster's CTAs lay theirs out (in place of the tiles) a row at a time and
+        // each finishes 8 / CS of them
+        int64_t* const part = reinterpret_cast<int64_t*>(S.tile);     // [warp][8][32 lanes]
         auto sum = [&](int c, int t, int y) {
             return (int64_t)acc[0][t][2 * y + c] + ((int64_t)acc[1][t][2 * y + c] << 8) + ((int64_t)acc[2][t][2 * y + c] << 16);
         };
         __syncthreads();                                              // the tiles are done with, S.z is complete
-        if (KS == 2) {
-#pragma unroll
-            for (int x = 0; x < 16; x++) part[(wid * 16 + x) * 32 + lane] = kg ? sum(x >> 3, x & 7, 0) : sum(x >> 3, x & 7, 1);
-            __syncthreads();
-        }
 #pragma unroll
         for (int y = 0; y < 2; y++) {
-            if (KS == 2 && y != kg) continue;
             const int r = y ? rb : ra;
-            const int64_t z = (int64_t)S.z[r];
+            if (CS > 1) {
+#pragma unroll
+                for (int x = 0; x < 8; x++) part[(wid * 8 + x) * 32 + lane] = sum(x >> 2, x & 3, y);
+                cluster_sync();
+            }
+            int64_t z = CS > 1 ? 0 : (int64_t)S.z[r];
+            if (CS > 1)
+#pragma unroll
+                for (int k = 0; k < CS; k++) z += ld_dsmem(mapa(saddr(&S.z[r]), (uint32_t)k));
             const bool none = (y ? lb > pb : la > pa) || z == 0;
             const int64_t F = 65536ll * ((y ? mb : ma) + STORE_W_SHIFT) - log2fix(none ? 1 : z, a.LOG2);
             const int32_t e = none ? 0 : __ldg(a.EXP2 + (F & 0xFFFF));
             const int64_t sh = 20 - (F >> 16);                        // the tiles hold 16 c: 4 digits more
             uint64_t any = 0;
-            int64_t* const out = a.out + ((size_t)(run.r0 + i0 + r) * H + h) * 64 + 16 * j;
+            int64_t* const out = a.out + ((size_t)(run.r0 + i0 + r) * H + h) * 64 + 16 * j + 4 * (wid & 1);
             // columns 2j, 2j + 1 of tile t: dims 16j + t, 16j + 8 + t
 #pragma unroll
-            for (int x = 0; x < 16; x += 2) {
+            for (int x = 0; x < 8; x += 2) {
+                if (CS > 1 && x / (8 / CS) != rank) continue;
                 int64_t o[2];
 #pragma unroll
                 for (int k = 0; k < 2; k++) {
-                    int64_t num = sum(x >> 3, (x + k) & 7, y);
-                    if (KS == 2) num += part[((wid ^ QG) * 16 + x + k) * 32 + lane];
+                    int64_t num = CS > 1 ? 0 : sum(x >> 2, (x + k) & 3, y);
+                    if (CS > 1)
+#pragma unroll
+                        for (int m = 0; m < CS; m++) num += ld_dsmem(mapa(saddr(&part[(wid * 8 + x + k) * 32 + lane]), (uint32_t)m));
                     num *= e;                                          // at most 2^46 2^17
                     o[k] = sh > 0 ? ((num >> (sh - 1)) + 1) >> 1 : (int64_t)((uint64_t)num << -sh);
                     any |= mag(o[k]);
                 }
                 if (r < nr) {
+                    int64_t* const to = out + 8 * (x >> 2) + (x & 3);
                     if (wide & 2) {
-                        *reinterpret_cast<longlong2*>(out + x) = make_longlong2(o[0], o[1]);
+                        *reinterpret_cast<longlong2*>(to) = make_longlong2(o[0], o[1]);
                     } else {
-                        out[x] = o[0];
-                        out[x + 1] = o[1];
+                        to[0] = o[0];
+                        to[1] = o[1];
                     }
                 }
             }
@@ -732,6 +763,7 @@ __global__ void __launch_bounds__(SM_THREADS, 2) k_store_attend_many(StoreAttend
                 any |= __shfl_xor_sync(0xffffffffu, any, 2);
                 if (j == 0 && r < nr) atomicOr((unsigned long long*)&a.or_out[run.r0 + i0 + r], (unsigned long long)any);
             }
+            if (CS > 1) cluster_sync();                                // the others have read this CTA's sums
         }
     }
 }
@@ -788,28 +820,28 @@ cudaError_t store_init() {
     if (e == cudaSuccess) e = cudaFuncSetAttribute(k_store_attend_few<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, SF_MOST_KEYS * SF_BYTES);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(k_store_attend_few<4>, cudaFuncAttributeMaxDynamicSharedMemorySize, SF_MOST_KEYS * SF_BYTES);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(k_store_attend_few<8>, cudaFuncAttributeMaxDynamicSharedMemorySize, SF_MOST_KEYS * SF_BYTES);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(k_store_attend_many<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, SM_SMEM_MOST);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(k_store_attend_many<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, SM_SMEM_MOST);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(k_store_attend_many<4>, cudaFuncAttributeMaxDynamicSharedMemorySize, SM_SMEM_MOST);
     return e;
 }
 
-namespace {
-template <int QG>
-cudaError_t attend_many(const StoreAttend& a, StoreLaunch how, int wide) {
-    const int tiles = (a.rw.max_rows + 16 * QG - 1) / (16 * QG);
-    const int64_t items = (int64_t)tiles * a.st.H * a.rw.n_streams;
-    const size_t smem = sizeof(SmShared<QG>) + (size_t)(a.alen + 1) * 4;
-    return store_launch(how, k_store_attend_many<QG>, dim3((unsigned)std::min<int64_t>(items, 2 * how.sms)), SM_THREADS, smem, 1, a,
-                        tiles, wide);
-}
-}  // namespace
-
 cudaError_t store_attend(const StoreAttend& a, StoreLaunch how) {
     if (a.rw.n_streams == 0 || a.rw.rows == 0) return cudaSuccess;
     const int wide = (aligned16(a.q) && a.ldq % 2 == 0) | aligned16(a.out) << 1;
-    if (a.rw.max_rows > SM_FROM_ROWS && (int64_t)((a.rw.max_rows + 31) / 32) * a.st.H * a.rw.n_streams < INT32_MAX)
-        return (int64_t)((a.rw.max_rows + 63) / 64) * a.st.H * a.rw.n_streams >= how.sms ? attend_many<4>(a, how, wide)
-                                                                                          : attend_many<2>(a, how, wide);
+    const int64_t items = (int64_t)((a.rw.max_rows + SM_ROWS - 1) / SM_ROWS) * a.st.H * a.rw.n_streams;
+    if (a.rw.max_rows > SM_FROM_ROWS && items < INT32_MAX) {
+        const int tiles = (a.rw.max_rows + SM_ROWS - 1) / SM_ROWS;
+        const size_t smem = sizeof(SmShared) + (size_t)(a.alen + 1) * 4;
+        int cs = 1;
+        while (cs < 4 && items * cs * 2 <= how.sms * 2) cs *= 2;
+        const dim3 grid((unsigned)(std::min<int64_t>(items, how.sms * 2 / cs) * cs));
+        switch (cs) {
+            case 1: return store_launch(how, k_store_attend_many<1>, grid, SM_THREADS, smem, 1, a, tiles, wide);
+            case 2: return store_launch(how, k_store_attend_many<2>, grid, SM_THREADS, smem, 2, a, tiles, wide);
+            default: return store_launch(how, k_store_attend_many<4>, grid, SM_THREADS, smem, 4, a, tiles, wide);
+        }
+    }
     // blocks of 32 positions that a row may see
     int blocks = (a.st.lim + 31) / 32;
     if (a.window > 0 && a.window < a.st.lim) blocks = std::min(blocks, (a.window + 30) / 32 + 1);
