@@ -152,14 +152,22 @@ B2_DEV void turn3(const uint32_t* w, uint32_t& b0, uint32_t& b1, uint32_t& b2) {
 
 // a row's 64 query values at 15 bits, as two signed bytes q15 = 256 hi + lo, in a lane's pair (dims 2 lane, 2 lane + 1):
 // bytes hi, lo of the first, hi, lo of the second. Returns the row's shift u. Every lane of the warp takes part.
-B2_DEV int query_bytes(const int64_t* q, bool wide, int lane, uint32_t& word) {
-    int64_t x0, x1;
-    load_pair(q + 2 * lane, wide, x0, x1);
-    x0 = store_clamp(x0);
-    x1 = store_clamp(x1);
-    // the largest magnitude's bit length is that of the magnitudes' OR
-    const int u = max((int)__reduce_max_sync(0xffffffffu, (uint32_t)bitlen_u(mag(x0) | mag(x1))) - 14, 0);
-    const int a = (int)rnd64(x0, u), b = (int)rnd64(x1, u);
+B2_DEV int query_bytes(int64_t x0, int64_t x1, uint32_t& word) {
+    int u, a, b;
+    if (__all_sync(0xffffffffu, x0 == (int32_t)x0 && x1 == (int32_t)x1)) {       // the usual case: 32 bits hold them
+        const int y0 = (int)x0, y1 = (int)x1;
+        const uint32_t m = (uint32_t)abs(y0) | (uint32_t)abs(y1);                // (|-2^31| is 2^31 unsigned)
+        u = max(18 - __clz((int)__reduce_or_sync(0xffffffffu, m)), 0);
+        a = rnd32(y0, u);
+        b = rnd32(y1, u);
+    } else {
+        x0 = store_clamp(x0);
+        x1 = store_clamp(x1);
+        // the largest magnitude's bit length is that of the magnitudes' OR
+        u = max((int)__reduce_max_sync(0xffffffffu, (uint32_t)bitlen_u(mag(x0) | mag(x1))) - 14, 0);
+        a = (int)rnd64(x0, u);
+        b = (int)rnd64(x1, u);
+    }
     // byte 0: a + 128 >> 8, byte 1: a, byte 2: b + 128 >> 8, byte 3: b
     word = __byte_perm(__byte_perm(a + 128, a, 0x41), __byte_perm(b + 128, b, 0x41), 0x5410);
     return u;
@@ -200,7 +208,9 @@ __global__ void __launch_bounds__(SF_WARPS * 32) k_store_attend_few(StoreAttend 
     const int from = lo - b0 * 32, to = p - b0 * 32;                 // visible: from <= local key <= to
 
     uint32_t word, q0[2], q1[2];                                     // B operands of the two halves
-    const int u = query_bytes(a.q + (size_t)row * a.ldq + h * 64, wide & 1, lane, word);
+    int64_t x0, x1;
+    load_pair(a.q + (size_t)row * a.ldq + h * 64 + 2 * lane, wide & 1, x0, x1);
+    const int u = query_bytes(x0, x1, word);
     {
         const uint32_t pick = (g & 1) ? 0x5151u : 0x4040u;           // odd columns the low bytes
 #pragma unroll
@@ -405,8 +415,7 @@ B2_DEV uint32_t shr_u32(uint32_t x, uint32_t s) {     // 0 for s > 31
     return r;
 }
 
-template <int CS>
-__global__ void __launch_bounds__(SM_THREADS, 2) k_store_attend_many(StoreAttend a, int tiles, int wide) {
+__global__ void __launch_bounds__(SM_THREADS, 2) k_store_attend_many(StoreAttend a, int tiles, int cs, int wide) {
     griddep_wait();
     griddep_launch();
     extern __shared__ __align__(16) uint8_t sm[];
@@ -414,18 +423,33 @@ __global__ void __launch_bounds__(SM_THREADS, 2) k_store_attend_many(StoreAttend
     int32_t* const TAB = reinterpret_cast<int32_t*>(sm + sizeof(SmShared));   // [alen + 1], 0 at the end
     constexpr int ROWS = SM_ROWS, KEYS = SM_KEYS;
     const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, g = lane >> 2, j = lane & 3;
-    const int pair = wid >> 1, blk = wid & 1, rank = CS > 1 ? (int)cluster_rank() : 0;   // blk: the warp's block of a tile
+    const int pair = wid >> 1, blk = wid & 1, rank = cs > 1 ? (int)cluster_rank() : 0;   // blk: the warp's block of a tile
     const int H = a.st.H, alen = a.alen;
     for (int i = tid; i < alen; i += SM_THREADS) TAB[i] = __ldg(a.ARR + i);
     if (tid == 0) TAB[alen] = 0;
-    const uint32_t items = (uint32_t)(tiles * H * a.rw.n_streams);     // below 2^31 (the launch sees to it)
-    for (uint32_t item = blockIdx.x / CS; item < items; item += gridDim.x / CS) {
+    const uint32_t items = (uint32_t)(tiles * H * a.rw.n_streams), step = gridDim.x / cs;   // below 2^31 (the launch sees to it)
+    // an item's entries of the row table, read one item ahead
+    int n_r0 = 0, n_r1 = 0, n_pos = 0, n_first = 0;
+    auto ahead = [&](uint32_t item) {
+        if (item < items) {
+            const int s = item % a.rw.n_streams;
+            n_r0 = a.rw.cu ? a.rw.cu[s] : s;
+            n_r1 = a.rw.cu ? a.rw.cu[s + 1] : s + 1;
+            n_pos = a.rw.pos[s];
+            n_first = a.first ? a.first[s] : 0;
+        }
+    };
+    ahead(blockIdx.x / cs);
+    for (uint32_t item = blockIdx.x / cs; item < items; item += step) {
         const uint32_t sh_ = item / a.rw.n_streams;
         const int s = item - sh_ * a.rw.n_streams, h = sh_ % H, tile = tiles - 1 - (int)(sh_ / H);
         StoreRun run;
-        if (!store_run(a.rw, s, a.st.lim, run, a.err) || tile * ROWS >= run.n) continue;
+        const bool some = store_run(a.rw, n_r0, n_r1, n_pos, a.st.lim, run, a.err);
+        const int from = max(0, n_first);
+        ahead(item + step);
+        if (!some || tile * ROWS >= run.n) continue;
         const int i0 = tile * ROWS, nr = min(ROWS, run.n - i0);
-        const int from = a.first ? max(0, a.first[s]) : 0, win = a.window > 0 ? a.window : 0x40000000;
+        const int win = a.window > 0 ? a.window : 0x40000000;
         const int p_first = run.p0 + i0, p_last = p_first + nr - 1;
         const int k_lo = max(from, p_first - win + 1);       // the first row sees the earliest position
         __syncthreads();                                      // the item before is done with shared memory
@@ -434,6 +458,32 @@ __global__ void __launch_bounds__(SM_THREADS, 2) k_store_attend_many(StoreAttend
                 a.out[((size_t)(run.r0 + i0 + (t >> 6)) * H + h) * 64 + (t & 63)] = 0;
             continue;
         }
+        const int k0 = k_lo & ~31, k1 = (p_last | 31) + 1, all = (k1 - k0 + KEYS - 1) / KEYS;
+        // this CTA's tiles: t0 .. t1 - 1
+        const int per = cs > 1 ? (all + cs - 1) / cs : all, t0 = rank * per, t1 = min(all, t0 + per);
+        const size_t base = kv_index(s, a.layer, h, k0, a.st.L, H, a.st.ctx);
+
+        // ---- a tile on its way: copied as it is, then unpacked. A warp takes 8 keys, and byte b of the words of 32 values
+        // (dims 8g + 2b, 8g + 2b + 1); positions from k1 on are neither copied nor used
+        auto fetch = [&](int t, bool values) {
+            if (t < t1) {
+                const int left = k1 - k0 - t * KEYS;
+                const size_t e = base + (size_t)t * KEYS;
+                SmRaw& R = S.raw[t & 1];
+                if (((tid & 127) >> 1) < left) {
+                    if (tid < 128) copy16(&R.k[0][0] + tid * 16, a.st.k + e * 32 + tid * 16);
+                    else if (values) copy16(&R.v[0][0] + (tid - 128) * 16, a.st.v + e * 32 + (tid - 128) * 16);
+                }
+                if (tid < 8) {
+                    if (tid * 8 < left) copy16(&R.ks[tid * 8][0], a.st.ks + e * 2 + tid * 16);
+                } else if (tid < 12) {
+                    if ((tid - 8) * 16 < left) copy16(&R.vs[(tid - 8) * 16], a.st.vs + e + (tid - 8) * 16);
+                }
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+        fetch(t0, false);
+        fetch(t0 + 1, false);
         if (tid == 0) {
             S.umax = 0;
             S.slow = 0;
@@ -443,16 +493,23 @@ __global__ void __launch_bounds__(SM_THREADS, 2) k_store_attend_many(StoreAttend
             S.z[r] = 0;
         }
         __syncthreads();
-#pragma unroll 2
-        for (int r = wid; r < ROWS; r += SM_WARPS) {
-            uint32_t word = 0;
-            int u = 0;
-            if (r < nr) u = query_bytes(a.q + (size_t)(run.r0 + i0 + r) * a.ldq + h * 64, wide & 1, lane, word);
-            S.q[r][lane] = word;
-            if (lane == 0) {
-                S.u[r] = u;
-                atomicMax(&S.umax, u);
+        {
+            int64_t x[SM_ROWS / SM_WARPS][2];
+#pragma unroll
+            for (int k = 0; k < SM_ROWS / SM_WARPS; k++) {
+                const int r = wid + k * SM_WARPS;
+                x[k][0] = x[k][1] = 0;
+                if (r < nr) load_pair(a.q + (size_t)(run.r0 + i0 + r) * a.ldq + h * 64 + 2 * lane, wide & 1, x[k][0], x[k][1]);
             }
+            int most = 0;
+#pragma unroll
+            for (int k = 0; k < SM_ROWS / SM_WARPS; k++) {
+                const int r = wid + k * SM_WARPS;
+                const int u = query_bytes(x[k][0], x[k][1], S.q[r][lane]);
+                if (lane == 0) S.u[r] = u;
+                most = max(most, u);
+            }
+            if (lane == 0) atomicMax(&S.umax, most);
         }
         __syncthreads();
         // this lane's rows and their A operands: [plane][half][even row g, even g + 8, odd g, odd g + 8]
@@ -463,10 +520,10 @@ __global__ void __launch_bounds__(SM_THREADS, 2) k_store_attend_many(StoreAttend
 #pragma unroll
             for (int y = 0; y < 2; y++) {
                 const uint32_t* w = &S.q[y ? rb : ra][16 * x + 4 * j];
-                const uint32_t t0 = __byte_perm(w[0], w[1], 0x6240), t1 = __byte_perm(w[2], w[3], 0x6240);   // hi: even, even, odd, odd
+                const uint32_t h0 = __byte_perm(w[0], w[1], 0x6240), h1 = __byte_perm(w[2], w[3], 0x6240);   // hi: even, even, odd, odd
                 const uint32_t l0 = __byte_perm(w[0], w[1], 0x7351), l1 = __byte_perm(w[2], w[3], 0x7351);   // lo
-                q[0][x][y] = __byte_perm(t0, t1, 0x5410);
-                q[0][x][2 + y] = __byte_perm(t0, t1, 0x7632);
+                q[0][x][y] = __byte_perm(h0, h1, 0x5410);
+                q[0][x][2 + y] = __byte_perm(h0, h1, 0x7632);
                 q[1][x][y] = __byte_perm(l0, l1, 0x5410);
                 q[1][x][2 + y] = __byte_perm(l0, l1, 0x7632);
             }
@@ -475,27 +532,6 @@ __global__ void __launch_bounds__(SM_THREADS, 2) k_store_attend_many(StoreAttend
         const int la = max(from, pa - win + 1), lb = max(from, pb - win + 1);
         const int w_p0 = min(p_first + pair * 16, p_last), w_p1 = min(p_first + pair * 16 + 15, p_last);
         const int w_l0 = max(from, w_p0 - win + 1), w_l1 = max(from, w_p1 - win + 1);
-        const int k0 = k_lo & ~31, k1 = (p_last | 31) + 1, all = (k1 - k0 + KEYS - 1) / KEYS;
-        // this CTA's tiles: t0 .. t1 - 1
-        const int per = CS > 1 ? (all + CS - 1) / CS : all, t0 = rank * per, t1 = min(all, t0 + per);
-        const size_t base = kv_index(s, a.layer, h, 0, a.st.L, H, a.st.ctx);
-
-        // ---- a tile on its way: copied as it is, then unpacked. A warp takes 8 keys, and byte b of the words of 32 values
-        // (dims 8g + 2b, 8g + 2b + 1); positions from k1 on are neither copied nor used
-        auto fetch = [&](int t, bool values) {
-            const int kt = k0 + t * KEYS;
-            SmRaw& R = S.raw[t & 1];
-            if (t < t1) {
-                const int key = (tid & 127) >> 1, off = (tid & 1) * 16;
-                if (kt + key < k1) {
-                    if (tid < 128) copy16(&R.k[key][off], a.st.k + (base + kt + key) * 32 + off);
-                    else if (values) copy16(&R.v[key][off], a.st.v + (base + kt + key) * 32 + off);
-                }
-                if (tid < 8 && kt + tid * 8 < k1) copy16(&R.ks[tid * 8][0], a.st.ks + (base + kt + tid * 8) * 2);
-                if (tid >= 128 && tid < 132 && kt + (tid - 128) * 16 < k1) copy16(&R.vs[(tid - 128) * 16], a.st.vs + base + kt + (tid - 128) * 16);
-            }
-            asm volatile("cp.async.commit_group;" ::: "memory");
-        };
         auto arrived = [&]() { asm volatile("cp.async.wait_group 0;" ::: "memory"); };   // a barrier makes it everybody's
         auto put = [&](int t, bool values) {
             const SmRaw& R = S.raw[t & 1];
@@ -503,7 +539,8 @@ __global__ void __launch_bounds__(SM_THREADS, 2) k_store_attend_many(StoreAttend
             {
                 const int kl = wid * 8 + g;
                 const uint2 w = *reinterpret_cast<const uint2*>(&R.k[kl][8 * j]);
-                const int s0 = R.ks[kl][0], s1 = R.ks[kl][1], big = max(s0, s1);
+                const int both = *reinterpret_cast<const int16_t*>(&R.ks[kl][0]);
+                const int s0 = (int8_t)both, s1 = both >> 8, big = max(s0, s1);
                 const int up0 = s0 - big + 3, up1 = s1 - big + 3;
                 const uint32_t less0 = 0x80808080u - (0x08080808u << up0), less1 = 0x80808080u - (0x08080808u << up1);
                 T.k[wid][lane] = make_uint4(even_up(w.x, up0, less0), odd_up(w.x, up0, less0), even_up(w.y, up1, less1), odd_up(w.y, up1, less1));
@@ -562,17 +599,19 @@ __global__ void __launch_bounds__(SM_THREADS, 2) k_store_attend_many(StoreAttend
                 }
             }
         };
-        // a pass over the CTA's tiles: tile t in the works, t + 1 unpacked, t + 2 on its way
+        // a pass over the CTA's tiles: tile t in the works, t + 1 unpacked, t + 2 on its way; its first two are already
         auto pass = [&](bool values, auto work) {
-            fetch(t0, values);
             arrived();
             __syncthreads();
-            fetch(t0 + 1, values);
             if (t0 < t1) put(t0, values);
-            arrived();
             __syncthreads();
             for (int t = t0; t < t1; t++) {
-                fetch(t + 2, values);
+                if (t + 2 < t1) {
+                    fetch(t + 2, values);
+                } else if (!values && t + 1 == t1) {   // both buffers are free: the next pass's first tiles
+                    fetch(t0, true);
+                    fetch(t0 + 1, true);
+                }
                 work(S.tile[t & 1], k0 + t * KEYS);
                 if (t + 1 < t1) put(t + 1, values);
                 arrived();
@@ -592,7 +631,11 @@ __global__ void __launch_bounds__(SM_THREADS, 2) k_store_attend_many(StoreAttend
         };
         pass1(std::false_type());
         const bool slow = S.slow;         // some key's score shifts up (or not down): all again with the general form
-        if (slow) pass1(std::true_type());
+        if (slow) {
+            fetch(t0, false);             // (the second pass's tiles are fetched again after it)
+            fetch(t0 + 1, false);
+            pass1(std::true_type());
+        }
         mw = __reduce_max_sync(0xffffffffu, mw);
         ma = max(ma, mw);
         mb = max(mb, mw);
@@ -609,10 +652,9 @@ __global__ void __launch_bounds__(SM_THREADS, 2) k_store_attend_many(StoreAttend
             atomicMax(&S.ym[ra].y, ma);
             atomicMax(&S.ym[rb].y, mb);
         }
-        if (CS > 1) {
+        if (cs > 1) {
             cluster_sync();
-#pragma unroll
-            for (int k = 0; k < CS; k++) {
+            for (int k = 0; k < cs; k++) {
                 const int64_t oa = ld_dsmem(mapa(saddr(&S.ym[ra]), (uint32_t)k)), ob = ld_dsmem(mapa(saddr(&S.ym[rb]), (uint32_t)k));
                 ya = max(ya, (int32_t)oa);
                 yb = max(yb, (int32_t)ob);
@@ -625,6 +667,12 @@ __global__ void __launch_bounds__(SM_THREADS, 2) k_store_attend_many(StoreAttend
             yb = S.ym[rb].x;
             ma = S.ym[ra].y;
             mb = S.ym[rb].y;
+        }
+        // the next item's queries into L2 (a row is four lines)
+        if (item + step < items && n_r0 >= 0 && n_r1 <= a.rw.rows) {
+            const uint32_t nsh = (item + step) / a.rw.n_streams;
+            const int row = n_r0 + (tiles - 1 - (int)(nsh / H)) * ROWS + (tid >> 2);
+            if (row < n_r1) asm volatile("prefetch.global.L2 [%0];" ::"l"(a.q + (size_t)row * a.ldq + (nsh % H) * 64 + (tid & 3) * 16));
         }
         // twice the largest score: a digit below the last rounds up with it
         const uint32_t sa = (uint32_t)(((ya >> 1) + (ya & 1)) * 2), sb = (uint32_t)(((yb >> 1) + (yb & 1)) * 2);
@@ -709,61 +757,67 @@ __global__ void __launch_bounds__(SM_THREADS, 2) k_store_attend_many(StoreAttend
         atomicAdd(&S.z[ra], (unsigned long long)za);
         atomicAdd(&S.z[rb], (unsigned long long)zb);
         // a lane's 8 sums of each of its rows; a cluster's CTAs lay theirs out (in place of the tiles) a row at a time and
-        // each finishes 8 / CS of them
+        // each finishes some of them
         int64_t* const part = reinterpret_cast<int64_t*>(S.tile);     // [warp][8][32 lanes]
         auto sum = [&](int c, int t, int y) {
-            return (int64_t)acc[0][t][2 * y + c] + ((int64_t)acc[1][t][2 * y + c] << 8) + ((int64_t)acc[2][t][2 * y + c] << 16);
+            return (int64_t)acc[0][t][2 * y + c] + (int64_t)acc[1][t][2 * y + c] * 256 + (int64_t)acc[2][t][2 * y + c] * 65536;
         };
-        __syncthreads();                                              // the tiles are done with, S.z is complete
+        if (cs > 1) cluster_sync();                                   // the tiles are done with, S.z is complete
+        else __syncthreads();
+        uint32_t e[2];
+        int sh[2];
+#pragma unroll
+        for (int y = 0; y < 2; y++) {
+            int64_t z = 0;
+            for (int k = 0; k < cs; k++) z += cs > 1 ? ld_dsmem(mapa(saddr(&S.z[y ? rb : ra]), (uint32_t)k)) : (int64_t)S.z[y ? rb : ra];
+            const bool none = (y ? lb > pb : la > pa) || z == 0;
+            const int64_t F = 65536ll * ((y ? mb : ma) + STORE_W_SHIFT) - log2fix(none ? 1 : z, a.LOG2);
+            e[y] = none ? 0 : (uint32_t)__ldg(a.EXP2 + (F & 0xFFFF));
+            sh[y] = 19 - (int)(F >> 16);                              // less one, and 4 digits more: the tiles hold 16 c
+        }
 #pragma unroll
         for (int y = 0; y < 2; y++) {
             const int r = y ? rb : ra;
-            if (CS > 1) {
+            if (cs > 1) {
 #pragma unroll
                 for (int x = 0; x < 8; x++) part[(wid * 8 + x) * 32 + lane] = sum(x >> 2, x & 3, y);
                 cluster_sync();
             }
-            int64_t z = CS > 1 ? 0 : (int64_t)S.z[r];
-            if (CS > 1)
-#pragma unroll
-                for (int k = 0; k < CS; k++) z += ld_dsmem(mapa(saddr(&S.z[r]), (uint32_t)k));
-            const bool none = (y ? lb > pb : la > pa) || z == 0;
-            const int64_t F = 65536ll * ((y ? mb : ma) + STORE_W_SHIFT) - log2fix(none ? 1 : z, a.LOG2);
-            const int32_t e = none ? 0 : __ldg(a.EXP2 + (F & 0xFFFF));
-            const int64_t sh = 20 - (F >> 16);                        // the tiles hold 16 c: 4 digits more
-            uint64_t any = 0;
             int64_t* const out = a.out + ((size_t)(run.r0 + i0 + r) * H + h) * 64 + 16 * j + 4 * (wid & 1);
             // columns 2j, 2j + 1 of tile t: dims 16j + t, 16j + 8 + t
+            int64_t o[8];
 #pragma unroll
-            for (int x = 0; x < 8; x += 2) {
-                if (CS > 1 && x / (8 / CS) != rank) continue;
-                int64_t o[2];
+            for (int x = 0; x < 8; x++) {
+                if (cs > 1 && (x >> 1) % cs != rank) continue;
+                int64_t num = cs > 1 ? 0 : sum(x >> 2, x & 3, y);
+                if (cs > 1)
+                    for (int m = 0; m < cs; m++) num += ld_dsmem(mapa(saddr(&part[(wid * 8 + x) * 32 + lane]), (uint32_t)m));
+                num *= (int64_t)e[y];                                  // at most 2^46 2^17
+                o[x] = sh[y] >= 0 ? ((num >> sh[y]) + 1) >> 1 : (int64_t)((uint64_t)num << (-1 - sh[y]));
+            }
+            if (r < nr) {
 #pragma unroll
-                for (int k = 0; k < 2; k++) {
-                    int64_t num = CS > 1 ? 0 : sum(x >> 2, (x + k) & 3, y);
-                    if (CS > 1)
-#pragma unroll
-                        for (int m = 0; m < CS; m++) num += ld_dsmem(mapa(saddr(&part[(wid * 8 + x + k) * 32 + lane]), (uint32_t)m));
-                    num *= e;                                          // at most 2^46 2^17
-                    o[k] = sh > 0 ? ((num >> (sh - 1)) + 1) >> 1 : (int64_t)((uint64_t)num << -sh);
-                    any |= mag(o[k]);
-                }
-                if (r < nr) {
+                for (int x = 0; x < 8; x += 2) {
+                    if (cs > 1 && (x >> 1) % cs != rank) continue;
                     int64_t* const to = out + 8 * (x >> 2) + (x & 3);
                     if (wide & 2) {
-                        *reinterpret_cast<longlong2*>(to) = make_longlong2(o[0], o[1]);
+                        *reinterpret_cast<longlong2*>(to) = make_longlong2(o[x], o[x + 1]);
                     } else {
-                        to[0] = o[0];
-                        to[1] = o[1];
+                        to[0] = o[x];
+                        to[1] = o[x + 1];
                     }
                 }
             }
             if (a.or_out) {
+                uint64_t any = 0;
+#pragma unroll
+                for (int x = 0; x < 8; x++)
+                    if (cs == 1 || (x >> 1) % cs == rank) any |= mag(o[x]);
                 any |= __shfl_xor_sync(0xffffffffu, any, 1);
                 any |= __shfl_xor_sync(0xffffffffu, any, 2);
                 if (j == 0 && r < nr) atomicOr((unsigned long long*)&a.or_out[run.r0 + i0 + r], (unsigned long long)any);
             }
-            if (CS > 1) cluster_sync();                                // the others have read this CTA's sums
+            if (cs > 1) cluster_sync();                                // the others have read this CTA's sums
         }
     }
 }
@@ -811,19 +865,43 @@ cudaError_t store_read(const Store4& st, const StoreRows& rw, int layer, int64_t
     return store_launch(how, k_store_read, grid, SW_WARPS * 32, 0, 1, st, rw, layer, k, v, wide, err);
 }
 
-constexpr int SM_FROM_ROWS = 4;
+constexpr int SM_FROM_ROWS = 4, SM_FIXED = 4;
 constexpr int SM_SMEM_MOST = 200 * 1024;
 constexpr int SF_MOST_KEYS = 8192;   // of a CTA: 64 KB of shared memory
 
-cudaError_t store_init() {
-    cudaError_t e = cudaFuncSetAttribute(k_store_attend_few<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, SF_MOST_KEYS * SF_BYTES);
+size_t many_smem(int alen) { return sizeof(SmShared) + (size_t)(alen + 1) * 4; }
+
+cudaError_t store_init(int alen, StorePlan& plan) {
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&plan.sms, cudaDevAttrMultiProcessorCount, device);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(k_store_attend_few<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, SF_MOST_KEYS * SF_BYTES);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(k_store_attend_few<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, SF_MOST_KEYS * SF_BYTES);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(k_store_attend_few<4>, cudaFuncAttributeMaxDynamicSharedMemorySize, SF_MOST_KEYS * SF_BYTES);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(k_store_attend_few<8>, cudaFuncAttributeMaxDynamicSharedMemorySize, SF_MOST_KEYS * SF_BYTES);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(k_store_attend_many<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, SM_SMEM_MOST);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(k_store_attend_many<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, SM_SMEM_MOST);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(k_store_attend_many<4>, cudaFuncAttributeMaxDynamicSharedMemorySize, SM_SMEM_MOST);
-    return e;
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(k_store_attend_many, cudaFuncAttributeMaxDynamicSharedMemorySize, SM_SMEM_MOST);
+    if (e != cudaSuccess) return e;
+    int fit = 0;
+    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, k_store_attend_many, SM_THREADS, many_smem(alen));
+    if (e != cudaSuccess) return e;
+    plan.many[1] = fit * plan.sms;
+    for (int cs = 2; cs <= STORE_MAX_CLUSTER; cs++) {
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(cs);
+        cfg.blockDim = dim3(SM_THREADS);
+        cfg.dynamicSmemBytes = many_smem(alen);
+        cudaLaunchAttribute at[1];
+        at[0].id = cudaLaunchAttributeClusterDimension;
+        at[0].val.clusterDim.x = cs;
+        at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+        cfg.attrs = at;
+        cfg.numAttrs = 1;
+        if (cudaOccupancyMaxActiveClusters(&plan.many[cs], k_store_attend_many, &cfg) != cudaSuccess) {
+            plan.many[cs] = 0;
+            cudaGetLastError();
+        }
+    }
+    return cudaSuccess;
 }
 
 cudaError_t store_attend(const StoreAttend& a, StoreLaunch how) {
@@ -832,22 +910,31 @@ cudaError_t store_attend(const StoreAttend& a, StoreLaunch how) {
     const int64_t items = (int64_t)((a.rw.max_rows + SM_ROWS - 1) / SM_ROWS) * a.st.H * a.rw.n_streams;
     if (a.rw.max_rows > SM_FROM_ROWS && items < INT32_MAX) {
         const int tiles = (a.rw.max_rows + SM_ROWS - 1) / SM_ROWS;
-        const size_t smem = sizeof(SmShared) + (size_t)(a.alen + 1) * 4;
+        const size_t smem = many_smem(a.alen);
+        // fewer items than the GPU holds: their keys split over clusters, in two tiles a CTA at least, by the time that a
+        // split would take (waves x tiles a CTA, an item's start and end counted as SM_FIXED tiles)
+        const int keys = a.window > 0 ? std::min(a.st.lim, std::min(a.window, a.st.lim) + SM_ROWS) : a.st.lim;
+        const int all = (keys + SM_KEYS - 1) / SM_KEYS;
         int cs = 1;
-        while (cs < 4 && items * cs * 2 <= how.sms * 2) cs *= 2;
-        const dim3 grid((unsigned)(std::min<int64_t>(items, how.sms * 2 / cs) * cs));
-        switch (cs) {
-            case 1: return store_launch(how, k_store_attend_many<1>, grid, SM_THREADS, smem, 1, a, tiles, wide);
-            case 2: return store_launch(how, k_store_attend_many<2>, grid, SM_THREADS, smem, 2, a, tiles, wide);
-            default: return store_launch(how, k_store_attend_many<4>, grid, SM_THREADS, smem, 4, a, tiles, wide);
+        int64_t least = INT64_MAX;
+        for (int k = 1; k <= STORE_MAX_CLUSTER && (k == 1 || k * 2 <= all); k++) {
+            const int fit = how.plan->many[k];
+            if (fit < 1) continue;
+            const int64_t t = (items + fit - 1) / fit * ((all + k - 1) / k + SM_FIXED);
+            if (t < least) {
+                least = t;
+                cs = k;
+            }
         }
+        const dim3 grid((unsigned)(std::min<int64_t>(items, std::max(how.plan->many[cs], 1)) * cs));
+        return store_launch(how, k_store_attend_many, grid, SM_THREADS, smem, cs, a, tiles, cs, wide);
     }
     // blocks of 32 positions that a row may see
     int blocks = (a.st.lim + 31) / 32;
     if (a.window > 0 && a.window < a.st.lim) blocks = std::min(blocks, (a.window + 30) / 32 + 1);
     const int64_t units = (int64_t)a.rw.n_streams * a.rw.max_rows * a.st.H;
     int cs = 1;
-    while (cs < 8 && ((units * cs < how.sms * 2 && blocks >= cs * 8) || blocks * 32 > cs * SF_MOST_KEYS)) cs *= 2;
+    while (cs < 8 && ((units * cs < how.plan->sms * 2 && blocks >= cs * 8) || blocks * 32 > cs * SF_MOST_KEYS)) cs *= 2;
     const int chunk = (blocks + cs - 1) / cs * 32;
     const dim3 grid(a.rw.max_rows * cs, a.st.H, a.rw.n_streams);
     const size_t smem = (size_t)chunk * SF_BYTES;
@@ -872,7 +959,8 @@ struct b2_store {
     std::string err;
     Store4 st{};
     int32_t *ARR = nullptr, *LOG2 = nullptr, *EXP2 = nullptr;
-    int alen = 0, sms = 148;
+    int alen = 0;
+    StorePlan plan;
     uint32_t* d_err = nullptr;
     std::vector<void*> allocs;
 };
@@ -940,8 +1028,7 @@ void store_release(b2_store* h) {
 
 int store_build(b2_store* h, const int64_t* arrival, int64_t n_arrival, const int64_t* log2, const int64_t* exp2) {
     const b2_store_config& c = h->cfg;
-    SCK(store_init());
-    SCK(cudaDeviceGetAttribute(&h->sms, cudaDevAttrMultiProcessorCount, h->device));
+    SCK(store_init((int)n_arrival, h->plan));
     if (arrival[0] < 1) return sfail(h, B2_ERR_VALUE, "b2_store_create: arrival[0] = %lld (at least 1)", (long long)arrival[0]);
     // one piece for the error words and the tables, one for the store
     std::vector<int32_t> t(4, 0);
@@ -1035,7 +1122,7 @@ int b2_store_write(b2_store* h, int32_t layer, const int64_t* k, int64_t ldk, co
         OnDevice on(h->device);
         SCK(on.e);
         SCK(store_write(h->st, StoreRows{cu, pos, n_streams, rows, max_rows}, layer, k, ldk, v, ldv, h->d_err,
-                        StoreLaunch{(cudaStream_t)stream, false, h->sms}));
+                        StoreLaunch{(cudaStream_t)stream, false, &h->plan}));
         return (int)B2_OK;
     });
 }
@@ -1050,7 +1137,7 @@ int b2_store_read(b2_store* h, int32_t layer, const int32_t* cu, const int32_t* 
         OnDevice on(h->device);
         SCK(on.e);
         SCK(store_read(h->st, StoreRows{cu, pos, n_streams, rows, max_rows}, layer, k, v, h->d_err,
-                       StoreLaunch{(cudaStream_t)stream, false, h->sms}));
+                       StoreLaunch{(cudaStream_t)stream, false, &h->plan}));
         return (int)B2_OK;
     });
 }
@@ -1069,7 +1156,7 @@ int b2_store_attend(b2_store* h, int32_t layer, const int64_t* q, int64_t ldq, c
         SCK(on.e);
         StoreAttend a{h->st, StoreRows{cu, pos, n_streams, rows, max_rows}, layer, q, ldq, first, window, h->ARR, h->alen,
                       h->LOG2, h->EXP2, out, nullptr, h->d_err};
-        SCK(store_attend(a, StoreLaunch{(cudaStream_t)stream, false, h->sms}));
+        SCK(store_attend(a, StoreLaunch{(cudaStream_t)stream, false, &h->plan}));
         return (int)B2_OK;
     });
 }

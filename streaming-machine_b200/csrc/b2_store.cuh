@@ -51,14 +51,20 @@ struct StoreAttend {
     uint32_t* err;
 };
 
+// what the launches are sized by, once per device (the current one) and arrival table; to be called before the first launch
+constexpr int STORE_MAX_CLUSTER = 8;
+struct StorePlan {
+    int sms = 0;                               // the device's SM count
+    int many[STORE_MAX_CLUSTER + 1] = {0};     // clusters of 1 .. 8 CTAs of the many-row arrival that fit at once (0: none)
+};
+cudaError_t store_init(int alen, StorePlan& plan);
+
 // how the launches below are made: on `stream`, as programmatic dependent launches where pdl is set
 struct StoreLaunch {
     cudaStream_t stream;
     bool pdl;
-    int sms;           // the device's SM count
+    const StorePlan* plan;
 };
-
-cudaError_t store_init();   // once per device (current), before the first launch there
 
 cudaError_t store_write(const Store4& st, const StoreRows& rw, int layer, const int64_t* k, int64_t ldk, const int64_t* v,
                         int64_t ldv, uint32_t* err, StoreLaunch how);
@@ -110,26 +116,27 @@ B2_DEV int32_t store_score(int32_t dot, int r) {
     return (int32_t)((uint32_t)dot << (up & 31));
 }
 
-// the rows of stream s; false: nothing to do (no rows, or an inconsistent table, which is flagged)
+// the rows of a stream by its entries of the row table; false: nothing to do (no rows, or an entry that does not fit the
+// call, which is flagged)
 struct StoreRun { int r0, n, p0; };
-B2_DEV bool store_run(const StoreRows& w, int s, int lim, StoreRun& run, uint32_t* err) {
-    const int r0 = w.cu ? w.cu[s] : s, r1 = w.cu ? w.cu[s + 1] : s + 1;
+B2_DEV bool store_run(const StoreRows& w, int r0, int r1, int p0, int lim, StoreRun& run, uint32_t* err) {
     run.r0 = r0;
     run.n = 0;
-    run.p0 = 0;
+    run.p0 = p0;
     if (r0 < 0 || r1 < r0 || r1 > w.rows || r1 - r0 > w.max_rows) {
         set_err(err, DERR_ROWS);
         return false;
     }
     if (r1 == r0) return false;
-    const int p0 = w.pos[s];
     if (p0 < 0 || p0 > lim - (r1 - r0)) {
         set_err(err, DERR_POS);
         return false;
     }
     run.n = r1 - r0;
-    run.p0 = p0;
     return true;
+}
+B2_DEV bool store_run(const StoreRows& w, int s, int lim, StoreRun& run, uint32_t* err) {
+    return store_run(w, w.cu ? w.cu[s] : s, w.cu ? w.cu[s + 1] : s + 1, w.pos[s], lim, run, err);
 }
 #endif
 
