@@ -93,7 +93,10 @@ int b2_set_array(b2_handle* h, const char* name, const int64_t* data, int64_t n)
  * base2_layer0.py, base2_stream_fr2.swift:407-428): 1 makes every decode step take layer 0's qkv piles from two stored
  * rows, wte . W and wpe . W of the qkv.0 bank (built as exact int64 piles at the next b2_alloc_streams, 0.95 GB for
  * GPT-2 124M), instead of the bank product: the same bits, refused (B2_ERR_ARG) when an embedded value can reach 2^15,
- * where to16 would round the row; 0 (default) drops them. */
+ * where to16 would round the row; 0 (default) drops them. "store_bits": 4 makes the next b2_alloc_streams hold the
+ * streams' keys and values in 4 bits (67 bytes a position and head in place of 396; b2_store_* below says what is held and
+ * how the arrival reads it; Pythia's turn comes before it), 16 (default) as the reference does; 4 is refused with a float
+ * arrival or turn, with "entry_tables", and for tables that b2_store_create would refuse. */
 int b2_set_scalar(b2_handle* h, const char* name, int64_t v);
 
 /* All arrays given: build the device layouts. */

@@ -9,6 +9,7 @@
 #include <stdio.h>
 #include <string.h>
 
+#include <algorithm>
 #include <cmath>
 #include <mutex>
 #include <string>
@@ -16,6 +17,7 @@
 
 #include "../../include/base2.h"
 #include "b2_kernels.cuh"
+#include "b2_store.cuh"
 #include "b2_tc.cuh"
 
 using namespace b2;
@@ -66,6 +68,15 @@ struct b2_handle {
     // stream slots + key/value store
     int n_slots = 0, max_ctx = 0;
     KV kv{};
+    // "store_bits" 4: the key/value store held in 4 bits (kv's arrays stay empty); the rows of the pass under way as the
+    // store's kernels take them, and the streams' tables of a prompt-pass chunk
+    int store_bits = 16, store_want = 16;   // of the allocated streams; of the next b2_alloc_streams
+    int tables4_bad = 0;                    // bits: a table (arrival, log2, exp2) outside what those kernels take
+    Store4 st4{};
+    StorePlan plan4;
+    StoreRows rows4{};
+    uint8_t* mem4 = nullptr;
+    int32_t *cu4 = nullptr, *pos4 = nullptr;
     int32_t *slot_len = nullptr, *slot_tok = nullptr;
     bool primed = false;
 
@@ -429,6 +440,31 @@ int run_attend(b2_handle* h, int rows, int l, uint64_t* or_out, cudaStream_t st,
               : launch(h, B2_PROF_ATTEND, "attend", k_attend<4, false>, grid, 128, sm, st, aa);
 }
 
+// "store_bits" 4, after layer l's qkv bank (q, k, v in QKV's rows): (Pythia's turn,) the rows' keys and values into the
+// 4-bit store, then the arrival over it
+int run_store4(b2_handle* h, int rows, int l, uint64_t* or_out, cudaStream_t st) {
+    const int d = h->cfg.d_model;
+    const bool py = h->cfg.kind == B2_PYTHIA;
+    const int hs = py ? 192 : 64;                       // Pythia's columns are per head q, k, v
+    const StoreLaunch how{st, h->pdl && h->prof.timing != 1, &h->plan4};
+    int rc;
+    if (py && (rc = launch(h, B2_PROF_HEADS, "turn", k_turn, rows, 256, 0, st, h->QKV, rows, (const int32_t*)h->row_pos,
+                           h->cfg.n_head, h->st4.lim, (const int32_t*)h->COS, (const int32_t*)h->SIN, h->d_err)))
+        return rc;
+    prof_begin(h, B2_PROF_HEADS, st);
+    cudaError_t e = store_write(h->st4, h->rows4, l, StoreVec{h->QKV + (py ? 64 : d), 3 * d, hs},
+                                StoreVec{h->QKV + (py ? 128 : 2 * d), 3 * d, hs}, h->d_err, how, stamp_slot(h, B2_PROF_HEADS));
+    prof_end(h, B2_PROF_HEADS, st);
+    if (e != cudaSuccess) return fail(h, B2_ERR_CUDA, "launch store_write: %s", cudaGetErrorString(e));
+    StoreAttend a{h->st4, h->rows4, l, StoreVec{h->QKV, 3 * d, hs}, nullptr, 0, h->ARR, h->alen, h->LOG2, h->EXP2, h->ATT,
+                  or_out, h->d_err, stamp_slot(h, B2_PROF_ATTEND)};
+    prof_begin(h, B2_PROF_ATTEND, st);
+    e = store_attend(a, how);
+    prof_end(h, B2_PROF_ATTEND, st);
+    if (e != cudaSuccess) return fail(h, B2_ERR_CUDA, "launch store_attend: %s", cudaGetErrorString(e));
+    return B2_OK;
+}
+
 // Pythia's layer norm (pythia_base2.py:100-110) of rows of X (gathered by src_rows when given) into out [rows][d]
 int run_gauge(b2_handle* h, const int64_t* X, const int32_t* src_rows, int rows, int ni, int64_t* out, cudaStream_t st,
               uint64_t* or_out = nullptr, int ni2 = -1, int64_t* out2 = nullptr, uint64_t* or_out2 = nullptr) {
@@ -461,12 +497,16 @@ int run_rows_pythia(b2_handle* h, int rows, const int32_t* hrows, const int32_t*
         if ((rc = run_gauge(h, h->R, nullptr, rows, 2 * l, h->ATT, st))) return rc;
         if ((rc = run_quant(h, h->ATT, d, nullptr, rows, 0, st))) return rc;
         if ((rc = run_bank(h, 4 * l + 0, EPI_PLAIN_OUT, rows, h->QKV, 3 * d, nullptr, st))) return rc;
-        if ((rc = launch(h, B2_PROF_HEADS, "heads_pythia", k_heads_pythia, dim3(rows, 3 * H), 32, 0, st,
-                         (const int64_t*)h->QKV, rows, (const int32_t*)h->row_slot, (const int32_t*)h->row_pos, l, h->kv,
-                         (int)h->rot, (const int32_t*)h->COS, (const int32_t*)h->SIN, h->q16, h->qexp, h->d_err,
-                         (const double*)h->cosf, (const double*)h->sinf, h->qraw, stamp_slot(h, B2_PROF_HEADS))))
-            return rc;
-        if ((rc = run_attend(h, rows, l, nullptr, st, nblocks))) return rc;
+        if (h->store_bits == 4) {
+            if ((rc = run_store4(h, rows, l, nullptr, st))) return rc;
+        } else {
+            if ((rc = launch(h, B2_PROF_HEADS, "heads_pythia", k_heads_pythia, dim3(rows, 3 * H), 32, 0, st,
+                             (const int64_t*)h->QKV, rows, (const int32_t*)h->row_slot, (const int32_t*)h->row_pos, l, h->kv,
+                             (int)h->rot, (const int32_t*)h->COS, (const int32_t*)h->SIN, h->q16, h->qexp, h->d_err,
+                             (const double*)h->cosf, (const double*)h->sinf, h->qraw, stamp_slot(h, B2_PROF_HEADS))))
+                return rc;
+            if ((rc = run_attend(h, rows, l, nullptr, st, nblocks))) return rc;
+        }
         if ((rc = run_gauge(h, h->R, nullptr, rows, 2 * l + 1, h->HID, st))) return rc;
         if ((rc = run_quant(h, h->HID, d, nullptr, rows, 0, st))) return rc;
         if ((rc = run_bank(h, 4 * l + 2, EPI_PLAIN_EDGE, rows, h->HID, F, nullptr, st))) return rc;
@@ -499,15 +539,19 @@ int run_rows(b2_handle* h, int rows, const int32_t* hrows, const int32_t* hmap, 
         // which also needs the keys at full width)
         const TcHeads hd{h->q16, h->qexp, h->kv, h->row_slot, h->row_pos, l};
         bool heads_done = false;
-        const bool want_heads = h->fuse_heads && !(h->flags & B2_ARRIVAL_FLOAT);
+        const bool want_heads = h->fuse_heads && !(h->flags & B2_ARRIVAL_FLOAT) && h->store_bits != 4;
         if ((rc = run_bank(h, 4 * l + 0, EPI_GAUGED, rows, h->QKV, 3 * d, nullptr, st, want_heads ? &hd : nullptr,
                            &heads_done)))
             return rc;
-        if (!heads_done &&
-            (rc = launch(h, B2_PROF_HEADS, "heads", k_heads, dim3(rows, 3 * H), 32, 0, st, h->QKV, rows, h->row_slot,
-                         h->row_pos, l, h->kv, h->q16, h->qexp, h->d_err)))
-            return rc;
-        if ((rc = run_attend(h, rows, l, nullptr, st, nblocks))) return rc;
+        if (h->store_bits == 4) {
+            if ((rc = run_store4(h, rows, l, nullptr, st))) return rc;
+        } else {
+            if (!heads_done &&
+                (rc = launch(h, B2_PROF_HEADS, "heads", k_heads, dim3(rows, 3 * H), 32, 0, st, h->QKV, rows, h->row_slot,
+                             h->row_pos, l, h->kv, h->q16, h->qexp, h->d_err)))
+                return rc;
+            if ((rc = run_attend(h, rows, l, nullptr, st, nblocks))) return rc;
+        }
         if ((rc = run_quant(h, h->ATT, d, nullptr, rows, 0, st))) return rc;
         if ((rc = run_bank(h, 4 * l + 1, EPI_PLAIN_ADD, rows, h->R, d, nullptr, st))) return rc;
         if ((rc = run_quant(h, h->R, d, nullptr, rows, 1, st))) return rc;
@@ -624,11 +668,16 @@ int run_decode_wq(b2_handle* h, int n, cudaStream_t st) {
             prof_end(h, B2_PROF_BANK, st);
             if (rc) return fail(h, B2_ERR_CUDA, "entry qkv: %s", cudaGetErrorString((cudaError_t)rc));
             heads_done = true;
-        } else if ((rc = run_bank(h, 4 * l, EPI_GAUGED, n, h->QKV, 3 * d, nullptr, st, &hd, &heads_done, &q))) {
+        } else if ((rc = run_bank(h, 4 * l, EPI_GAUGED, n, h->QKV, 3 * d, nullptr, st, h->store_bits == 4 ? nullptr : &hd,
+                                  &heads_done, &q))) {
             return rc;
         }
-        if (!heads_done) return fail(h, B2_ERR_STATE, "qkv bank %d: heads16 not done in its epilogue", l);
-        if ((rc = run_attend(h, n, l, o0 + FUSED_ROWS, st, 0, true))) return rc;
+        if (h->store_bits == 4) {
+            if ((rc = run_store4(h, n, l, o0 + FUSED_ROWS, st))) return rc;
+        } else {
+            if (!heads_done) return fail(h, B2_ERR_STATE, "qkv bank %d: heads16 not done in its epilogue", l);
+            if ((rc = run_attend(h, n, l, o0 + FUSED_ROWS, st, 0, true))) return rc;
+        }
         q = wq_args(h, 4 * l + 1, h->ATT, d, o0 + FUSED_ROWS);
         if ((rc = run_bank(h, 4 * l + 1, EPI_PLAIN_ADD, n, h->R, d, nullptr, st, nullptr, nullptr, &q, o0 + 2 * FUSED_ROWS)))
             return rc;
@@ -677,16 +726,17 @@ int run_decode_wq_pythia(b2_handle* h, int n, cudaStream_t st) {
         hd.COS = h->COS;
         hd.SIN = h->SIN;
         bool heads_done = false;
-        if ((rc = run_bank(h, 4 * l + 0, EPI_PLAIN_OUT, n, h->QKV, 3 * d, nullptr, st, h->fuse_heads ? &hd : nullptr,
+        const bool four = h->store_bits == 4;
+        if ((rc = run_bank(h, 4 * l + 0, EPI_PLAIN_OUT, n, h->QKV, 3 * d, nullptr, st, h->fuse_heads && !four ? &hd : nullptr,
                            &heads_done, &q)))
             return rc;
-        if (!heads_done &&
+        if (!four && !heads_done &&
             (rc = launch(h, B2_PROF_HEADS, "heads_pythia", k_heads_pythia, dim3(n, 3 * H), 32, 0, st,
                          (const int64_t*)h->QKV, n, (const int32_t*)h->row_slot, (const int32_t*)h->row_pos, l, h->kv,
                          (int)h->rot, (const int32_t*)h->COS, (const int32_t*)h->SIN, h->q16, h->qexp, h->d_err,
                          (const double*)nullptr, (const double*)nullptr, (int64_t*)nullptr, stamp_slot(h, B2_PROF_HEADS))))
             return rc;
-        if ((rc = run_attend(h, n, l, o0 + FUSED_ROWS, st, 0, true))) return rc;
+        if ((rc = four ? run_store4(h, n, l, o0 + FUSED_ROWS, st) : run_attend(h, n, l, o0 + FUSED_ROWS, st, 0, true))) return rc;
         // MLP branch from the same R: fc + bend -> mproj; then both branches into R (mproj, proj)
         q = wq_args(h, 4 * l + 2, h->G2, d, o0 + 2 * FUSED_ROWS);
         if ((rc = run_bank(h, 4 * l + 2, EPI_PLAIN_EDGE, n, h->HID, F, nullptr, st, nullptr, nullptr, &q,
@@ -753,6 +803,7 @@ int read_device_error(b2_handle* h) {
     if (e & DERR_RANGE)
         return fail(h, B2_ERR_VALUE, "a value passed the range the reference asserts (turn input >= 2^31, a power or the "
                     "arrival's sum past int64; device check, bits 0x%x)", e);
+    if (e & DERR_ROWS) return fail(h, B2_ERR_DEVICE, "a stream's rows did not fit the 4-bit store's call (device check, bits 0x%x)", e);
     return fail(h, B2_ERR_DEVICE, "a token id was out of range (device check, bits 0x%x)", e);
 }
 
@@ -878,6 +929,13 @@ int b2_set_array(b2_handle* h, const char* name, const int64_t* data, int64_t n)
     CK(cudaSetDevice(h->device));
     const b2_config& c = h->cfg;
     int rc;
+    const int t4 = !strcmp(name, "arrival") ? 1 : (!strcmp(name, "log2") ? 2 : (!strcmp(name, "exp2") ? 4 : 0));
+    if (t4) {
+        const int64_t lo = t4 == 4 ? 65536 : 0, hi = t4 == 1 ? STORE_MAX_ARR : (t4 == 2 ? 65536 : 131071);
+        bool ok = t4 != 1 || (n <= STORE_MAX_ALEN && data[0] >= 1);
+        for (int64_t i = 0; i < n && ok; i++) ok = data[i] >= lo && data[i] <= hi;
+        h->tables4_bad = (h->tables4_bad & ~t4) | (ok ? 0 : t4);
+    }
     if (!strcmp(name, "wte") || !strcmp(name, "wpe")) {
         int64_t want = (int64_t)(name[1] == 't' ? c.vocab : c.n_ctx) * c.d_model;
         if (n != want) return fail(h, B2_ERR_ARG, "%s: %lld values, want %lld", name, (long long)n, (long long)want);
@@ -924,9 +982,19 @@ int b2_set_scalar(b2_handle* h, const char* name, int64_t v) {
         drop_graph(h);
         return B2_OK;
     }
+    if (!strcmp(name, "store_bits")) {   // the key/value store of the next b2_alloc_streams: 16 bits or 4
+        if (v != 16 && v != 4) return fail(h, B2_ERR_ARG, "store_bits = %lld (16 or 4)", (long long)v);
+        if (v == 4 && (h->flags & (B2_ARRIVAL_FLOAT | B2_TURN_FLOAT)))
+            return fail(h, B2_ERR_ARG, "store_bits 4: the handle's arrival or turn is in float64");
+        if (v == 4 && h->entry) return fail(h, B2_ERR_ARG, "store_bits 4 and entry_tables exclude one another");
+        h->store_want = (int)v;
+        return B2_OK;
+    }
     if (!strcmp(name, "entry_tables")) {   // GPT-2: layer 0's qkv piles of a decode step from stored rows (0 or 1)
         if ((v != 0 && v != 1) || (v && h->cfg.kind != B2_GPT2))
             return fail(h, B2_ERR_ARG, "entry_tables = %lld (0 or 1, GPT-2 only)", (long long)v);
+        if (v && (h->store_bits == 4 || h->store_want == 4))
+            return fail(h, B2_ERR_ARG, "store_bits 4 and entry_tables exclude one another");
         h->entry = (int)v;
         if (!v) {
             dfree(h, h->entry_w);
@@ -1121,12 +1189,19 @@ int b2_alloc_streams(b2_handle* h, int32_t n_streams, int32_t max_ctx) {
         return fail(h, B2_ERR_ARG, "b2_alloc_streams: n_streams %d, max_ctx %d (model n_ctx %d)", n_streams, max_ctx, h->cfg.n_ctx);
     CK(cudaSetDevice(h->device));
     const b2_config& c = h->cfg;
+    if (h->store_want == 4) {
+        if (max_ctx > STORE_MAX_CTX) return fail(h, B2_ERR_ARG, "store_bits 4: max_ctx %d (at most %d)", max_ctx, STORE_MAX_CTX);
+        if (n_streams > 65535) return fail(h, B2_ERR_ARG, "store_bits 4: n_streams %d (at most 65535)", n_streams);
+        if (h->tables4_bad)
+            return fail(h, B2_ERR_VALUE, "store_bits 4: the arrival table has 1 .. %d entries in [0, %d], the first at least 1, log2's are "
+                        "in [0, 65536], exp2's in [65536, 131071] (bits 0x%x)", STORE_MAX_ALEN, STORE_MAX_ARR, h->tables4_bad);
+    }
     // drop old stream/row buffers
     void* old[] = {h->pf_blocks, h->sigf, h->qraw, h->kv.kraw, h->row_or, h->wq_acc, h->wq_nsat, h->wq_ctr, h->fr_C, h->fr_HIS,
                    h->fr_p5v, h->fr_p5i, h->fr_list, h->fr_cnt, h->fr_sv, h->fr_si, h->G2, h->race_v,
                    h->race_i, h->kv.k, h->kv.kmask, h->kv.kexp, h->kv.v, h->slot_len, h->slot_tok, h->row_slot, h->row_pos,
                    h->row_tok, h->R, h->QKV, h->ATT, h->HID, h->x16, h->ex, h->q16, h->qexp, h->LS, h->head_rows,
-                   h->race_out, h->logits};
+                   h->race_out, h->logits, h->mem4, h->cu4, h->pos4};
     for (void* p : old) dfree(h, p);
     tc_rows_free(h->tcr);
     drop_graph(h);
@@ -1137,15 +1212,31 @@ int b2_alloc_streams(b2_handle* h, int32_t n_streams, int32_t max_ctx) {
     h->qraw = nullptr;
     h->kv.kraw = nullptr;
     h->pf_blocks = nullptr;
+    h->mem4 = nullptr;
+    h->cu4 = h->pos4 = nullptr;
+    h->kv.k = nullptr;
+    h->kv.kmask = nullptr;
+    h->kv.kexp = nullptr;
+    h->kv.v = nullptr;
+    h->st4 = Store4{};
+    h->store_bits = h->store_want;
     const int L = c.n_layer, H = c.n_head, d = c.d_model, F = c.d_ff;
     const int ctx_stride = (max_ctx + 15) / 16 * 16;
     size_t nkv = (size_t)n_streams * L * H * ctx_stride;
     int rc;
     h->kv.L = L; h->kv.H = H; h->kv.ctx = ctx_stride; h->kv.lim = max_ctx;
-    if ((rc = dalloc(h, &h->kv.k, nkv * 64))) return rc;
-    if ((rc = dalloc(h, &h->kv.kmask, nkv))) return rc;
-    if ((rc = dalloc(h, &h->kv.kexp, nkv))) return rc;
-    if ((rc = dalloc(h, &h->kv.v, nkv * 64))) return rc;
+    if (h->store_bits == 4) {
+        CK(store_init(h->alen, h->plan4));
+        const size_t bytes = store_layout(h->st4, n_streams, L, H, max_ctx, nullptr);
+        if ((rc = dalloc(h, &h->mem4, bytes)) || (rc = dalloc(h, &h->cu4, n_streams + 1)) || (rc = dalloc(h, &h->pos4, n_streams))) return rc;
+        store_layout(h->st4, n_streams, L, H, max_ctx, h->mem4);
+        CK(cudaMemset(h->mem4, 0, bytes));
+    } else {
+        if ((rc = dalloc(h, &h->kv.k, nkv * 64))) return rc;
+        if ((rc = dalloc(h, &h->kv.kmask, nkv))) return rc;
+        if ((rc = dalloc(h, &h->kv.kexp, nkv))) return rc;
+        if ((rc = dalloc(h, &h->kv.v, nkv * 64))) return rc;
+    }
     if ((h->flags & B2_ARRIVAL_FLOAT) && (rc = dalloc(h, &h->kv.kraw, nkv * 64))) return rc;
     if ((rc = dalloc(h, &h->row_or, (size_t)4 * L * FUSED_ROWS))) return rc;
     CK(cudaMemset(h->row_or, 0, sizeof(uint64_t) * 4 * L * FUSED_ROWS));
@@ -1260,7 +1351,25 @@ int b2_prefill(b2_handle* h, const int32_t* ids, const int32_t* lens, int32_t n_
             }
             // the arrival's query blocks: runs of up to pf_qb consecutive positions of one stream
             int nblocks = 0;
-            if (h->pf_qb) {
+            if (h->store_bits == 4) {   // the 4-bit store's kernels take the chunk's streams: first rows and positions
+                const int s0 = rs[r0], s1 = rs[r0 + rows - 1];
+                std::vector<int32_t> cu, pos;
+                int most = 0;
+                for (int s = s0, i = 0; s <= s1; s++) {
+                    const int from = i;
+                    cu.push_back(from);
+                    pos.push_back(rp[r0 + from]);
+                    while (i < rows && rs[r0 + i] == s) i++;
+                    most = std::max(most, i - from);
+                }
+                cu.push_back(rows);
+                if (cudaMemcpyAsync(h->cu4, cu.data(), sizeof(int32_t) * cu.size(), cudaMemcpyHostToDevice, st) != cudaSuccess ||
+                    cudaMemcpyAsync(h->pos4, pos.data(), sizeof(int32_t) * pos.size(), cudaMemcpyHostToDevice, st) != cudaSuccess) {
+                    rc = fail(h, B2_ERR_CUDA, "prefill stream table copy");
+                    break;
+                }
+                h->rows4 = StoreRows{h->cu4, h->pos4, (int)pos.size(), rows, most, s0};
+            } else if (h->pf_qb) {
                 std::vector<PrefillBlock> bl;
                 for (int i = 0; i < rows;) {
                     const size_t g = r0 + i;
@@ -1298,6 +1407,7 @@ int b2_prefill(b2_handle* h, const int32_t* ids, const int32_t* lens, int32_t n_
 namespace {
 // one decode step for slots 0..n-1 (row r = slot r); words into the call's GenDesc, words by slot into race_out
 int step_body(b2_handle* h, int n, cudaStream_t st) {
+    h->rows4 = StoreRows{nullptr, h->row_pos, n, n, 1, 0};
     if (wq_ok(h, n) || wq_pythia_ok(h, n)) {
         int rc = h->cfg.kind == B2_PYTHIA ? run_decode_wq_pythia(h, n, st) : run_decode_wq(h, n, st);
         if (rc) return rc;

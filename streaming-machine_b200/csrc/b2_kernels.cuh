@@ -264,6 +264,24 @@ __global__ void k_heads_pythia(const int64_t* __restrict__ QKV, int rows, const 
     }
 }
 
+// Pythia's turn of q and k in their qkv rows (pythia_base2.py:116-124, the arithmetic of k_heads_pythia), for the 4-bit
+// store, whose kernels take whole rows: 16 dims a head, pairs (t, t + 8), a thread a pair
+__global__ void __launch_bounds__(256) k_turn(int64_t* __restrict__ QKV, int rows, const int32_t* __restrict__ row_pos, int H, int lim,
+                                              const int32_t* __restrict__ COS, const int32_t* __restrict__ SIN, uint32_t* err) {
+    griddep_wait();
+    griddep_launch();
+    const int r = blockIdx.x, pos = row_pos[r];
+    if (r >= rows || pos < 0 || pos >= lim) return;          // flagged by the store's kernels (DERR_POS)
+    for (int i = threadIdx.x; i < H * 16; i += 256) {
+        const int t = i & 7, kind = (i >> 3) & 1, h = i >> 4;
+        int64_t* x = QKV + (size_t)r * 192 * H + h * 192 + kind * 64 + t;
+        const int64_t a = x[0], b = x[8], c = COS[(size_t)pos * 8 + t], s = SIN[(size_t)pos * 8 + t];
+        if ((mag(a) | mag(b)) >= (1ull << 31)) set_err(err, DERR_RANGE);
+        x[0] = rshift(wsub(wmul(a, c), wmul(b, s)), 30);
+        x[8] = rshift(wadd(wmul(b, c), wmul(a, s)), 30);
+    }
+}
+
 // ---------------------------------------------------------------------------------------------------------------------
 // bank epilogues (base2.py:62-76, 78-83)
 // ---------------------------------------------------------------------------------------------------------------------

@@ -34,10 +34,10 @@ B2_DEV void load_pair(const int64_t* p, bool wide, int64_t& a, int64_t& b) {
     }
 }
 
-__global__ void __launch_bounds__(SW_WARPS * 32) k_store_write(Store4 st, StoreRows rw, int layer, const int64_t* __restrict__ K,
-                                                               int64_t ldk, const int64_t* __restrict__ V, int64_t ldv,
-                                                               int wide, uint32_t* err) {
+__global__ void __launch_bounds__(SW_WARPS * 32) k_store_write(Store4 st, StoreRows rw, int layer, StoreVec K, StoreVec V,
+                                                               int wide, uint32_t* err, uint64_t* stamp) {
     griddep_wait();
+    stamp_begin(stamp);
     griddep_launch();
     const int s = blockIdx.y, lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
     StoreRun run;
@@ -46,9 +46,9 @@ __global__ void __launch_bounds__(SW_WARPS * 32) k_store_write(Store4 st, StoreR
     const int i = item / (2 * st.H), part = item - i * 2 * st.H, h = part < st.H ? part : part - st.H;
     if (i >= run.n) return;
     const bool key = part < st.H;
-    const int64_t* x = key ? K + (size_t)(run.r0 + i) * ldk : V + (size_t)(run.r0 + i) * ldv;
+    const int64_t* x = key ? K.x + (size_t)(run.r0 + i) * K.ld + h * K.hs : V.x + (size_t)(run.r0 + i) * V.ld + h * V.hs;
     int64_t a, b;
-    load_pair(x + h * 64 + 2 * lane, wide, a, b);
+    load_pair(x + 2 * lane, wide, a, b);
     a = store_clamp(a);
     b = store_clamp(b);
     const uint32_t t = (uint32_t)bitlen_u(mag(a) > mag(b) ? mag(a) : mag(b));
@@ -59,7 +59,7 @@ __global__ void __launch_bounds__(SW_WARPS * 32) k_store_write(Store4 st, StoreR
         sh = max(min(max((int)half - 3, 0), STORE_MAX_SHIFT), sh - 3);
     }
     const uint8_t c = (uint8_t)((store_code(a, sh) & 15) | (store_code(b, sh) << 4));
-    const size_t e = kv_index(s, layer, h, run.p0 + i, st.L, st.H, st.ctx);
+    const size_t e = kv_index(rw.slot0 + s, layer, h, run.p0 + i, st.L, st.H, st.ctx);
     if (key) {
         st.k[e * 32 + key_byte(lane)] = c;
         if ((lane & 15) == 0) st.ks[e * 2 + (lane >> 4)] = (int8_t)sh;
@@ -83,7 +83,7 @@ __global__ void __launch_bounds__(SW_WARPS * 32) k_store_read(Store4 st, StoreRo
     const bool key = part < st.H;
     int64_t* out = key ? K : V;
     if (!out) return;
-    const size_t e = kv_index(s, layer, h, run.p0 + i, st.L, st.H, st.ctx);
+    const size_t e = kv_index(rw.slot0 + s, layer, h, run.p0 + i, st.L, st.H, st.ctx);
     const int c = key ? (int)(int8_t)st.k[e * 32 + key_byte(lane)] : (int)(int8_t)st.v[e * 32 + lane];
     const int sh = key ? st.ks[e * 2 + (lane >> 4)] : st.vs[e];
     const int lo = (int)((uint32_t)c << 28) >> 28, hi = c >> 4;
@@ -176,6 +176,7 @@ B2_DEV int query_bytes(int64_t x0, int64_t x1, uint32_t& word) {
 template <int CS>
 __global__ void __launch_bounds__(SF_WARPS * 32) k_store_attend_few(StoreAttend a, int chunk, int wide) {
     griddep_wait();
+    stamp_begin(a.stamp);
     griddep_launch();
     extern __shared__ __align__(16) uint8_t sm[];
     int32_t* const SC = reinterpret_cast<int32_t*>(sm);              // [chunk]
@@ -201,7 +202,7 @@ __global__ void __launch_bounds__(SF_WARPS * 32) k_store_attend_few(StoreAttend 
     const int first_block = lo >> 5, blocks = (p >> 5) - first_block + 1;
     const int per = CS > 1 ? (blocks + CS - 1) / CS : blocks;
     const int b0 = first_block + rank * per, nb = max(0, min(per, blocks - rank * per));
-    const size_t base = kv_index(s, a.layer, h, 0, a.st.L, H, a.st.ctx) + (size_t)b0 * 32;
+    const size_t base = kv_index(a.rw.slot0 + s, a.layer, h, 0, a.st.L, H, a.st.ctx) + (size_t)b0 * 32;
     const uint8_t* const K = a.st.k + base * 32;
     const uint8_t* const V = a.st.v + base * 32;
     const int8_t* const KS = a.st.ks + base * 2;
@@ -209,7 +210,7 @@ __global__ void __launch_bounds__(SF_WARPS * 32) k_store_attend_few(StoreAttend 
 
     uint32_t word, q0[2], q1[2];                                     // B operands of the two halves
     int64_t x0, x1;
-    load_pair(a.q + (size_t)row * a.ldq + h * 64 + 2 * lane, wide & 1, x0, x1);
+    load_pair(a.q.x + (size_t)row * a.q.ld + h * a.q.hs + 2 * lane, wide & 1, x0, x1);
     const int u = query_bytes(x0, x1, word);
     {
         const uint32_t pick = (g & 1) ? 0x5151u : 0x4040u;           // odd columns the low bytes
@@ -406,6 +407,11 @@ B2_DEV uint32_t even_up(uint32_t w, int up, uint32_t less) {
 B2_DEV uint32_t odd_up(uint32_t w, int up, uint32_t less) {
     return ((((w & 0xF0F0F0F0u) ^ 0x80808080u) >> (4 - up)) + less) ^ 0x80808080u;
 }
+// bits from .. to of a word (none where from > to; either may lie outside)
+B2_DEV uint32_t seen(int from, int to) {
+    if (from > 31 || to < 0 || from > to) return 0u;
+    return (0xFFFFFFFFu << max(from, 0)) & (0xFFFFFFFFu >> (31 - min(to, 31)));
+}
 B2_DEV void copy16(void* to, const void* from) {      // 16 bytes, asynchronously, past L1
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(saddr(to)), "l"(from) : "memory");
 }
@@ -417,6 +423,7 @@ B2_DEV uint32_t shr_u32(uint32_t x, uint32_t s) {     // 0 for s > 31
 
 __global__ void __launch_bounds__(SM_THREADS, 2) k_store_attend_many(StoreAttend a, int tiles, int cs, int wide) {
     griddep_wait();
+    stamp_begin(a.stamp);
     griddep_launch();
     extern __shared__ __align__(16) uint8_t sm[];
     SmShared& S = *reinterpret_cast<SmShared*>(sm);
@@ -461,7 +468,7 @@ __global__ void __launch_bounds__(SM_THREADS, 2) k_store_attend_many(StoreAttend
         const int k0 = k_lo & ~31, k1 = (p_last | 31) + 1, all = (k1 - k0 + KEYS - 1) / KEYS;
         // this CTA's tiles: t0 .. t1 - 1
         const int per = cs > 1 ? (all + cs - 1) / cs : all, t0 = rank * per, t1 = min(all, t0 + per);
-        const size_t base = kv_index(s, a.layer, h, k0, a.st.L, H, a.st.ctx);
+        const size_t base = kv_index(a.rw.slot0 + s, a.layer, h, k0, a.st.L, H, a.st.ctx);
 
         // ---- a tile on its way: copied as it is, then unpacked. A warp takes 8 keys, and byte b of the words of 32 values
         // (dims 8g + 2b, 8g + 2b + 1); positions from k1 on are neither copied nor used
@@ -499,7 +506,7 @@ __global__ void __launch_bounds__(SM_THREADS, 2) k_store_attend_many(StoreAttend
             for (int k = 0; k < SM_ROWS / SM_WARPS; k++) {
                 const int r = wid + k * SM_WARPS;
                 x[k][0] = x[k][1] = 0;
-                if (r < nr) load_pair(a.q + (size_t)(run.r0 + i0 + r) * a.ldq + h * 64 + 2 * lane, wide & 1, x[k][0], x[k][1]);
+                if (r < nr) load_pair(a.q.x + (size_t)(run.r0 + i0 + r) * a.q.ld + h * a.q.hs + 2 * lane, wide & 1, x[k][0], x[k][1]);
             }
             int most = 0;
 #pragma unroll
@@ -582,6 +589,7 @@ __global__ void __launch_bounds__(SM_THREADS, 2) k_store_attend_many(StoreAttend
         int ya, yb, ma, mb, mw;
         auto largest = [&](const SmTile& T, int kb, auto slow, auto whole) {
             if (decltype(whole)::value) mw = max(mw, T.vs[blk * 32 + lane]);
+            const uint32_t seen_a = seen(la - kb, pa - kb), seen_b = seen(lb - kb, pb - kb);
 #pragma unroll
             for (int n = 0; n < 4; n++) {
                 int y[4];
@@ -591,11 +599,12 @@ __global__ void __launch_bounds__(SM_THREADS, 2) k_store_attend_many(StoreAttend
                     yb = max(yb, max(y[2], y[3]));
                 } else {
                     const int2 vs = *reinterpret_cast<const int2*>(&T.vs[blk * 32 + n * 8 + 2 * j]);
-                    const int key = kb + n * 8 + 2 * j;
-                    if (key >= la && key <= pa) { ya = max(ya, y[0]); ma = max(ma, vs.x); }
-                    if (key + 1 >= la && key + 1 <= pa) { ya = max(ya, y[1]); ma = max(ma, vs.y); }
-                    if (key >= lb && key <= pb) { yb = max(yb, y[2]); mb = max(mb, vs.x); }
-                    if (key + 1 >= lb && key + 1 <= pb) { yb = max(yb, y[3]); mb = max(mb, vs.y); }
+                    // bits 0 and 1: whether each row sees keys 2j and 2j + 1
+                    const uint32_t sa_ = seen_a >> (n * 8 + 2 * j), sb_ = seen_b >> (n * 8 + 2 * j);
+                    ya = max(ya, max((sa_ & 1) ? y[0] : INT32_MIN, (sa_ & 2) ? y[1] : INT32_MIN));
+                    yb = max(yb, max((sb_ & 1) ? y[2] : INT32_MIN, (sb_ & 2) ? y[3] : INT32_MIN));
+                    ma = max(ma, max((sa_ & 1) ? vs.x : 0, (sa_ & 2) ? vs.y : 0));
+                    mb = max(mb, max((sb_ & 1) ? vs.x : 0, (sb_ & 2) ? vs.y : 0));
                 }
             }
         };
@@ -672,7 +681,7 @@ __global__ void __launch_bounds__(SM_THREADS, 2) k_store_attend_many(StoreAttend
         if (item + step < items && n_r0 >= 0 && n_r1 <= a.rw.rows) {
             const uint32_t nsh = (item + step) / a.rw.n_streams;
             const int row = n_r0 + (tiles - 1 - (int)(nsh / H)) * ROWS + (tid >> 2);
-            if (row < n_r1) asm volatile("prefetch.global.L2 [%0];" ::"l"(a.q + (size_t)row * a.ldq + (nsh % H) * 64 + (tid & 3) * 16));
+            if (row < n_r1) asm volatile("prefetch.global.L2 [%0];" ::"l"(a.q.x + (size_t)row * a.q.ld + (int)(nsh % H) * a.q.hs + (tid & 3) * 16));
         }
         // twice the largest score: a digit below the last rounds up with it
         const uint32_t sa = (uint32_t)(((ya >> 1) + (ya & 1)) * 2), sb = (uint32_t)(((yb >> 1) + (yb & 1)) * 2);
@@ -689,6 +698,7 @@ __global__ void __launch_bounds__(SM_THREADS, 2) k_store_attend_many(StoreAttend
         auto weights = [&](const SmTile& T, int kb, auto slow, auto whole) {
             uint32_t p[3][4];                 // the weights' planes as A operands
             int32_t s_a = 0, s_b = 0;         // 8 entries of at most 2^24
+            const uint32_t seen_a = seen(la - kb, pa - kb), seen_b = seen(lb - kb, pb - kb);
 #pragma unroll
             for (int n = 0; n < 4; n += 2) {
                 uint32_t wa[4], wb[4];
@@ -703,11 +713,11 @@ __global__ void __launch_bounds__(SM_THREADS, 2) k_store_attend_many(StoreAttend
 #pragma unroll
                     for (int c = 0; c < 4; c++) d[c] = min(d[c], (uint32_t)alen);
                     if (!decltype(whole)::value) {
-                        const int key = kb + (n + x) * 8 + 2 * j;
-                        if (!(key >= la && key <= pa)) d[0] = alen;
-                        if (!(key + 1 >= la && key + 1 <= pa)) d[1] = alen;
-                        if (!(key >= lb && key <= pb)) d[2] = alen;
-                        if (!(key + 1 >= lb && key + 1 <= pb)) d[3] = alen;
+                        const uint32_t sa_ = seen_a >> ((n + x) * 8 + 2 * j), sb_ = seen_b >> ((n + x) * 8 + 2 * j);
+                        d[0] = (sa_ & 1) ? d[0] : alen;
+                        d[1] = (sa_ & 2) ? d[1] : alen;
+                        d[2] = (sb_ & 1) ? d[2] : alen;
+                        d[3] = (sb_ & 2) ? d[3] : alen;
                     }
                     const int v[4] = {TAB[d[0]], TAB[d[1]], TAB[d[2]], TAB[d[3]]};
                     s_a += v[0] + v[1];
@@ -848,14 +858,15 @@ cudaError_t store_launch(StoreLaunch how, void (*kernel)(KArgs...), dim3 grid, i
     return cudaLaunchKernelEx(&cfg, kernel, ((KArgs)args)...);
 }
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+bool pairs(const StoreVec& v) { return aligned16(v.x) && v.ld % 2 == 0 && v.hs % 2 == 0; }   // every pair of dims in one load
 }  // namespace
 
-cudaError_t store_write(const Store4& st, const StoreRows& rw, int layer, const int64_t* k, int64_t ldk, const int64_t* v,
-                        int64_t ldv, uint32_t* err, StoreLaunch how) {
+cudaError_t store_write(const Store4& st, const StoreRows& rw, int layer, const StoreVec& k, const StoreVec& v, uint32_t* err,
+                        StoreLaunch how, uint64_t* stamp) {
     if (rw.n_streams == 0 || rw.rows == 0) return cudaSuccess;
-    const int wide = aligned16(k) && aligned16(v) && ldk % 2 == 0 && ldv % 2 == 0;
+    const int wide = pairs(k) && pairs(v);
     const dim3 grid((unsigned)(((int64_t)rw.max_rows * 2 * st.H + SW_WARPS - 1) / SW_WARPS), rw.n_streams);
-    return store_launch(how, k_store_write, grid, SW_WARPS * 32, 0, 1, st, rw, layer, k, ldk, v, ldv, wide, err);
+    return store_launch(how, k_store_write, grid, SW_WARPS * 32, 0, 1, st, rw, layer, k, v, wide, err, stamp);
 }
 
 cudaError_t store_read(const Store4& st, const StoreRows& rw, int layer, int64_t* k, int64_t* v, uint32_t* err, StoreLaunch how) {
@@ -906,7 +917,7 @@ cudaError_t store_init(int alen, StorePlan& plan) {
 
 cudaError_t store_attend(const StoreAttend& a, StoreLaunch how) {
     if (a.rw.n_streams == 0 || a.rw.rows == 0) return cudaSuccess;
-    const int wide = (aligned16(a.q) && a.ldq % 2 == 0) | aligned16(a.out) << 1;
+    const int wide = pairs(a.q) | aligned16(a.out) << 1;
     const int64_t items = (int64_t)((a.rw.max_rows + SM_ROWS - 1) / SM_ROWS) * a.st.H * a.rw.n_streams;
     if (a.rw.max_rows > SM_FROM_ROWS && items < INT32_MAX) {
         const int tiles = (a.rw.max_rows + SM_ROWS - 1) / SM_ROWS;
@@ -1034,7 +1045,7 @@ int store_build(b2_store* h, const int64_t* arrival, int64_t n_arrival, const in
     std::vector<int32_t> t(4, 0);
     t.reserve(4 + 2 * 65536 + (size_t)n_arrival);
     int rc;
-    if ((rc = table32(h, t, log2, 65536, 0, 65536, "log2")) || (rc = table32(h, t, exp2, 65536, 65536, 131072, "exp2")) ||
+    if ((rc = table32(h, t, log2, 65536, 0, 65536, "log2")) || (rc = table32(h, t, exp2, 65536, 65536, 131071, "exp2")) ||
         (rc = table32(h, t, arrival, n_arrival, 0, STORE_MAX_ARR, "arrival")))
         return rc;
     int32_t* d = nullptr;
@@ -1121,7 +1132,7 @@ int b2_store_write(b2_store* h, int32_t layer, const int64_t* k, int64_t ldk, co
                          (long long)ldk, (const void*)v, (long long)ldv, (long long)d);
         OnDevice on(h->device);
         SCK(on.e);
-        SCK(store_write(h->st, StoreRows{cu, pos, n_streams, rows, max_rows}, layer, k, ldk, v, ldv, h->d_err,
+        SCK(store_write(h->st, StoreRows{cu, pos, n_streams, rows, max_rows}, layer, StoreVec{k, ldk, 64}, StoreVec{v, ldv, 64}, h->d_err,
                         StoreLaunch{(cudaStream_t)stream, false, &h->plan}));
         return (int)B2_OK;
     });
@@ -1154,7 +1165,7 @@ int b2_store_attend(b2_store* h, int32_t layer, const int64_t* q, int64_t ldq, c
                          (const void*)out, window);
         OnDevice on(h->device);
         SCK(on.e);
-        StoreAttend a{h->st, StoreRows{cu, pos, n_streams, rows, max_rows}, layer, q, ldq, first, window, h->ARR, h->alen,
+        StoreAttend a{h->st, StoreRows{cu, pos, n_streams, rows, max_rows}, layer, StoreVec{q, ldq, 64}, first, window, h->ARR, h->alen,
                       h->LOG2, h->EXP2, out, nullptr, h->d_err};
         SCK(store_attend(a, StoreLaunch{(cudaStream_t)stream, false, &h->plan}));
         return (int)B2_OK;

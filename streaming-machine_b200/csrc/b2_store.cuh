@@ -27,19 +27,27 @@ struct Store4 {
     int lim;           // positions a stream may hold
 };
 
-// a call's rows: stream i gives rows cu[i] .. cu[i + 1] - 1 (cu == nullptr: row i), its first at position pos[i]
+// a call's rows: stream i (slot slot0 + i) gives rows cu[i] .. cu[i + 1] - 1 (cu == nullptr: row i), its first at
+// position pos[i]
 struct StoreRows {
-    const int32_t* cu;
-    const int32_t* pos;
-    int n_streams, rows, max_rows;
+    const int32_t* cu = nullptr;
+    const int32_t* pos = nullptr;
+    int n_streams = 0, rows = 0, max_rows = 0;
+    int slot0 = 0;
+};
+
+// int64 rows of heads: row r's head h at x + r * ld + h * hs
+struct StoreVec {
+    const int64_t* x;
+    int64_t ld;
+    int hs;
 };
 
 struct StoreAttend {
     Store4 st;
     StoreRows rw;
     int layer;
-    const int64_t* q;      // row r's head h at q + r * ldq + 64 h
-    int64_t ldq;
+    StoreVec q;
     const int32_t* first;  // optional [n_streams]: the first position that a stream still sees
     int window;            // 0, or how many positions a row sees (its own the last)
     const int32_t* ARR;
@@ -49,6 +57,7 @@ struct StoreAttend {
     int64_t* out;          // [rows][H][64]
     uint64_t* or_out;      // optional [rows]: OR of |out| per row (the next bank's to16 shift)
     uint32_t* err;
+    uint64_t* stamp = nullptr;   // b2_profile mode 2
 };
 
 // what the launches are sized by, once per device (the current one) and arrival table; to be called before the first launch
@@ -66,8 +75,8 @@ struct StoreLaunch {
     const StorePlan* plan;
 };
 
-cudaError_t store_write(const Store4& st, const StoreRows& rw, int layer, const int64_t* k, int64_t ldk, const int64_t* v,
-                        int64_t ldv, uint32_t* err, StoreLaunch how);
+cudaError_t store_write(const Store4& st, const StoreRows& rw, int layer, const StoreVec& k, const StoreVec& v, uint32_t* err,
+                        StoreLaunch how, uint64_t* stamp = nullptr);
 cudaError_t store_read(const Store4& st, const StoreRows& rw, int layer, int64_t* k, int64_t* v, uint32_t* err, StoreLaunch how);
 cudaError_t store_attend(const StoreAttend& a, StoreLaunch how);
 

@@ -111,10 +111,13 @@ class Engine:
     Pythia's "embed.w") on one GPU, with `n_streams` independent streams of up to `max_ctx` positions."""
 
     def __init__(self, M: dict, device: int = 0, n_streams: int = 1, max_ctx: int = 1024,
-                 gauge: str = "int", edge: str = "int", arrival: str = "int", turn: str = "int", layout: dict | None = None):
+                 gauge: str = "int", edge: str = "int", arrival: str = "int", turn: str = "int", layout: dict | None = None,
+                 store_bits: int = 16):
         """gauge=/edge=/arrival= "float" (and Pythia's turn=) put that stage back to float64, as the reference's
         switches do (base2.py:10-11, pythia_base2.py:20). layout: the banks' tensor-core layouts computed ahead of time
-        ({bank: {wh, wl, cc, cckb}}, streaming_machine_b200.layout.read_tc_layout), uploaded instead of built."""
+        ({bank: {wh, wl, cc, cckb}}, streaming_machine_b200.layout.read_tc_layout), uploaded instead of built. store_bits:
+        4 holds the streams' keys and values in 4 bits (67 bytes a position and head in place of 396; see store.Store for
+        what is held and how the arrival reads it), 16 as the reference does."""
         torch = _torch()
         self.torch = torch
         self.device = torch.device("cuda", device)
@@ -164,6 +167,8 @@ class Engine:
             self._call("b2_set_scalar", h, k.encode(), _scalar(M, k))
         self._call("b2_finalize", h)
         self.n_streams, self.max_ctx = 0, 0
+        if store_bits != 16:
+            self._call("b2_set_scalar", h, b"store_bits", store_bits)
         self.alloc_streams(n_streams, max_ctx)
 
     # ---- plumbing ---------------------------------------------------------------------------------------------
