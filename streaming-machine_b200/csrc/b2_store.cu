@@ -18,8 +18,10 @@
 namespace b2 {
 
 // ---------------------------------------------------------------------------------------------------------------------
-// write: a warp holds one head row (64 int64, two a lane). The shift is the bit length of the largest magnitude less 3:
-// a warp maximum of bit lengths, over each half of 32 dims for keys, over all 64 for values.
+// write: a warp holds a head's key or value of U consecutive rows, a row (64 int64) in 16-byte loads of two dims a lane,
+// all asked for before the first is used. The shift is the bit length of the OR of the magnitudes less 3 (the OR has the
+// largest one's bit length): a warp reduction for each half of 32 dims of a key, for all 64 of a value. Bound by the
+// memory's latency at U = 1 (a decode step), by its bandwidth at U = 8.
 // ---------------------------------------------------------------------------------------------------------------------
 constexpr int SW_WARPS = 8;
 
@@ -34,66 +36,112 @@ B2_DEV void load_pair(const int64_t* p, bool wide, int64_t& a, int64_t& b) {
     }
 }
 
+// the warp's head part and its first row among the stream's (U rows a warp)
+template <int U>
+B2_DEV bool store_item(int H, int n, int& part, int& i) {
+    const int item = blockIdx.x * SW_WARPS + (threadIdx.x >> 5), up = item / (2 * H);
+    part = item - up * 2 * H;
+    i = up * U;
+    return i < n;
+}
+
+template <int U>
 __global__ void __launch_bounds__(SW_WARPS * 32) k_store_write(Store4 st, StoreRows rw, int layer, StoreVec K, StoreVec V,
                                                                int wide, uint32_t* err, uint64_t* stamp) {
     griddep_wait();
     stamp_begin(stamp);
     griddep_launch();
-    const int s = blockIdx.y, lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+    const int s = blockIdx.y, lane = threadIdx.x & 31;
     StoreRun run;
-    if (!store_run(rw, s, st.lim, run, err)) return;
-    const int item = blockIdx.x * SW_WARPS + wid;            // (row of the stream, key or value, head)
-    const int i = item / (2 * st.H), part = item - i * 2 * st.H, h = part < st.H ? part : part - st.H;
-    if (i >= run.n) return;
+    int part, i;
+    if (!store_run(rw, s, st.lim, run, err) || !store_item<U>(st.H, run.n, part, i)) return;
     const bool key = part < st.H;
-    const int64_t* x = key ? K.x + (size_t)(run.r0 + i) * K.ld + h * K.hs : V.x + (size_t)(run.r0 + i) * V.ld + h * V.hs;
-    int64_t a, b;
-    load_pair(x + 2 * lane, wide, a, b);
-    a = store_clamp(a);
-    b = store_clamp(b);
-    const uint32_t t = (uint32_t)bitlen_u(mag(a) > mag(b) ? mag(a) : mag(b));
-    const int whole = max((int)__reduce_max_sync(0xffffffffu, t) - 3, 0);
-    int sh = min(whole, STORE_MAX_SHIFT);
-    if (key) {                                               // lanes 0 .. 15 hold dims 0 .. 31
-        const uint32_t half = __reduce_max_sync(lane < 16 ? 0xffffu : 0xffff0000u, t);
-        sh = max(min(max((int)half - 3, 0), STORE_MAX_SHIFT), sh - 3);
+    const int h = key ? part : part - st.H;
+    const StoreVec& X = key ? K : V;
+    const int64_t* x = X.x + (size_t)(run.r0 + i) * X.ld + h * X.hs + 2 * lane;
+    int64_t a[U], b[U];
+#pragma unroll
+    for (int t = 0; t < U; t++) {
+        a[t] = b[t] = 0;
+        if (i + t < run.n) load_pair(x + (size_t)t * X.ld, wide, a[t], b[t]);
     }
-    const uint8_t c = (uint8_t)((store_code(a, sh) & 15) | (store_code(b, sh) << 4));
     const size_t e = kv_index(rw.slot0 + s, layer, h, run.p0 + i, st.L, st.H, st.ctx);
+    uint8_t* const codes = key ? st.k + e * 32 + key_byte(lane) : st.v + e * 32 + lane;
+    int mine = 0;                                        // the shift that this lane stores
+#pragma unroll
+    for (int t = 0; t < U; t++) {
+        int sh0, sh1, c0, c1;                            // the shifts of the lower and the upper half, the codes
+        if (__all_sync(0xffffffffu, a[t] == (int32_t)a[t] && b[t] == (int32_t)b[t])) {     // the usual case: 32 bits hold them
+            const int y0 = (int)a[t], y1 = (int)b[t];
+            const uint32_t m = (uint32_t)abs(y0) | (uint32_t)abs(y1);
+            const uint32_t lo = __reduce_or_sync(0xffffffffu, lane < 16 ? m : 0u), hi = __reduce_or_sync(0xffffffffu, lane < 16 ? 0u : m);
+            const int big = max(29 - __clz((int)(lo | hi)), 0);
+            sh0 = key ? max(max(29 - __clz((int)lo), 0), big - 3) : big;
+            sh1 = key ? max(max(29 - __clz((int)hi), 0), big - 3) : big;
+            const int sh = lane < 16 ? sh0 : sh1;
+            c0 = max(min(rnd32(y0, sh), 7), -8);
+            c1 = max(min(rnd32(y1, sh), 7), -8);
+        } else {
+            const int64_t y0 = store_clamp(a[t]), y1 = store_clamp(b[t]);
+            const uint32_t m = (uint32_t)bitlen_u(mag(y0) | mag(y1));
+            const int lo = (int)__reduce_max_sync(0xffffffffu, lane < 16 ? m : 0u), hi = (int)__reduce_max_sync(0xffffffffu, lane < 16 ? 0u : m);
+            const int big = min(max(max(lo, hi) - 3, 0), STORE_MAX_SHIFT);
+            sh0 = key ? max(min(max(lo - 3, 0), STORE_MAX_SHIFT), big - 3) : big;
+            sh1 = key ? max(min(max(hi - 3, 0), STORE_MAX_SHIFT), big - 3) : big;
+            const int sh = lane < 16 ? sh0 : sh1;
+            c0 = store_code(y0, sh);
+            c1 = store_code(y1, sh);
+        }
+        if (i + t < run.n) codes[t * 32] = (uint8_t)((c0 & 15) | (c1 << 4));
+        if (key) mine = lane == 2 * t ? sh0 : (lane == 2 * t + 1 ? sh1 : mine);
+        else mine = lane == t ? sh0 : mine;
+    }
+    const int rows = min(U, run.n - i);
     if (key) {
-        st.k[e * 32 + key_byte(lane)] = c;
-        if ((lane & 15) == 0) st.ks[e * 2 + (lane >> 4)] = (int8_t)sh;
+        if (lane < 2 * rows) st.ks[e * 2 + lane] = (int8_t)mine;
     } else {
-        st.v[e * 32 + lane] = c;
-        if (lane == 0) st.vs[e] = (int8_t)sh;
+        if (lane < rows) st.vs[e + lane] = (int8_t)mine;
     }
 }
 
-// read: the values that the codes stand for, c 2^s; a warp a head row, as above
+// read: the values that the codes stand for, c 2^s; a warp a head's key or value of U consecutive rows, as above
+template <int U>
 __global__ void __launch_bounds__(SW_WARPS * 32) k_store_read(Store4 st, StoreRows rw, int layer, int64_t* __restrict__ K,
                                                               int64_t* __restrict__ V, int wide, uint32_t* err) {
     griddep_wait();
     griddep_launch();
-    const int s = blockIdx.y, lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+    const int s = blockIdx.y, lane = threadIdx.x & 31;
     StoreRun run;
-    if (!store_run(rw, s, st.lim, run, err)) return;
-    const int item = blockIdx.x * SW_WARPS + wid;
-    const int i = item / (2 * st.H), part = item - i * 2 * st.H, h = part < st.H ? part : part - st.H;
-    if (i >= run.n) return;
+    int part, i;
+    if (!store_run(rw, s, st.lim, run, err) || !store_item<U>(st.H, run.n, part, i)) return;
     const bool key = part < st.H;
+    const int h = key ? part : part - st.H;
     int64_t* out = key ? K : V;
     if (!out) return;
     const size_t e = kv_index(rw.slot0 + s, layer, h, run.p0 + i, st.L, st.H, st.ctx);
-    const int c = key ? (int)(int8_t)st.k[e * 32 + key_byte(lane)] : (int)(int8_t)st.v[e * 32 + lane];
-    const int sh = key ? st.ks[e * 2 + (lane >> 4)] : st.vs[e];
-    const int lo = (int)((uint32_t)c << 28) >> 28, hi = c >> 4;
-    const int64_t a = (int64_t)((uint64_t)(int64_t)lo << sh), b = (int64_t)((uint64_t)(int64_t)hi << sh);
+    const uint8_t* const codes = key ? st.k + e * 32 + key_byte(lane) : st.v + e * 32 + lane;
+    const int8_t* const shifts = key ? st.ks + e * 2 + (lane >> 4) : st.vs + e;
+    int c[U], sh[U];
+#pragma unroll
+    for (int t = 0; t < U; t++) {
+        c[t] = sh[t] = 0;
+        if (i + t < run.n) {
+            c[t] = (int8_t)codes[t * 32];
+            sh[t] = shifts[key ? t * 2 : t];
+        }
+    }
     int64_t* o = out + ((size_t)(run.r0 + i) * st.H + h) * 64 + 2 * lane;
-    if (wide) {
-        *reinterpret_cast<longlong2*>(o) = make_longlong2(a, b);
-    } else {
-        o[0] = a;
-        o[1] = b;
+#pragma unroll
+    for (int t = 0; t < U; t++, o += st.H * 64) {
+        if (i + t >= run.n) return;
+        const int lo = (int)((uint32_t)c[t] << 28) >> 28, hi = c[t] >> 4;
+        const int64_t a = (int64_t)((uint64_t)(int64_t)lo << sh[t]), b = (int64_t)((uint64_t)(int64_t)hi << sh[t]);
+        if (wide) {
+            *reinterpret_cast<longlong2*>(o) = make_longlong2(a, b);
+        } else {
+            o[0] = a;
+            o[1] = b;
+        }
     }
 }
 
@@ -861,19 +909,29 @@ bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 bool pairs(const StoreVec& v) { return aligned16(v.x) && v.ld % 2 == 0 && v.hs % 2 == 0; }   // every pair of dims in one load
 }  // namespace
 
+namespace {
+// rows a warp: one where streams give few (a decode step: more warps, the least latency), else eight
+constexpr int SW_ROWS = 8;
+dim3 row_grid(const Store4& st, const StoreRows& rw, int u) {
+    return dim3((unsigned)(((int64_t)((rw.max_rows + u - 1) / u) * 2 * st.H + SW_WARPS - 1) / SW_WARPS), rw.n_streams);
+}
+}  // namespace
+
 cudaError_t store_write(const Store4& st, const StoreRows& rw, int layer, const StoreVec& k, const StoreVec& v, uint32_t* err,
                         StoreLaunch how, uint64_t* stamp) {
     if (rw.n_streams == 0 || rw.rows == 0) return cudaSuccess;
     const int wide = pairs(k) && pairs(v);
-    const dim3 grid((unsigned)(((int64_t)rw.max_rows * 2 * st.H + SW_WARPS - 1) / SW_WARPS), rw.n_streams);
-    return store_launch(how, k_store_write, grid, SW_WARPS * 32, 0, 1, st, rw, layer, k, v, wide, err, stamp);
+    if (rw.max_rows < SW_ROWS)
+        return store_launch(how, k_store_write<1>, row_grid(st, rw, 1), SW_WARPS * 32, 0, 1, st, rw, layer, k, v, wide, err, stamp);
+    return store_launch(how, k_store_write<SW_ROWS>, row_grid(st, rw, SW_ROWS), SW_WARPS * 32, 0, 1, st, rw, layer, k, v, wide, err, stamp);
 }
 
 cudaError_t store_read(const Store4& st, const StoreRows& rw, int layer, int64_t* k, int64_t* v, uint32_t* err, StoreLaunch how) {
     if (rw.n_streams == 0 || rw.rows == 0) return cudaSuccess;
     const int wide = aligned16(k) && aligned16(v);
-    const dim3 grid((unsigned)(((int64_t)rw.max_rows * 2 * st.H + SW_WARPS - 1) / SW_WARPS), rw.n_streams);
-    return store_launch(how, k_store_read, grid, SW_WARPS * 32, 0, 1, st, rw, layer, k, v, wide, err);
+    if (rw.max_rows < SW_ROWS)
+        return store_launch(how, k_store_read<1>, row_grid(st, rw, 1), SW_WARPS * 32, 0, 1, st, rw, layer, k, v, wide, err);
+    return store_launch(how, k_store_read<SW_ROWS>, row_grid(st, rw, SW_ROWS), SW_WARPS * 32, 0, 1, st, rw, layer, k, v, wide, err);
 }
 
 constexpr int SM_FROM_ROWS = 4, SM_FIXED = 4;
