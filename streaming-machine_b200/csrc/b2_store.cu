@@ -18,10 +18,12 @@
 namespace b2 {
 
 // ---------------------------------------------------------------------------------------------------------------------
-// write: a warp holds a head's key or value of U consecutive rows, a row (64 int64) in 16-byte loads of two dims a lane,
-// all asked for before the first is used. The shift is the bit length of the OR of the magnitudes less 3 (the OR has the
-// largest one's bit length): a warp reduction for each half of 32 dims of a key, for all 64 of a value. Bound by the
-// memory's latency at U = 1 (a decode step), by its bandwidth at U = 8.
+// write: eight lanes hold a head's key or value (64 int64), lane i of them the pairs of dims i, i + 8, i + 16, i + 24, so
+// that a load of the eight is 128 bytes in a row and the first two pairs are the lower half's; U rows, all asked for before
+// the first is used. The shift is the bit length of the OR of the magnitudes less 3 (the OR has the largest one's bit
+// length). Bound by the memory's latency at U = 1 (a decode step); a prompt's by its bandwidth. One row a warp, two dims a
+// lane, took three times the instructions and was bound by them (40 against 28 us, 4.6 TB/s, for
+// 32 x 512 prompts of 12 heads).
 // ---------------------------------------------------------------------------------------------------------------------
 constexpr int SW_WARPS = 8;
 
@@ -51,56 +53,77 @@ __global__ void __launch_bounds__(SW_WARPS * 32) k_store_write(Store4 st, StoreR
     griddep_wait();
     stamp_begin(stamp);
     griddep_launch();
-    const int s = blockIdx.y, lane = threadIdx.x & 31;
+    const int s = blockIdx.y, sub = threadIdx.x & 7;
     StoreRun run;
-    int part, i;
-    if (!store_run(rw, s, st.lim, run, err) || !store_item<U>(st.H, run.n, part, i)) return;
+    if (!store_run(rw, s, st.lim, run, err)) return;
+    // the eight lanes' head part and first row: U = 1 the parts of a row in turn, else four neighbours' rows in turn
+    const int item = blockIdx.x * (SW_WARPS * 4) + (threadIdx.x >> 3);
+    const int part = U == 1 ? item % (2 * st.H) : (item >> 2) % (2 * st.H);
+    const int i = U == 1 ? item / (2 * st.H) : ((item >> 2) / (2 * st.H) * 4 + (item & 3)) * U;
+    if (!__any_sync(0xffffffffu, i < run.n)) return;             // past a short stream's rows
     const bool key = part < st.H;
     const int h = key ? part : part - st.H;
-    const StoreVec& X = key ? K : V;
-    const int64_t* x = X.x + (size_t)(run.r0 + i) * X.ld + h * X.hs + 2 * lane;
-    int64_t a[U], b[U];
+    const StoreVec X = key ? K : V;
+    const int64_t* x = X.x + (size_t)(run.r0 + i) * X.ld + h * X.hs + 2 * sub;
+    int64_t v[U][8];
 #pragma unroll
-    for (int t = 0; t < U; t++) {
-        a[t] = b[t] = 0;
-        if (i + t < run.n) load_pair(x + (size_t)t * X.ld, wide, a[t], b[t]);
-    }
-    const size_t e = kv_index(rw.slot0 + s, layer, h, run.p0 + i, st.L, st.H, st.ctx);
-    uint8_t* const codes = key ? st.k + e * 32 + key_byte(lane) : st.v + e * 32 + lane;
-    int mine = 0;                                        // the shift that this lane stores
+    for (int t = 0; t < U; t++)
 #pragma unroll
-    for (int t = 0; t < U; t++) {
-        int sh0, sh1, c0, c1;                            // the shifts of the lower and the upper half, the codes
-        if (__all_sync(0xffffffffu, a[t] == (int32_t)a[t] && b[t] == (int32_t)b[t])) {     // the usual case: 32 bits hold them
-            const int y0 = (int)a[t], y1 = (int)b[t];
-            const uint32_t m = (uint32_t)abs(y0) | (uint32_t)abs(y1);
-            const uint32_t lo = __reduce_or_sync(0xffffffffu, lane < 16 ? m : 0u), hi = __reduce_or_sync(0xffffffffu, lane < 16 ? 0u : m);
-            const int big = max(29 - __clz((int)(lo | hi)), 0);
-            sh0 = key ? max(max(29 - __clz((int)lo), 0), big - 3) : big;
-            sh1 = key ? max(max(29 - __clz((int)hi), 0), big - 3) : big;
-            const int sh = lane < 16 ? sh0 : sh1;
-            c0 = max(min(rnd32(y0, sh), 7), -8);
-            c1 = max(min(rnd32(y1, sh), 7), -8);
-        } else {
-            const int64_t y0 = store_clamp(a[t]), y1 = store_clamp(b[t]);
-            const uint32_t m = (uint32_t)bitlen_u(mag(y0) | mag(y1));
-            const int lo = (int)__reduce_max_sync(0xffffffffu, lane < 16 ? m : 0u), hi = (int)__reduce_max_sync(0xffffffffu, lane < 16 ? 0u : m);
-            const int big = min(max(max(lo, hi) - 3, 0), STORE_MAX_SHIFT);
-            sh0 = key ? max(min(max(lo - 3, 0), STORE_MAX_SHIFT), big - 3) : big;
-            sh1 = key ? max(min(max(hi - 3, 0), STORE_MAX_SHIFT), big - 3) : big;
-            const int sh = lane < 16 ? sh0 : sh1;
-            c0 = store_code(y0, sh);
-            c1 = store_code(y1, sh);
+        for (int k = 0; k < 4; k++) {
+            v[t][2 * k] = v[t][2 * k + 1] = 0;
+            if (i + t < run.n) load_pair(x + (size_t)t * X.ld + 16 * k, wide, v[t][2 * k], v[t][2 * k + 1]);
         }
-        if (i + t < run.n) codes[t * 32] = (uint8_t)((c0 & 15) | (c1 << 4));
-        if (key) mine = lane == 2 * t ? sh0 : (lane == 2 * t + 1 ? sh1 : mine);
-        else mine = lane == t ? sh0 : mine;
-    }
-    const int rows = min(U, run.n - i);
-    if (key) {
-        if (lane < 2 * rows) st.ks[e * 2 + lane] = (int8_t)mine;
-    } else {
-        if (lane < rows) st.vs[e + lane] = (int8_t)mine;
+    const size_t e = kv_index(rw.slot0 + s, layer, h, run.p0 + i, st.L, st.H, st.ctx);
+    uint8_t* const codes = key ? st.k + e * 32 + key_byte(sub) : st.v + e * 32 + sub;
+    const int step1 = key ? 16 : 8, step2 = key ? 4 : 16;        // from pair i to i + 8, to i + 16
+#pragma unroll
+    for (int t = 0; t < U; t++) {
+        uint32_t past = 0;                                       // nonzero where 32 bits do not hold a value
+#pragma unroll
+        for (int k = 0; k < 8; k++) past |= (uint32_t)(v[t][k] >> 32) ^ (uint32_t)((int32_t)v[t][k] >> 31);
+        int sh[2], c[8];
+        if (__all_sync(0xffffffffu, past == 0)) {                // the usual case
+            uint32_t m[2] = {0, 0};
+#pragma unroll
+            for (int k = 0; k < 8; k++) m[k >> 2] |= (uint32_t)abs((int)v[t][k]);
+#pragma unroll
+            for (int o = 1; o < 8; o <<= 1) {
+                m[0] |= __shfl_xor_sync(0xffffffffu, m[0], o);
+                m[1] |= __shfl_xor_sync(0xffffffffu, m[1], o);
+            }
+            const int big = max(29 - __clz((int)(m[0] | m[1])), 0);
+#pragma unroll
+            for (int k = 0; k < 2; k++) sh[k] = key ? max(max(29 - __clz((int)m[k]), 0), big - 3) : big;
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const int down = max(sh[k >> 2] - 1, 0), one = sh[k >> 2] > 0;
+                c[k] = max(min((((int)v[t][k] >> down) + one) >> one, 7), -8);
+            }
+        } else {
+            uint64_t m[2] = {0, 0};
+#pragma unroll
+            for (int k = 0; k < 8; k++) m[k >> 2] |= mag(store_clamp(v[t][k]));
+#pragma unroll
+            for (int o = 1; o < 8; o <<= 1) {
+                m[0] |= __shfl_xor_sync(0xffffffffu, m[0], o);
+                m[1] |= __shfl_xor_sync(0xffffffffu, m[1], o);
+            }
+            const int big = min(max(bitlen_u(m[0] | m[1]) - 3, 0), STORE_MAX_SHIFT);
+#pragma unroll
+            for (int k = 0; k < 2; k++) sh[k] = key ? max(min(max(bitlen_u(m[k]) - 3, 0), STORE_MAX_SHIFT), big - 3) : big;
+#pragma unroll
+            for (int k = 0; k < 8; k++) c[k] = store_code(store_clamp(v[t][k]), sh[k >> 2]);
+        }
+        if (i + t < run.n) {
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                codes[t * 32 + (k & 1) * step1 + (k >> 1) * step2] = (uint8_t)((c[2 * k] & 15) | (c[2 * k + 1] << 4));
+            if (key) {
+                if (sub < 2) st.ks[(e + t) * 2 + sub] = (int8_t)(sub ? sh[1] : sh[0]);
+            } else if (sub == 0) {
+                st.vs[e + t] = (int8_t)sh[0];
+            }
+        }
     }
 }
 
@@ -921,9 +944,11 @@ cudaError_t store_write(const Store4& st, const StoreRows& rw, int layer, const 
                         StoreLaunch how, uint64_t* stamp) {
     if (rw.n_streams == 0 || rw.rows == 0) return cudaSuccess;
     const int wide = pairs(k) && pairs(v);
-    if (rw.max_rows < SW_ROWS)
-        return store_launch(how, k_store_write<1>, row_grid(st, rw, 1), SW_WARPS * 32, 0, 1, st, rw, layer, k, v, wide, err, stamp);
-    return store_launch(how, k_store_write<SW_ROWS>, row_grid(st, rw, SW_ROWS), SW_WARPS * 32, 0, 1, st, rw, layer, k, v, wide, err, stamp);
+    const bool few = rw.max_rows < SW_ROWS;
+    const int64_t items = few ? (int64_t)rw.max_rows * 2 * st.H : (int64_t)((rw.max_rows + SW_ROWS - 1) / SW_ROWS) * 4 * 2 * st.H;
+    const dim3 grid((unsigned)((items + SW_WARPS * 4 - 1) / (SW_WARPS * 4)), rw.n_streams);
+    return few ? store_launch(how, k_store_write<1>, grid, SW_WARPS * 32, 0, 1, st, rw, layer, k, v, wide, err, stamp)
+               : store_launch(how, k_store_write<2>, grid, SW_WARPS * 32, 0, 1, st, rw, layer, k, v, wide, err, stamp);
 }
 
 cudaError_t store_read(const Store4& st, const StoreRows& rw, int layer, int64_t* k, int64_t* v, uint32_t* err, StoreLaunch how) {
