@@ -493,9 +493,6 @@ B2_DEV uint32_t shr_u32(uint32_t x, uint32_t s) {     // 0 for s > 31
 }
 
 __global__ void __launch_bounds__(SM_THREADS, 2) k_store_attend_many(StoreAttend a, int tiles, int cs, int wide) {
-    griddep_wait();
-    stamp_begin(a.stamp);
-    griddep_launch();
     extern __shared__ __align__(16) uint8_t sm[];
     SmShared& S = *reinterpret_cast<SmShared*>(sm);
     int32_t* const TAB = reinterpret_cast<int32_t*>(sm + sizeof(SmShared));   // [alen + 1], 0 at the end
@@ -505,6 +502,9 @@ __global__ void __launch_bounds__(SM_THREADS, 2) k_store_attend_many(StoreAttend
     const int H = a.st.H, alen = a.alen;
     for (int i = tid; i < alen; i += SM_THREADS) TAB[i] = __ldg(a.ARR + i);
     if (tid == 0) TAB[alen] = 0;
+    griddep_wait();                       // (the table never changes: its copy need not wait)
+    stamp_begin(a.stamp);
+    griddep_launch();
     const uint32_t items = (uint32_t)(tiles * H * a.rw.n_streams), step = gridDim.x / cs;   // below 2^31 (the launch sees to it)
     // an item's entries of the row table, read one item ahead
     int n_r0 = 0, n_r1 = 0, n_pos = 0, n_first = 0;
@@ -1216,7 +1216,7 @@ int b2_store_write(b2_store* h, int32_t layer, const int64_t* k, int64_t ldk, co
         OnDevice on(h->device);
         SCK(on.e);
         SCK(store_write(h->st, StoreRows{cu, pos, n_streams, rows, max_rows}, layer, StoreVec{k, ldk, 64}, StoreVec{v, ldv, 64}, h->d_err,
-                        StoreLaunch{(cudaStream_t)stream, false, &h->plan}));
+                        StoreLaunch{(cudaStream_t)stream, true, &h->plan}));
         return (int)B2_OK;
     });
 }
@@ -1231,7 +1231,7 @@ int b2_store_read(b2_store* h, int32_t layer, const int32_t* cu, const int32_t* 
         OnDevice on(h->device);
         SCK(on.e);
         SCK(store_read(h->st, StoreRows{cu, pos, n_streams, rows, max_rows}, layer, k, v, h->d_err,
-                       StoreLaunch{(cudaStream_t)stream, false, &h->plan}));
+                       StoreLaunch{(cudaStream_t)stream, true, &h->plan}));
         return (int)B2_OK;
     });
 }
@@ -1250,7 +1250,7 @@ int b2_store_attend(b2_store* h, int32_t layer, const int64_t* q, int64_t ldq, c
         SCK(on.e);
         StoreAttend a{h->st, StoreRows{cu, pos, n_streams, rows, max_rows}, layer, StoreVec{q, ldq, 64}, first, window, h->ARR, h->alen,
                       h->LOG2, h->EXP2, out, nullptr, h->d_err};
-        SCK(store_attend(a, StoreLaunch{(cudaStream_t)stream, false, &h->plan}));
+        SCK(store_attend(a, StoreLaunch{(cudaStream_t)stream, true, &h->plan}));
         return (int)B2_OK;
     });
 }

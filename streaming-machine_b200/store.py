@@ -47,108 +47,122 @@ class Store:
 
     def _host(self, torch, kind: str, device: int, n_streams: int, max_ctx: int, n_head: int, n_layer: int):
         """The host side's own state (no device work)."""
-        self.torch, self.device = torch, torch.device(kind, device if kind == "cuda" else None)
+        cuda = kind == "cuda"
+        self.torch, self.device = torch, torch.device(kind, device if cuda else None)
         self.n_streams, self.max_ctx, self.n_head, self.n_layer = n_streams, max_ctx, n_head, n_layer
-        self._i64, self._i32 = torch.int64, torch.int32
+        self._tensor, self._i64, self._i32 = torch.Tensor, torch.int64, torch.int32
         self._row, self._flat, self._unit = (n_head, HEAD), (n_head * HEAD,), (HEAD, 1)
-        self._stream, self._index = torch._C._cuda_getCurrentRawStream if kind == "cuda" else (lambda i: None), device
+        self._stream, self._index = (torch._C._cuda_getCurrentRawStream, device) if cuda else (lambda i: None, -1)
         L = lib()
-        self._write, self._read, self._attend = L.b2_store_write, L.b2_store_read, L.b2_store_attend
+        self._f_write, self._f_read, self._f_attend = L.b2_store_write, L.b2_store_read, L.b2_store_attend
 
-    # ---- plumbing (a decode step calls these for every layer: the usual case is settled by a few comparisons) ----
-    def _call(self, fn, *args):
-        if not self.h:
-            raise ValueError("the store is closed")
-        rc = fn(self.h, *args, self._stream(self._index))
-        if rc:
-            raise B2Error(rc, lib().b2_store_last_error(self.h).decode())
-
+    # ---- plumbing ---------------------------------------------------------------------------------------------
+    # (a decode step comes here for every layer: the usual case is settled by a few comparisons, what is wrong with an
+    # argument is looked for only where they fail)
     def _rows(self, x, name: str):
         """(pointer, row stride) of int64 rows [rows, n_head, 64] or [rows, n_head * 64]; only the rows may be strided."""
-        self._on_device(x, name, self._i64)
-        shape, st = x.shape, x.stride()
-        d = self.n_head * HEAD
-        if shape[1:] == self._row and (st[1:] == self._unit or (self.n_head == 1 and st[2] == 1)) or \
-                shape[1:] == self._flat and st[1] == 1:
-            if st[0] >= d:
-                return x.data_ptr(), st[0]
-            if shape[0] <= 1:                                    # a single row's stride says nothing
-                return x.data_ptr(), d
-        raise ValueError(f"{name}: rows of [{self.n_head}, {HEAD}] (or {d}) values, one behind the other and apart, got shape "
-                         f"{tuple(shape)}, strides {st}")
+        if isinstance(x, self._tensor) and x.dtype is self._i64 and x.get_device() == self._index:
+            shape, st, d = x.shape, x.stride(), self.n_head * HEAD
+            if (shape[1:] == self._row and (st[1:] == self._unit or (self.n_head == 1 and st[2] == 1))) or \
+                    (shape[1:] == self._flat and st[1] == 1):
+                if st[0] >= d:
+                    return x.data_ptr(), st[0]
+                if shape[0] <= 1:                                # a single row's stride says nothing
+                    return x.data_ptr(), d
+            raise ValueError(f"{name}: rows of [{self.n_head}, {HEAD}] (or {d}) values, one behind the other and apart, got "
+                             f"shape {tuple(shape)}, strides {st}")
+        raise ValueError(f"{name}: a torch.int64 tensor on {self.device}, got {self._what(x)}")
 
-    def _on_device(self, x, name: str, dtype):
-        if not isinstance(x, self.torch.Tensor) or x.dtype is not dtype or x.device != self.device:
-            what = f"{x.dtype} on {x.device}" if isinstance(x, self.torch.Tensor) else type(x).__name__
-            raise ValueError(f"{name}: a {dtype} tensor on {self.device}, got {what}")
+    def _what(self, x) -> str:
+        return f"{x.dtype} on {x.device}" if isinstance(x, self._tensor) else type(x).__name__
 
     def _ints(self, x, name: str, n: int):
-        self._on_device(x, name, self._i32)
-        if x.shape != (n,) or (n > 1 and x.stride() != (1,)):
-            raise ValueError(f"{name}: {n} int32 values in a row, got shape {tuple(x.shape)}, strides {x.stride()}")
-        return x.data_ptr()
+        if isinstance(x, self._tensor) and x.dtype is self._i32 and x.get_device() == self._index and x.shape == (n,) and \
+                x.is_contiguous():
+            return x.data_ptr()
+        what = f"shape {tuple(x.shape)}, strides {x.stride()}, " if isinstance(x, self._tensor) else ""
+        raise ValueError(f"{name}: {n} torch.int32 values in a row on {self.device}, got {what}{self._what(x)}")
 
     def _table(self, pos, cu, rows: int, max_rows):
         """The row table's arguments: cu, pos, n_streams, rows, max_rows."""
-        n = len(pos) if isinstance(pos, self.torch.Tensor) and pos.dim() == 1 else -1
+        n = pos.shape[0] if isinstance(pos, self._tensor) and pos.dim() == 1 else -1
         p = self._ints(pos, "pos", n)
-        if cu is None:
-            if rows != n or max_rows not in (None, 1):
-                raise ValueError(f"without cu every stream gives one row: {rows} rows, {n} positions, max_rows {max_rows}")
-            return None, p, n, rows, 1
-        if max_rows is None:
-            raise ValueError("max_rows (the most rows a stream gives) goes with cu")
-        return self._ints(cu, "cu", n + 1), p, n, rows, max_rows
+        if cu is not None:
+            if max_rows is None:
+                raise ValueError("max_rows (the most rows a stream gives) goes with cu")
+            return self._ints(cu, "cu", n + 1), p, n, rows, max_rows
+        if rows != n or max_rows not in (None, 1):
+            raise ValueError(f"without cu every stream gives one row: {rows} rows, {n} positions, max_rows {max_rows}")
+        return None, p, n, rows, 1
 
     def _out(self, out, rows: int, name: str):
         shape = (rows, *self._row)
         if out is None:
             return self.torch.empty(shape, dtype=self._i64, device=self.device)
-        self._on_device(out, name, self._i64)
-        if out.shape != shape or not out.is_contiguous():
-            raise ValueError(f"{name}: a contiguous {shape}, got shape {tuple(out.shape)}, strides {out.stride()}")
-        return out
+        if isinstance(out, self._tensor) and out.dtype is self._i64 and out.get_device() == self._index and \
+                out.shape == shape and out.is_contiguous():
+            return out
+        what = f"shape {tuple(out.shape)}, strides {out.stride()}, " if isinstance(out, self._tensor) else ""
+        raise ValueError(f"{name}: a contiguous {shape} of torch.int64 on {self.device}, got {what}{self._what(out)}")
+
+    def _done(self, rc: int):
+        if rc:
+            raise B2Error(rc, lib().b2_store_last_error(self.h).decode())
+
+    def _open(self):
+        if not self.h:
+            raise ValueError("the store is closed")
+        return self.h
 
     # ---- the operators ----------------------------------------------------------------------------------------
     def write(self, k, v, pos, cu=None, max_rows: int | None = None, layer: int = 0):
         """Hold rows k, v (int64 [rows, n_head, 64], or rows of n_head * 64; rows may be strided, as slices of a qkv row
         are) at their streams' positions."""
-        (pk, ldk), (pv, ldv) = self._rows(k, "k"), self._rows(v, "v")
-        if k.shape[0] != v.shape[0]:
-            raise ValueError(f"{k.shape[0]} rows of keys, {v.shape[0]} of values")
-        self._call(self._write, layer, pk, ldk, pv, ldv, *self._table(pos, cu, k.shape[0], max_rows))
+        h = self._open()
+        (pk, ldk), (pv, ldv), rows = self._rows(k, "k"), self._rows(v, "v"), k.shape[0]
+        if rows != v.shape[0]:
+            raise ValueError(f"{rows} rows of keys, {v.shape[0]} of values")
+        cu, pos, n, rows, most = self._table(pos, cu, rows, max_rows)
+        rc = self._f_write(h, layer, pk, ldk, pv, ldv, cu, pos, n, rows, most, self._stream(self._index))
+        if rc:
+            self._done(rc)
 
     def read(self, pos, cu=None, max_rows: int | None = None, rows: int | None = None, layer: int = 0, out=None):
         """(k, v), int64 [rows, n_head, 64]: the values that the store holds at the rows' positions. rows: how many there
         are (with cu; its last entry). out: two tensors to fill instead of new ones. Rows that no stream has keep what
         `out` held."""
+        h = self._open()
         if rows is None:
             if cu is not None:
                 raise ValueError("rows (cu's last entry) goes with cu")
             rows = len(pos)
-        k, v = (self._out(o, rows, n) for o, n in zip(out if out is not None else (None, None), ("out k", "out v")))
-        self._call(self._read, layer, *self._table(pos, cu, rows, max_rows), k.data_ptr(), v.data_ptr())
+        k, v = (None, None) if out is None else out
+        k, v = self._out(k, rows, "out k"), self._out(v, rows, "out v")
+        cu, pos, n, rows, most = self._table(pos, cu, rows, max_rows)
+        rc = self._f_read(h, layer, cu, pos, n, rows, most, k.data_ptr(), v.data_ptr(), self._stream(self._index))
+        if rc:
+            self._done(rc)
         return k, v
 
     def attend(self, q, pos, cu=None, max_rows: int | None = None, window: int = 0, first=None, layer: int = 0, out=None):
         """The arrival of rows q (int64 [rows, n_head, 64], or rows of n_head * 64, strided or not) over the held keys and
         values: int64 [rows, n_head, 64]. A row at position p sees the positions from the largest of 0, first[stream] (if
         given) and p - window + 1 (if window > 0) to p; one that sees none gets zeros."""
+        h = self._open()
         pq, ldq = self._rows(q, "q")
-        out = self._out(out, q.shape[0], "out")
-        cu, p, n, rows, most = self._table(pos, cu, q.shape[0], max_rows)
-        f = self._ints(first, "first", n) if first is not None else None
-        self._call(self._attend, layer, pq, ldq, cu, p, f, n, rows, most, window, out.data_ptr())
+        rows = q.shape[0]
+        out = self._out(out, rows, "out")
+        cu, pos, n, rows, most = self._table(pos, cu, rows, max_rows)
+        f = None if first is None else self._ints(first, "first", n)
+        rc = self._f_attend(h, layer, pq, ldq, cu, pos, f, n, rows, most, window, out.data_ptr(), self._stream(self._index))
+        if rc:
+            self._done(rc)
         return out
 
     def sync(self):
         """Wait for the device and raise what its checks flagged (rows that do not fit the call, a position past the
         context): the streams concerned were skipped."""
-        if not self.h:
-            raise ValueError("the store is closed")
-        rc = lib().b2_store_sync(self.h)
-        if rc:
-            raise B2Error(rc, lib().b2_store_last_error(self.h).decode())
+        self._done(lib().b2_store_sync(self._open()))
 
     def close(self):
         if getattr(self, "h", None):
