@@ -169,8 +169,8 @@ __global__ void __launch_bounds__(SW_WARPS * 32) k_store_read(Store4 st, StoreRo
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// the arrival of few rows a stream (a decode step), one CTA of SF_WARPS warps per (row, head), or a cluster of CS sharing
-// its keys. The integer table softmax needs the largest score before any weight (a = ARR[start - score] does not factor),
+// the arrival of few rows a stream (a decode step), NW warps per (row, head): one where there are many (no barrier, four
+// units a CTA), else a CTA of 4 or 8, or a cluster of cs CTAs sharing the keys. The integer table softmax needs the largest score before any weight (a = ARR[start - score] does not factor),
 // so the keys are read once for the scores, which stay in shared memory, and the values once after it:
 //   pass 1  32 keys a warp: their codes as the A rows of m16n8k32 (16 c: the digits stay in a byte's upper half, no sign
 //           to extend), the query's two bytes as B columns, so the two products of a key meet in one lane; scores into
@@ -178,7 +178,6 @@ __global__ void __launch_bounds__(SW_WARPS * 32) k_store_read(Store4 st, StoreRo
 //   pass 2  a = ARR[start - score], Z += a, the weight's three bytes into three planes of shared memory
 //   pass 3  num: the planes as the A rows, the values' codes as B (4 keys x 8 dims of nibbles turned by byte permutes)
 // ---------------------------------------------------------------------------------------------------------------------
-constexpr int SF_WARPS = 4;
 constexpr int SF_BYTES = 8;      // shared memory a key: 4 score, 3 planes, 1 value shift
 
 B2_DEV void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -199,6 +198,12 @@ B2_DEV void mma_s8_first(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uin
 // eight 4-bit codes of a word as signed bytes 16 c: the even dims' and the odd dims'
 B2_DEV uint32_t even16(uint32_t w) { return (w << 4) & 0xF0F0F0F0u; }
 B2_DEV uint32_t odd16(uint32_t w) { return w & 0xF0F0F0F0u; }
+
+B2_DEV uint32_t shr_u32(uint32_t x, uint32_t s) {     // 0 for s > 31
+    uint32_t r;
+    asm("shr.u32 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(s));
+    return r;
+}
 
 // the same score from 16 dot (what the tensor cores give of 16 c): r16 = 32 - u - S
 B2_DEV int32_t score16(int32_t dot16, int r16) { return r16 >= 4 ? rnd32(dot16, r16) : store_score(dot16 >> 4, r16 - 4); }
@@ -244,21 +249,30 @@ B2_DEV int query_bytes(int64_t x0, int64_t x1, uint32_t& word) {
     return u;
 }
 
-template <int CS>
-__global__ void __launch_bounds__(SF_WARPS * 32) k_store_attend_few(StoreAttend a, int chunk, int wide) {
+template <int NW>
+B2_DEV void unit_sync() {
+    if (NW == 1) __syncwarp();
+    else __syncthreads();
+}
+
+template <int NW>
+__global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32) k_store_attend_few(StoreAttend a, int chunk, int cs, int wide) {
+    extern __shared__ __align__(16) uint8_t sm[];
+    constexpr int UN = NW == 1 ? 4 : 1;                              // (row, head) units a CTA
+    __shared__ int32_t s_max[NW], s_shift[NW], s_acc[UN][NW][3][64];
+    __shared__ int64_t s_z[NW], s_num[65];
+    __shared__ int2 s_own;                                           // cs > 1: this CTA's largest score and shift
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, wid = NW == 1 ? 0 : warp, un = NW == 1 ? warp : 0;
+    const int g = lane >> 2, j = lane & 3, ut = NW == 1 ? lane : threadIdx.x;      // ut: the thread of the unit
+    uint8_t* const mem = sm + (size_t)un * chunk * SF_BYTES;
+    int32_t* const SC = reinterpret_cast<int32_t*>(mem);             // [chunk]
+    uint8_t* const WP = mem + (size_t)chunk * 4;                     // [3][chunk]
+    int8_t* const VS = reinterpret_cast<int8_t*>(mem + (size_t)chunk * 7);   // [chunk]
     griddep_wait();
     stamp_begin(a.stamp);
     griddep_launch();
-    extern __shared__ __align__(16) uint8_t sm[];
-    int32_t* const SC = reinterpret_cast<int32_t*>(sm);              // [chunk]
-    uint8_t* const WP = sm + (size_t)chunk * 4;                      // [3][chunk]
-    int8_t* const VS = reinterpret_cast<int8_t*>(sm + (size_t)chunk * 7);   // [chunk]
-    __shared__ int32_t s_max[SF_WARPS], s_shift[SF_WARPS], s_acc[SF_WARPS][3][64];
-    __shared__ int64_t s_z[SF_WARPS], s_num[65];
-    __shared__ int2 s_own;                                           // CS > 1: this CTA's largest score and shift
-    const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, g = lane >> 2, j = lane & 3;
-    const int H = a.st.H, h = blockIdx.y, s = blockIdx.z, i = CS > 1 ? blockIdx.x / CS : blockIdx.x;
-    const int rank = CS > 1 ? (int)cluster_rank() : 0;
+    const int H = a.st.H, s = blockIdx.y, rank = cs > 1 ? (int)cluster_rank() : 0;
+    const int unit = NW == 1 ? blockIdx.x * UN + un : blockIdx.x / cs, i = unit / H, h = unit - i * H;
     StoreRun run;
     if (!store_run(a.rw, s, a.st.lim, run, a.err) || i >= run.n) return;   // the same for a whole cluster
     const int row = run.r0 + i, p = run.p0 + i;
@@ -266,50 +280,60 @@ __global__ void __launch_bounds__(SF_WARPS * 32) k_store_attend_few(StoreAttend 
     if (a.first) lo = max(lo, a.first[s]);
     int64_t* const out = a.out + ((size_t)row * H + h) * 64;
     if (lo > p) {
-        if (rank == 0 && threadIdx.x < 64) out[threadIdx.x] = 0;
+        for (int t = ut; t < 64 && rank == 0; t += NW * 32) out[t] = 0;
         return;
     }
-    // blocks of 32 positions; this CTA's are b0 .. b0 + nb - 1
-    const int first_block = lo >> 5, blocks = (p >> 5) - first_block + 1;
-    const int per = CS > 1 ? (blocks + CS - 1) / CS : blocks;
-    const int b0 = first_block + rank * per, nb = max(0, min(per, blocks - rank * per));
-    const size_t base = kv_index(a.rw.slot0 + s, a.layer, h, 0, a.st.L, H, a.st.ctx) + (size_t)b0 * 32;
-    const uint8_t* const K = a.st.k + base * 32;
-    const uint8_t* const V = a.st.v + base * 32;
-    const int8_t* const KS = a.st.ks + base * 2;
-    const int from = lo - b0 * 32, to = p - b0 * 32;                 // visible: from <= local key <= to
-
-    uint32_t word, q0[2], q1[2];                                     // B operands of the two halves
     int64_t x0, x1;
     load_pair(a.q.x + (size_t)row * a.q.ld + h * a.q.hs + 2 * lane, wide & 1, x0, x1);
+    // blocks of 32 positions; this CTA's are b0 .. b0 + nb - 1
+    const int first_block = lo >> 5, blocks = (p >> 5) - first_block + 1;
+    const int per = cs > 1 ? (blocks + cs - 1) / cs : blocks;
+    const int b0 = first_block + rank * per, nb = max(0, min(per, blocks - rank * per));
+    const size_t base = kv_index(a.rw.slot0 + s, a.layer, h, 0, a.st.L, H, a.st.ctx) + (size_t)b0 * 32;
+    const int from = lo - b0 * 32, to = p - b0 * 32;                 // visible: from <= local key <= to
+    const int mine = 16 * (j >> 1) + 8 * (j & 1) + g;                // of a block's keys the one whose score this lane finishes
+
+    // a block's keys: rows 8t + g, words j of both halves; this lane's key's shifts and its value's
+    struct Keys { uint2 w[4]; int ks, vs; };
+    auto keys = [&](int b, Keys& k) {
+        const size_t e = base + (size_t)b * 32;
+        const uint2* const from_ = reinterpret_cast<const uint2*>(a.st.k + (e + g) * 32 + 8 * j);
+#pragma unroll
+        for (int t = 0; t < 4; t++) k.w[t] = from_[t * 32];
+        k.ks = *reinterpret_cast<const int16_t*>(a.st.ks + (e + mine) * 2);
+        k.vs = a.st.vs[e + mine];
+    };
+    // a block's values: word g (dims 8g .. 8g + 7) of keys 8j .. 8j + 7
+    auto values = [&](int b, uint32_t (&w)[8]) {
+        const uint32_t* const from_ = reinterpret_cast<const uint32_t*>(a.st.v + (base + (size_t)b * 32 + 8 * j) * 32 + 4 * g);
+#pragma unroll
+        for (int t = 0; t < 8; t++) w[t] = from_[t * 8];
+    };
+    Keys k;
+    if (wid < nb) keys(wid, k);
+    uint32_t word, q0[2], q1[2];                                     // B operands of the two halves
     const int u = query_bytes(x0, x1, word);
     {
-        const uint32_t pick = (g & 1) ? 0x5151u : 0x4040u;           // odd columns the low bytes
+        const uint32_t pick = (g & 1) ? 0x51u : 0x40u;               // odd columns the low bytes
 #pragma unroll
         for (int x = 0; x < 2; x++) {
             uint32_t w[4];
 #pragma unroll
             for (int b = 0; b < 4; b++) w[b] = __shfl_sync(0xffffffffu, word, 16 * x + 4 * j + b);
-            const uint32_t e01 = __byte_perm(w[0], w[1], pick & 0xFF), e23 = __byte_perm(w[2], w[3], pick & 0xFF);
-            const uint32_t o01 = __byte_perm(w[0], w[1], (pick & 0xFF) + 0x22), o23 = __byte_perm(w[2], w[3], (pick & 0xFF) + 0x22);
-            q0[x] = __byte_perm(e01, e23, 0x5410);
-            q1[x] = __byte_perm(o01, o23, 0x5410);
+            q0[x] = __byte_perm(__byte_perm(w[0], w[1], pick), __byte_perm(w[2], w[3], pick), 0x5410);
+            q1[x] = __byte_perm(__byte_perm(w[0], w[1], pick + 0x22), __byte_perm(w[2], w[3], pick + 0x22), 0x5410);
         }
     }
     int32_t start = -STORE_LIM - 1;
     int M = 0;
-    for (int b = wid; b < nb; b += SF_WARPS) {
-        const int key = b * 32 + 16 * (j >> 1) + 8 * (j & 1) + g;    // the key whose score this lane finishes
-        uint2 w[4];
-#pragma unroll
-        for (int t = 0; t < 4; t++) w[t] = *reinterpret_cast<const uint2*>(K + (size_t)(b * 32 + 8 * t + g) * 32 + 8 * j);
-        const int ksw = *reinterpret_cast<const uint16_t*>(KS + (size_t)key * 2);
-        const int vs = a.st.vs[base + key];
-        int d[2][2][4] = {};                                         // [block of 16][half]
+    for (int b = wid; b < nb; b += NW) {
+        const Keys c = k;
+        if (b + NW < nb) keys(b + NW, k);                            // the next block's, while this one is worked on
+        int d[2][2][4];                                              // [16 keys][half]
 #pragma unroll
         for (int m = 0; m < 2; m++) {
-            mma_s8(d[m][0], even16(w[2 * m].x), even16(w[2 * m + 1].x), odd16(w[2 * m].x), odd16(w[2 * m + 1].x), q0[0], q1[0]);
-            mma_s8(d[m][1], even16(w[2 * m].y), even16(w[2 * m + 1].y), odd16(w[2 * m].y), odd16(w[2 * m + 1].y), q0[1], q1[1]);
+            mma_s8_first(d[m][0], even16(c.w[2 * m].x), even16(c.w[2 * m + 1].x), odd16(c.w[2 * m].x), odd16(c.w[2 * m + 1].x), q0[0], q1[0]);
+            mma_s8_first(d[m][1], even16(c.w[2 * m].y), even16(c.w[2 * m + 1].y), odd16(c.w[2 * m].y), odd16(c.w[2 * m + 1].y), q0[1], q1[1]);
         }
         int dot[2];
 #pragma unroll
@@ -318,63 +342,71 @@ __global__ void __launch_bounds__(SF_WARPS * 32) k_store_attend_few(StoreAttend 
             const int lw = (j & 2) ? ((j & 1) ? d[1][x][3] : d[1][x][1]) : ((j & 1) ? d[0][x][3] : d[0][x][1]);
             dot[x] = 256 * hi + lw;
         }
-        const int s0 = (int8_t)(ksw & 255), s1 = (int8_t)(ksw >> 8), S = max(s0, s1);
+        const int s0 = (int8_t)c.ks, s1 = c.ks >> 8, S = max(s0, s1), key = b * 32 + mine;
         const int32_t sc = score16((dot[0] << (s0 - S + 3)) + (dot[1] << (s1 - S + 3)), 32 - u - S);
         SC[key] = sc;
-        VS[key] = (int8_t)vs;
+        VS[key] = (int8_t)c.vs;
         if (key >= from && key <= to) {
             start = max(start, sc);
-            M = max(M, vs);
+            M = max(M, c.vs);
         }
     }
+    uint32_t v[8];
+    if (wid < nb) values(wid, v);                                    // on their way over the reductions
     start = __reduce_max_sync(0xffffffffu, start);
     M = __reduce_max_sync(0xffffffffu, M);
-    if (lane == 0) { s_max[wid] = start; s_shift[wid] = M; }
-    __syncthreads();
+    if (NW > 1) {
+        if (lane == 0) { s_max[wid] = start; s_shift[wid] = M; }
+        __syncthreads();
 #pragma unroll
-    for (int k = 0; k < SF_WARPS; k++) {
-        start = max(start, s_max[k]);
-        M = max(M, s_shift[k]);
-    }
-    if (CS > 1) {
-        if (threadIdx.x == 0) s_own = make_int2(start, M);
-        cluster_sync();
-#pragma unroll
-        for (int k = 0; k < CS; k++) {
-            const int64_t o = ld_dsmem(mapa(saddr(&s_own), (uint32_t)k));
-            start = max(start, (int32_t)o);
-            M = max(M, (int)(o >> 32));
+        for (int w = 0; w < NW; w++) {
+            start = max(start, s_max[w]);
+            M = max(M, s_shift[w]);
         }
+        if (cs > 1) {
+            if (threadIdx.x == 0) s_own = make_int2(start, M);
+            cluster_sync();
+            for (int c = 0; c < cs; c++) {
+                const int64_t o = ld_dsmem(mapa(saddr(&s_own), (uint32_t)c));
+                start = max(start, (int32_t)o);
+                M = max(M, (int)(o >> 32));
+            }
+        }
+    } else {
+        __syncwarp();
     }
     // ---- weights: four keys a thread
     int64_t z = 0;
-    for (int k = threadIdx.x * 4; k < nb * 32; k += SF_WARPS * 128) {
-        const int4 sc = *reinterpret_cast<const int4*>(SC + k);
-        const uint32_t v4 = *reinterpret_cast<const uint32_t*>(VS + k);
+    for (int t = ut * 4; t < nb * 32; t += NW * 128) {
+        const int4 sc = *reinterpret_cast<const int4*>(SC + t);
+        const uint32_t v4 = *reinterpret_cast<const uint32_t*>(VS + t);
         const int scs[4] = {sc.x, sc.y, sc.z, sc.w};
         uint32_t w[4];
+        int32_t four = 0;                                            // four entries of at most 2^24
 #pragma unroll
-        for (int t = 0; t < 4; t++) {
-            const int d = start - scs[t];
-            const bool seen = k + t >= from && k + t <= to && d < a.alen;
+        for (int x = 0; x < 4; x++) {
+            const int d = start - scs[x];
+            const bool seen = t + x >= from && t + x <= to && d < a.alen;
             const int av = seen ? __ldg(a.ARR + d) : 0;
-            z += av;
-            w[t] = seen ? (uint32_t)rnd32(av, min(STORE_W_SHIFT + M - (int)(int8_t)(v4 >> (8 * t)), 26)) : 0u;
+            four += av;
+            w[x] = (shr_u32(av, M - (int)(int8_t)(v4 >> (8 * x))) + 1) >> 1;
         }
+        z += four;
         uint32_t r[3];
         turn3(w, r[0], r[1], r[2]);
 #pragma unroll
-        for (int b = 0; b < 3; b++) *reinterpret_cast<uint32_t*>(WP + (size_t)b * chunk + k) = r[b];
+        for (int b = 0; b < 3; b++) *reinterpret_cast<uint32_t*>(WP + (size_t)b * chunk + t) = r[b];
     }
     z = warp_sum64(z);
-    if (lane == 0) s_z[wid] = z;
-    __syncthreads();
-    // ---- values: a lane takes word g (dims 8g .. 8g + 7) of keys 8j .. 8j + 7 of a block of 32
+    if (NW > 1 && lane == 0) s_z[wid] = z;
+    unit_sync<NW>();
+    // ---- values
     int acc[8][4] = {};
-    for (int b = wid; b < nb; b += SF_WARPS) {
+    for (int b = wid; b < nb; b += NW) {
         uint32_t w[8];
 #pragma unroll
-        for (int t = 0; t < 8; t++) w[t] = *reinterpret_cast<const uint32_t*>(V + (size_t)(b * 32 + 8 * j + t) * 32 + 4 * g);
+        for (int t = 0; t < 8; t++) w[t] = v[t];
+        if (b + NW < nb) values(b + NW, v);
         uint2 p8 = make_uint2(0, 0);
         if (g < 3) p8 = *reinterpret_cast<const uint2*>(WP + (size_t)g * chunk + b * 32 + 8 * j);
         uint32_t r0[4], r1[4];
@@ -390,49 +422,61 @@ __global__ void __launch_bounds__(SF_WARPS * 32) k_store_attend_few(StoreAttend 
     if (g < 3) {
 #pragma unroll
         for (int t = 0; t < 8; t++) {
-            s_acc[wid][g][16 * j + t] = acc[t][0];
-            s_acc[wid][g][16 * j + 8 + t] = acc[t][1];
+            s_acc[un][wid][g][16 * j + t] = acc[t][0];
+            s_acc[un][wid][g][16 * j + 8 + t] = acc[t][1];
         }
     }
-    __syncthreads();
-    int64_t num = 0;
-    if (threadIdx.x < 64) {
+    unit_sync<NW>();
+    // a thread finishes dim ut (a lone warp's lanes dim ut + 32 as well)
+    constexpr int DIMS = NW == 1 ? 2 : 1;
+    int64_t num[DIMS];
 #pragma unroll
-        for (int b = 0; b < 3; b++) {
-            int t = 0;
+    for (int x = 0; x < DIMS; x++) {
+        num[x] = 0;
+        if (ut + 32 * x < 64) {
 #pragma unroll
-            for (int k = 0; k < SF_WARPS; k++) t += s_acc[k][b][threadIdx.x];
-            num += (int64_t)t << (8 * b);
-        }
-        z = 0;
+            for (int b = 0; b < 3; b++) {
+                int t = 0;
 #pragma unroll
-        for (int k = 0; k < SF_WARPS; k++) z += s_z[k];
-    }
-    if (CS > 1) {
-        if (threadIdx.x < 64) {
-            s_num[threadIdx.x] = num;
-            if (threadIdx.x == 0) s_num[64] = z;
-        }
-        cluster_sync();
-        if (rank == 0 && threadIdx.x < 64) {
-            num = z = 0;
-#pragma unroll
-            for (int k = 0; k < CS; k++) {
-                num += ld_dsmem(mapa(saddr(&s_num[threadIdx.x]), (uint32_t)k));
-                z += ld_dsmem(mapa(saddr(&s_num[64]), (uint32_t)k));
+                for (int w = 0; w < NW; w++) t += s_acc[un][w][b][ut + 32 * x];
+                num[x] += (int64_t)t << (8 * b);
             }
         }
     }
-    if (rank == 0 && threadIdx.x < 64) {
-        const int64_t F = 65536ll * (M + STORE_W_SHIFT) - log2fix(z, a.LOG2);
-        const int64_t y = power(num >> 4, F, a.EXP2);                // the tiles hold 16 c
-        out[threadIdx.x] = y;
-        if (a.or_out) {
-            const uint64_t o = warp_or64(mag(y));
-            if (lane == 0) atomicOr((unsigned long long*)&a.or_out[row], (unsigned long long)o);
+    if (NW > 1) {
+        z = 0;
+#pragma unroll
+        for (int w = 0; w < NW; w++) z += s_z[w];
+        if (cs > 1) {
+            if (threadIdx.x < 64) {
+                s_num[threadIdx.x] = num[0];
+                if (threadIdx.x == 0) s_num[64] = z;
+            }
+            cluster_sync();
+            if (rank == 0 && threadIdx.x < 64) {
+                num[0] = z = 0;
+                for (int c = 0; c < cs; c++) {
+                    num[0] += ld_dsmem(mapa(saddr(&s_num[threadIdx.x]), (uint32_t)c));
+                    z += ld_dsmem(mapa(saddr(&s_num[64]), (uint32_t)c));
+                }
+            }
         }
     }
-    if (CS > 1) cluster_sync();                                      // rank 0 has read the others' sums
+    if (rank == 0 && ut < 64) {
+        const int64_t F = 65536ll * (M + STORE_W_SHIFT) - log2fix(z, a.LOG2);
+        uint64_t any = 0;
+#pragma unroll
+        for (int x = 0; x < DIMS; x++) {
+            const int64_t y = power(num[x] >> 4, F, a.EXP2);         // the tiles hold 16 c
+            out[ut + 32 * x] = y;
+            any |= mag(y);
+        }
+        if (a.or_out) {
+            any = warp_or64(any);
+            if (lane == 0) atomicOr((unsigned long long*)&a.or_out[row], (unsigned long long)any);
+        }
+    }
+    if (NW > 1 && cs > 1) cluster_sync();                            // rank 0 has read the others' sums
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -485,11 +529,6 @@ B2_DEV uint32_t seen(int from, int to) {
 }
 B2_DEV void copy16(void* to, const void* from) {      // 16 bytes, asynchronously, past L1
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(saddr(to)), "l"(from) : "memory");
-}
-B2_DEV uint32_t shr_u32(uint32_t x, uint32_t s) {     // 0 for s > 31
-    uint32_t r;
-    asm("shr.u32 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(s));
-    return r;
 }
 
 __global__ void __launch_bounds__(SM_THREADS, 2) k_store_attend_many(StoreAttend a, int tiles, int cs, int wide) {
@@ -962,6 +1001,8 @@ cudaError_t store_read(const Store4& st, const StoreRows& rw, int layer, int64_t
 constexpr int SM_FROM_ROWS = 4, SM_FIXED = 4;
 constexpr int SM_SMEM_MOST = 200 * 1024;
 constexpr int SF_MOST_KEYS = 8192;   // of a CTA: 64 KB of shared memory
+constexpr int SF_WARP_UNITS = 12, SF_WARP_BLOCKS = 32;   // a warp a unit: from so many units an SM on, up to 1,024 keys (32 KB a CTA)
+constexpr int SF_LONG = 16;          // blocks of 32 keys a CTA from which eight warps take them
 
 size_t many_smem(int alen) { return sizeof(SmShared) + (size_t)(alen + 1) * 4; }
 
@@ -969,8 +1010,6 @@ cudaError_t store_init(int alen, StorePlan& plan) {
     int device = 0;
     cudaError_t e = cudaGetDevice(&device);
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&plan.sms, cudaDevAttrMultiProcessorCount, device);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(k_store_attend_few<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, SF_MOST_KEYS * SF_BYTES);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(k_store_attend_few<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, SF_MOST_KEYS * SF_BYTES);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(k_store_attend_few<4>, cudaFuncAttributeMaxDynamicSharedMemorySize, SF_MOST_KEYS * SF_BYTES);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(k_store_attend_few<8>, cudaFuncAttributeMaxDynamicSharedMemorySize, SF_MOST_KEYS * SF_BYTES);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(k_store_attend_many, cudaFuncAttributeMaxDynamicSharedMemorySize, SM_SMEM_MOST);
@@ -1027,17 +1066,16 @@ cudaError_t store_attend(const StoreAttend& a, StoreLaunch how) {
     int blocks = (a.st.lim + 31) / 32;
     if (a.window > 0 && a.window < a.st.lim) blocks = std::min(blocks, (a.window + 30) / 32 + 1);
     const int64_t units = (int64_t)a.rw.n_streams * a.rw.max_rows * a.st.H;
-    int cs = 1;
-    while (cs < 8 && ((units * cs < how.plan->sms * 2 && blocks >= cs * 8) || blocks * 32 > cs * SF_MOST_KEYS)) cs *= 2;
-    const int chunk = (blocks + cs - 1) / cs * 32;
-    const dim3 grid(a.rw.max_rows * cs, a.st.H, a.rw.n_streams);
-    const size_t smem = (size_t)chunk * SF_BYTES;
-    switch (cs) {
-        case 1: return store_launch(how, k_store_attend_few<1>, grid, SF_WARPS * 32, smem, 1, a, chunk, wide);
-        case 2: return store_launch(how, k_store_attend_few<2>, grid, SF_WARPS * 32, smem, 2, a, chunk, wide);
-        case 4: return store_launch(how, k_store_attend_few<4>, grid, SF_WARPS * 32, smem, 4, a, chunk, wide);
-        default: return store_launch(how, k_store_attend_few<8>, grid, SF_WARPS * 32, smem, 8, a, chunk, wide);
+    if (units >= (int64_t)SF_WARP_UNITS * how.plan->sms && blocks <= SF_WARP_BLOCKS) {
+        const dim3 grid((unsigned)(((int64_t)a.rw.max_rows * a.st.H + 3) / 4), a.rw.n_streams);
+        return store_launch(how, k_store_attend_few<1>, grid, 128, (size_t)blocks * 32 * SF_BYTES * 4, 1, a, blocks * 32, 1, wide);
     }
+    int cs = 1;
+    while (cs < STORE_MAX_CLUSTER && ((units * cs < how.plan->sms * 2 && blocks >= cs * 8) || blocks * 32 > cs * SF_MOST_KEYS)) cs *= 2;
+    const int chunk = (blocks + cs - 1) / cs * 32;
+    const dim3 grid((unsigned)((int64_t)a.rw.max_rows * a.st.H * cs), a.rw.n_streams);
+    if (chunk >= SF_LONG * 32) return store_launch(how, k_store_attend_few<8>, grid, 256, (size_t)chunk * SF_BYTES, cs, a, chunk, cs, wide);
+    return store_launch(how, k_store_attend_few<4>, grid, 128, (size_t)chunk * SF_BYTES, cs, a, chunk, cs, wide);
 }
 
 }  // namespace b2

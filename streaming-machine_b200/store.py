@@ -151,7 +151,10 @@ class Store:
         h = self._open()
         pq, ldq = self._rows(q, "q")
         rows = q.shape[0]
-        out = self._out(out, rows, "out")
+        if out is None and q.dim() == 3 and q.is_contiguous():
+            out = self.torch.empty_like(q)               # (what _out makes, in less time)
+        else:
+            out = self._out(out, rows, "out")
         cu, pos, n, rows, most = self._table(pos, cu, rows, max_rows)
         f = None if first is None else self._ints(first, "first", n)
         rc = self._f_attend(h, layer, pq, ldq, cu, pos, f, n, rows, most, window, out.data_ptr(), self._stream(self._index))
