@@ -256,9 +256,10 @@ B2_DEV void unit_sync() {
 }
 
 template <int NW>
-__global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32) k_store_attend_few(StoreAttend a, int chunk, int cs, int wide) {
+__global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, NW == 1 ? 7 : (NW == 4 ? 6 : (NW == 8 ? 3 : 1))) k_store_attend_few(StoreAttend a, int chunk, int cs, int wide) {
     extern __shared__ __align__(16) uint8_t sm[];
     constexpr int UN = NW == 1 ? 4 : 1;                              // (row, head) units a CTA
+    constexpr int PF = NW == 16 ? 2 : 1;                             // blocks of 32 keys that a warp has on their way
     __shared__ int32_t s_max[NW], s_shift[NW], s_acc[UN][NW][3][64];
     __shared__ int64_t s_z[NW], s_num[65];
     __shared__ int2 s_own;                                           // cs > 1: this CTA's largest score and shift
@@ -309,8 +310,10 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32) k_store_attend_few(St
 #pragma unroll
         for (int t = 0; t < 8; t++) w[t] = from_[t * 8];
     };
-    Keys k;
-    if (wid < nb) keys(wid, k);
+    Keys k[PF];
+#pragma unroll
+    for (int f = 0; f < PF; f++)
+        if (wid + f * NW < nb) keys(wid + f * NW, k[f]);
     uint32_t word, q0[2], q1[2];                                     // B operands of the two halves
     const int u = query_bytes(x0, x1, word);
     {
@@ -326,9 +329,7 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32) k_store_attend_few(St
     }
     int32_t start = -STORE_LIM - 1;
     int M = 0;
-    for (int b = wid; b < nb; b += NW) {
-        const Keys c = k;
-        if (b + NW < nb) keys(b + NW, k);                            // the next block's, while this one is worked on
+    auto score_block = [&](int b, const Keys& c) {
         int d[2][2][4];                                              // [16 keys][half]
 #pragma unroll
         for (int m = 0; m < 2; m++) {
@@ -350,9 +351,22 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32) k_store_attend_few(St
             start = max(start, sc);
             M = max(M, c.vs);
         }
+    };
+    for (int b = wid; b < nb; b += NW * PF) {
+        Keys c[PF];
+#pragma unroll
+        for (int f = 0; f < PF; f++) c[f] = k[f];
+#pragma unroll
+        for (int f = 0; f < PF; f++)                                 // the next blocks', while these are worked on
+            if (b + (PF + f) * NW < nb) keys(b + (PF + f) * NW, k[f]);
+#pragma unroll
+        for (int f = 0; f < PF; f++)
+            if (b + f * NW < nb) score_block(b + f * NW, c[f]);
     }
-    uint32_t v[8];
-    if (wid < nb) values(wid, v);                                    // on their way over the reductions
+    uint32_t v[PF][8];
+#pragma unroll
+    for (int f = 0; f < PF; f++)
+        if (wid + f * NW < nb) values(wid + f * NW, v[f]);           // on their way over the reductions
     start = __reduce_max_sync(0xffffffffu, start);
     M = __reduce_max_sync(0xffffffffu, M);
     if (NW > 1) {
@@ -402,20 +416,28 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32) k_store_attend_few(St
     unit_sync<NW>();
     // ---- values
     int acc[8][4] = {};
-    for (int b = wid; b < nb; b += NW) {
-        uint32_t w[8];
+    for (int b = wid; b < nb; b += NW * PF) {
+        uint32_t w[PF][8];
 #pragma unroll
-        for (int t = 0; t < 8; t++) w[t] = v[t];
-        if (b + NW < nb) values(b + NW, v);
-        uint2 p8 = make_uint2(0, 0);
-        if (g < 3) p8 = *reinterpret_cast<const uint2*>(WP + (size_t)g * chunk + b * 32 + 8 * j);
-        uint32_t r0[4], r1[4];
-        turn4(w, r0);
-        turn4(w + 4, r1);
+        for (int f = 0; f < PF; f++)
 #pragma unroll
-        for (int t = 0; t < 4; t++) {
-            mma_u8s8(acc[2 * t], p8.x, 0, p8.y, 0, even16(r0[t]), even16(r1[t]));
-            mma_u8s8(acc[2 * t + 1], p8.x, 0, p8.y, 0, odd16(r0[t]), odd16(r1[t]));
+            for (int t = 0; t < 8; t++) w[f][t] = v[f][t];
+#pragma unroll
+        for (int f = 0; f < PF; f++)
+            if (b + (PF + f) * NW < nb) values(b + (PF + f) * NW, v[f]);
+#pragma unroll
+        for (int f = 0; f < PF; f++) {
+            if (b + f * NW >= nb) break;
+            uint2 p8 = make_uint2(0, 0);
+            if (g < 3) p8 = *reinterpret_cast<const uint2*>(WP + (size_t)g * chunk + (b + f * NW) * 32 + 8 * j);
+            uint32_t r0[4], r1[4];
+            turn4(w[f], r0);
+            turn4(w[f] + 4, r1);
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+                mma_u8s8(acc[2 * t], p8.x, 0, p8.y, 0, even16(r0[t]), even16(r1[t]));
+                mma_u8s8(acc[2 * t + 1], p8.x, 0, p8.y, 0, odd16(r0[t]), odd16(r1[t]));
+            }
         }
     }
     // row g of the tiles is plane g; columns 2j, 2j + 1 of tile t are dims 16j + t and 16j + 8 + t
@@ -464,10 +486,13 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32) k_store_attend_few(St
     }
     if (rank == 0 && ut < 64) {
         const int64_t F = 65536ll * (M + STORE_W_SHIFT) - log2fix(z, a.LOG2);
+        const uint32_t e = (uint32_t)__ldg(a.EXP2 + (F & 0xFFFF));
+        const int down = 19 - (int)(F >> 16);                        // power's shift less one, and 4 digits more: 16 c
         uint64_t any = 0;
 #pragma unroll
         for (int x = 0; x < DIMS; x++) {
-            const int64_t y = power(num[x] >> 4, F, a.EXP2);         // the tiles hold 16 c
+            const int64_t n = num[x] * (int64_t)e;                   // at most 2^46 2^17
+            const int64_t y = down >= 0 ? ((n >> down) + 1) >> 1 : (int64_t)((uint64_t)n << (-1 - down));
             out[ut + 32 * x] = y;
             any |= mag(y);
         }
@@ -1002,7 +1027,7 @@ constexpr int SM_FROM_ROWS = 4, SM_FIXED = 4;
 constexpr int SM_SMEM_MOST = 200 * 1024;
 constexpr int SF_MOST_KEYS = 8192;   // of a CTA: 64 KB of shared memory
 constexpr int SF_WARP_UNITS = 12, SF_WARP_BLOCKS = 32;   // a warp a unit: from so many units an SM on, up to 1,024 keys (32 KB a CTA)
-constexpr int SF_LONG = 16;          // blocks of 32 keys a CTA from which eight warps take them
+constexpr int SF_LONG = 32, SF_VERY_LONG = 64;   // blocks of 32 keys
 
 size_t many_smem(int alen) { return sizeof(SmShared) + (size_t)(alen + 1) * 4; }
 
@@ -1012,6 +1037,7 @@ cudaError_t store_init(int alen, StorePlan& plan) {
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&plan.sms, cudaDevAttrMultiProcessorCount, device);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(k_store_attend_few<4>, cudaFuncAttributeMaxDynamicSharedMemorySize, SF_MOST_KEYS * SF_BYTES);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(k_store_attend_few<8>, cudaFuncAttributeMaxDynamicSharedMemorySize, SF_MOST_KEYS * SF_BYTES);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(k_store_attend_few<16>, cudaFuncAttributeMaxDynamicSharedMemorySize, SF_MOST_KEYS * SF_BYTES);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(k_store_attend_many, cudaFuncAttributeMaxDynamicSharedMemorySize, SM_SMEM_MOST);
     if (e != cudaSuccess) return e;
     int fit = 0;
@@ -1070,12 +1096,20 @@ cudaError_t store_attend(const StoreAttend& a, StoreLaunch how) {
         const dim3 grid((unsigned)(((int64_t)a.rw.max_rows * a.st.H + 3) / 4), a.rw.n_streams);
         return store_launch(how, k_store_attend_few<1>, grid, 128, (size_t)blocks * 32 * SF_BYTES * 4, 1, a, blocks * 32, 1, wide);
     }
+    // a cluster costs about 1.3 us (its barriers), a warp's block of 32 keys 0.5 (from L2) to 1.2 us (from HBM): the keys are
+    // split where that leaves half the SMs idle, and while there is a long run of keys for every CTA of two an SM
     int cs = 1;
-    while (cs < STORE_MAX_CLUSTER && ((units * cs < how.plan->sms * 2 && blocks >= cs * 8) || blocks * 32 > cs * SF_MOST_KEYS)) cs *= 2;
-    const int chunk = (blocks + cs - 1) / cs * 32;
+    while (cs < STORE_MAX_CLUSTER && ((units * cs * 2 <= how.plan->sms && blocks >= SF_LONG && blocks >= cs * 8) ||
+                                      (units * cs < how.plan->sms * 2 && blocks >= cs * SF_VERY_LONG) ||
+                                      blocks * 32 > cs * SF_MOST_KEYS))
+        cs *= 2;
+    const int each = (blocks + cs - 1) / cs, chunk = each * 32;
     const dim3 grid((unsigned)((int64_t)a.rw.max_rows * a.st.H * cs), a.rw.n_streams);
-    if (chunk >= SF_LONG * 32) return store_launch(how, k_store_attend_few<8>, grid, 256, (size_t)chunk * SF_BYTES, cs, a, chunk, cs, wide);
-    return store_launch(how, k_store_attend_few<4>, grid, 128, (size_t)chunk * SF_BYTES, cs, a, chunk, cs, wide);
+    const size_t smem = (size_t)chunk * SF_BYTES;
+    if (each >= SF_VERY_LONG && units * cs <= how.plan->sms)       // 16 warps: one CTA an SM
+        return store_launch(how, k_store_attend_few<16>, grid, 512, smem, cs, a, chunk, cs, wide);
+    if (each >= SF_LONG) return store_launch(how, k_store_attend_few<8>, grid, 256, smem, cs, a, chunk, cs, wide);
+    return store_launch(how, k_store_attend_few<4>, grid, 128, smem, cs, a, chunk, cs, wide);
 }
 
 }  // namespace b2
