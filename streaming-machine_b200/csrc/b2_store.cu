@@ -535,9 +535,9 @@ struct SmShared {
         uint32_t q[SM_ROWS][33];         // the rows' query bytes, until every lane has its operands
         uint4 p[SM_WARPS][3][32];        // a block's weights on the way to the pair's other warp
     };
-    unsigned long long z[SM_ROWS];
-    int2 ym[SM_ROWS];                    // the CTA's largest score (twice) and value shift
-    int32_t u[SM_ROWS], umax, slow;
+    int64_t z[SM_WARPS][16];             // a warp's rows: their sums of entries,
+    int2 ym[SM_WARPS][16];               // largest score (twice) and value shift
+    int32_t u[SM_ROWS], most[SM_WARPS], slow;
 };
 
 // bytes c 2^up of the word's even and odd codes; up = 0 .. 3: c + 8 moves up, 8 2^up comes off again (less: 128 - 8 2^up)
@@ -569,26 +569,34 @@ __global__ void __launch_bounds__(SM_THREADS, 2) k_store_attend_many(StoreAttend
     griddep_wait();                       // (the table never changes: its copy need not wait)
     stamp_begin(a.stamp);
     griddep_launch();
-    const uint32_t items = (uint32_t)(tiles * H * a.rw.n_streams), step = gridDim.x / cs;   // below 2^31 (the launch sees to it)
+    // items: streams run fastest, then heads, then the tiles of rows from the last on; below 2^31 (the launch sees to it).
+    // One cluster's next item is `step` further, taken apart once
+    const int n_str = a.rw.n_streams, step = gridDim.x / cs;
+    const int d_s = step % n_str, d_h = step / n_str % H, d_t = step / n_str / H;
+    int s = blockIdx.x / cs % n_str, h = blockIdx.x / cs / n_str % H, t_ = blockIdx.x / cs / n_str / H;
     // an item's entries of the row table, read one item ahead
     int n_r0 = 0, n_r1 = 0, n_pos = 0, n_first = 0;
-    auto ahead = [&](uint32_t item) {
-        if (item < items) {
-            const int s = item % a.rw.n_streams;
+    auto ahead = [&](int s, int t) {
+        if (t < tiles) {
             n_r0 = a.rw.cu ? a.rw.cu[s] : s;
             n_r1 = a.rw.cu ? a.rw.cu[s + 1] : s + 1;
             n_pos = a.rw.pos[s];
             n_first = a.first ? a.first[s] : 0;
         }
     };
-    ahead(blockIdx.x / cs);
-    for (uint32_t item = blockIdx.x / cs; item < items; item += step) {
-        const uint32_t sh_ = item / a.rw.n_streams;
-        const int s = item - sh_ * a.rw.n_streams, h = sh_ % H, tile = tiles - 1 - (int)(sh_ / H);
+    ahead(s, t_);
+    int n_s, n_h, n_t;
+    for (; t_ < tiles; s = n_s, h = n_h, t_ = n_t) {
+        n_s = s + d_s;
+        n_h = h + d_h;
+        n_t = t_ + d_t;
+        if (n_s >= n_str) { n_s -= n_str; n_h++; }
+        if (n_h >= H) { n_h -= H; n_t++; }
+        const int tile = tiles - 1 - t_;
         StoreRun run;
         const bool some = store_run(a.rw, n_r0, n_r1, n_pos, a.st.lim, run, a.err);
         const int from = max(0, n_first);
-        ahead(item + step);
+        ahead(n_s, n_t);
         if (!some || tile * ROWS >= run.n) continue;
         const int i0 = tile * ROWS, nr = min(ROWS, run.n - i0);
         const int win = a.window > 0 ? a.window : 0x40000000;
@@ -626,15 +634,7 @@ __global__ void __launch_bounds__(SM_THREADS, 2) k_store_attend_many(StoreAttend
         };
         fetch(t0, false);
         fetch(t0 + 1, false);
-        if (tid == 0) {
-            S.umax = 0;
-            S.slow = 0;
-        }
-        for (int r = tid; r < ROWS; r += SM_THREADS) {
-            S.ym[r] = make_int2(INT32_MIN, 0);
-            S.z[r] = 0;
-        }
-        __syncthreads();
+        if (tid == 0) S.slow = 0;
         {
             int64_t x[SM_ROWS / SM_WARPS][2];
 #pragma unroll
@@ -651,7 +651,7 @@ __global__ void __launch_bounds__(SM_THREADS, 2) k_store_attend_many(StoreAttend
                 if (lane == 0) S.u[r] = u;
                 most = max(most, u);
             }
-            if (lane == 0) atomicMax(&S.umax, most);
+            if (lane == 0) S.most[wid] = most;
         }
         __syncthreads();
         // this lane's rows and their A operands: [plane][half][even row g, even g + 8, odd g, odd g + 8]
@@ -669,7 +669,10 @@ __global__ void __launch_bounds__(SM_THREADS, 2) k_store_attend_many(StoreAttend
                 q[1][x][y] = __byte_perm(l0, l1, 0x5410);
                 q[1][x][2 + y] = __byte_perm(l0, l1, 0x7632);
             }
-        const int ua = S.u[ra], ub = S.u[rb], umax = S.umax;
+        const int ua = S.u[ra], ub = S.u[rb];
+        int umax = 0;
+#pragma unroll
+        for (int w = 0; w < SM_WARPS; w++) umax = max(umax, S.most[w]);
         const int pa = min(p_first + ra, p_last), pb = min(p_first + rb, p_last);      // rows past the last repeat it
         const int la = max(from, pa - win + 1), lb = max(from, pb - win + 1);
         const int w_p0 = min(p_first + pair * 16, p_last), w_p1 = min(p_first + pair * 16 + 15, p_last);
@@ -791,32 +794,26 @@ __global__ void __launch_bounds__(SM_THREADS, 2) k_store_attend_many(StoreAttend
             mb = max(mb, __shfl_xor_sync(0xffffffffu, mb, o));
         }
         if (j == 0) {
-            atomicMax(&S.ym[ra].x, ya);
-            atomicMax(&S.ym[rb].x, yb);
-            atomicMax(&S.ym[ra].y, ma);
-            atomicMax(&S.ym[rb].y, mb);
+            S.ym[wid][g] = make_int2(ya, ma);
+            S.ym[wid][g + 8] = make_int2(yb, mb);
         }
-        if (cs > 1) {
-            cluster_sync();
-            for (int k = 0; k < cs; k++) {
-                const int64_t oa = ld_dsmem(mapa(saddr(&S.ym[ra]), (uint32_t)k)), ob = ld_dsmem(mapa(saddr(&S.ym[rb]), (uint32_t)k));
+        if (cs > 1) cluster_sync();
+        else __syncthreads();
+        for (int k = 0; k < cs; k++)
+#pragma unroll
+            for (int w = 0; w < 2; w++) {            // the pair's two warps, in every CTA of the cluster
+                const int2* const at = &S.ym[2 * pair + w][g];
+                const int64_t oa = cs > 1 ? ld_dsmem(mapa(saddr(at), (uint32_t)k)) : *reinterpret_cast<const int64_t*>(at);
+                const int64_t ob = cs > 1 ? ld_dsmem(mapa(saddr(at + 8), (uint32_t)k)) : *reinterpret_cast<const int64_t*>(at + 8);
                 ya = max(ya, (int32_t)oa);
                 yb = max(yb, (int32_t)ob);
                 ma = max(ma, (int)(oa >> 32));
                 mb = max(mb, (int)(ob >> 32));
             }
-        } else {
-            __syncthreads();
-            ya = S.ym[ra].x;
-            yb = S.ym[rb].x;
-            ma = S.ym[ra].y;
-            mb = S.ym[rb].y;
-        }
         // the next item's queries into L2 (a row is four lines)
-        if (item + step < items && n_r0 >= 0 && n_r1 <= a.rw.rows) {
-            const uint32_t nsh = (item + step) / a.rw.n_streams;
-            const int row = n_r0 + (tiles - 1 - (int)(nsh / H)) * ROWS + (tid >> 2);
-            if (row < n_r1) asm volatile("prefetch.global.L2 [%0];" ::"l"(a.q.x + (size_t)row * a.q.ld + (int)(nsh % H) * a.q.hs + (tid & 3) * 16));
+        if (n_t < tiles && n_r0 >= 0 && n_r1 <= a.rw.rows) {
+            const int row = n_r0 + (tiles - 1 - n_t) * ROWS + (tid >> 2);
+            if (row < n_r1) asm volatile("prefetch.global.L2 [%0];" ::"l"(a.q.x + (size_t)row * a.q.ld + n_h * a.q.hs + (tid & 3) * 16));
         }
         // twice the largest score: a digit below the last rounds up with it
         const uint32_t sa = (uint32_t)(((ya >> 1) + (ya & 1)) * 2), sb = (uint32_t)(((yb >> 1) + (yb & 1)) * 2);
@@ -899,8 +896,15 @@ __global__ void __launch_bounds__(SM_THREADS, 2) k_store_attend_many(StoreAttend
         };
         if (slow) pass2(std::true_type());
         else pass2(std::false_type());
-        atomicAdd(&S.z[ra], (unsigned long long)za);
-        atomicAdd(&S.z[rb], (unsigned long long)zb);
+#pragma unroll
+        for (int o = 1; o < 4; o <<= 1) {
+            za += __shfl_xor_sync(0xffffffffu, za, o);
+            zb += __shfl_xor_sync(0xffffffffu, zb, o);
+        }
+        if (j == 0) {
+            S.z[wid][g] = za;
+            S.z[wid][g + 8] = zb;
+        }
         // a lane's 8 sums of each of its rows; a cluster's CTAs lay theirs out (in place of the tiles) a row at a time and
         // each finishes some of them
         int64_t* const part = reinterpret_cast<int64_t*>(S.tile);     // [warp][8][32 lanes]
@@ -914,7 +918,12 @@ __global__ void __launch_bounds__(SM_THREADS, 2) k_store_attend_many(StoreAttend
 #pragma unroll
         for (int y = 0; y < 2; y++) {
             int64_t z = 0;
-            for (int k = 0; k < cs; k++) z += cs > 1 ? ld_dsmem(mapa(saddr(&S.z[y ? rb : ra]), (uint32_t)k)) : (int64_t)S.z[y ? rb : ra];
+            for (int k = 0; k < cs; k++)
+#pragma unroll
+                for (int w = 0; w < 2; w++) {
+                    const int64_t* const at = &S.z[2 * pair + w][g + 8 * y];
+                    z += cs > 1 ? ld_dsmem(mapa(saddr(at), (uint32_t)k)) : *at;
+                }
             const bool none = (y ? lb > pb : la > pa) || z == 0;
             const int64_t F = 65536ll * ((y ? mb : ma) + STORE_W_SHIFT) - log2fix(none ? 1 : z, a.LOG2);
             e[y] = none ? 0 : (uint32_t)__ldg(a.EXP2 + (F & 0xFFFF));
@@ -933,12 +942,20 @@ __global__ void __launch_bounds__(SM_THREADS, 2) k_store_attend_many(StoreAttend
             int64_t o[8];
 #pragma unroll
             for (int x = 0; x < 8; x++) {
-                if (cs > 1 && (x >> 1) % cs != rank) continue;
-                int64_t num = cs > 1 ? 0 : sum(x >> 2, x & 3, y);
-                if (cs > 1)
-                    for (int m = 0; m < cs; m++) num += ld_dsmem(mapa(saddr(&part[(wid * 8 + x) * 32 + lane]), (uint32_t)m));
-                num *= (int64_t)e[y];                                  // at most 2^46 2^17
-                o[x] = sh[y] >= 0 ? ((num >> sh[y]) + 1) >> 1 : (int64_t)((uint64_t)num << (-1 - sh[y]));
+                o[x] = 0;
+                if (cs == 1) {
+                    o[x] = sum(x >> 2, x & 3, y);
+                } else if ((x >> 1) % cs == rank) {
+                    for (int m = 0; m < cs; m++) o[x] += ld_dsmem(mapa(saddr(&part[(wid * 8 + x) * 32 + lane]), (uint32_t)m));
+                }
+                o[x] *= (int64_t)e[y];                                 // at most 2^46 2^17
+            }
+            if (sh[y] >= 0) {
+#pragma unroll
+                for (int x = 0; x < 8; x++) o[x] = ((o[x] >> sh[y]) + 1) >> 1;
+            } else {
+#pragma unroll
+                for (int x = 0; x < 8; x++) o[x] = (int64_t)((uint64_t)o[x] << (-1 - sh[y]));
             }
             if (r < nr) {
 #pragma unroll
@@ -1023,7 +1040,7 @@ cudaError_t store_read(const Store4& st, const StoreRows& rw, int layer, int64_t
     return store_launch(how, k_store_read<SW_ROWS>, row_grid(st, rw, SW_ROWS), SW_WARPS * 32, 0, 1, st, rw, layer, k, v, wide, err);
 }
 
-constexpr int SM_FROM_ROWS = 4, SM_FIXED = 4;
+constexpr int SM_FROM_ROWS = 20, SM_FIXED = 4;
 constexpr int SM_SMEM_MOST = 200 * 1024;
 constexpr int SF_MOST_KEYS = 8192;   // of a CTA: 64 KB of shared memory
 constexpr int SF_WARP_UNITS = 12, SF_WARP_BLOCKS = 32;   // a warp a unit: from so many units an SM on, up to 1,024 keys (32 KB a CTA)
