@@ -180,18 +180,19 @@ int b2_check_wait(b2_handle* h, void* stream);
  *           magnitude, s = min(max(t - 3, 0), 44), and at least the larger half's s less 3; codes c = rnd(x, s) kept in
  *           [-8, 7]. A value head row: the same with one shift over the 64.
  *   read    c 2^s.
- *   attend  (base2.py:85-100 over the held keys and values) q15 = rnd(q, u), u = max(bit length - 14, 0); the score of
- *           key k = c 2^s is q15 . k 2^u over 8 at 2^-10, rounded (and held below 2^30); start = the largest;
+ *   attend  (base2.py:85-100 over the held keys and values; q kept below 2^47 as well) q15 = rnd(q, u), u = max(bit
+ *           length - 14, 0); the score of key k = c 2^s is q15 . k 2^u over 8 at 2^-10, rounded (and held below 2^30); start = the largest;
  *           a = arrival[start - score], 0 past the table; Z = sum a; w = rnd(a, 1 + M - s), s the value's shift and M
  *           the largest of the visible keys'; out = power(sum w c, 65536 (M + 1) - log2fix(Z)). Every sum is exact, so
  *           the result does not depend on the order or on how a call is split.
  * Streams: stream i's rows are cu[i] .. cu[i + 1] - 1 of the call's rows (cu [n_streams + 1]; NULL: one row a stream,
- * rows = n_streams), its first row at position pos[i]; max_rows is a bound on a stream's rows (1 with cu = NULL). Rows
+ * rows = n_streams), its first row at position pos[i]; max_rows is any bound on a stream's rows (1 with cu = NULL). Rows
  * that no stream has are neither read nor written. cu, pos, first, k, v, q, out are DEVICE pointers; row r's head h is
  * at r * ld + 64 h (ld in elements, at least 64 n_head). Work is queued on `stream`; nothing is allocated, copied to
  * the host or kept between calls, so calls may be captured into a graph, and calls that do not write what another one
- * reads or writes may run at once. A stream whose rows do not fit the call or whose positions pass the context is
- * skipped and flagged: b2_store_sync reports it (B2_ERR_ARG, B2_ERR_CTX). */
+ * reads or writes may run at once on several streams (the host's calls on one store come one after the other). out may be
+ * q itself. A stream whose rows do not fit the call or whose positions pass the context is skipped and flagged:
+ * b2_store_sync reports it (B2_ERR_ARG, B2_ERR_CTX). */
 typedef struct b2_store b2_store;
 typedef struct {
     int32_t n_slots;    /* streams, 1 .. 65535 */
@@ -201,8 +202,9 @@ typedef struct {
 } b2_store_config;
 
 /* A store on `device`, every position standing for zeros. arrival [n_arrival] (1 .. 32768 entries in [0, 2^24], the first
- * at least 1), log2 and exp2 [65536]: the machine's tables (base2_convert.py:50-59), HOST pointers. After an error *out, where it
- * is not NULL, holds the message (b2_store_last_error) and is to be destroyed. */
+ * at least 1), log2 [65536] in [0, 65536] and exp2 [65536] in [65536, 131071]: the machine's tables
+ * (base2_convert.py:50-59), HOST pointers. After an error *out, where it is not NULL, holds the message
+ * (b2_store_last_error) and is to be destroyed. */
 int b2_store_create(const b2_store_config* cfg, int device, const int64_t* arrival, int64_t n_arrival, const int64_t* log2,
                     const int64_t* exp2, b2_store** out);
 

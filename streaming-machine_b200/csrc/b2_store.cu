@@ -85,7 +85,7 @@ __global__ void __launch_bounds__(SW_WARPS * 32) k_store_write(Store4 st, StoreR
         if (__all_sync(0xffffffffu, past == 0)) {                // the usual case
             uint32_t m[2] = {0, 0};
 #pragma unroll
-            for (int k = 0; k < 8; k++) m[k >> 2] |= (uint32_t)abs((int)v[t][k]);
+            for (int k = 0; k < 8; k++) m[k >> 2] |= mag32((int32_t)v[t][k]);
 #pragma unroll
             for (int o = 1; o < 8; o <<= 1) {
                 m[0] |= __shfl_xor_sync(0xffffffffu, m[0], o);
@@ -226,27 +226,44 @@ B2_DEV void turn3(const uint32_t* w, uint32_t& b0, uint32_t& b1, uint32_t& b2) {
     b2 = __byte_perm(__byte_perm(w[0], w[1], 0x0062), __byte_perm(w[2], w[3], 0x0062), 0x5410);
 }
 
-// a row's 64 query values at 15 bits, as two signed bytes q15 = 256 hi + lo, in a lane's pair (dims 2 lane, 2 lane + 1):
-// bytes hi, lo of the first, hi, lo of the second. Returns the row's shift u. Every lane of the warp takes part.
-B2_DEV int query_bytes(int64_t x0, int64_t x1, uint32_t& word) {
-    int u, a, b;
-    if (__all_sync(0xffffffffu, x0 == (int32_t)x0 && x1 == (int32_t)x1)) {       // the usual case: 32 bits hold them
-        const int y0 = (int)x0, y1 = (int)x1;
-        const uint32_t m = (uint32_t)abs(y0) | (uint32_t)abs(y1);                // (|-2^31| is 2^31 unsigned)
-        u = max(18 - __clz((int)__reduce_or_sync(0xffffffffu, m)), 0);
-        a = rnd32(y0, u);
-        b = rnd32(y1, u);
+// N rows' 64 query values at 15 bits, as two signed bytes q15 = 256 hi + lo, in a lane's pair (dims 2 lane, 2 lane + 1):
+// bytes hi, lo of the first, hi, lo of the second. u: the rows' shifts. Every lane of the warp takes part.
+template <int N>
+B2_DEV void query_bytes(const int64_t (&x)[N][2], uint32_t (&word)[N], int (&u)[N]) {
+    uint32_t past = 0;                                                            // nonzero where 32 bits do not hold a value
+#pragma unroll
+    for (int k = 0; k < N; k++)
+#pragma unroll
+        for (int t = 0; t < 2; t++) past |= (uint32_t)(x[k][t] >> 32) ^ (uint32_t)((int32_t)x[k][t] >> 31);
+    int a[N], b[N];
+    if (__all_sync(0xffffffffu, past == 0)) {                                     // the usual case
+#pragma unroll
+        for (int k = 0; k < N; k++) {
+            const int y0 = (int)x[k][0], y1 = (int)x[k][1];
+            // the largest magnitude's bit length is that of the magnitudes' OR
+            u[k] = max(18 - __clz((int)__reduce_or_sync(0xffffffffu, mag32(y0) | mag32(y1))), 0);
+            const int down = max(u[k] - 1, 0), one = u[k] > 0;
+            a[k] = ((y0 >> down) + one) >> one;
+            b[k] = ((y1 >> down) + one) >> one;
+        }
     } else {
-        x0 = store_clamp(x0);
-        x1 = store_clamp(x1);
-        // the largest magnitude's bit length is that of the magnitudes' OR
-        u = max((int)__reduce_max_sync(0xffffffffu, (uint32_t)bitlen_u(mag(x0) | mag(x1))) - 14, 0);
-        a = (int)rnd64(x0, u);
-        b = (int)rnd64(x1, u);
+#pragma unroll 1
+        for (int k = 0; k < N; k++) {
+            int64_t y0 = 0, y1 = 0;
+#pragma unroll
+            for (int t = 0; t < N; t++)                                           // (a register of the array by constants)
+                if (t == k) { y0 = store_clamp(x[t][0]); y1 = store_clamp(x[t][1]); }
+            const int r = max((int)__reduce_max_sync(0xffffffffu, (uint32_t)bitlen_u(mag(y0) | mag(y1))) - 14, 0);
+            const int c = (int)rnd64(y0, r), d = (int)rnd64(y1, r);
+#pragma unroll
+            for (int t = 0; t < N; t++)
+                if (t == k) { u[t] = r; a[t] = c; b[t] = d; }
+        }
     }
     // byte 0: a + 128 >> 8, byte 1: a, byte 2: b + 128 >> 8, byte 3: b
-    word = __byte_perm(__byte_perm(a + 128, a, 0x41), __byte_perm(b + 128, b, 0x41), 0x5410);
-    return u;
+#pragma unroll
+    for (int k = 0; k < N; k++)
+        word[k] = __byte_perm(__byte_perm(a[k] + 128, a[k], 0x41), __byte_perm(b[k] + 128, b[k], 0x41), 0x5410);
 }
 
 template <int NW>
@@ -284,8 +301,8 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, NW == 1 ? 7 : (NW == 
         for (int t = ut; t < 64 && rank == 0; t += NW * 32) out[t] = 0;
         return;
     }
-    int64_t x0, x1;
-    load_pair(a.q.x + (size_t)row * a.q.ld + h * a.q.hs + 2 * lane, wide & 1, x0, x1);
+    int64_t x[1][2];
+    load_pair(a.q.x + (size_t)row * a.q.ld + h * a.q.hs + 2 * lane, wide & 1, x[0][0], x[0][1]);
     // blocks of 32 positions; this CTA's are b0 .. b0 + nb - 1
     const int first_block = lo >> 5, blocks = (p >> 5) - first_block + 1;
     const int per = cs > 1 ? (blocks + cs - 1) / cs : blocks;
@@ -314,15 +331,17 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, NW == 1 ? 7 : (NW == 
 #pragma unroll
     for (int f = 0; f < PF; f++)
         if (wid + f * NW < nb) keys(wid + f * NW, k[f]);
-    uint32_t word, q0[2], q1[2];                                     // B operands of the two halves
-    const int u = query_bytes(x0, x1, word);
+    uint32_t words[1], q0[2], q1[2];                                 // q0, q1: B operands of the two halves
+    int us[1];
+    query_bytes(x, words, us);
+    const int u = us[0];
     {
         const uint32_t pick = (g & 1) ? 0x51u : 0x40u;               // odd columns the low bytes
 #pragma unroll
         for (int x = 0; x < 2; x++) {
             uint32_t w[4];
 #pragma unroll
-            for (int b = 0; b < 4; b++) w[b] = __shfl_sync(0xffffffffu, word, 16 * x + 4 * j + b);
+            for (int b = 0; b < 4; b++) w[b] = __shfl_sync(0xffffffffu, words[0], 16 * x + 4 * j + b);
             q0[x] = __byte_perm(__byte_perm(w[0], w[1], pick), __byte_perm(w[2], w[3], pick), 0x5410);
             q1[x] = __byte_perm(__byte_perm(w[0], w[1], pick + 0x22), __byte_perm(w[2], w[3], pick + 0x22), 0x5410);
         }
@@ -643,13 +662,14 @@ __global__ void __launch_bounds__(SM_THREADS, 2) k_store_attend_many(StoreAttend
                 x[k][0] = x[k][1] = 0;
                 if (r < nr) load_pair(a.q.x + (size_t)(run.r0 + i0 + r) * a.q.ld + h * a.q.hs + 2 * lane, wide & 1, x[k][0], x[k][1]);
             }
-            int most = 0;
+            uint32_t words[SM_ROWS / SM_WARPS];
+            int us[SM_ROWS / SM_WARPS], most = 0;
+            query_bytes(x, words, us);
 #pragma unroll
             for (int k = 0; k < SM_ROWS / SM_WARPS; k++) {
-                const int r = wid + k * SM_WARPS;
-                const int u = query_bytes(x[k][0], x[k][1], S.q[r][lane]);
-                if (lane == 0) S.u[r] = u;
-                most = max(most, u);
+                S.q[wid + k * SM_WARPS][lane] = words[k];
+                if (lane == 0) S.u[wid + k * SM_WARPS] = us[k];
+                most = max(most, us[k]);
             }
             if (lane == 0) S.most[wid] = most;
         }
@@ -802,13 +822,17 @@ __global__ void __launch_bounds__(SM_THREADS, 2) k_store_attend_many(StoreAttend
         for (int k = 0; k < cs; k++)
 #pragma unroll
             for (int w = 0; w < 2; w++) {            // the pair's two warps, in every CTA of the cluster
-                const int2* const at = &S.ym[2 * pair + w][g];
-                const int64_t oa = cs > 1 ? ld_dsmem(mapa(saddr(at), (uint32_t)k)) : *reinterpret_cast<const int64_t*>(at);
-                const int64_t ob = cs > 1 ? ld_dsmem(mapa(saddr(at + 8), (uint32_t)k)) : *reinterpret_cast<const int64_t*>(at + 8);
-                ya = max(ya, (int32_t)oa);
-                yb = max(yb, (int32_t)ob);
-                ma = max(ma, (int)(oa >> 32));
-                mb = max(mb, (int)(ob >> 32));
+                int2 oa = S.ym[2 * pair + w][g], ob = S.ym[2 * pair + w][g + 8];
+                if (cs > 1) {
+                    const int64_t a8 = ld_dsmem(mapa(saddr(&S.ym[2 * pair + w][g]), (uint32_t)k));
+                    const int64_t b8 = ld_dsmem(mapa(saddr(&S.ym[2 * pair + w][g + 8]), (uint32_t)k));
+                    oa = make_int2((int)a8, (int)(a8 >> 32));
+                    ob = make_int2((int)b8, (int)(b8 >> 32));
+                }
+                ya = max(ya, oa.x);
+                yb = max(yb, ob.x);
+                ma = max(ma, oa.y);
+                mb = max(mb, ob.y);
             }
         // the next item's queries into L2 (a row is four lines)
         if (n_t < tiles && n_r0 >= 0 && n_r1 <= a.rw.rows) {
@@ -921,8 +945,8 @@ __global__ void __launch_bounds__(SM_THREADS, 2) k_store_attend_many(StoreAttend
             for (int k = 0; k < cs; k++)
 #pragma unroll
                 for (int w = 0; w < 2; w++) {
-                    const int64_t* const at = &S.z[2 * pair + w][g + 8 * y];
-                    z += cs > 1 ? ld_dsmem(mapa(saddr(at), (uint32_t)k)) : *at;
+                    if (cs > 1) z += ld_dsmem(mapa(saddr(&S.z[2 * pair + w][g + 8 * y]), (uint32_t)k));
+                    else z += S.z[2 * pair + w][g + 8 * y];
                 }
             const bool none = (y ? lb > pb : la > pa) || z == 0;
             const int64_t F = 65536ll * ((y ? mb : ma) + STORE_W_SHIFT) - log2fix(none ? 1 : z, a.LOG2);
@@ -1177,7 +1201,10 @@ struct OnDevice {
 #define SCK(call)                                                                                     \
     do {                                                                                              \
         cudaError_t e_ = (call);                                                                      \
-        if (e_ != cudaSuccess) return sfail(h, B2_ERR_CUDA, "%s: %s", #call, cudaGetErrorString(e_)); \
+        if (e_ != cudaSuccess) {                                                                      \
+            cudaGetLastError(); /* nothing is left behind for the next call's check */                \
+            return sfail(h, B2_ERR_CUDA, "%s: %s", #call, cudaGetErrorString(e_));                    \
+        }                                                                                             \
     } while (0)
 
 template <class T>
@@ -1242,8 +1269,7 @@ int check_rows(b2_store* h, const char* what, int32_t layer, const int32_t* cu, 
     const b2_store_config& c = h->cfg;
     if (layer < 0 || layer >= c.n_layer) return sfail(h, B2_ERR_ARG, "%s: layer %d of %d", what, layer, c.n_layer);
     if (n_streams < 0 || n_streams > c.n_slots) return sfail(h, B2_ERR_ARG, "%s: n_streams %d of %d slots", what, n_streams, c.n_slots);
-    if (rows < 0 || max_rows < 0 || max_rows > c.max_ctx)
-        return sfail(h, B2_ERR_ARG, "%s: rows %d, max_rows %d (context %d)", what, rows, max_rows, c.max_ctx);
+    if (rows < 0 || max_rows < 0) return sfail(h, B2_ERR_ARG, "%s: rows %d, max_rows %d", what, rows, max_rows);
     if (!cu && (rows != n_streams || max_rows != (rows ? 1 : max_rows)))
         return sfail(h, B2_ERR_ARG, "%s: without cu every stream gives one row (rows %d, n_streams %d, max_rows %d)", what, rows,
                      n_streams, max_rows);
@@ -1279,7 +1305,10 @@ int b2_store_create(const b2_store_config* cfg, int device, const int64_t* arriv
         cfg->n_head > 1024 || cfg->max_ctx < 1 || cfg->max_ctx > STORE_MAX_CTX)
         return B2_ERR_ARG;
     OnDevice on(device);
-    if (on.e != cudaSuccess) return B2_ERR_CUDA;
+    if (on.e != cudaSuccess) {
+        cudaGetLastError();
+        return B2_ERR_CUDA;
+    }
     b2_store* h = new (std::nothrow) b2_store();
     if (!h) return B2_ERR_NOMEM;
     const int rc = guarded(h, [&] {
@@ -1304,7 +1333,7 @@ int b2_store_write(b2_store* h, int32_t layer, const int64_t* k, int64_t ldk, co
                          (long long)ldk, (const void*)v, (long long)ldv, (long long)d);
         OnDevice on(h->device);
         SCK(on.e);
-        SCK(store_write(h->st, StoreRows{cu, pos, n_streams, rows, max_rows}, layer, StoreVec{k, ldk, 64}, StoreVec{v, ldv, 64}, h->d_err,
+        SCK(store_write(h->st, StoreRows{cu, pos, n_streams, rows, std::min(max_rows, h->cfg.max_ctx)}, layer, StoreVec{k, ldk, 64}, StoreVec{v, ldv, 64}, h->d_err,
                         StoreLaunch{(cudaStream_t)stream, true, &h->plan}));
         return (int)B2_OK;
     });
@@ -1319,7 +1348,7 @@ int b2_store_read(b2_store* h, int32_t layer, const int32_t* cu, const int32_t* 
         if (rows && !k && !v) return sfail(h, B2_ERR_ARG, "b2_store_read: neither k nor v asked for");
         OnDevice on(h->device);
         SCK(on.e);
-        SCK(store_read(h->st, StoreRows{cu, pos, n_streams, rows, max_rows}, layer, k, v, h->d_err,
+        SCK(store_read(h->st, StoreRows{cu, pos, n_streams, rows, std::min(max_rows, h->cfg.max_ctx)}, layer, k, v, h->d_err,
                        StoreLaunch{(cudaStream_t)stream, true, &h->plan}));
         return (int)B2_OK;
     });
@@ -1337,7 +1366,7 @@ int b2_store_attend(b2_store* h, int32_t layer, const int64_t* q, int64_t ldq, c
                          (const void*)out, window);
         OnDevice on(h->device);
         SCK(on.e);
-        StoreAttend a{h->st, StoreRows{cu, pos, n_streams, rows, max_rows}, layer, StoreVec{q, ldq, 64}, first, window, h->ARR, h->alen,
+        StoreAttend a{h->st, StoreRows{cu, pos, n_streams, rows, std::min(max_rows, h->cfg.max_ctx)}, layer, StoreVec{q, ldq, 64}, first, window, h->ARR, h->alen,
                       h->LOG2, h->EXP2, out, nullptr, h->d_err};
         SCK(store_attend(a, StoreLaunch{(cudaStream_t)stream, true, &h->plan}));
         return (int)B2_OK;

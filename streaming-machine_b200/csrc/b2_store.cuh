@@ -106,6 +106,7 @@ inline size_t store_layout(Store4& st, int n_slots, int L, int H, int max_ctx, v
 // x 2^-s to nearest, halves up, s >= 0: with no carry past the word (base2.py:18-22 wherever that does not overflow)
 B2_DEV int32_t rnd32(int32_t x, int s) { return s > 0 ? ((x >> (s - 1)) + 1) >> 1 : x; }
 B2_DEV int64_t rnd64(int64_t x, int s) { return s > 0 ? ((x >> (s - 1)) + 1) >> 1 : x; }
+B2_DEV uint32_t mag32(int32_t x) { return x < 0 ? 0u - (uint32_t)x : (uint32_t)x; }
 B2_DEV int64_t store_clamp(int64_t x) { return x < -STORE_TOP ? -STORE_TOP : (x > STORE_TOP - 1 ? STORE_TOP - 1 : x); }
 B2_DEV int store_code(int64_t x, int s) {
     const int64_t c = rnd64(x, s);

@@ -77,7 +77,7 @@ def test_head_counts(T, heads):
 
 
 @pytest.mark.parametrize("window", [1, 2, 16, 33, 1000])
-@pytest.mark.parametrize("rows", [[1, 1, 1], [20, 3, 1]])
+@pytest.mark.parametrize("rows", [[1, 1, 1], [20, 3, 1], [70, 21, 1]])
 def test_windows(T, window, rows):
     run(T, np.random.default_rng(window), 1, [90, 32, 5], rows, window=window)
 
@@ -87,12 +87,15 @@ def test_dropped_beginnings_and_empty_rows(T):
     and a negative first is none."""
     run(T, np.random.default_rng(3), 2, [50, 50, 10, 5], [3, 3, 4, 1], first=[17, 53, 12, -7])
     run(T, np.random.default_rng(4), 2, [50, 40], [1, 1], first=[51, 40], window=9)
+    run(T, np.random.default_rng(4), 1, [50, 50, 10, 5], [70, 30, 25, 1], first=[97, 81, 12, 6])
+    run(T, np.random.default_rng(4), 1, [50, 40], [30, 22], first=[70, 20], window=11)
 
 
 @pytest.mark.parametrize("size", [2.0 ** -16, 0.01, 40.0, 2.0 ** 20, 2.0 ** 40])
 def test_query_sizes(T, size):
     """Scores from zeros to ones that are held at their limit (and weights from all alike to a single one)."""
     run(T, np.random.default_rng(5), 1, [40], [2], size=size)
+    run(T, np.random.default_rng(5), 1, [40], [33], size=size)
 
 
 def test_extremes(T):
@@ -126,6 +129,7 @@ def test_other_tables(T):
         T2 = dict(T, arrival=arr.astype(np.int64))
         run(T2, rng, 1, [30, 2], [1, 1])
         run(T2, rng, 1, [30, 2], [20, 3])
+        run(T2, rng, 1, [30, 2], [40, 3])
 
 
 def test_layers_and_slots_are_apart(T):
@@ -240,7 +244,7 @@ def test_refusals(T):
     pos = i32([0, 0])
     for call in (lambda: st.write(x, x, pos, layer=2), lambda: st.write(x, x, pos, layer=-1),
                  lambda: st.attend(x, pos, window=-1), lambda: st.write(x[:1].expand(3, 1, 64).contiguous(), x[:1].expand(3, 1, 64).contiguous(), i32([0, 0, 0])),
-                 lambda: st.attend(x, pos, cu=i32([0, 1, 2]), max_rows=17), lambda: st.attend(x, pos, cu=i32([0, 1, 2]), max_rows=0),
+                 lambda: st.attend(x, pos, cu=i32([0, 1, 2]), max_rows=-1), lambda: st.attend(x, pos, cu=i32([0, 1, 2]), max_rows=0),
                  lambda: st.attend(x, i32([]), cu=i32([0]), max_rows=1)):
         with pytest.raises(engine.B2Error) as ex:
             call()
@@ -297,5 +301,123 @@ def test_captured_and_on_another_stream(T):
                 st.attend(q, pos, out=out)
             side.synchronize()
         assert np.array_equal(out.cpu().numpy(), pl.attend(q.cpu().numpy(), at))
+    st.sync()
+    st.close()
+
+
+def run_long(T, rng, heads, held, rows, window=0, first=None, max_rows=None):
+    """As run(), for many keys: the numpy reference."""
+    n = len(held)
+    st = make(T, n, max(h + r for h, r in zip(held, rows)), heads)[0]
+    pl = ref.FastStore(T, heads, n)
+    try:
+        total = [h + r for h, r in zip(held, rows)]
+        cu = np.concatenate([[0], np.cumsum(total)])
+        k, v = values(rng, cu[-1], heads, 1.0), values(rng, cu[-1], heads, 0.3)
+        st.write(dev(k), dev(v), i32([0] * n), cu=i32(cu), max_rows=max(total))
+        for s in range(n):
+            pl.write(s, k[cu[s]:cu[s + 1]], v[cu[s]:cu[s + 1]])
+        cu = np.concatenate([[0], np.cumsum(rows)])
+        q = values(rng, cu[-1], heads, 1.5)
+        got = st.attend(dev(q), i32(held), cu=i32(cu), max_rows=max_rows or max(rows), window=window,
+                        first=None if first is None else i32(first)).cpu().numpy()
+        st.sync()
+        for s in range(n):
+            want = pl.attend(s, q[cu[s]:cu[s + 1]], held[s], window, 0 if first is None else first[s])
+            assert np.array_equal(got[cu[s]:cu[s + 1]], want), s
+    finally:
+        st.close()
+
+
+@pytest.mark.parametrize("heads,held,rows", [
+    (1, [2100, 40], [1, 1]), (12, [1030] * 5 + [3] * 11, [1] * 16), (1, [20000], [1]), (12, [60, 99, 7] * 50, [1] * 150),
+    (2, [40000, 33000, 5], [1, 2, 1]), (5, [4100], [20]),
+    (2, [700, 3], [40, 64]), (1, [3000], [130]), (3, [6000, 50], [64, 1]), (12, [0] * 8, [200, 130, 64, 65, 127, 128, 1, 30])])
+def test_long_and_many(T, heads, held, rows):
+    """Every shape of launch: a warp, 4, 8 and 16 warps a row and head, keys split over clusters of 2 to 8 CTAs, for few
+    rows and for many; streams much shorter than the longest beside it."""
+    run_long(T, np.random.default_rng(len(held) + heads), heads, held, rows)
+
+
+@pytest.mark.parametrize("rows", [[1, 1], [18, 3], [90, 22]])
+def test_long_windows(T, rows):
+    run_long(T, np.random.default_rng(16), 2, [3000, 1500], rows, window=1111, first=[0, 1490])
+
+
+def test_max_rows_is_a_bound(T):
+    """A bound that no stream reaches, up to the whole context: the same results by whichever kernel it leads to."""
+    for bound in (3, 20, 21, 64, 400):
+        run_long(T, np.random.default_rng(17), 2, [390, 0, 100], [2, 3, 1], max_rows=bound)
+
+
+def test_far_into_memory(T):
+    """A store whose arrays pass 2^32 bytes: its last stream's last positions."""
+    st, pl = make(T, 256, 65536, 12)
+    rng = np.random.default_rng(18)
+    pos = np.zeros(256, np.int32)
+    cu = np.zeros(257, np.int32)
+    pos[255], cu[256] = 65536 - 40, 40
+    k, v, q = (values(rng, 40, 12, s) for s in (1.0, 0.3, 1.5))
+    st.write(dev(k), dev(v), i32(pos), cu=i32(cu), max_rows=40)
+    got = st.attend(dev(q), i32(pos), cu=i32(cu), max_rows=40, window=9)
+    one = pos.copy()
+    one[255] = 65535
+    cu1 = np.minimum(cu, 1)
+    last = st.attend(dev(q[39:]), i32(one), cu=i32(cu1), max_rows=1, window=9)
+    back = st.read(i32(pos), cu=i32(cu), max_rows=40, rows=40)
+    st.sync()
+    st.close()
+    for s in (slice(0, 2),):                                       # two heads of the twelve, by the slow reference
+        pl.H = 2
+        pl.write(k[:, s], v[:, s], [65536 - 40], [0, 40])
+        want = pl.attend(q[:, s], [65536 - 40], [0, 40], window=9)
+        assert np.array_equal(got[9:, s].cpu().numpy(), want[9:]) and np.array_equal(last[:, s].cpu().numpy(), want[39:])
+        for b, w in zip(back, pl.read([65536 - 40], [0, 40])):
+            assert np.array_equal(b[:, s].cpu().numpy(), w)
+
+
+def test_out_may_be_the_queries(T):
+    import torch
+    for rows in ([1, 1], [25, 70]):
+        rng = np.random.default_rng(19)
+        st, _ = make(T, 2, 200, 3)
+        cu = np.concatenate([[0], np.cumsum(rows)])
+        hist = [dev(values(rng, 400, 3, s)) for s in (1.0, 0.3)]
+        st.write(*hist, i32([0, 0]), cu=i32([0, 200, 400]), max_rows=200)
+        q = dev(values(rng, cu[-1], 3, 1.5))
+        want = st.attend(q, i32([100, 130]), cu=i32(cu), max_rows=max(rows))
+        assert st.attend(q, i32([100, 130]), cu=i32(cu), max_rows=max(rows), out=q) is q
+        assert torch.equal(q, want)
+        st.sync()
+        st.close()
+
+
+def test_calls_at_once(T):
+    """Two streams of work on one store (readers of one half of the slots, a writer of the other), many times over."""
+    import torch
+    rng = np.random.default_rng(20)
+    st, _ = make(T, 4, 700, 4)
+    hist = [dev(values(rng, 4 * 600, 4, s)) for s in (1.0, 0.3)]
+    cu = i32([0, 600, 1200, 1800, 2400])
+    st.write(*hist, i32([0] * 4), cu=cu, max_rows=600)
+    q1, q2 = dev(values(rng, 2, 4, 1.5)), dev(values(rng, 100, 4, 1.5))
+    args1, args2 = (i32([599, 400]),), (i32([550, 550]),)
+    cu2 = i32([0, 50, 100])
+    want1, want2 = st.attend(q1, *args1), st.attend(q2, *args2, cu=cu2, max_rows=50)
+    # the writer rewrites the positions 600 .. 649 of all four: nobody reads those
+    more = [dev(values(rng, 200, 4, s)) for s in (1.0, 0.3)]
+    cuw, posw = i32([0, 50, 100, 150, 200]), i32([600] * 4)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(30):
+        with torch.cuda.stream(streams[0]):
+            got.append((want1, st.attend(q1, *args1)))
+        with torch.cuda.stream(streams[1]):
+            got.append((want2, st.attend(q2, *args2, cu=cu2, max_rows=50)))
+        with torch.cuda.stream(streams[2]):
+            st.write(*more, posw, cu=cuw, max_rows=50)
+    torch.cuda.synchronize()
+    assert all(torch.equal(w, g) for w, g in got)
     st.sync()
     st.close()

@@ -177,3 +177,53 @@ def test_refusals_and_context(eng, M):
         e.step()
     assert ex.value.code == 4
     assert e.prefill(ids).shape == (2,)                            # and the handle goes on
+
+
+@pytest.mark.parametrize("switch", [dict(gauge="float"), dict(edge="float")])
+def test_beside_float_stages(M, switch):
+    """The stage switches that leave the arrival whole: a prompt pass equals its steps (the CUDA-core banks' path)."""
+    from streaming_machine_b200 import engine
+    e = engine.Engine(layers(M, 1), n_streams=2, max_ctx=48, store_bits=4, **switch)
+    try:
+        ids = np.random.default_rng(15).integers(0, V, (2, 30))
+        _, want = e.prefill(ids, logits=True)
+        e.prefill(ids[:, :28])
+        for t in (28, 29):
+            _, got = e.step(ids[:, t], logits=True)
+        assert np.array_equal(got, want)
+    finally:
+        e.close()
+
+
+@pytest.mark.parametrize("kind", ["gpt2", "pythia"])
+def test_profiled_steps(kind, eng, peng):
+    """b2_profile's modes count the store's launches in their classes and change no words."""
+    e = shape(eng if kind == "gpt2" else peng, 2, 64)
+    ids = np.random.default_rng(16).integers(0, V, (2, 20))
+    want = e.generate(ids, 4)
+    for mode in (0, 1, 2):
+        e._call("b2_profile", e.h, mode)
+        assert np.array_equal(e.generate(ids, 4), want)
+        _, classes = e.profile_read()
+        assert classes["attend"][0] == 4 * 2 and classes["heads"][0] == 4 * 2 * (2 if kind == "pythia" else 1)
+        if mode:
+            assert classes["attend"][1] > 0
+    e._call("b2_profile", e.h, 0)
+
+
+def test_launch_shapes_of_the_decode_paths(M):
+    """The switches of the decode path give the same words over the 4-bit store."""
+    import os
+    from streaming_machine_b200 import engine
+    ids = np.random.default_rng(17).integers(0, V, (3, 20))
+    got = []
+    for env in ({}, {"B2_WQ": "0"}, {"B2_GRAPH": "0"}, {"B2_PDL": "0"}, {"B2_FUSE_HEADS": "0"}):
+        os.environ.update(env)
+        try:
+            e = engine.Engine(layers(M, 2), n_streams=3, max_ctx=48, store_bits=4)
+        finally:
+            for k in env:
+                del os.environ[k]
+        got.append(e.generate(ids, 6))
+        e.close()
+    assert all(np.array_equal(g, got[0]) for g in got)

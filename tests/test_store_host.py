@@ -102,3 +102,16 @@ def test_create_refuses_before_it_touches_a_device():
         assert getattr(L, f)(None, *args) == 1
     assert L.b2_store_last_error(None) == b"null store"
     L.b2_store_destroy(None)
+
+
+def test_the_two_references_agree():
+    """FastStore (numpy) against Store (Python's whole numbers)."""
+    from streaming_machine_b200 import convert
+    T = convert.tables()
+    rng = np.random.default_rng(42)
+    slow, fast = ref.Store(T, 2), ref.FastStore(T, 2, 1)
+    k, v, q = (np.round(rng.standard_normal((30, 2, 64)) * s * 65536 * 2.0 ** rng.integers(-5, 2, (30, 2, 1))).astype(np.int64) for s in (1.0, 0.3, 2.0))
+    slow.write(k, v, [0], [0, 30])
+    fast.write(0, k, v)
+    for window, first in ((0, 0), (7, 0), (0, 12), (9, 25)):
+        assert np.array_equal(fast.attend(0, q, 0, window, first), slow.attend(q, [0], [0, 30], window, [first]))
