@@ -201,12 +201,16 @@ typedef struct {
     int32_t max_ctx;    /* positions of a stream, 1 .. 65536 */
 } b2_store_config;
 
+/* The bytes of device memory that a store takes (-1: a configuration or table length that b2_store_create refuses). */
+int64_t b2_store_size(const b2_store_config* cfg, int64_t n_arrival);
+
 /* A store on `device`, every position standing for zeros. arrival [n_arrival] (1 .. 32768 entries in [0, 2^24], the first
  * at least 1), log2 [65536] in [0, 65536] and exp2 [65536] in [65536, 131071]: the machine's tables
- * (base2_convert.py:50-59), HOST pointers. After an error *out, where it is not NULL, holds the message
- * (b2_store_last_error) and is to be destroyed. */
+ * (base2_convert.py:50-59), HOST pointers. memory: b2_store_size bytes of that device's memory, 32-byte aligned, for as long
+ * as the store lives (a host whose own allocator owns the GPU's memory), or NULL: the library allocates. Waits for the
+ * device. After an error *out, where it is not NULL, holds the message (b2_store_last_error) and is to be destroyed. */
 int b2_store_create(const b2_store_config* cfg, int device, const int64_t* arrival, int64_t n_arrival, const int64_t* log2,
-                    const int64_t* exp2, b2_store** out);
+                    const int64_t* exp2, void* memory, b2_store** out);
 
 /* Put rows into the store (the key/value append; base2.py:93 with 4 bits for to16's 16). */
 int b2_store_write(b2_store* s, int32_t layer, const int64_t* k, int64_t ldk, const int64_t* v, int64_t ldv, const int32_t* cu,

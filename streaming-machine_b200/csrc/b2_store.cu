@@ -6,6 +6,7 @@
 
 #include <algorithm>
 #include <exception>
+#include <mutex>
 #include <new>
 #include <string>
 #include <type_traits>
@@ -1072,10 +1073,9 @@ constexpr int SF_LONG = 32, SF_VERY_LONG = 64;   // blocks of 32 keys
 
 size_t many_smem(int alen) { return sizeof(SmShared) + (size_t)(alen + 1) * 4; }
 
-cudaError_t store_init(int alen, StorePlan& plan) {
-    int device = 0;
-    cudaError_t e = cudaGetDevice(&device);
-    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&plan.sms, cudaDevAttrMultiProcessorCount, device);
+namespace {
+cudaError_t make_plan(int device, int alen, StorePlan& plan) {
+    cudaError_t e = cudaDeviceGetAttribute(&plan.sms, cudaDevAttrMultiProcessorCount, device);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(k_store_attend_few<4>, cudaFuncAttributeMaxDynamicSharedMemorySize, SF_MOST_KEYS * SF_BYTES);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(k_store_attend_few<8>, cudaFuncAttributeMaxDynamicSharedMemorySize, SF_MOST_KEYS * SF_BYTES);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(k_store_attend_few<16>, cudaFuncAttributeMaxDynamicSharedMemorySize, SF_MOST_KEYS * SF_BYTES);
@@ -1102,6 +1102,27 @@ cudaError_t store_init(int alen, StorePlan& plan) {
         }
     }
     return cudaSuccess;
+}
+
+// the plans made so far: a few devices and table lengths a process
+std::mutex g_plan_mu;
+struct PlanAt { int device, alen; StorePlan plan; };
+std::vector<PlanAt> g_plans;
+}  // namespace
+
+cudaError_t store_init(int alen, StorePlan& plan) {
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess) return e;
+    std::lock_guard<std::mutex> lock(g_plan_mu);
+    for (const PlanAt& p : g_plans)
+        if (p.device == device && p.alen == alen) {
+            plan = p.plan;
+            return cudaSuccess;
+        }
+    e = make_plan(device, alen, plan);
+    if (e == cudaSuccess) g_plans.push_back(PlanAt{device, alen, plan});
+    return e;
 }
 
 cudaError_t store_attend(const StoreAttend& a, StoreLaunch how) {
@@ -1169,7 +1190,7 @@ struct b2_store {
     int alen = 0;
     StorePlan plan;
     uint32_t* d_err = nullptr;
-    std::vector<void*> allocs;
+    void* own = nullptr;      // the memory, where the library allocated it
 };
 
 namespace {
@@ -1207,57 +1228,70 @@ struct OnDevice {
         }                                                                                             \
     } while (0)
 
-template <class T>
-int salloc(b2_store* h, T** p, size_t n) {
-    void* q = nullptr;
-    const cudaError_t e = cudaMalloc(&q, n * sizeof(T));
-    if (e != cudaSuccess) {
-        cudaGetLastError();      // an allocation that failed leaves nothing behind for the next call's check
-        return sfail(h, B2_ERR_NOMEM, "cudaMalloc(%zu bytes): %s", n * sizeof(T), cudaGetErrorString(e));
-    }
-    h->allocs.push_back(q);
-    *p = (T*)q;
-    return B2_OK;
-}
-
-int table32(b2_store* h, std::vector<int32_t>& t, const int64_t* src, int64_t n, int64_t lo, int64_t hi, const char* name) {
+// a table's entries as 32 bits; where one lies outside [lo, hi], an error that names it
+int table32(b2_store* h, int32_t* to, const int64_t* from, int64_t n, int64_t lo, int64_t hi, const char* name) {
+    int64_t least = from[0], most = from[0];
     for (int64_t i = 0; i < n; i++) {
-        if (src[i] < lo || src[i] > hi)
-            return sfail(h, B2_ERR_VALUE, "b2_store_create: %s[%lld] = %lld outside [%lld, %lld]", name, (long long)i,
-                         (long long)src[i], (long long)lo, (long long)hi);
-        t.push_back((int32_t)src[i]);
+        least = std::min(least, from[i]);
+        most = std::max(most, from[i]);
+        to[i] = (int32_t)from[i];
     }
-    return B2_OK;
+    if (least >= lo && most <= hi) return B2_OK;
+    return sfail(h, B2_ERR_VALUE, "b2_store_create: %s holds %lld .. %lld, its entries lie in [%lld, %lld]", name, (long long)least,
+                 (long long)most, (long long)lo, (long long)hi);
 }
 
 void store_release(b2_store* h) {
-    for (void* p : h->allocs) cudaFree(p);
-    h->allocs.clear();
+    if (h->own) cudaFree(h->own);
+    h->own = nullptr;
     h->d_err = nullptr;
 }
 
-int store_build(b2_store* h, const int64_t* arrival, int64_t n_arrival, const int64_t* log2, const int64_t* exp2) {
+// the store's one piece of memory: the arrays, then (16-byte aligned) four error words and the tables
+constexpr size_t TABLE_WORDS = 4 + 2 * 65536;
+size_t store_bytes(const b2_store_config& c, int64_t n_arrival, Store4* st = nullptr, void* at = nullptr, size_t* tables = nullptr) {
+    Store4 tmp;
+    const size_t n = (store_layout(st ? *st : tmp, c.n_slots, c.n_layer, c.n_head, c.max_ctx, at) + 15) / 16 * 16;
+    if (tables) *tables = n;
+    return n + (TABLE_WORDS + (size_t)n_arrival) * sizeof(int32_t);
+}
+
+bool config_ok(const b2_store_config* c, int64_t n_arrival) {
+    return c && n_arrival >= 1 && n_arrival <= STORE_MAX_ALEN && c->n_slots >= 1 && c->n_slots <= 65535 && c->n_layer >= 1 &&
+           c->n_layer <= 1024 && c->n_head >= 1 && c->n_head <= 1024 && c->max_ctx >= 1 && c->max_ctx <= STORE_MAX_CTX;
+}
+
+int store_build(b2_store* h, const int64_t* arrival, int64_t n_arrival, const int64_t* log2, const int64_t* exp2, void* memory) {
     const b2_store_config& c = h->cfg;
-    SCK(store_init((int)n_arrival, h->plan));
     if (arrival[0] < 1) return sfail(h, B2_ERR_VALUE, "b2_store_create: arrival[0] = %lld (at least 1)", (long long)arrival[0]);
-    // one piece for the error words and the tables, one for the store
-    std::vector<int32_t> t(4, 0);
-    t.reserve(4 + 2 * 65536 + (size_t)n_arrival);
+    std::vector<int32_t> t(TABLE_WORDS + (size_t)n_arrival, 0);
     int rc;
-    if ((rc = table32(h, t, log2, 65536, 0, 65536, "log2")) || (rc = table32(h, t, exp2, 65536, 65536, 131071, "exp2")) ||
-        (rc = table32(h, t, arrival, n_arrival, 0, STORE_MAX_ARR, "arrival")))
+    if ((rc = table32(h, t.data() + 4, log2, 65536, 0, 65536, "log2")) ||
+        (rc = table32(h, t.data() + 4 + 65536, exp2, 65536, 65536, 131071, "exp2")) ||
+        (rc = table32(h, t.data() + TABLE_WORDS, arrival, n_arrival, 0, STORE_MAX_ARR, "arrival")))
         return rc;
-    int32_t* d = nullptr;
-    uint8_t* mem = nullptr;
-    const size_t bytes = store_layout(h->st, c.n_slots, c.n_layer, c.n_head, c.max_ctx, nullptr);
-    if ((rc = salloc(h, &mem, bytes)) || (rc = salloc(h, &d, t.size()))) return rc;
-    store_layout(h->st, c.n_slots, c.n_layer, c.n_head, c.max_ctx, mem);
-    SCK(cudaMemset(mem, 0, bytes));
+    SCK(store_init((int)n_arrival, h->plan));
+    uint8_t* mem = (uint8_t*)memory;
+    if (!mem) {
+        const size_t bytes = store_bytes(c, n_arrival);
+        const cudaError_t e = cudaMalloc(&h->own, bytes);
+        if (e != cudaSuccess) {
+            cudaGetLastError();
+            h->own = nullptr;
+            return sfail(h, B2_ERR_NOMEM, "b2_store_create: cudaMalloc(%zu bytes): %s", bytes, cudaGetErrorString(e));
+        }
+        mem = (uint8_t*)h->own;
+    }
+    size_t tables = 0;
+    store_bytes(c, n_arrival, &h->st, mem, &tables);
+    SCK(cudaDeviceSynchronize());        // given memory may still be in use by earlier work
+    SCK(cudaMemset(mem, 0, tables));
+    int32_t* const d = (int32_t*)(mem + tables);
     SCK(cudaMemcpy(d, t.data(), sizeof(int32_t) * t.size(), cudaMemcpyHostToDevice));
     SCK(cudaDeviceSynchronize());
     h->LOG2 = d + 4;
     h->EXP2 = h->LOG2 + 65536;
-    h->ARR = h->EXP2 + 65536;
+    h->ARR = d + TABLE_WORDS;
     h->alen = (int)n_arrival;
     h->d_err = (uint32_t*)d;
     return B2_OK;
@@ -1296,14 +1330,15 @@ extern "C" {
 
 const char* b2_store_last_error(const b2_store* h) { return h ? h->err.c_str() : "null store"; }
 
+int64_t b2_store_size(const b2_store_config* cfg, int64_t n_arrival) {
+    return config_ok(cfg, n_arrival) ? (int64_t)store_bytes(*cfg, n_arrival) : -1;
+}
+
 int b2_store_create(const b2_store_config* cfg, int device, const int64_t* arrival, int64_t n_arrival, const int64_t* log2,
-                    const int64_t* exp2, b2_store** out) {
+                    const int64_t* exp2, void* memory, b2_store** out) {
     if (!out) return B2_ERR_ARG;
     *out = nullptr;
-    if (!cfg || !arrival || !log2 || !exp2 || n_arrival < 1 || n_arrival > STORE_MAX_ALEN) return B2_ERR_ARG;
-    if (cfg->n_slots < 1 || cfg->n_slots > 65535 || cfg->n_layer < 1 || cfg->n_layer > 1024 || cfg->n_head < 1 ||
-        cfg->n_head > 1024 || cfg->max_ctx < 1 || cfg->max_ctx > STORE_MAX_CTX)
-        return B2_ERR_ARG;
+    if (!config_ok(cfg, n_arrival) || !arrival || !log2 || !exp2 || ((uintptr_t)memory & 31)) return B2_ERR_ARG;
     OnDevice on(device);
     if (on.e != cudaSuccess) {
         cudaGetLastError();
@@ -1314,7 +1349,7 @@ int b2_store_create(const b2_store_config* cfg, int device, const int64_t* arriv
     const int rc = guarded(h, [&] {
         h->cfg = *cfg;
         h->device = device;
-        return store_build(h, arrival, n_arrival, log2, exp2);
+        return store_build(h, arrival, n_arrival, log2, exp2, memory);
     });
     *out = h;      // on an error the store holds its message; b2_store_destroy frees it all the same
     if (rc) store_release(h);

@@ -27,8 +27,8 @@ STATUS = {0: "OK", 1: "ERR_ARG", 2: "ERR_CUDA", 3: "ERR_NOMEM", 4: "ERR_CTX", 5:
 EXPORTS = ("b2_create", "b2_set_bank", "b2_set_array", "b2_set_scalar", "b2_finalize", "b2_alloc_streams",
            "b2_prefill", "b2_step", "b2_generate", "b2_step_host", "b2_bank", "b2_gauge", "b2_bank_noalloc",
            "b2_rewind", "b2_profile", "b2_profile_read", "b2_sync", "b2_check_wait", "b2_set_bank_layout",
-           "b2_get_bank_layout", "b2_last_error", "b2_destroy", "b2_abi_version", "b2_store_create", "b2_store_write",
-           "b2_store_read", "b2_store_attend", "b2_store_sync", "b2_store_last_error", "b2_store_destroy")
+           "b2_get_bank_layout", "b2_last_error", "b2_destroy", "b2_abi_version", "b2_store_size", "b2_store_create",
+           "b2_store_write", "b2_store_read", "b2_store_attend", "b2_store_sync", "b2_store_last_error", "b2_store_destroy")
 PROF_CLASSES = ("bank", "attend", "quant", "heads", "race", "other")
 
 
@@ -79,7 +79,8 @@ def lib():
         L.b2_last_error.restype = cp
         L.b2_destroy.argtypes = [vp]
         L.b2_destroy.restype = None
-        L.b2_store_create.argtypes = [ctypes.POINTER(StoreConfig), ctypes.c_int, vp, i64, vp, vp, ctypes.POINTER(vp)]
+        L.b2_store_size.argtypes = [ctypes.POINTER(StoreConfig), i64]
+        L.b2_store_create.argtypes = [ctypes.POINTER(StoreConfig), ctypes.c_int, vp, i64, vp, vp, vp, ctypes.POINTER(vp)]
         L.b2_store_write.argtypes = [vp, i32, vp, i64, vp, i64, vp, vp, i32, i32, i32, vp]
         L.b2_store_read.argtypes = [vp, i32, vp, vp, i32, i32, i32, vp, vp, vp]
         L.b2_store_attend.argtypes = [vp, i32, vp, i64, vp, vp, vp, i32, i32, i32, i32, vp, vp]
@@ -90,7 +91,7 @@ def lib():
         L.b2_store_destroy.restype = None
         for f in EXPORTS:
             if f not in ("b2_last_error", "b2_destroy", "b2_store_last_error", "b2_store_destroy"):
-                getattr(L, f).restype = ctypes.c_int
+                getattr(L, f).restype = i64 if f == "b2_store_size" else ctypes.c_int
         _lib = L
     return _lib
 

@@ -36,8 +36,11 @@ class Store:
             raise ValueError("the log2 and exp2 tables have 65,536 entries")
         h = ctypes.c_void_p()
         cfg = StoreConfig(n_streams, n_layer, n_head, max_ctx)
+        size = lib().b2_store_size(ctypes.byref(cfg), t[0].size)
+        # torch's allocator gives the memory (and keeps it between stores)
+        self._memory = self.torch.empty(max(size, 0), dtype=self.torch.uint8, device=self.device)
         rc = lib().b2_store_create(ctypes.byref(cfg), device, t[0].ctypes.data, t[0].size, t[1].ctypes.data, t[2].ctypes.data,
-                                   ctypes.byref(h))
+                                   self._memory.data_ptr(), ctypes.byref(h))
         self.h = h if h.value else None
         if rc:
             msg = lib().b2_store_last_error(self.h).decode() if self.h else f"b2_store_create failed ({n_streams} streams, " \
@@ -97,8 +100,6 @@ class Store:
 
     def _out(self, out, rows: int, name: str):
         shape = (rows, *self._row)
-        if out is None:
-            return self.torch.empty(shape, dtype=self._i64, device=self.device)
         if isinstance(out, self._tensor) and out.dtype is self._i64 and out.get_device() == self._index and \
                 out.shape == shape and out.is_contiguous():
             return out
@@ -136,8 +137,10 @@ class Store:
             if cu is not None:
                 raise ValueError("rows (cu's last entry) goes with cu")
             rows = len(pos)
-        k, v = (None, None) if out is None else out
-        k, v = self._out(k, rows, "out k"), self._out(v, rows, "out v")
+        if out is None:
+            k, v = self.torch.empty((2, rows, *self._row), dtype=self._i64, device=self.device).unbind(0)
+        else:
+            k, v = self._out(out[0], rows, "out k"), self._out(out[1], rows, "out v")
         cu, pos, n, rows, most = self._table(pos, cu, rows, max_rows)
         rc = self._f_read(h, layer, cu, pos, n, rows, most, k.data_ptr(), v.data_ptr(), self._stream(self._index))
         if rc:
@@ -151,10 +154,12 @@ class Store:
         h = self._open()
         pq, ldq = self._rows(q, "q")
         rows = q.shape[0]
-        if out is None and q.dim() == 3 and q.is_contiguous():
-            out = self.torch.empty_like(q)               # (what _out makes, in less time)
-        else:
+        if out is not None:
             out = self._out(out, rows, "out")
+        elif q.dim() == 3 and q.is_contiguous():
+            out = self.torch.empty_like(q)               # (the quickest)
+        else:
+            out = q.new_empty((rows, *self._row))
         cu, pos, n, rows, most = self._table(pos, cu, rows, max_rows)
         f = None if first is None else self._ints(first, "first", n)
         rc = self._f_attend(h, layer, pq, ldq, cu, pos, f, n, rows, most, window, out.data_ptr(), self._stream(self._index))
@@ -169,8 +174,8 @@ class Store:
 
     def close(self):
         if getattr(self, "h", None):
-            lib().b2_store_destroy(self.h)
-            self.h = None
+            lib().b2_store_destroy(self.h)               # (waits for the device)
+            self.h = self._memory = None
 
     def __del__(self):
         try:

@@ -236,9 +236,8 @@ def test_refusals(T):
     with pytest.raises(engine.B2Error) as ex:
         store.Store(T, 1, 65537, 1)
     assert ex.value.code == 1
-    with pytest.raises(engine.B2Error) as ex:
-        store.Store(T, 65535, 65536, 1024, n_layer=1024)     # far past the device's memory
-    assert ex.value.code == 3
+    with pytest.raises(torch.OutOfMemoryError):
+        store.Store(T, 1000, 65536, 12, n_layer=12)              # 632 GB
     st, _ = make(T, 2, 16, 1, layers=2)
     x = torch.zeros(2, 1, 64, dtype=torch.int64, device="cuda")
     pos = i32([0, 0])
@@ -421,3 +420,35 @@ def test_calls_at_once(T):
     assert all(torch.equal(w, g) for w, g in got)
     st.sync()
     st.close()
+
+
+def test_the_library_allocates(T):
+    """The C ABI with memory = NULL: the library's own allocation, and its refusal of one that does not fit."""
+    import ctypes
+    import torch
+    from streaming_machine_b200 import engine, store
+    L = engine.lib()
+    t = [np.ascontiguousarray(T[k], dtype=np.int64) for k in ("arrival", "log2", "exp2")]
+
+    def create(*cfg):
+        h = ctypes.c_void_p()
+        rc = L.b2_store_create(ctypes.byref(engine.StoreConfig(*cfg)), 0, t[0].ctypes.data, t[0].size, t[1].ctypes.data,
+                               t[2].ctypes.data, None, ctypes.byref(h))
+        return rc, h
+    rc, h = create(1000, 12, 12, 65536)
+    assert rc == 3 and b"cudaMalloc" in L.b2_store_last_error(h)
+    assert L.b2_store_sync(h) == 1                             # a store that was not made refuses every call
+    L.b2_store_destroy(h)
+    rc, h = create(2, 1, 3, 40)
+    assert rc == 0
+    rng = np.random.default_rng(21)
+    k, v, q = (dev(values(rng, 2, 3, s)) for s in (1.0, 0.3, 1.5))
+    pos, out = i32([0, 0]), torch.zeros(2, 3, 64, dtype=torch.int64, device="cuda")
+    torch.cuda.synchronize()
+    assert L.b2_store_write(h, 0, k.data_ptr(), 192, v.data_ptr(), 192, None, pos.data_ptr(), 2, 2, 1, None) == 0
+    assert L.b2_store_attend(h, 0, q.data_ptr(), 192, None, pos.data_ptr(), None, 2, 2, 1, 0, out.data_ptr(), None) == 0
+    assert L.b2_store_sync(h) == 0
+    L.b2_store_destroy(h)
+    pl = ref.Store(T, 3)
+    pl.write(k.cpu().numpy(), v.cpu().numpy(), [0, 0])
+    assert np.array_equal(out.cpu().numpy(), pl.attend(q.cpu().numpy(), [0, 0]))

@@ -88,12 +88,16 @@ def test_create_refuses_before_it_touches_a_device():
     t = np.ones(65536, np.int64)
     h = ctypes.c_void_p()
 
-    def create(cfg, arr=t, n=100, log2=t, exp2=t):
+    def create(cfg, arr=t, n=100, log2=t, exp2=t, mem=None):
         ptr = [a.ctypes.data if a is not None else None for a in (arr, log2, exp2)]
-        return L.b2_store_create(ctypes.byref(engine.StoreConfig(*cfg)), 0, ptr[0], n, ptr[1], ptr[2], ctypes.byref(h))
+        return L.b2_store_create(ctypes.byref(engine.StoreConfig(*cfg)), 0, ptr[0], n, ptr[1], ptr[2], mem, ctypes.byref(h))
     for cfg in ((0, 1, 1, 1), (65536, 1, 1, 1), (1, 0, 1, 1), (1, 1025, 1, 1), (1, 1, 0, 1), (1, 1, 1025, 1), (1, 1, 1, 0),
                 (1, 1, 1, 65537), (-1, 1, 1, 1)):
         assert create(cfg) == 1 and not h.value
+        assert L.b2_store_size(ctypes.byref(engine.StoreConfig(*cfg)), 100) == -1
+    assert create((1, 1, 1, 1), mem=4096 + 16) == 1 and not h.value        # memory that is not 32-byte aligned
+    # 67 bytes a position and head (positions in 32s), the error words and the tables
+    assert L.b2_store_size(ctypes.byref(engine.StoreConfig(3, 2, 5, 33)), 100) == 3 * 2 * 5 * 64 * 67 + 4 * (4 + 131072 + 100)
     for kw in (dict(arr=None), dict(log2=None), dict(exp2=None), dict(n=0), dict(n=-5), dict(n=32769)):
         assert create((1, 1, 1, 1), **kw) == 1 and not h.value
     for f, args in (("b2_store_write", (0, None, 0, None, 0, None, None, 0, 0, 0, None)),
