@@ -191,7 +191,7 @@ int b2_check_wait(b2_handle* h, void* stream);
  * at r * ld + 64 h (ld in elements, at least 64 n_head). Work is queued on `stream`; nothing is allocated, copied to
  * the host or kept between calls, so calls may be captured into a graph, and calls that do not write what another one
  * reads or writes may run at once on several streams (the host's calls on one store come one after the other). out may be
- * q itself. A stream whose rows do not fit the call or whose positions pass the context is skipped and flagged:
+ * q itself (not a step's k or v). A stream whose rows do not fit the call or whose positions pass the context is skipped and flagged:
  * b2_store_sync reports it (B2_ERR_ARG, B2_ERR_CTX). */
 typedef struct b2_store b2_store;
 typedef struct {
@@ -226,6 +226,12 @@ int b2_store_read(b2_store* s, int32_t layer, const int32_t* cu, const int32_t* 
 int b2_store_attend(b2_store* s, int32_t layer, const int64_t* q, int64_t ldq, const int32_t* cu, const int32_t* pos,
                     const int32_t* first, int32_t n_streams, int32_t rows, int32_t max_rows, int32_t window, int64_t* out,
                     void* stream);
+
+/* A decode step's b2_store_write and b2_store_attend of one row a stream (row i is stream i's, at position pos[i]) in one
+ * launch: the same results. */
+int b2_store_step(b2_store* s, int32_t layer, const int64_t* q, int64_t ldq, const int64_t* k, int64_t ldk, const int64_t* v,
+                  int64_t ldv, const int32_t* pos, const int32_t* first, int32_t n_streams, int32_t window, int64_t* out,
+                  void* stream);
 
 /* Wait for queued work and report what the device checks flagged since the last call. */
 int b2_store_sync(b2_store* s);

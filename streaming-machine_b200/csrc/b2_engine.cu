@@ -441,25 +441,33 @@ int run_attend(b2_handle* h, int rows, int l, uint64_t* or_out, cudaStream_t st,
 }
 
 // "store_bits" 4, after layer l's qkv bank (q, k, v in QKV's rows): (Pythia's turn,) the rows' keys and values into the
-// 4-bit store, then the arrival over it
+// 4-bit store and the arrival over it; a decode step's in one launch
 int run_store4(b2_handle* h, int rows, int l, uint64_t* or_out, cudaStream_t st) {
     const int d = h->cfg.d_model;
-    const bool py = h->cfg.kind == B2_PYTHIA;
+    const bool py = h->cfg.kind == B2_PYTHIA, step = !h->rows4.cu;
     const int hs = py ? 192 : 64;                       // Pythia's columns are per head q, k, v
     const StoreLaunch how{st, h->pdl && h->prof.timing != 1, &h->plan4};
-    int rc;
-    if (py && (rc = launch(h, B2_PROF_HEADS, "turn", k_turn, rows, 256, 0, st, h->QKV, rows, (const int32_t*)h->row_pos,
-                           h->cfg.n_head, h->st4.lim, (const int32_t*)h->COS, (const int32_t*)h->SIN, h->d_err)))
-        return rc;
-    prof_begin(h, B2_PROF_HEADS, st);
-    cudaError_t e = store_write(h->st4, h->rows4, l, StoreVec{h->QKV + (py ? 64 : d), 3 * d, hs},
-                                StoreVec{h->QKV + (py ? 128 : 2 * d), 3 * d, hs}, h->d_err, how, stamp_slot(h, B2_PROF_HEADS));
-    prof_end(h, B2_PROF_HEADS, st);
-    if (e != cudaSuccess) return fail(h, B2_ERR_CUDA, "launch store_write: %s", cudaGetErrorString(e));
     StoreAttend a{h->st4, h->rows4, l, StoreVec{h->QKV, 3 * d, hs}, nullptr, 0, h->ARR, h->alen, h->LOG2, h->EXP2, h->ATT,
-                  or_out, h->d_err, stamp_slot(h, B2_PROF_ATTEND)};
+                  or_out, h->d_err};
+    a.k = StoreVec{h->QKV + (py ? 64 : d), 3 * d, hs};
+    a.v = StoreVec{h->QKV + (py ? 128 : 2 * d), 3 * d, hs};
+    int rc;
+    cudaError_t e;
+    if (!step) {
+        if (py && (rc = launch(h, B2_PROF_HEADS, "turn", k_turn, rows, 256, 0, st, h->QKV, rows, (const int32_t*)h->row_pos,
+                               h->cfg.n_head, h->st4.lim, (const int32_t*)h->COS, (const int32_t*)h->SIN, h->d_err)))
+            return rc;
+        prof_begin(h, B2_PROF_HEADS, st);
+        e = store_write(h->st4, h->rows4, l, a.k, a.v, h->d_err, how, stamp_slot(h, B2_PROF_HEADS));
+        prof_end(h, B2_PROF_HEADS, st);
+        if (e != cudaSuccess) return fail(h, B2_ERR_CUDA, "launch store_write: %s", cudaGetErrorString(e));
+    } else if (py) {
+        a.COS = h->COS;
+        a.SIN = h->SIN;
+    }
+    a.stamp = stamp_slot(h, B2_PROF_ATTEND);
     prof_begin(h, B2_PROF_ATTEND, st);
-    e = store_attend(a, how);
+    e = step ? store_step(a, how) : store_attend(a, how);
     prof_end(h, B2_PROF_ATTEND, st);
     if (e != cudaSuccess) return fail(h, B2_ERR_CUDA, "launch store_attend: %s", cudaGetErrorString(e));
     return B2_OK;

@@ -267,13 +267,43 @@ B2_DEV void query_bytes(const int64_t (&x)[N][2], uint32_t (&word)[N], int (&u)[
         word[k] = __byte_perm(__byte_perm(a[k] + 128, a[k], 0x41), __byte_perm(b[k] + 128, b[k], 0x41), 0x5410);
 }
 
+// a head row held by a warp (lane l: dims 2l, 2l + 1), put into the store at element e (k_store_write's arithmetic)
+B2_DEV void put_row(const Store4& st, size_t e, bool key, int64_t x0, int64_t x1, int lane) {
+    x0 = store_clamp(x0);
+    x1 = store_clamp(x1);
+    const uint32_t t = (uint32_t)bitlen_u(mag(x0) | mag(x1));
+    const int lo = (int)__reduce_max_sync(0xffffffffu, lane < 16 ? t : 0u), hi = (int)__reduce_max_sync(0xffffffffu, lane < 16 ? 0u : t);
+    const int big = min(max(max(lo, hi) - 3, 0), STORE_MAX_SHIFT);
+    const int sh = key ? max(min(max((lane < 16 ? lo : hi) - 3, 0), STORE_MAX_SHIFT), big - 3) : big;
+    const uint8_t c = (uint8_t)((store_code(x0, sh) & 15) | (store_code(x1, sh) << 4));
+    if (key) {
+        st.k[e * 32 + key_byte(lane)] = c;
+        if ((lane & 15) == 0) st.ks[e * 2 + (lane >> 4)] = (int8_t)sh;
+    } else {
+        st.v[e * 32 + lane] = c;
+        if (lane == 0) st.vs[e] = (int8_t)sh;
+    }
+}
+
+// Pythia's turn of such a row (pythia_base2.py:116-124, the arithmetic of k_turn): dims t and t + 8, t < 8, lie four lanes
+// apart
+B2_DEV void turn_row(int64_t& x0, int64_t& x1, int lane, int pos, const int32_t* COS, const int32_t* SIN, uint32_t* err) {
+    const int64_t o0 = __shfl_xor_sync(0xffffffffu, x0, 4), o1 = __shfl_xor_sync(0xffffffffu, x1, 4);
+    if (lane >= 8) return;
+    if ((mag(x0) | mag(x1)) >= (1ull << 31)) set_err(err, DERR_RANGE);
+    const size_t t = (size_t)pos * 8 + 2 * (lane & 3);
+    const int64_t c0 = COS[t], s0 = SIN[t], c1 = COS[t + 1], s1 = SIN[t + 1];
+    x0 = rshift(lane < 4 ? wsub(wmul(x0, c0), wmul(o0, s0)) : wadd(wmul(x0, c0), wmul(o0, s0)), 30);
+    x1 = rshift(lane < 4 ? wsub(wmul(x1, c1), wmul(o1, s1)) : wadd(wmul(x1, c1), wmul(o1, s1)), 30);
+}
+
 template <int NW>
 B2_DEV void unit_sync() {
     if (NW == 1) __syncwarp();
     else __syncthreads();
 }
 
-template <int NW>
+template <int NW, bool PUT>
 __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, NW == 1 ? 7 : (NW == 4 ? 6 : (NW == 8 ? 3 : 1))) k_store_attend_few(StoreAttend a, int chunk, int cs, int wide) {
     extern __shared__ __align__(16) uint8_t sm[];
     constexpr int UN = NW == 1 ? 4 : 1;                              // (row, head) units a CTA
@@ -298,7 +328,19 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, NW == 1 ? 7 : (NW == 
     int lo = a.window > 0 ? max(0, p - a.window + 1) : 0;
     if (a.first) lo = max(lo, a.first[s]);
     int64_t* const out = a.out + ((size_t)row * H + h) * 64;
+    // PUT: the row's own key and value, by the warp whose block they fall into
+    auto put = [&]() {
+        const size_t e = kv_index(a.rw.slot0 + s, a.layer, h, p, a.st.L, H, a.st.ctx);
+        int64_t k0, k1, v0, v1;
+        load_pair(a.k.x + (size_t)row * a.k.ld + h * a.k.hs + 2 * lane, wide & 4, k0, k1);
+        load_pair(a.v.x + (size_t)row * a.v.ld + h * a.v.hs + 2 * lane, wide & 8, v0, v1);
+        if (a.COS) turn_row(k0, k1, lane, p, a.COS, a.SIN, a.err);
+        put_row(a.st, e, true, k0, k1, lane);
+        put_row(a.st, e, false, v0, v1, lane);
+        __syncwarp();                                                // the warp's own loads come after it
+    };
     if (lo > p) {
+        if (PUT && rank == 0 && wid == 0) put();
         for (int t = ut; t < 64 && rank == 0; t += NW * 32) out[t] = 0;
         return;
     }
@@ -328,10 +370,12 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, NW == 1 ? 7 : (NW == 
 #pragma unroll
         for (int t = 0; t < 8; t++) w[t] = from_[t * 8];
     };
+    if (PUT && nb > 0 && b0 + nb - 1 == p >> 5 && (nb - 1) % NW == wid) put();
     Keys k[PF];
 #pragma unroll
     for (int f = 0; f < PF; f++)
         if (wid + f * NW < nb) keys(wid + f * NW, k[f]);
+    if (PUT && a.COS) turn_row(x[0][0], x[0][1], lane, p, a.COS, a.SIN, a.err);
     uint32_t words[1], q0[2], q1[2];                                 // q0, q1: B operands of the two halves
     int us[1];
     query_bytes(x, words, us);
@@ -1065,7 +1109,8 @@ cudaError_t store_read(const Store4& st, const StoreRows& rw, int layer, int64_t
     return store_launch(how, k_store_read<SW_ROWS>, row_grid(st, rw, SW_ROWS), SW_WARPS * 32, 0, 1, st, rw, layer, k, v, wide, err);
 }
 
-constexpr int SM_FROM_ROWS = 20, SM_FIXED = 4;
+constexpr int SM_FROM_ROWS = 20;     // rows a stream up to which the few-row kernel is quicker (between 12 and 48, by the context)
+constexpr int SM_FIXED = 4, SM_SPLIT = 6;
 constexpr int SM_SMEM_MOST = 200 * 1024;
 constexpr int SF_MOST_KEYS = 8192;   // of a CTA: 64 KB of shared memory
 constexpr int SF_WARP_UNITS = 12, SF_WARP_BLOCKS = 32;   // a warp a unit: from so many units an SM on, up to 1,024 keys (32 KB a CTA)
@@ -1076,9 +1121,12 @@ size_t many_smem(int alen) { return sizeof(SmShared) + (size_t)(alen + 1) * 4; }
 namespace {
 cudaError_t make_plan(int device, int alen, StorePlan& plan) {
     cudaError_t e = cudaDeviceGetAttribute(&plan.sms, cudaDevAttrMultiProcessorCount, device);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(k_store_attend_few<4>, cudaFuncAttributeMaxDynamicSharedMemorySize, SF_MOST_KEYS * SF_BYTES);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(k_store_attend_few<8>, cudaFuncAttributeMaxDynamicSharedMemorySize, SF_MOST_KEYS * SF_BYTES);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(k_store_attend_few<16>, cudaFuncAttributeMaxDynamicSharedMemorySize, SF_MOST_KEYS * SF_BYTES);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(k_store_attend_few<4, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, SF_MOST_KEYS * SF_BYTES);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(k_store_attend_few<4, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, SF_MOST_KEYS * SF_BYTES);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(k_store_attend_few<8, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, SF_MOST_KEYS * SF_BYTES);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(k_store_attend_few<8, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, SF_MOST_KEYS * SF_BYTES);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(k_store_attend_few<16, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, SF_MOST_KEYS * SF_BYTES);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(k_store_attend_few<16, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, SF_MOST_KEYS * SF_BYTES);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(k_store_attend_many, cudaFuncAttributeMaxDynamicSharedMemorySize, SM_SMEM_MOST);
     if (e != cudaSuccess) return e;
     int fit = 0;
@@ -1125,38 +1173,16 @@ cudaError_t store_init(int alen, StorePlan& plan) {
     return e;
 }
 
-cudaError_t store_attend(const StoreAttend& a, StoreLaunch how) {
-    if (a.rw.n_streams == 0 || a.rw.rows == 0) return cudaSuccess;
-    const int wide = pairs(a.q) | aligned16(a.out) << 1;
-    const int64_t items = (int64_t)((a.rw.max_rows + SM_ROWS - 1) / SM_ROWS) * a.st.H * a.rw.n_streams;
-    if (a.rw.max_rows > SM_FROM_ROWS && items < INT32_MAX) {
-        const int tiles = (a.rw.max_rows + SM_ROWS - 1) / SM_ROWS;
-        const size_t smem = many_smem(a.alen);
-        // fewer items than the GPU holds: their keys split over clusters, in two tiles a CTA at least, by the time that a
-        // split would take (waves x tiles a CTA, an item's start and end counted as SM_FIXED tiles)
-        const int keys = a.window > 0 ? std::min(a.st.lim, std::min(a.window, a.st.lim) + SM_ROWS) : a.st.lim;
-        const int all = (keys + SM_KEYS - 1) / SM_KEYS;
-        int cs = 1;
-        int64_t least = INT64_MAX;
-        for (int k = 1; k <= STORE_MAX_CLUSTER && (k == 1 || k * 2 <= all); k++) {
-            const int fit = how.plan->many[k];
-            if (fit < 1) continue;
-            const int64_t t = (items + fit - 1) / fit * ((all + k - 1) / k + SM_FIXED);
-            if (t < least) {
-                least = t;
-                cs = k;
-            }
-        }
-        const dim3 grid((unsigned)(std::min<int64_t>(items, std::max(how.plan->many[cs], 1)) * cs));
-        return store_launch(how, k_store_attend_many, grid, SM_THREADS, smem, cs, a, tiles, cs, wide);
-    }
+namespace {
+template <bool PUT>
+cudaError_t attend_few(const StoreAttend& a, StoreLaunch how, int wide) {
     // blocks of 32 positions that a row may see
     int blocks = (a.st.lim + 31) / 32;
     if (a.window > 0 && a.window < a.st.lim) blocks = std::min(blocks, (a.window + 30) / 32 + 1);
     const int64_t units = (int64_t)a.rw.n_streams * a.rw.max_rows * a.st.H;
     if (units >= (int64_t)SF_WARP_UNITS * how.plan->sms && blocks <= SF_WARP_BLOCKS) {
         const dim3 grid((unsigned)(((int64_t)a.rw.max_rows * a.st.H + 3) / 4), a.rw.n_streams);
-        return store_launch(how, k_store_attend_few<1>, grid, 128, (size_t)blocks * 32 * SF_BYTES * 4, 1, a, blocks * 32, 1, wide);
+        return store_launch(how, k_store_attend_few<1, PUT>, grid, 128, (size_t)blocks * 32 * SF_BYTES * 4, 1, a, blocks * 32, 1, wide);
     }
     // a cluster costs about 1.3 us (its barriers), a warp's block of 32 keys 0.5 (from L2) to 1.2 us (from HBM): the keys are
     // split where that leaves half the SMs idle, and while there is a long run of keys for every CTA of two an SM
@@ -1169,9 +1195,48 @@ cudaError_t store_attend(const StoreAttend& a, StoreLaunch how) {
     const dim3 grid((unsigned)((int64_t)a.rw.max_rows * a.st.H * cs), a.rw.n_streams);
     const size_t smem = (size_t)chunk * SF_BYTES;
     if (each >= SF_VERY_LONG && units * cs <= how.plan->sms)       // 16 warps: one CTA an SM
-        return store_launch(how, k_store_attend_few<16>, grid, 512, smem, cs, a, chunk, cs, wide);
-    if (each >= SF_LONG) return store_launch(how, k_store_attend_few<8>, grid, 256, smem, cs, a, chunk, cs, wide);
-    return store_launch(how, k_store_attend_few<4>, grid, 128, smem, cs, a, chunk, cs, wide);
+        return store_launch(how, k_store_attend_few<16, PUT>, grid, 512, smem, cs, a, chunk, cs, wide);
+    if (each >= SF_LONG) return store_launch(how, k_store_attend_few<8, PUT>, grid, 256, smem, cs, a, chunk, cs, wide);
+    return store_launch(how, k_store_attend_few<4, PUT>, grid, 128, smem, cs, a, chunk, cs, wide);
+}
+int wide_bits(const StoreAttend& a) {
+    return pairs(a.q) | aligned16(a.out) << 1 | pairs(a.k) << 2 | pairs(a.v) << 3;
+}
+}  // namespace
+
+cudaError_t store_step(const StoreAttend& a, StoreLaunch how) {
+    if (a.rw.n_streams == 0 || a.rw.rows == 0) return cudaSuccess;
+    return attend_few<true>(a, how, wide_bits(a));
+}
+
+cudaError_t store_attend(const StoreAttend& a, StoreLaunch how) {
+    if (a.rw.n_streams == 0 || a.rw.rows == 0) return cudaSuccess;
+    const int wide = wide_bits(a);
+    const int64_t items = (int64_t)((a.rw.max_rows + SM_ROWS - 1) / SM_ROWS) * a.st.H * a.rw.n_streams;
+    if (a.rw.max_rows > SM_FROM_ROWS && items < INT32_MAX) {
+        const int tiles = (a.rw.max_rows + SM_ROWS - 1) / SM_ROWS;
+        const size_t smem = many_smem(a.alen);
+        // fewer items than half of what the GPU holds: their keys split over clusters, in two tiles a CTA at least, by the
+        // time that a split would take (waves x tiles a CTA, an item's start and end counted as SM_FIXED tiles, a cluster's
+        // barriers and sums as SM_SPLIT more: 2 x 256 rows on 8,000 positions 263 us whole, 182 on clusters of five; 8 x 64
+        // on 500 30 us whole, 33 on pairs)
+        const int keys = a.window > 0 ? std::min(a.st.lim, std::min(a.window, a.st.lim) + SM_ROWS) : a.st.lim;
+        const int all = (keys + SM_KEYS - 1) / SM_KEYS;
+        int cs = 1;
+        int64_t least = INT64_MAX;
+        for (int k = 1; k <= STORE_MAX_CLUSTER && (k == 1 || (k * 2 <= all && items * 2 <= how.plan->many[1])); k++) {
+            const int fit = how.plan->many[k];
+            if (fit < 1) continue;
+            const int64_t t = (items + fit - 1) / fit * ((all + k - 1) / k + SM_FIXED + (k > 1 ? SM_SPLIT : 0));
+            if (t < least) {
+                least = t;
+                cs = k;
+            }
+        }
+        const dim3 grid((unsigned)(std::min<int64_t>(items, std::max(how.plan->many[cs], 1)) * cs));
+        return store_launch(how, k_store_attend_many, grid, SM_THREADS, smem, cs, a, tiles, cs, wide);
+    }
+    return attend_few<false>(a, how, wide);
 }
 
 }  // namespace b2
@@ -1404,6 +1469,28 @@ int b2_store_attend(b2_store* h, int32_t layer, const int64_t* q, int64_t ldq, c
         StoreAttend a{h->st, StoreRows{cu, pos, n_streams, rows, std::min(max_rows, h->cfg.max_ctx)}, layer, StoreVec{q, ldq, 64}, first, window, h->ARR, h->alen,
                       h->LOG2, h->EXP2, out, nullptr, h->d_err};
         SCK(store_attend(a, StoreLaunch{(cudaStream_t)stream, true, &h->plan}));
+        return (int)B2_OK;
+    });
+}
+
+int b2_store_step(b2_store* h, int32_t layer, const int64_t* q, int64_t ldq, const int64_t* k, int64_t ldk, const int64_t* v,
+                  int64_t ldv, const int32_t* pos, const int32_t* first, int32_t n_streams, int32_t window, int64_t* out,
+                  void* stream) {
+    if (!h || !h->d_err) return B2_ERR_ARG;
+    return guarded(h, [&] {
+        int rc = check_rows(h, "b2_store_step", layer, nullptr, pos, n_streams, n_streams, n_streams ? 1 : 0);
+        if (rc) return rc;
+        const int64_t d = 64ll * h->cfg.n_head;
+        if (window < 0 || (n_streams && (!q || !k || !v || !out || ldq < d || ldk < d || ldv < d)))
+            return sfail(h, B2_ERR_ARG, "b2_store_step: q %p (stride %lld), k %p (%lld), v %p (%lld), out %p, window %d", (const void*)q,
+                         (long long)ldq, (const void*)k, (long long)ldk, (const void*)v, (long long)ldv, (const void*)out, window);
+        OnDevice on(h->device);
+        SCK(on.e);
+        StoreAttend a{h->st, StoreRows{nullptr, pos, n_streams, n_streams, 1}, layer, StoreVec{q, ldq, 64}, first, window, h->ARR,
+                      h->alen, h->LOG2, h->EXP2, out, nullptr, h->d_err};
+        a.k = StoreVec{k, ldk, 64};
+        a.v = StoreVec{v, ldv, 64};
+        SCK(store_step(a, StoreLaunch{(cudaStream_t)stream, true, &h->plan}));
         return (int)B2_OK;
     });
 }

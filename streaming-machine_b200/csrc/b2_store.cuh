@@ -58,6 +58,10 @@ struct StoreAttend {
     uint64_t* or_out;      // optional [rows]: OR of |out| per row (the next bank's to16 shift)
     uint32_t* err;
     uint64_t* stamp = nullptr;   // b2_profile mode 2
+    // store_step: the rows' own keys and values, held first (one row a stream); Pythia's turn of q and k before it, where
+    // COS is given ([positions][8] at 2^-30)
+    StoreVec k{nullptr, 0, 0}, v{nullptr, 0, 0};
+    const int32_t *COS = nullptr, *SIN = nullptr;
 };
 
 // what the launches are sized by, once per device (the current one) and arrival table; to be called before the first launch
@@ -79,6 +83,7 @@ cudaError_t store_write(const Store4& st, const StoreRows& rw, int layer, const 
                         StoreLaunch how, uint64_t* stamp = nullptr);
 cudaError_t store_read(const Store4& st, const StoreRows& rw, int layer, int64_t* k, int64_t* v, uint32_t* err, StoreLaunch how);
 cudaError_t store_attend(const StoreAttend& a, StoreLaunch how);
+cudaError_t store_step(const StoreAttend& a, StoreLaunch how);   // a.rw.max_rows = 1
 
 constexpr int64_t STORE_TOP = 1ll << 47;          // magnitudes are held below this
 constexpr int32_t STORE_LIM = (1 << 30) - 1;      // scores are held between -STORE_LIM and STORE_LIM

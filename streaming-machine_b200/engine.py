@@ -28,7 +28,7 @@ EXPORTS = ("b2_create", "b2_set_bank", "b2_set_array", "b2_set_scalar", "b2_fina
            "b2_prefill", "b2_step", "b2_generate", "b2_step_host", "b2_bank", "b2_gauge", "b2_bank_noalloc",
            "b2_rewind", "b2_profile", "b2_profile_read", "b2_sync", "b2_check_wait", "b2_set_bank_layout",
            "b2_get_bank_layout", "b2_last_error", "b2_destroy", "b2_abi_version", "b2_store_size", "b2_store_create",
-           "b2_store_write", "b2_store_read", "b2_store_attend", "b2_store_sync", "b2_store_last_error", "b2_store_destroy")
+           "b2_store_write", "b2_store_read", "b2_store_attend", "b2_store_step", "b2_store_sync", "b2_store_last_error", "b2_store_destroy")
 PROF_CLASSES = ("bank", "attend", "quant", "heads", "race", "other")
 
 
@@ -84,6 +84,7 @@ def lib():
         L.b2_store_write.argtypes = [vp, i32, vp, i64, vp, i64, vp, vp, i32, i32, i32, vp]
         L.b2_store_read.argtypes = [vp, i32, vp, vp, i32, i32, i32, vp, vp, vp]
         L.b2_store_attend.argtypes = [vp, i32, vp, i64, vp, vp, vp, i32, i32, i32, i32, vp, vp]
+        L.b2_store_step.argtypes = [vp, i32, vp, i64, vp, i64, vp, i64, vp, vp, i32, i32, vp, vp]
         L.b2_store_sync.argtypes = [vp]
         L.b2_store_last_error.argtypes = [vp]
         L.b2_store_last_error.restype = cp

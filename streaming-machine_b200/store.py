@@ -5,6 +5,7 @@
     st = store.Store(convert.tables(), n_streams=64, max_ctx=1024, n_head=12)
     st.write(k, v, pos)              # one new position per stream: k, v [64, 12, 64] int64, pos [64] int32
     y = st.attend(q, pos)            # [64, 12, 64] int64: what each row takes from its stream's positions 0 .. pos
+    y = st.step(q, k, v, pos)        # both in one launch
     k4, v4 = st.read(pos)            # the values that the store holds for those positions
 
 Numbers are whole, at the stream's scale 2^-16; include/base2.h has the formulas. A prompt pass gives many rows per
@@ -57,7 +58,7 @@ class Store:
         self._row, self._flat, self._unit = (n_head, HEAD), (n_head * HEAD,), (HEAD, 1)
         self._stream, self._index = (torch._C._cuda_getCurrentRawStream, device) if cuda else (lambda i: None, -1)
         L = lib()
-        self._f_write, self._f_read, self._f_attend = L.b2_store_write, L.b2_store_read, L.b2_store_attend
+        self._f_write, self._f_read, self._f_attend, self._f_step = L.b2_store_write, L.b2_store_read, L.b2_store_attend, L.b2_store_step
 
     # ---- plumbing ---------------------------------------------------------------------------------------------
     # (a decode step comes here for every layer: the usual case is settled by a few comparisons, what is wrong with an
@@ -72,6 +73,8 @@ class Store:
                     return x.data_ptr(), st[0]
                 if shape[0] <= 1:                                # a single row's stride says nothing
                     return x.data_ptr(), d
+            if shape[:1] == (0,) and shape[1:] in (self._row, self._flat):
+                return x.data_ptr(), d                           # no rows: no stride says anything
             raise ValueError(f"{name}: rows of [{self.n_head}, {HEAD}] (or {d}) values, one behind the other and apart, got "
                              f"shape {tuple(shape)}, strides {st}")
         raise ValueError(f"{name}: a torch.int64 tensor on {self.device}, got {self._what(x)}")
@@ -163,6 +166,25 @@ class Store:
         cu, pos, n, rows, most = self._table(pos, cu, rows, max_rows)
         f = None if first is None else self._ints(first, "first", n)
         rc = self._f_attend(h, layer, pq, ldq, cu, pos, f, n, rows, most, window, out.data_ptr(), self._stream(self._index))
+        if rc:
+            self._done(rc)
+        return out
+
+    def step(self, q, k, v, pos, window: int = 0, first=None, layer: int = 0, out=None):
+        """A decode step, write() and attend() of one row a stream in one launch: row i is stream i's, at position pos[i]."""
+        h = self._open()
+        (pq, ldq), (pk, ldk), (pv, ldv), n = self._rows(q, "q"), self._rows(k, "k"), self._rows(v, "v"), q.shape[0]
+        if k.shape[0] != n or v.shape[0] != n:
+            raise ValueError(f"{n} rows of queries, {k.shape[0]} of keys, {v.shape[0]} of values")
+        if out is not None:
+            out = self._out(out, n, "out")
+        elif q.dim() == 3 and q.is_contiguous():
+            out = self.torch.empty_like(q)
+        else:
+            out = q.new_empty((n, *self._row))
+        p = self._ints(pos, "pos", n)
+        f = None if first is None else self._ints(first, "first", n)
+        rc = self._f_step(h, layer, pq, ldq, pk, ldk, pv, ldv, p, f, n, window, out.data_ptr(), self._stream(self._index))
         if rc:
             self._done(rc)
         return out

@@ -452,3 +452,60 @@ def test_the_library_allocates(T):
     pl = ref.Store(T, 3)
     pl.write(k.cpu().numpy(), v.cpu().numpy(), [0, 0])
     assert np.array_equal(out.cpu().numpy(), pl.attend(q.cpu().numpy(), [0, 0]))
+
+
+@pytest.mark.parametrize("n,heads,ctx", [(1, 12, 100), (3, 2, 33), (64, 12, 160), (150, 12, 70), (2, 1, 5000), (16, 12, 1040), (1, 1, 30000)])
+def test_step_is_write_and_attend(T, n, heads, ctx):
+    """step() on one store, write() and attend() on another, token by token at every place in a block of 32 positions, with
+    windows and dropped beginnings (that leave a row nothing): the same outputs and the same store."""
+    import torch
+    rng = np.random.default_rng(n + ctx)
+    a, b = make(T, n, ctx, heads)[0], make(T, n, ctx, heads)[0]
+    start = max(ctx - 34, 0)
+    hist = [dev(values(rng, n * start, heads, s)) for s in (1.0, 0.3)]
+    for st in (a, b):
+        st.write(*hist, i32([0] * n), cu=i32(np.arange(n + 1) * start), max_rows=start)
+    qkv = torch.zeros(n, 3 * heads * 64 + 1, dtype=torch.int64, device="cuda")
+    for t in range(min(34, ctx)):
+        pos = i32(start + t - rng.integers(0, t + 1, n))
+        window = int(rng.choice([0, 0, 1, 40, ctx]))
+        first = i32(rng.integers(0, ctx + 4, n)) if t % 3 == 2 else None
+        x = values(rng, n, 3 * heads, 1.0)
+        if t % 5 == 4:
+            x[:, :, 0] = rng.choice([-2 ** 63, 2 ** 46, 2 ** 31, 0], (n, 3 * heads))
+        qkv[:, t % 2:t % 2 + 3 * heads * 64] = dev(x.reshape(n, -1))
+        q, k, v = (qkv[:, t % 2 + i * heads * 64:t % 2 + (i + 1) * heads * 64] for i in range(3))
+        got = a.step(q, k, v, pos, window=window, first=first)
+        b.write(k, v, pos)
+        assert torch.equal(got, b.attend(q, pos, window=window, first=first)), t
+    rows = i32(np.arange(n + 1) * ctx)
+    for u, w in zip(a.read(i32([0] * n), cu=rows, max_rows=ctx, rows=n * ctx), b.read(i32([0] * n), cu=rows, max_rows=ctx, rows=n * ctx)):
+        assert torch.equal(u, w)
+    a.sync()
+    b.sync()
+    a.close()
+    b.close()
+
+
+def test_step_refusals_and_flags(T):
+    import torch
+    from streaming_machine_b200 import engine
+    st, _ = make(T, 2, 16, 1)
+    x = torch.zeros(2, 1, 64, dtype=torch.int64, device="cuda")
+    pos = i32([0, 0])
+    for call in (lambda: st.step(x, x, x, pos, layer=1), lambda: st.step(x, x, x, pos, window=-1),
+                 lambda: st.step(*[torch.zeros(3, 1, 64, dtype=torch.int64, device="cuda")] * 3, i32([0, 0, 0]))):
+        with pytest.raises(engine.B2Error) as ex:
+            call()
+        assert ex.value.code == 1
+    for call in (lambda: st.step(x, x[:1], x, pos), lambda: st.step(x, x, x[:1], pos), lambda: st.step(x, x, x, i32([0]))):
+        with pytest.raises(ValueError):
+            call()
+    st.step(x, x, x, i32([16, 3]))
+    with pytest.raises(engine.B2Error) as ex:
+        st.sync()
+    assert ex.value.code == 4
+    empty = torch.zeros(0, 1, 64, dtype=torch.int64, device="cuda")
+    assert st.step(empty, empty, empty, i32([])).shape == (0, 1, 64)
+    st.sync()
+    st.close()

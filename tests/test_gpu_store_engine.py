@@ -205,7 +205,8 @@ def test_profiled_steps(kind, eng, peng):
         e._call("b2_profile", e.h, mode)
         assert np.array_equal(e.generate(ids, 4), want)
         _, classes = e.profile_read()
-        assert classes["attend"][0] == 4 * 2 and classes["heads"][0] == 4 * 2 * (2 if kind == "pythia" else 1)
+        assert classes["attend"][0] == 4 * 2                       # the prompt pass and three steps of two layers
+        assert classes["heads"][0] == 2 * (2 if kind == "pythia" else 1)   # the prompt pass's write (and turn)
         if mode:
             assert classes["attend"][1] > 0
     e._call("b2_profile", e.h, 0)

@@ -53,6 +53,7 @@ def test_rows_are_refused():
     p, ld = st._rows(qkv[:, 192:384], "k")
     assert ld == 576 and p == qkv.data_ptr() + 192 * 8
     assert st._rows(qkv[:, 192:384].unflatten(1, (3, 64)), "k")[1] == 576
+    assert st._rows(torch.from_numpy(np.zeros((0, 3, 64), np.int64)), "k")[1] == 192      # (strides of zero)
     for bad in (good.to(torch.int32), good.float(), good[:, :2], good.transpose(0, 1), good[..., ::2], good[:, :, :32],
                 torch.zeros(5, 3, 128, dtype=torch.int64)[..., ::2], good.view(15, 64), torch.zeros(1, 192, dtype=torch.int64).expand(5, 192),
                 np.zeros((5, 3, 64), np.int64)):
