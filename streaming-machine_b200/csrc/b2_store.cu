@@ -22,9 +22,9 @@ namespace b2 {
 // write: eight lanes hold a head's key or value (64 int64), lane i of them the pairs of dims i, i + 8, i + 16, i + 24, so
 // that a load of the eight is 128 bytes in a row and the first two pairs are the lower half's; U rows, all asked for before
 // the first is used. The shift is the bit length of the OR of the magnitudes less 3 (the OR has the largest one's bit
-// length). Bound by the memory's latency at U = 1 (a decode step); a prompt's by its bandwidth. One row a warp, two dims a
-// lane, took three times the instructions and was bound by them (40 against 28 us, 4.6 TB/s, for
-// 32 x 512 prompts of 12 heads).
+// length). U = 1 where streams give few rows (a decode step, bound by the memory's latency: 1.7 us for 64 rows of 12 heads in
+// a graph), 2 for prompts, bound by its bandwidth: 28 us for 12,600 rows (4.6 TB/s). A row a warp, two dims a lane, took three
+// times the instructions and was bound by them (40 us).
 // ---------------------------------------------------------------------------------------------------------------------
 constexpr int SW_WARPS = 8;
 
@@ -171,13 +171,19 @@ __global__ void __launch_bounds__(SW_WARPS * 32) k_store_read(Store4 st, StoreRo
 
 // ---------------------------------------------------------------------------------------------------------------------
 // the arrival of few rows a stream (a decode step), NW warps per (row, head): one where there are many (no barrier, four
-// units a CTA), else a CTA of 4 or 8, or a cluster of cs CTAs sharing the keys. The integer table softmax needs the largest score before any weight (a = ARR[start - score] does not factor),
-// so the keys are read once for the scores, which stay in shared memory, and the values once after it:
+// units a CTA), else a CTA of 4, 8 or 16, or a cluster of cs CTAs sharing the keys (attend_few has the rule). The integer
+// table softmax needs the largest score before any weight (a = ARR[start - score] does not factor), so the keys are read
+// once for the scores, which stay in shared memory, and the values once after it:
 //   pass 1  32 keys a warp: their codes as the A rows of m16n8k32 (16 c: the digits stay in a byte's upper half, no sign
 //           to extend), the query's two bytes as B columns, so the two products of a key meet in one lane; scores into
 //           shared memory, the largest score and value shift by warp maxima
 //   pass 2  a = ARR[start - score], Z += a, the weight's three bytes into three planes of shared memory
 //   pass 3  num: the planes as the A rows, the values' codes as B (4 keys x 8 dims of nibbles turned by byte permutes)
+// PUT (store_step): the warp into whose block the row's own position falls holds its key and value first.
+// Bound by the chain of dependent steps where there are few units (3.4 us for 17 keys in a graph, 7.5 for 16 x 1,024), by
+// instruction issue where there are many (512 x 192: 23 us, 2.6 TB/s; about 240 instructions a warp and block of 32 keys,
+// 1.6 an SM and clock) and by both on long contexts (4 x 32,768: 32 us, 3.2 TB/s). Copies of the next blocks into L2 ahead
+// of their loads, and two blocks in flight a warp below 16 warps, gave nothing or cost occupancy.
 // ---------------------------------------------------------------------------------------------------------------------
 constexpr int SF_BYTES = 8;      // shared memory a key: 4 score, 3 planes, 1 value shift
 
@@ -272,7 +278,8 @@ B2_DEV void put_row(const Store4& st, size_t e, bool key, int64_t x0, int64_t x1
     x0 = store_clamp(x0);
     x1 = store_clamp(x1);
     const uint32_t t = (uint32_t)bitlen_u(mag(x0) | mag(x1));
-    const int lo = (int)__reduce_max_sync(0xffffffffu, lane < 16 ? t : 0u), hi = (int)__reduce_max_sync(0xffffffffu, lane < 16 ? 0u : t);
+    const int lo = (int)__reduce_max_sync(0xffffffffu, lane < 16 ? t : 0u);
+    const int hi = (int)__reduce_max_sync(0xffffffffu, lane < 16 ? 0u : t);
     const int big = min(max(max(lo, hi) - 3, 0), STORE_MAX_SHIFT);
     const int sh = key ? max(min(max((lane < 16 ? lo : hi) - 3, 0), STORE_MAX_SHIFT), big - 3) : big;
     const uint8_t c = (uint8_t)((store_code(x0, sh) & 15) | (store_code(x1, sh) << 4));
@@ -304,7 +311,8 @@ B2_DEV void unit_sync() {
 }
 
 template <int NW, bool PUT>
-__global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, NW == 1 ? 7 : (NW == 4 ? 6 : (NW == 8 ? 3 : 1))) k_store_attend_few(StoreAttend a, int chunk, int cs, int wide) {
+__global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, NW == 1 ? 7 : (NW == 4 ? 6 : (NW == 8 ? 3 : 1)))
+    k_store_attend_few(StoreAttend a, int chunk, int cs, int wide) {
     extern __shared__ __align__(16) uint8_t sm[];
     constexpr int UN = NW == 1 ? 4 : 1;                              // (row, head) units a CTA
     constexpr int PF = NW == 16 ? 2 : 1;                             // blocks of 32 keys that a warp has on their way
@@ -397,8 +405,9 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, NW == 1 ? 7 : (NW == 
         int d[2][2][4];                                              // [16 keys][half]
 #pragma unroll
         for (int m = 0; m < 2; m++) {
-            mma_s8_first(d[m][0], even16(c.w[2 * m].x), even16(c.w[2 * m + 1].x), odd16(c.w[2 * m].x), odd16(c.w[2 * m + 1].x), q0[0], q1[0]);
-            mma_s8_first(d[m][1], even16(c.w[2 * m].y), even16(c.w[2 * m + 1].y), odd16(c.w[2 * m].y), odd16(c.w[2 * m + 1].y), q0[1], q1[1]);
+            const uint2 wa = c.w[2 * m], wb = c.w[2 * m + 1];
+            mma_s8_first(d[m][0], even16(wa.x), even16(wb.x), odd16(wa.x), odd16(wb.x), q0[0], q1[0]);
+            mma_s8_first(d[m][1], even16(wa.y), even16(wb.y), odd16(wa.y), odd16(wb.y), q0[1], q1[1]);
         }
         int dot[2];
 #pragma unroll
@@ -525,7 +534,7 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, NW == 1 ? 7 : (NW == 
                 int t = 0;
 #pragma unroll
                 for (int w = 0; w < NW; w++) t += s_acc[un][w][b][ut + 32 * x];
-                num[x] += (int64_t)t << (8 * b);
+                num[x] += (int64_t)t * (1 << 8 * b);
             }
         }
     }
@@ -570,7 +579,7 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, NW == 1 ? 7 : (NW == 
 
 // ---------------------------------------------------------------------------------------------------------------------
 // the arrival of many rows a stream (a prompt pass): a CTA of 8 warps takes 64 consecutive rows of one head, a pair of warps
-// 16 of them; where that gives too few CTAs, a cluster of CS shares the rows' keys. Tiles of 64 keys (and values) are copied
+// 16 of them; where that gives too few CTAs, a cluster of cs shares the rows' keys. Tiles of 64 keys (and values) are copied
 // into shared memory two ahead (cp.async), then unpacked once for all the rows as signed bytes in the order of the tensor
 // cores' B operands (c 2^(s - S + 3) for keys, 16 c for values); a warp forms the scores of one of a tile's two blocks of 32.
 //   pass 1  every score (m16n8k32, the query's two bytes one after the other), the rows' largest and largest value shift
@@ -580,6 +589,11 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, NW == 1 ? 7 : (NW == 
 //           swap those through shared memory and each adds w c for half of the 64 dims: 48 registers of sums a lane in
 //           place of 96, which lets 16 warps share an SM
 // CTAs are persistent so that the table is copied twice an SM, the longest rows first.
+// Bound by the integer work of a (row, key) pair, about 21 operations over both passes (the score's two byte planes, its
+// shift, the table's index, the weight's rounding and bytes), and by the latency of an item's start and end: 228 us for
+// 32 prompts of 300 to 512 (84 of them the items' queries, sums and outputs, 43 pass 1), 182 us for 2 x 256 rows on 8,000
+// positions. IPC 1.7; the tensor cores' share of the time is a sixth. Of 128 rows on 16 warps a CTA it took 246 us (one CTA
+// an SM: nothing runs while it waits), with the sums of all 64 dims in one warp (8 warps an SM) 288.
 // ---------------------------------------------------------------------------------------------------------------------
 constexpr int SM_WARPS = 8, SM_THREADS = SM_WARPS * 32, SM_ROWS = 64, SM_KEYS = 64;
 struct SmRaw {
@@ -705,7 +719,8 @@ __global__ void __launch_bounds__(SM_THREADS, 2) k_store_attend_many(StoreAttend
             for (int k = 0; k < SM_ROWS / SM_WARPS; k++) {
                 const int r = wid + k * SM_WARPS;
                 x[k][0] = x[k][1] = 0;
-                if (r < nr) load_pair(a.q.x + (size_t)(run.r0 + i0 + r) * a.q.ld + h * a.q.hs + 2 * lane, wide & 1, x[k][0], x[k][1]);
+                const int64_t* const from_ = a.q.x + (size_t)(run.r0 + i0 + r) * a.q.ld + h * a.q.hs + 2 * lane;
+                if (r < nr) load_pair(from_, wide & 1, x[k][0], x[k][1]);
             }
             uint32_t words[SM_ROWS / SM_WARPS];
             int us[SM_ROWS / SM_WARPS], most = 0;
@@ -727,8 +742,9 @@ __global__ void __launch_bounds__(SM_THREADS, 2) k_store_attend_many(StoreAttend
 #pragma unroll
             for (int y = 0; y < 2; y++) {
                 const uint32_t* w = &S.q[y ? rb : ra][16 * x + 4 * j];
-                const uint32_t h0 = __byte_perm(w[0], w[1], 0x6240), h1 = __byte_perm(w[2], w[3], 0x6240);   // hi: even, even, odd, odd
-                const uint32_t l0 = __byte_perm(w[0], w[1], 0x7351), l1 = __byte_perm(w[2], w[3], 0x7351);   // lo
+                // hi bytes of two words: even, even, odd, odd; lo bytes the same
+                const uint32_t h0 = __byte_perm(w[0], w[1], 0x6240), h1 = __byte_perm(w[2], w[3], 0x6240);
+                const uint32_t l0 = __byte_perm(w[0], w[1], 0x7351), l1 = __byte_perm(w[2], w[3], 0x7351);
                 q[0][x][y] = __byte_perm(h0, h1, 0x5410);
                 q[0][x][2 + y] = __byte_perm(h0, h1, 0x7632);
                 q[1][x][y] = __byte_perm(l0, l1, 0x5410);
@@ -753,7 +769,8 @@ __global__ void __launch_bounds__(SM_THREADS, 2) k_store_attend_many(StoreAttend
                 const int s0 = (int8_t)both, s1 = both >> 8, big = max(s0, s1);
                 const int up0 = s0 - big + 3, up1 = s1 - big + 3;
                 const uint32_t less0 = 0x80808080u - (0x08080808u << up0), less1 = 0x80808080u - (0x08080808u << up1);
-                T.k[wid][lane] = make_uint4(even_up(w.x, up0, less0), odd_up(w.x, up0, less0), even_up(w.y, up1, less1), odd_up(w.y, up1, less1));
+                T.k[wid][lane] = make_uint4(even_up(w.x, up0, less0), odd_up(w.x, up0, less0), even_up(w.y, up1, less1),
+                                            odd_up(w.y, up1, less1));
                 if (j == 0) {
                     T.kr[kl] = 27 - big;
                     if (27 - big < umax && k0 + t * KEYS + kl < k1) S.slow = 1;
@@ -882,7 +899,8 @@ __global__ void __launch_bounds__(SM_THREADS, 2) k_store_attend_many(StoreAttend
         // the next item's queries into L2 (a row is four lines)
         if (n_t < tiles && n_r0 >= 0 && n_r1 <= a.rw.rows) {
             const int row = n_r0 + (tiles - 1 - n_t) * ROWS + (tid >> 2);
-            if (row < n_r1) asm volatile("prefetch.global.L2 [%0];" ::"l"(a.q.x + (size_t)row * a.q.ld + n_h * a.q.hs + (tid & 3) * 16));
+            const int64_t* const line = a.q.x + (size_t)row * a.q.ld + n_h * a.q.hs + (tid & 3) * 16;
+            if (row < n_r1) asm volatile("prefetch.global.L2 [%0];" ::"l"(line));
         }
         // twice the largest score: a digit below the last rounds up with it
         const uint32_t sa = (uint32_t)(((ya >> 1) + (ya & 1)) * 2), sb = (uint32_t)(((yb >> 1) + (yb & 1)) * 2);
@@ -1109,11 +1127,15 @@ cudaError_t store_read(const Store4& st, const StoreRows& rw, int layer, int64_t
     return store_launch(how, k_store_read<SW_ROWS>, row_grid(st, rw, SW_ROWS), SW_WARPS * 32, 0, 1, st, rw, layer, k, v, wide, err);
 }
 
-constexpr int SM_FROM_ROWS = 20;     // rows a stream up to which the few-row kernel is quicker (between 12 and 48, by the context)
+// rows a stream up to which the few-row kernel is quicker: it overtakes between 12 (16 streams on 8,000 positions) and 48 (on
+// 100); at 12 and 48 rows of 4 streams on 2,000 it takes 21 and 64 us, the many-row kernel 38 and 40
+constexpr int SM_FROM_ROWS = 20;
 constexpr int SM_FIXED = 4, SM_SPLIT = 6;
 constexpr int SM_SMEM_MOST = 200 * 1024;
 constexpr int SF_MOST_KEYS = 8192;   // of a CTA: 64 KB of shared memory
-constexpr int SF_WARP_UNITS = 12, SF_WARP_BLOCKS = 32;   // a warp a unit: from so many units an SM on, up to 1,024 keys (32 KB a CTA)
+// a warp a unit: from so many units an SM on (100 x 900, 8 an SM: 45 us against 28; 200 x 160, 16 an SM: 10.8 against 14.8),
+// up to 1,024 keys (32 KB a CTA)
+constexpr int SF_WARP_UNITS = 12, SF_WARP_BLOCKS = 32;
 constexpr int SF_LONG = 32, SF_VERY_LONG = 64;   // blocks of 32 keys
 
 size_t many_smem(int alen) { return sizeof(SmShared) + (size_t)(alen + 1) * 4; }
@@ -1121,13 +1143,13 @@ size_t many_smem(int alen) { return sizeof(SmShared) + (size_t)(alen + 1) * 4; }
 namespace {
 cudaError_t make_plan(int device, int alen, StorePlan& plan) {
     cudaError_t e = cudaDeviceGetAttribute(&plan.sms, cudaDevAttrMultiProcessorCount, device);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(k_store_attend_few<4, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, SF_MOST_KEYS * SF_BYTES);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(k_store_attend_few<4, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, SF_MOST_KEYS * SF_BYTES);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(k_store_attend_few<8, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, SF_MOST_KEYS * SF_BYTES);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(k_store_attend_few<8, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, SF_MOST_KEYS * SF_BYTES);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(k_store_attend_few<16, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, SF_MOST_KEYS * SF_BYTES);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(k_store_attend_few<16, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, SF_MOST_KEYS * SF_BYTES);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(k_store_attend_many, cudaFuncAttributeMaxDynamicSharedMemorySize, SM_SMEM_MOST);
+    void (*const few[])(StoreAttend, int, int, int) = {k_store_attend_few<4, false>, k_store_attend_few<4, true>,
+                                                       k_store_attend_few<8, false>, k_store_attend_few<8, true>,
+                                                       k_store_attend_few<16, false>, k_store_attend_few<16, true>};
+    for (auto f : few)
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, SF_MOST_KEYS * SF_BYTES);
+    if (e == cudaSuccess)
+        e = cudaFuncSetAttribute(k_store_attend_many, cudaFuncAttributeMaxDynamicSharedMemorySize, SM_SMEM_MOST);
     if (e != cudaSuccess) return e;
     int fit = 0;
     e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, k_store_attend_many, SM_THREADS, many_smem(alen));
@@ -1182,7 +1204,8 @@ cudaError_t attend_few(const StoreAttend& a, StoreLaunch how, int wide) {
     const int64_t units = (int64_t)a.rw.n_streams * a.rw.max_rows * a.st.H;
     if (units >= (int64_t)SF_WARP_UNITS * how.plan->sms && blocks <= SF_WARP_BLOCKS) {
         const dim3 grid((unsigned)(((int64_t)a.rw.max_rows * a.st.H + 3) / 4), a.rw.n_streams);
-        return store_launch(how, k_store_attend_few<1, PUT>, grid, 128, (size_t)blocks * 32 * SF_BYTES * 4, 1, a, blocks * 32, 1, wide);
+        const int chunk = blocks * 32;
+        return store_launch(how, k_store_attend_few<1, PUT>, grid, 128, (size_t)chunk * SF_BYTES * 4, 1, a, chunk, 1, wide);
     }
     // a cluster costs about 1.3 us (its barriers), a warp's block of 32 keys 0.5 (from L2) to 1.2 us (from HBM): the keys are
     // split where that leaves half the SMs idle, and while there is a long run of keys for every CTA of two an SM
@@ -1377,6 +1400,11 @@ int check_rows(b2_store* h, const char* what, int32_t layer, const int32_t* cu, 
     return B2_OK;
 }
 
+// a bound past the context says no more than the context
+StoreRows call_rows(const b2_store* h, const int32_t* cu, const int32_t* pos, int32_t n_streams, int32_t rows, int32_t max_rows) {
+    return StoreRows{cu, pos, n_streams, rows, std::min(max_rows, h->cfg.max_ctx)};
+}
+
 // nothing that is thrown (memory for a message, a table) passes the C boundary
 template <class F>
 int guarded(b2_store* h, F f) {
@@ -1433,7 +1461,7 @@ int b2_store_write(b2_store* h, int32_t layer, const int64_t* k, int64_t ldk, co
                          (long long)ldk, (const void*)v, (long long)ldv, (long long)d);
         OnDevice on(h->device);
         SCK(on.e);
-        SCK(store_write(h->st, StoreRows{cu, pos, n_streams, rows, std::min(max_rows, h->cfg.max_ctx)}, layer, StoreVec{k, ldk, 64}, StoreVec{v, ldv, 64}, h->d_err,
+        SCK(store_write(h->st, call_rows(h, cu, pos, n_streams, rows, max_rows), layer, StoreVec{k, ldk, 64}, StoreVec{v, ldv, 64}, h->d_err,
                         StoreLaunch{(cudaStream_t)stream, true, &h->plan}));
         return (int)B2_OK;
     });
@@ -1448,7 +1476,7 @@ int b2_store_read(b2_store* h, int32_t layer, const int32_t* cu, const int32_t* 
         if (rows && !k && !v) return sfail(h, B2_ERR_ARG, "b2_store_read: neither k nor v asked for");
         OnDevice on(h->device);
         SCK(on.e);
-        SCK(store_read(h->st, StoreRows{cu, pos, n_streams, rows, std::min(max_rows, h->cfg.max_ctx)}, layer, k, v, h->d_err,
+        SCK(store_read(h->st, call_rows(h, cu, pos, n_streams, rows, max_rows), layer, k, v, h->d_err,
                        StoreLaunch{(cudaStream_t)stream, true, &h->plan}));
         return (int)B2_OK;
     });
@@ -1466,7 +1494,7 @@ int b2_store_attend(b2_store* h, int32_t layer, const int64_t* q, int64_t ldq, c
                          (const void*)out, window);
         OnDevice on(h->device);
         SCK(on.e);
-        StoreAttend a{h->st, StoreRows{cu, pos, n_streams, rows, std::min(max_rows, h->cfg.max_ctx)}, layer, StoreVec{q, ldq, 64}, first, window, h->ARR, h->alen,
+        StoreAttend a{h->st, call_rows(h, cu, pos, n_streams, rows, max_rows), layer, StoreVec{q, ldq, 64}, first, window, h->ARR, h->alen,
                       h->LOG2, h->EXP2, out, nullptr, h->d_err};
         SCK(store_attend(a, StoreLaunch{(cudaStream_t)stream, true, &h->plan}));
         return (int)B2_OK;
