@@ -22,6 +22,12 @@ import numpy as np
 from .engine import B2Error, StoreConfig, _torch, lib
 
 HEAD = 64
+INT32_MIN, INT32_MAX = -2 ** 31, 2 ** 31 - 1
+
+
+def _i32(x: int) -> int:
+    """A number as the C ABI's int32 takes it: one outside stands for the nearest (ctypes would drop its upper bits)."""
+    return x if INT32_MIN <= x <= INT32_MAX else (INT32_MIN if x < 0 else INT32_MAX)
 
 
 class Store:
@@ -36,7 +42,7 @@ class Store:
         if t[1].size != 65536 or t[2].size != 65536:
             raise ValueError("the log2 and exp2 tables have 65,536 entries")
         h = ctypes.c_void_p()
-        cfg = StoreConfig(n_streams, n_layer, n_head, max_ctx)
+        cfg = StoreConfig(*(_i32(x) for x in (n_streams, n_layer, n_head, max_ctx)))
         size = lib().b2_store_size(ctypes.byref(cfg), t[0].size)
         # torch's allocator gives the memory (and keeps it between stores)
         self._memory = self.torch.empty(max(size, 0), dtype=self.torch.uint8, device=self.device)
@@ -96,7 +102,7 @@ class Store:
         if cu is not None:
             if max_rows is None:
                 raise ValueError("max_rows (the most rows a stream gives) goes with cu")
-            return self._ints(cu, "cu", n + 1), p, n, rows, max_rows
+            return self._ints(cu, "cu", n + 1), p, _i32(n), rows, _i32(max_rows)
         if rows != n or max_rows not in (None, 1):
             raise ValueError(f"without cu every stream gives one row: {rows} rows, {n} positions, max_rows {max_rows}")
         return None, p, n, rows, 1
@@ -127,7 +133,7 @@ class Store:
         if rows != v.shape[0]:
             raise ValueError(f"{rows} rows of keys, {v.shape[0]} of values")
         cu, pos, n, rows, most = self._table(pos, cu, rows, max_rows)
-        rc = self._f_write(h, layer, pk, ldk, pv, ldv, cu, pos, n, rows, most, self._stream(self._index))
+        rc = self._f_write(h, _i32(layer), pk, ldk, pv, ldv, cu, pos, n, rows, most, self._stream(self._index))
         if rc:
             self._done(rc)
 
@@ -145,7 +151,7 @@ class Store:
         else:
             k, v = self._out(out[0], rows, "out k"), self._out(out[1], rows, "out v")
         cu, pos, n, rows, most = self._table(pos, cu, rows, max_rows)
-        rc = self._f_read(h, layer, cu, pos, n, rows, most, k.data_ptr(), v.data_ptr(), self._stream(self._index))
+        rc = self._f_read(h, _i32(layer), cu, pos, n, rows, most, k.data_ptr(), v.data_ptr(), self._stream(self._index))
         if rc:
             self._done(rc)
         return k, v
@@ -165,7 +171,7 @@ class Store:
             out = q.new_empty((rows, *self._row))
         cu, pos, n, rows, most = self._table(pos, cu, rows, max_rows)
         f = None if first is None else self._ints(first, "first", n)
-        rc = self._f_attend(h, layer, pq, ldq, cu, pos, f, n, rows, most, window, out.data_ptr(), self._stream(self._index))
+        rc = self._f_attend(h, _i32(layer), pq, ldq, cu, pos, f, n, rows, most, _i32(window), out.data_ptr(), self._stream(self._index))
         if rc:
             self._done(rc)
         return out
@@ -184,7 +190,7 @@ class Store:
             out = q.new_empty((n, *self._row))
         p = self._ints(pos, "pos", n)
         f = None if first is None else self._ints(first, "first", n)
-        rc = self._f_step(h, layer, pq, ldq, pk, ldk, pv, ldv, p, f, n, window, out.data_ptr(), self._stream(self._index))
+        rc = self._f_step(h, _i32(layer), pq, ldq, pk, ldk, pv, ldv, p, f, n, _i32(window), out.data_ptr(), self._stream(self._index))
         if rc:
             self._done(rc)
         return out

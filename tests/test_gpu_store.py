@@ -1,5 +1,7 @@
 """The 4-bit key/value store on the GPU against the formulas in plain Python (store_reference.py), bit for bit: every
 result is a whole number, so the tolerance is zero."""
+import os
+
 import numpy as np
 import pytest
 
@@ -509,3 +511,67 @@ def test_step_refusals_and_flags(T):
     assert st.step(empty, empty, empty, i32([])).shape == (0, 1, 64)
     st.sync()
     st.close()
+
+
+FIRST_CALLS = """
+import sys, numpy as np, torch
+from streaming_machine_b200 import convert, store
+def i32(x): return torch.tensor(x, dtype=torch.int32, device="cuda")
+g = torch.Generator(device="cuda").manual_seed(1)
+def x(*s): return torch.randint(-2 ** 17, 2 ** 17, s, dtype=torch.int64, device="cuda", generator=g)
+st, other = (store.Store(convert.tables(), 3, 96, 2) for _ in range(2))
+cu, zero, pos, end = i32([0, 30, 60, 90]), i32([0, 0, 0]), i32([30, 30, 30]), i32([31, 31, 31])
+k, v, q = x(90, 2, 64), x(90, 2, 64), x(90, 2, 64)
+src = [x(3, 2, 64) for _ in range(3)]
+q1, k1, v1 = (torch.zeros_like(s) for s in src)
+out = torch.full((3, 2, 64), -7, dtype=torch.int64, device="cuda")
+pinned = torch.zeros(90, 2, 64, dtype=torch.int64).pin_memory()
+side = torch.cuda.Stream()
+torch.cuda.synchronize()
+def work(st, capture):
+    for a, b in zip((q1, k1, v1), src):
+        a.copy_(b)                                           # a copy on the device before
+    st.write(k, v, zero, cu=cu, max_rows=30)
+    fork = torch.cuda.Event()
+    fork.record()
+    with torch.cuda.stream(side):                            # two readers at once
+        side.wait_event(fork)
+        many = st.attend(q, zero, cu=cu, max_rows=30)
+        join = torch.cuda.Event()
+        join.record()
+    few = st.attend(q1, i32_29)
+    torch.cuda.current_stream().wait_event(join)
+    step = st.step(q1, k1, v1, pos)                          # behind both
+    out.zero_()                                              # a fill between two calls
+    st.attend(q1, pos, out=out)
+    held = st.read(zero, cu=cu, max_rows=30, rows=90)
+    pinned.copy_(held[0], non_blocking=True)                 # a copy to the host behind
+    return many, few, step, held
+i32_29 = i32([29, 29, 29])
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):                                # the process's first calls
+    got = work(st, True)
+for _ in range(2):
+    graph.replay()
+torch.cuda.synchronize()
+host, o = pinned.clone(), out.clone()
+want = work(other, False)
+torch.cuda.synchronize()
+flat = lambda r: (r[0], r[1], r[2], *r[3])
+assert all(torch.equal(a, b) for a, b in zip(flat(got), flat(want)))
+assert torch.equal(host, want[3][0].cpu()) and torch.equal(o, out) and torch.equal(out, want[2])
+assert not torch.equal(want[1], want[2]) and int(want[2].abs().max()) > 0
+st.sync()
+other.sync()
+print("same")
+"""
+
+
+def test_first_calls_captured_and_forked():
+    """A process's first calls inside a capture, on two streams that part and meet, with copies and fills between them:
+    replayed, the plain calls' results."""
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", FIRST_CALLS], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "same" in r.stdout, r.stdout + r.stderr

@@ -61,6 +61,31 @@ def test_rows_are_refused():
             st._rows(bad, "k")
 
 
+def test_numbers_past_32_bits_stay_large():
+    """layer, window, max_rows beyond an int32: what reaches the library is as far out, not the number's lower bits."""
+    st = _bare()
+    st.h, calls = object(), []
+
+    def call(*a):
+        calls.append(a)
+        return 0
+    st._f_write = st._f_read = st._f_attend = st._f_step = call
+    x = torch.zeros(4, 3, 64, dtype=torch.int64)
+    pos, cu = torch.zeros(4, dtype=torch.int32), torch.arange(5, dtype=torch.int32)
+    big = 2 ** 32
+    st.write(x, x, pos, cu=cu, max_rows=big + 1, layer=big)
+    assert calls[-1][1] == calls[-1][-2] == 2 ** 31 - 1
+    st.read(pos, cu=cu, rows=4, max_rows=big + 1, layer=-big)
+    assert calls[-1][1] == -2 ** 31 and calls[-1][6] == 2 ** 31 - 1
+    st.attend(x, pos, window=big + 5, layer=big)
+    assert calls[-1][1] == calls[-1][-3] == 2 ** 31 - 1
+    st.step(x, x, x, pos, window=-big + 5, layer=big + 1)
+    assert calls[-1][1] == 2 ** 31 - 1 and calls[-1][-3] == -2 ** 31
+    st.attend(x, pos, window=5, layer=1)
+    assert calls[-1][1] == 1 and calls[-1][-3] == 5
+    st.h = None
+
+
 def test_tables_are_refused():
     st = _bare()
     pos = torch.zeros(4, dtype=torch.int32)
