@@ -191,7 +191,7 @@ int b2_check_wait(b2_handle* h, void* stream);
  * at r * ld + 64 h (ld in elements, at least 64 n_head). Work is queued on `stream`; nothing is allocated, copied to
  * the host or kept between calls, so calls may be captured into a graph, and calls that do not write what another one
  * reads or writes may run at once on several streams (the host's calls on one store come one after the other). out may be
- * q itself (not a step's k or v). A stream whose rows do not fit the call or whose positions pass the context is skipped and flagged:
+ * q itself, or a step's k or v. A stream whose rows do not fit the call or whose positions pass the context is skipped and flagged:
  * b2_store_sync reports it (B2_ERR_ARG, B2_ERR_CTX). */
 typedef struct b2_store b2_store;
 typedef struct {

@@ -349,6 +349,7 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, NW == 1 ? 7 : (NW == 
     };
     if (lo > p) {
         if (PUT && rank == 0 && wid == 0) put();
+        if (PUT) unit_sync<NW>();                                    // out may be k or v
         for (int t = ut; t < 64 && rank == 0; t += NW * 32) out[t] = 0;
         return;
     }

@@ -489,6 +489,28 @@ def test_step_is_write_and_attend(T, n, heads, ctx):
     b.close()
 
 
+@pytest.mark.parametrize("ctx", [100, 5000])
+def test_step_out_may_be_an_input(T, ctx):
+    """step() into its own q, k or v, rows that see nothing among them: the outputs and the store of a step into new memory."""
+    import torch
+    rng = np.random.default_rng(ctx)
+    pos, first = i32([ctx - 1, 40, 70]), i32([0, 41, 71])
+    hist = [dev(values(rng, 3 * (ctx - 1), 12, s)) for s in (1.0, 0.3)]
+    x = [dev(values(rng, 3, 12, s)) for s in (1.5, 1.0, 0.3)]
+    want = None
+    for into in (None, 0, 1, 2):
+        st, _ = make(T, 3, ctx, 12)
+        st.write(*hist, i32([0] * 3), cu=i32(np.arange(4) * (ctx - 1)), max_rows=ctx - 1)
+        args = [t.clone() for t in x]
+        y = st.step(*args, pos, first=first, out=None if into is None else args[into])
+        held = st.read(i32([0] * 3), cu=i32(np.arange(4) * ctx), max_rows=ctx, rows=3 * ctx)
+        st.sync()
+        want = want or (y, *held)
+        assert all(torch.equal(a, b) for a, b in zip((y, *held), want)), into
+        assert int(y[0].abs().max()) > 0 and int(y[1:].abs().max()) == 0
+        st.close()
+
+
 def test_step_refusals_and_flags(T):
     import torch
     from streaming_machine_b200 import engine
