@@ -591,12 +591,13 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, NW == 1 ? 7 : (NW == 
 //           place of 96, which lets 16 warps share an SM
 // CTAs are persistent so that the table is copied twice an SM, the longest rows first.
 // Bound by the integer work of a (row, key) pair, about 21 operations over both passes (the score's two byte planes, its
-// shift, the table's index, the weight's rounding and bytes), and by the latency of an item's start and end: 228 us for
+// shift, the table's index, the weight's rounding and bytes), and by the latency of an item's start and end: 195 us for
 // 32 prompts of 300 to 512 (84 of them the items' queries, sums and outputs, 43 pass 1), 182 us for 2 x 256 rows on 8,000
 // positions. IPC 1.7; the tensor cores' share of the time is a sixth. Of 128 rows on 16 warps a CTA it took 246 us (one CTA
 // an SM: nothing runs while it waits), with the sums of all 64 dims in one warp (8 warps an SM) 288.
 // ---------------------------------------------------------------------------------------------------------------------
 constexpr int SM_WARPS = 8, SM_THREADS = SM_WARPS * 32, SM_ROWS = 64, SM_KEYS = 64;
+constexpr int SM_STREAMS = 1024;         // up to so many streams the items are listed
 struct SmRaw {
     uint8_t k[SM_KEYS][32], v[SM_KEYS][32];
     int8_t ks[SM_KEYS][2], vs[SM_KEYS];
@@ -617,6 +618,7 @@ struct SmShared {
     int64_t z[SM_WARPS][16];             // a warp's rows: their sums of entries,
     int2 ym[SM_WARPS][16];               // largest score (twice) and value shift
     int32_t u[SM_ROWS], most[SM_WARPS], slow;
+    uint16_t rows[SM_STREAMS];           // how many items of rows each stream has (of a head)
 };
 
 // bytes c 2^up of the word's even and odd codes; up = 0 .. 3: c + 8 moves up, 8 2^up comes off again (less: 128 - 8 2^up)
@@ -643,39 +645,82 @@ __global__ void __launch_bounds__(SM_THREADS, 2) k_store_attend_many(StoreAttend
     const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, g = lane >> 2, j = lane & 3;
     const int pair = wid >> 1, blk = wid & 1, rank = cs > 1 ? (int)cluster_rank() : 0;   // blk: the warp's block of a tile
     const int H = a.st.H, alen = a.alen;
-    for (int i = tid; i < alen; i += SM_THREADS) TAB[i] = __ldg(a.ARR + i);
-    if (tid == 0) TAB[alen] = 0;
+    for (int i = tid; i < alen / 4; i += SM_THREADS) copy16(TAB + 4 * i, a.ARR + 4 * i);
+    for (int i = alen / 4 * 4 + tid; i <= alen; i += SM_THREADS) TAB[i] = i < alen ? __ldg(a.ARR + i) : 0;
     griddep_wait();                       // (the table never changes: its copy need not wait)
     stamp_begin(a.stamp);
     griddep_launch();
-    // items: streams run fastest, then heads, then the tiles of rows from the last on; below 2^31 (the launch sees to it).
-    // One cluster's next item is `step` further, taken apart once
-    const int n_str = a.rw.n_streams, step = gridDim.x / cs;
-    const int d_s = step % n_str, d_h = step / n_str % H, d_t = step / n_str / H;
-    int s = blockIdx.x / cs % n_str, h = blockIdx.x / cs / n_str % H, t_ = blockIdx.x / cs / n_str / H;
+    // The items: the streams' last tiles of 64 rows before those ahead of them (a stream's first is tile 0), then by heads, then
+    // by streams; below 2^31 (the launch sees to it). Cluster me of W takes one of every W, there and back (me, 2 W - 1 - me,
+    // 2 W + me, ..), so that the loads come out even: 32 prompts of 300 to 512 rows 195 us, 200 one way, 227 where the
+    // streams that lack a tile keep their places; 4 of 512 rows 38, 51, 49. Past SM_STREAMS streams they do
+    const int n_str = a.rw.n_streams, me = blockIdx.x / cs, W = gridDim.x / cs;
+    const bool listed = n_str <= SM_STREAMS;
+    int w_tile = tiles - 1, w_of = n_str;                     // the walk: at items of tile w_tile, w_of streams have one,
+    uint32_t w_from = 0, round = 0;                           // the first is item w_from
+    if (listed) {
+        for (int s = tid; s < n_str; s += SM_THREADS) {
+            StoreRun run;
+            S.rows[s] = (uint16_t)(store_run(a.rw, s, a.st.lim, run, a.err) ? (run.n + ROWS - 1) / ROWS : 0);
+        }
+        __syncthreads();
+    }
+    auto streams_with = [&](int tile) {                       // every warp counts for itself
+        int c = 0;
+        for (int s = lane; s - lane < n_str; s += 32) c += __popc(__ballot_sync(0xffffffffu, s < n_str && S.rows[s] > tile));
+        return c;
+    };
+    if (listed) {
+        int most = 0;
+        for (int s = lane; s < n_str; s += 32) most = max(most, (int)S.rows[s]);
+        w_tile = __reduce_max_sync(0xffffffffu, most) - 1;
+        w_of = streams_with(w_tile);
+    }
+    // the next item: its tile (-1: there is none), head and stream
+    auto next = [&](int& tile, int& h, int& s) {
+        const uint32_t k = round * W + ((round & 1) ? W - 1 - me : me);
+        round++;
+        while (w_tile >= 0 && k >= w_from + (uint32_t)(w_of * H)) {
+            w_from += w_of * H;
+            w_tile--;
+            if (listed && w_tile >= 0) w_of = streams_with(w_tile);
+        }
+        tile = w_tile;
+        if (w_tile < 0) return;
+        h = (k - w_from) / w_of;
+        s = (k - w_from) - h * w_of;
+        if (listed && w_of < n_str) {                         // the s-th of those that have this tile
+            int left = s;
+            for (int at = 0;; at += 32) {
+                const uint32_t has = __ballot_sync(0xffffffffu, at + lane < n_str && S.rows[at + lane] > w_tile);
+                if (left < __popc(has)) {
+                    const bool it = (has >> lane & 1) && __popc(has & ((1u << lane) - 1)) == left;
+                    s = at + __ffs(__ballot_sync(0xffffffffu, it)) - 1;
+                    break;
+                }
+                left -= __popc(has);
+            }
+        }
+    };
     // an item's entries of the row table, read one item ahead
     int n_r0 = 0, n_r1 = 0, n_pos = 0, n_first = 0;
-    auto ahead = [&](int s, int t) {
-        if (t < tiles) {
+    auto ahead = [&](int s, int tile) {
+        if (tile >= 0) {
             n_r0 = a.rw.cu ? a.rw.cu[s] : s;
             n_r1 = a.rw.cu ? a.rw.cu[s + 1] : s + 1;
             n_pos = a.rw.pos[s];
             n_first = a.first ? a.first[s] : 0;
         }
     };
-    ahead(s, t_);
-    int n_s, n_h, n_t;
-    for (; t_ < tiles; s = n_s, h = n_h, t_ = n_t) {
-        n_s = s + d_s;
-        n_h = h + d_h;
-        n_t = t_ + d_t;
-        if (n_s >= n_str) { n_s -= n_str; n_h++; }
-        if (n_h >= H) { n_h -= H; n_t++; }
-        const int tile = tiles - 1 - t_;
+    int tile, h, s, n_tile, n_h, n_s;
+    next(tile, h, s);
+    ahead(s, tile);
+    for (; tile >= 0; tile = n_tile, h = n_h, s = n_s) {
+        next(n_tile, n_h, n_s);
         StoreRun run;
         const bool some = store_run(a.rw, n_r0, n_r1, n_pos, a.st.lim, run, a.err);
         const int from = max(0, n_first);
-        ahead(n_s, n_t);
+        ahead(n_s, n_tile);
         if (!some || tile * ROWS >= run.n) continue;
         const int i0 = tile * ROWS, nr = min(ROWS, run.n - i0);
         const int win = a.window > 0 ? a.window : 0x40000000;
@@ -898,8 +943,8 @@ __global__ void __launch_bounds__(SM_THREADS, 2) k_store_attend_many(StoreAttend
                 mb = max(mb, ob.y);
             }
         // the next item's queries into L2 (a row is four lines)
-        if (n_t < tiles && n_r0 >= 0 && n_r1 <= a.rw.rows) {
-            const int row = n_r0 + (tiles - 1 - n_t) * ROWS + (tid >> 2);
+        if (n_tile >= 0 && n_r0 >= 0 && n_r1 <= a.rw.rows) {
+            const int row = n_r0 + n_tile * ROWS + (tid >> 2);
             const int64_t* const line = a.q.x + (size_t)row * a.q.ld + n_h * a.q.hs + (tid & 3) * 16;
             if (row < n_r1) asm volatile("prefetch.global.L2 [%0];" ::"l"(line));
         }
