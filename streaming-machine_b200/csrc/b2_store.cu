@@ -185,7 +185,19 @@ __global__ void __launch_bounds__(SW_WARPS * 32) k_store_read(Store4 st, StoreRo
 // 1.6 an SM and clock) and by both on long contexts (4 x 32,768: 32 us, 3.2 TB/s). Copies of the next blocks into L2 ahead
 // of their loads, and two blocks in flight a warp below 16 warps, gave nothing or cost occupancy.
 // ---------------------------------------------------------------------------------------------------------------------
-constexpr int SF_BYTES = 8;      // shared memory a key: 4 score, 3 planes, 1 value shift
+constexpr int SF_BYTES = 5;      // shared memory a key: 4 its score, later 3 of them its weight's planes; 1 its value's shift
+// a warp's ring of blocks of 32 keys (or values) on their way
+struct SfBlock {
+    uint8_t codes[32][32];
+    int8_t ks[32][2], vs[32];
+};
+constexpr int SF_RING = 4;
+B2_DEV void copy16(void* to, const void* from) {      // 16 bytes, asynchronously, past L1
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(saddr(to)), "l"(from) : "memory");
+}
+B2_DEV void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+B2_DEV void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 B2_DEV void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -310,21 +322,21 @@ B2_DEV void unit_sync() {
     else __syncthreads();
 }
 
-template <int NW, bool PUT>
+template <int NW, bool PUT, bool RING>
 __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, NW == 1 ? 7 : (NW == 4 ? 6 : (NW == 8 ? 3 : 1)))
     k_store_attend_few(StoreAttend a, int chunk, int cs, int wide) {
     extern __shared__ __align__(16) uint8_t sm[];
     constexpr int UN = NW == 1 ? 4 : 1;                              // (row, head) units a CTA
-    constexpr int PF = NW == 16 ? 2 : 1;                             // blocks of 32 keys that a warp has on their way
+    constexpr int D = SF_RING, PF = NW == 16 ? 2 : 1;                // blocks of 32 keys that a warp has on their way (PF: in registers)
     __shared__ int32_t s_max[NW], s_shift[NW], s_acc[UN][NW][3][64];
     __shared__ int64_t s_z[NW], s_num[65];
     __shared__ int2 s_own;                                           // cs > 1: this CTA's largest score and shift
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, wid = NW == 1 ? 0 : warp, un = NW == 1 ? warp : 0;
     const int g = lane >> 2, j = lane & 3, ut = NW == 1 ? lane : threadIdx.x;      // ut: the thread of the unit
-    uint8_t* const mem = sm + (size_t)un * chunk * SF_BYTES;
-    int32_t* const SC = reinterpret_cast<int32_t*>(mem);             // [chunk]
-    uint8_t* const WP = mem + (size_t)chunk * 4;                     // [3][chunk]
-    int8_t* const VS = reinterpret_cast<int8_t*>(mem + (size_t)chunk * 7);   // [chunk]
+    SfBlock* const ring = reinterpret_cast<SfBlock*>(sm) + warp * D;
+    uint8_t* const mem = sm + (RING ? (NW == 1 ? 4 : NW) * D * sizeof(SfBlock) : 0) + (size_t)un * chunk * SF_BYTES;
+    int32_t* const SC = reinterpret_cast<int32_t*>(mem);             // [chunk]; then of four keys each the three planes' words
+    int8_t* const VS = reinterpret_cast<int8_t*>(mem + (size_t)chunk * 4);   // [chunk]
     griddep_wait();
     stamp_begin(a.stamp);
     griddep_launch();
@@ -361,29 +373,58 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, NW == 1 ? 7 : (NW == 
     const int b0 = first_block + rank * per, nb = max(0, min(per, blocks - rank * per));
     const size_t base = kv_index(a.rw.slot0 + s, a.layer, h, 0, a.st.L, H, a.st.ctx) + (size_t)b0 * 32;
     const int from = lo - b0 * 32, to = p - b0 * 32;                 // visible: from <= local key <= to
-    const int mine = 16 * (j >> 1) + 8 * (j & 1) + g;                // of a block's keys the one whose score this lane finishes
+    // of a block's keys the one whose score this lane finishes, and its place: a block's scores, shifts and planes are kept in
+    // the order of the values' operands, key 4m + x at 8x + m
+    const int mine = 16 * (j >> 1) + 8 * (j & 1) + g, place = 8 * (mine & 3) + (mine >> 2);
 
+    // a block on its way: the i-th of this warp's, b0 + wid + i NW; the warp's lanes wait for their own copies, then meet
+    auto fetch = [&](int i, bool values) {
+        const int b = wid + i * NW;
+        if (b < nb) {
+            SfBlock& r = ring[i % D];
+            const size_t e = base + (size_t)b * 32;
+            const uint8_t* const from_ = (values ? a.st.v : a.st.k) + e * 32 + lane * 16;
+            copy16(&r.codes[0][0] + lane * 16, from_);
+            copy16(&r.codes[0][0] + 512 + lane * 16, from_ + 512);
+            if (!values) {
+                if (lane < 4) copy16(&r.ks[0][0] + lane * 16, a.st.ks + e * 2 + lane * 16);
+                else if (lane < 6) copy16(r.vs + (lane - 4) * 16, a.st.vs + e + (lane - 4) * 16);
+            }
+        }
+        copies_end();
+    };
+    auto arrived = [&](int i, bool values) {                         // block i is here; the one D - 1 behind it sets out
+        copies_wait<D - 2>();
+        __syncwarp();
+        fetch(i + D - 1, values);
+    };
     // a block's keys: rows 8t + g, words j of both halves; this lane's key's shifts and its value's
     struct Keys { uint2 w[4]; int ks, vs; };
-    auto keys = [&](int b, Keys& k) {
-        const size_t e = base + (size_t)b * 32;
-        const uint2* const from_ = reinterpret_cast<const uint2*>(a.st.k + (e + g) * 32 + 8 * j);
+    auto keys = [&](const uint8_t* codes, const int8_t* ks, const int8_t* vs, Keys& k) {
 #pragma unroll
-        for (int t = 0; t < 4; t++) k.w[t] = from_[t * 32];
-        k.ks = *reinterpret_cast<const int16_t*>(a.st.ks + (e + mine) * 2);
-        k.vs = a.st.vs[e + mine];
+        for (int t = 0; t < 4; t++) k.w[t] = *reinterpret_cast<const uint2*>(codes + (8 * t + g) * 32 + 8 * j);
+        k.ks = *reinterpret_cast<const int16_t*>(ks + 2 * mine);
+        k.vs = vs[mine];
     };
-    // a block's values: word g (dims 8g .. 8g + 7) of keys 8j .. 8j + 7
-    auto values = [&](int b, uint32_t (&w)[8]) {
-        const uint32_t* const from_ = reinterpret_cast<const uint32_t*>(a.st.v + (base + (size_t)b * 32 + 8 * j) * 32 + 4 * g);
+    auto keys_at = [&](int b, Keys& k) {
+        const size_t e = base + (size_t)b * 32;
+        keys(a.st.k + e * 32, a.st.ks + e * 2, a.st.vs + e, k);
+    };
+    // a block's values: word g (dims 8g .. 8g + 7) of keys j, j + 4, ..
+    auto values = [&](const uint8_t* codes, uint32_t (&w)[8]) {
 #pragma unroll
-        for (int t = 0; t < 8; t++) w[t] = from_[t * 8];
+        for (int t = 0; t < 8; t++) w[t] = *reinterpret_cast<const uint32_t*>(codes + (4 * t + j) * 32 + 4 * g);
     };
     if (PUT && nb > 0 && b0 + nb - 1 == p >> 5 && (nb - 1) % NW == wid) put();
     Keys k[PF];
+    if (RING) {
 #pragma unroll
-    for (int f = 0; f < PF; f++)
-        if (wid + f * NW < nb) keys(wid + f * NW, k[f]);
+        for (int i = 0; i < D - 1; i++) fetch(i, false);
+    } else {
+#pragma unroll
+        for (int f = 0; f < PF; f++)
+            if (wid + f * NW < nb) keys_at(wid + f * NW, k[f]);
+    }
     if (PUT && a.COS) turn_row(x[0][0], x[0][1], lane, p, a.COS, a.SIN, a.err);
     uint32_t words[1], q0[2], q1[2];                                 // q0, q1: B operands of the two halves
     int us[1];
@@ -419,28 +460,41 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, NW == 1 ? 7 : (NW == 
         }
         const int s0 = (int8_t)c.ks, s1 = c.ks >> 8, S = max(s0, s1), key = b * 32 + mine;
         const int32_t sc = score16((dot[0] << (s0 - S + 3)) + (dot[1] << (s1 - S + 3)), 32 - u - S);
-        SC[key] = sc;
-        VS[key] = (int8_t)c.vs;
+        SC[b * 32 + place] = sc;
+        VS[b * 32 + place] = (int8_t)c.vs;
         if (key >= from && key <= to) {
             start = max(start, sc);
             M = max(M, c.vs);
         }
     };
-    for (int b = wid; b < nb; b += NW * PF) {
-        Keys c[PF];
+    uint32_t v[PF][8];
+    if (RING) {
+        for (int i = 0, b = wid; b < nb; i++, b += NW) {
+            arrived(i, false);
+            const SfBlock& r = ring[i % D];
+            Keys c;
+            keys(&r.codes[0][0], &r.ks[0][0], r.vs, c);
+            score_block(b, c);
+        }
+        __syncwarp();                                                // the ring is free
 #pragma unroll
-        for (int f = 0; f < PF; f++) c[f] = k[f];
+        for (int i = 0; i < D - 1; i++) fetch(i, true);              // on their way over the reductions
+    } else {
+        for (int b = wid; b < nb; b += NW * PF) {
+            Keys c[PF];
 #pragma unroll
-        for (int f = 0; f < PF; f++)                                 // the next blocks', while these are worked on
-            if (b + (PF + f) * NW < nb) keys(b + (PF + f) * NW, k[f]);
+            for (int f = 0; f < PF; f++) c[f] = k[f];
+#pragma unroll
+            for (int f = 0; f < PF; f++)                             // the next blocks', while these are worked on
+                if (b + (PF + f) * NW < nb) keys_at(b + (PF + f) * NW, k[f]);
+#pragma unroll
+            for (int f = 0; f < PF; f++)
+                if (b + f * NW < nb) score_block(b + f * NW, c[f]);
+        }
 #pragma unroll
         for (int f = 0; f < PF; f++)
-            if (b + f * NW < nb) score_block(b + f * NW, c[f]);
+            if (wid + f * NW < nb) values(a.st.v + (base + (size_t)(wid + f * NW) * 32) * 32, v[f]);
     }
-    uint32_t v[PF][8];
-#pragma unroll
-    for (int f = 0; f < PF; f++)
-        if (wid + f * NW < nb) values(wid + f * NW, v[f]);           // on their way over the reductions
     start = __reduce_max_sync(0xffffffffu, start);
     M = __reduce_max_sync(0xffffffffu, M);
     if (NW > 1) {
@@ -468,13 +522,14 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, NW == 1 ? 7 : (NW == 
     for (int t = ut * 4; t < nb * 32; t += NW * 128) {
         const int4 sc = *reinterpret_cast<const int4*>(SC + t);
         const uint32_t v4 = *reinterpret_cast<const uint32_t*>(VS + t);
-        const int scs[4] = {sc.x, sc.y, sc.z, sc.w};
+        const int scs[4] = {sc.x, sc.y, sc.z, sc.w}, key0 = (t & ~31) + 4 * (t & 7) + ((t >> 3) & 3);
         uint32_t w[4];
         int32_t four = 0;                                            // four entries of at most 2^24
 #pragma unroll
         for (int x = 0; x < 4; x++) {
             const int d = start - scs[x];
-            const bool seen = t + x >= from && t + x <= to && d < a.alen;
+            const int key = key0 + 4 * x;
+            const bool seen = key >= from && key <= to && d < a.alen;
             const int av = seen ? __ldg(a.ARR + d) : 0;
             four += av;
             w[x] = (shr_u32(av, M - (int)(int8_t)(v4 >> (8 * x))) + 1) >> 1;
@@ -482,36 +537,47 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, NW == 1 ? 7 : (NW == 
         z += four;
         uint32_t r[3];
         turn3(w, r[0], r[1], r[2]);
-#pragma unroll
-        for (int b = 0; b < 3; b++) *reinterpret_cast<uint32_t*>(WP + (size_t)b * chunk + t) = r[b];
+        *reinterpret_cast<uint4*>(SC + t) = make_uint4(r[0], r[1], r[2], 0);
     }
     z = warp_sum64(z);
     if (NW > 1 && lane == 0) s_z[wid] = z;
     unit_sync<NW>();
     // ---- values
     int acc[8][4] = {};
-    for (int b = wid; b < nb; b += NW * PF) {
-        uint32_t w[PF][8];
+    auto add_block = [&](int b, const uint32_t (&w)[8]) {
+        uint32_t p0 = 0, p1 = 0, r0[4], r1[4];
+        if (g < 3) {
+            p0 = (uint32_t)SC[b * 32 + 8 * j + g];
+            p1 = (uint32_t)SC[b * 32 + 8 * j + 4 + g];
+        }
+        turn4(w, r0);
+        turn4(w + 4, r1);
 #pragma unroll
-        for (int f = 0; f < PF; f++)
+        for (int t = 0; t < 4; t++) {
+            mma_u8s8(acc[2 * t], p0, 0, p1, 0, even16(r0[t]), even16(r1[t]));
+            mma_u8s8(acc[2 * t + 1], p0, 0, p1, 0, odd16(r0[t]), odd16(r1[t]));
+        }
+    };
+    if (RING) {
+        for (int i = 0, b = wid; b < nb; i++, b += NW) {
+            arrived(i, true);
+            uint32_t w[8];
+            values(&ring[i % D].codes[0][0], w);
+            add_block(b, w);
+        }
+    } else {
+        for (int b = wid; b < nb; b += NW * PF) {
+            uint32_t w[PF][8];
 #pragma unroll
-            for (int t = 0; t < 8; t++) w[f][t] = v[f][t];
+            for (int f = 0; f < PF; f++)
 #pragma unroll
-        for (int f = 0; f < PF; f++)
-            if (b + (PF + f) * NW < nb) values(b + (PF + f) * NW, v[f]);
+                for (int t = 0; t < 8; t++) w[f][t] = v[f][t];
 #pragma unroll
-        for (int f = 0; f < PF; f++) {
-            if (b + f * NW >= nb) break;
-            uint2 p8 = make_uint2(0, 0);
-            if (g < 3) p8 = *reinterpret_cast<const uint2*>(WP + (size_t)g * chunk + (b + f * NW) * 32 + 8 * j);
-            uint32_t r0[4], r1[4];
-            turn4(w[f], r0);
-            turn4(w[f] + 4, r1);
+            for (int f = 0; f < PF; f++)
+                if (b + (PF + f) * NW < nb) values(a.st.v + (base + (size_t)(b + (PF + f) * NW) * 32) * 32, v[f]);
 #pragma unroll
-            for (int t = 0; t < 4; t++) {
-                mma_u8s8(acc[2 * t], p8.x, 0, p8.y, 0, even16(r0[t]), even16(r1[t]));
-                mma_u8s8(acc[2 * t + 1], p8.x, 0, p8.y, 0, odd16(r0[t]), odd16(r1[t]));
-            }
+            for (int f = 0; f < PF; f++)
+                if (b + f * NW < nb) add_block(b + f * NW, w[f]);
         }
     }
     // row g of the tiles is plane g; columns 2j, 2j + 1 of tile t are dims 16j + t and 16j + 8 + t
@@ -632,9 +698,6 @@ B2_DEV uint32_t odd_up(uint32_t w, int up, uint32_t less) {
 B2_DEV uint32_t seen(int from, int to) {
     if (from > 31 || to < 0 || from > to) return 0u;
     return (0xFFFFFFFFu << max(from, 0)) & (0xFFFFFFFFu >> (31 - min(to, 31)));
-}
-B2_DEV void copy16(void* to, const void* from) {      // 16 bytes, asynchronously, past L1
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(saddr(to)), "l"(from) : "memory");
 }
 
 __global__ void __launch_bounds__(SM_THREADS, 2) k_store_attend_many(StoreAttend a, int tiles, int cs, int wide) {
@@ -1182,18 +1245,24 @@ constexpr int SF_MOST_KEYS = 8192;   // of a CTA: 64 KB of shared memory
 // a warp a unit: from so many units an SM on (100 x 900, 8 an SM: 45 us against 28; 200 x 160, 16 an SM: 10.8 against 14.8),
 // up to 1,024 keys (32 KB a CTA)
 constexpr int SF_WARP_UNITS = 12, SF_WARP_BLOCKS = 32;
+// blocks of 32 keys a warp from which they come through the ring, three on their way: 100 x 900 (8 blocks) 26.6 us straight into
+// registers, 22.8 through the ring, 512 x 192 (6) 22.3 and 21.1, 4 x 32,768 (16) 30.8 and 29.3; but 200 x 160 (5) 10.1 and 11.0,
+// 16 x 1,024 (4) 7.1 and 8.1: a copy into shared memory and the load from it come later than a load
+constexpr int SF_RING_FROM = 6;
 constexpr int SF_LONG = 32, SF_VERY_LONG = 64;   // blocks of 32 keys
 
+size_t few_smem(int warps, int keys, bool ring) { return (ring ? warps * SF_RING * sizeof(SfBlock) : 0) + (size_t)keys * SF_BYTES; }
 size_t many_smem(int alen) { return sizeof(SmShared) + (size_t)(alen + 1) * 4; }
 
 namespace {
 cudaError_t make_plan(int device, int alen, StorePlan& plan) {
     cudaError_t e = cudaDeviceGetAttribute(&plan.sms, cudaDevAttrMultiProcessorCount, device);
-    void (*const few[])(StoreAttend, int, int, int) = {k_store_attend_few<4, false>, k_store_attend_few<4, true>,
-                                                       k_store_attend_few<8, false>, k_store_attend_few<8, true>,
-                                                       k_store_attend_few<16, false>, k_store_attend_few<16, true>};
+    void (*const few[])(StoreAttend, int, int, int) = {k_store_attend_few<1, false, false>, k_store_attend_few<1, false, true>, k_store_attend_few<1, true, false>, k_store_attend_few<1, true, true>,
+        k_store_attend_few<4, false, false>, k_store_attend_few<4, false, true>, k_store_attend_few<4, true, false>, k_store_attend_few<4, true, true>,
+        k_store_attend_few<8, false, false>, k_store_attend_few<8, false, true>, k_store_attend_few<8, true, false>, k_store_attend_few<8, true, true>,
+        k_store_attend_few<16, false, false>, k_store_attend_few<16, false, true>, k_store_attend_few<16, true, false>, k_store_attend_few<16, true, true>};
     for (auto f : few)
-        if (e == cudaSuccess) e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, SF_MOST_KEYS * SF_BYTES);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)few_smem(16, SF_MOST_KEYS, true));
     if (e == cudaSuccess)
         e = cudaFuncSetAttribute(k_store_attend_many, cudaFuncAttributeMaxDynamicSharedMemorySize, SM_SMEM_MOST);
     if (e != cudaSuccess) return e;
@@ -1242,6 +1311,15 @@ cudaError_t store_init(int alen, StorePlan& plan) {
 }
 
 namespace {
+// NW warps a (row, head) (a CTA of four for one warp), `each` blocks of 32 keys a CTA at most
+template <int NW, bool PUT>
+cudaError_t few_launch(const StoreAttend& a, StoreLaunch how, int wide, dim3 grid, int each, int cs) {
+    const int chunk = each * 32, warps = NW == 1 ? 4 : NW;
+    const bool ring = each >= NW * SF_RING_FROM;
+    return store_launch(how, ring ? k_store_attend_few<NW, PUT, true> : k_store_attend_few<NW, PUT, false>, grid, warps * 32,
+                        few_smem(warps, NW == 1 ? chunk * 4 : chunk, ring), cs, a, chunk, cs, wide);
+}
+
 template <bool PUT>
 cudaError_t attend_few(const StoreAttend& a, StoreLaunch how, int wide) {
     // blocks of 32 positions that a row may see
@@ -1249,9 +1327,7 @@ cudaError_t attend_few(const StoreAttend& a, StoreLaunch how, int wide) {
     if (a.window > 0 && a.window < a.st.lim) blocks = std::min(blocks, (a.window + 30) / 32 + 1);
     const int64_t units = (int64_t)a.rw.n_streams * a.rw.max_rows * a.st.H;
     if (units >= (int64_t)SF_WARP_UNITS * how.plan->sms && blocks <= SF_WARP_BLOCKS) {
-        const dim3 grid((unsigned)(((int64_t)a.rw.max_rows * a.st.H + 3) / 4), a.rw.n_streams);
-        const int chunk = blocks * 32;
-        return store_launch(how, k_store_attend_few<1, PUT>, grid, 128, (size_t)chunk * SF_BYTES * 4, 1, a, chunk, 1, wide);
+        return few_launch<1, PUT>(a, how, wide, dim3((unsigned)(((int64_t)a.rw.max_rows * a.st.H + 3) / 4), a.rw.n_streams), blocks, 1);
     }
     // a cluster costs about 1.3 us (its barriers), a warp's block of 32 keys 0.5 (from L2) to 1.2 us (from HBM): the keys are
     // split where that leaves half the SMs idle, and while there is a long run of keys for every CTA of two an SM
@@ -1260,13 +1336,11 @@ cudaError_t attend_few(const StoreAttend& a, StoreLaunch how, int wide) {
                                       (units * cs < how.plan->sms * 2 && blocks >= cs * SF_VERY_LONG) ||
                                       blocks * 32 > cs * SF_MOST_KEYS))
         cs *= 2;
-    const int each = (blocks + cs - 1) / cs, chunk = each * 32;
+    const int each = (blocks + cs - 1) / cs;
     const dim3 grid((unsigned)((int64_t)a.rw.max_rows * a.st.H * cs), a.rw.n_streams);
-    const size_t smem = (size_t)chunk * SF_BYTES;
-    if (each >= SF_VERY_LONG && units * cs <= how.plan->sms)       // 16 warps: one CTA an SM
-        return store_launch(how, k_store_attend_few<16, PUT>, grid, 512, smem, cs, a, chunk, cs, wide);
-    if (each >= SF_LONG) return store_launch(how, k_store_attend_few<8, PUT>, grid, 256, smem, cs, a, chunk, cs, wide);
-    return store_launch(how, k_store_attend_few<4, PUT>, grid, 128, smem, cs, a, chunk, cs, wide);
+    if (each >= SF_VERY_LONG && units * cs <= how.plan->sms) return few_launch<16, PUT>(a, how, wide, grid, each, cs);   // one CTA an SM
+    if (each >= SF_LONG) return few_launch<8, PUT>(a, how, wide, grid, each, cs);
+    return few_launch<4, PUT>(a, how, wide, grid, each, cs);
 }
 int wide_bits(const StoreAttend& a) {
     return pairs(a.q) | aligned16(a.out) << 1 | pairs(a.k) << 2 | pairs(a.v) << 3;

@@ -333,7 +333,8 @@ def run_long(T, rng, heads, held, rows, window=0, first=None, max_rows=None):
 @pytest.mark.parametrize("heads,held,rows", [
     (1, [2100, 40], [1, 1]), (12, [1030] * 5 + [3] * 11, [1] * 16), (1, [20000], [1]), (12, [60, 99, 7] * 50, [1] * 150),
     (2, [40000, 33000, 5], [1, 2, 1]), (5, [4100], [20]),
-    (2, [700, 3], [40, 64]), (1, [3000], [130]), (3, [6000, 50], [64, 1]), (12, [0] * 8, [200, 130, 64, 65, 127, 128, 1, 30])])
+    (12, [199, 60] * 75, [1] * 150), (1, [900, 77] * 50, [1] * 100), (2, [1630, 9] * 25, [1] * 50), (6, [13000] * 3 + [40] * 5, [1] * 8),
+    (1, [60001], [1]), (2, [700, 3], [40, 64]), (1, [3000], [130]), (3, [6000, 50], [64, 1]), (12, [0] * 8, [200, 130, 64, 65, 127, 128, 1, 30])])
 def test_long_and_many(T, heads, held, rows):
     """Every shape of launch: a warp, 4, 8 and 16 warps a row and head, keys split over clusters of 2 to 8 CTAs, for few
     rows and for many; streams much shorter than the longest beside it."""
@@ -456,7 +457,8 @@ def test_the_library_allocates(T):
     assert np.array_equal(out.cpu().numpy(), pl.attend(q.cpu().numpy(), [0, 0]))
 
 
-@pytest.mark.parametrize("n,heads,ctx", [(1, 12, 100), (3, 2, 33), (64, 12, 160), (150, 12, 70), (2, 1, 5000), (16, 12, 1040), (1, 1, 30000)])
+@pytest.mark.parametrize("n,heads,ctx", [(1, 12, 100), (3, 2, 33), (64, 12, 160), (150, 12, 70), (2, 1, 5000), (16, 12, 1040), (1, 1, 30000),
+                                         (150, 12, 190), (100, 1, 930), (50, 2, 1650), (1, 1, 60000)])
 def test_step_is_write_and_attend(T, n, heads, ctx):
     """step() on one store, write() and attend() on another, token by token at every place in a block of 32 positions, with
     windows and dropped beginnings (that leave a row nothing): the same outputs and the same store."""
