@@ -1236,20 +1236,25 @@ cudaError_t store_read(const Store4& st, const StoreRows& rw, int layer, int64_t
     return store_launch(how, k_store_read<SW_ROWS>, row_grid(st, rw, SW_ROWS), SW_WARPS * 32, 0, 1, st, rw, layer, k, v, wide, err);
 }
 
-// rows a stream up to which the few-row kernel is quicker: it overtakes between 12 (16 streams on 8,000 positions) and 48 (on
-// 100); at 12 and 48 rows of 4 streams on 2,000 it takes 21 and 64 us, the many-row kernel 38 and 40
-constexpr int SM_FROM_ROWS = 20;
+// the few-row kernel is quicker up to so many rows a stream (4 streams on 2,000 positions: 12 rows 21 us, the many-row kernel 38;
+// 32 rows 50 and 40), and of more rows while there is little to do in all: (row, head)s times their blocks of 32 keys and a
+// start of SF_START more, an SM (one prompt of 64 rows 8.8 and 14.3 us, of 256 13.5 and 20.6, 2 x 48 rows on 700 19 and 27; past
+// it 8 x 32 rows on 500 32.6 and 29.7, 16 prompts of 64 19.2 and 16.4)
+constexpr int SM_FROM_ROWS = 20, SF_START = 3, SF_LITTLE = 340;
 constexpr int SM_FIXED = 4, SM_SPLIT = 6;
 constexpr int SM_SMEM_MOST = 200 * 1024;
-constexpr int SF_MOST_KEYS = 8192;   // of a CTA: 64 KB of shared memory
-// a warp a unit: from so many units an SM on (100 x 900, 8 an SM: 45 us against 28; 200 x 160, 16 an SM: 10.8 against 14.8),
-// up to 1,024 keys (32 KB a CTA)
+constexpr int SF_MOST_KEYS = 8192;   // of a CTA: 40 KB of shared memory
+// a warp a unit where units are many and short: from SF_WARP_UNITS an SM on up to 1,024 keys (20 KB a CTA; 200 x 160, 16 an SM:
+// 10.1 us against 13.6), below that where their blocks of 32 keys are at most twice the units an SM less five (64 x 160, 5 an SM
+// of 5 blocks: 5.8 against 6.1, 64 x 256 7.7 against 6.9; 140 x 256, 11 an SM of 8: 9.5 against 13.3, 100 x 900 30 against 23)
 constexpr int SF_WARP_UNITS = 12, SF_WARP_BLOCKS = 32;
 // blocks of 32 keys a warp from which they come through the ring, three on their way: 100 x 900 (8 blocks) 26.6 us straight into
 // registers, 22.8 through the ring, 512 x 192 (6) 22.3 and 21.1, 4 x 32,768 (16) 30.8 and 29.3; but 200 x 160 (5) 10.1 and 11.0,
 // 16 x 1,024 (4) 7.1 and 8.1: a copy into shared memory and the load from it come later than a load
 constexpr int SF_RING_FROM = 6;
-constexpr int SF_LONG = 32, SF_VERY_LONG = 64;   // blocks of 32 keys
+// blocks of 32 keys a CTA from which it has 8 warps: 32 where there are few CTAs (16 x 1,024, 192 of them: 7.1 us against 8.2
+// with four; 20 x 1,024, 240: 8.9 against 8.2), else 48, where the ring begins (64 x 1,024 20.7 against 16.4 with four)
+constexpr int SF_LONG = 32, SF_LONG_MANY = SF_RING_FROM * 8, SF_VERY_LONG = 64;
 
 size_t few_smem(int warps, int keys, bool ring) { return (ring ? warps * SF_RING * sizeof(SfBlock) : 0) + (size_t)keys * SF_BYTES; }
 size_t many_smem(int alen) { return sizeof(SmShared) + (size_t)(alen + 1) * 4; }
@@ -1320,26 +1325,30 @@ cudaError_t few_launch(const StoreAttend& a, StoreLaunch how, int wide, dim3 gri
                         few_smem(warps, NW == 1 ? chunk * 4 : chunk, ring), cs, a, chunk, cs, wide);
 }
 
+// blocks of 32 positions that a row may see
+int few_blocks(const StoreAttend& a) {
+    const int blocks = (a.st.lim + 31) / 32;
+    return a.window > 0 && a.window < a.st.lim ? std::min(blocks, (a.window + 30) / 32 + 1) : blocks;
+}
+
 template <bool PUT>
 cudaError_t attend_few(const StoreAttend& a, StoreLaunch how, int wide) {
-    // blocks of 32 positions that a row may see
-    int blocks = (a.st.lim + 31) / 32;
-    if (a.window > 0 && a.window < a.st.lim) blocks = std::min(blocks, (a.window + 30) / 32 + 1);
+    const int blocks = few_blocks(a);
     const int64_t units = (int64_t)a.rw.n_streams * a.rw.max_rows * a.st.H;
-    if (units >= (int64_t)SF_WARP_UNITS * how.plan->sms && blocks <= SF_WARP_BLOCKS) {
+    const int sms = how.plan->sms;
+    if (blocks <= SF_WARP_BLOCKS && (units >= (int64_t)SF_WARP_UNITS * sms || (int64_t)(blocks + 5) * sms <= 2 * units))
         return few_launch<1, PUT>(a, how, wide, dim3((unsigned)(((int64_t)a.rw.max_rows * a.st.H + 3) / 4), a.rw.n_streams), blocks, 1);
-    }
     // a cluster costs about 1.3 us (its barriers), a warp's block of 32 keys 0.5 (from L2) to 1.2 us (from HBM): the keys are
     // split where that leaves half the SMs idle, and while there is a long run of keys for every CTA of two an SM
     int cs = 1;
-    while (cs < STORE_MAX_CLUSTER && ((units * cs * 2 <= how.plan->sms && blocks >= SF_LONG && blocks >= cs * 8) ||
-                                      (units * cs < how.plan->sms * 2 && blocks >= cs * SF_VERY_LONG) ||
+    while (cs < STORE_MAX_CLUSTER && ((units * cs * 2 <= sms && blocks >= SF_LONG && blocks >= cs * 8) ||
+                                      (units * cs < sms * 2 && blocks >= cs * SF_VERY_LONG) ||
                                       blocks * 32 > cs * SF_MOST_KEYS))
         cs *= 2;
     const int each = (blocks + cs - 1) / cs;
     const dim3 grid((unsigned)((int64_t)a.rw.max_rows * a.st.H * cs), a.rw.n_streams);
-    if (each >= SF_VERY_LONG && units * cs <= how.plan->sms) return few_launch<16, PUT>(a, how, wide, grid, each, cs);   // one CTA an SM
-    if (each >= SF_LONG) return few_launch<8, PUT>(a, how, wide, grid, each, cs);
+    if (each >= SF_VERY_LONG && units * cs <= sms) return few_launch<16, PUT>(a, how, wide, grid, each, cs);   // one CTA an SM
+    if (each >= SF_LONG_MANY || (each >= SF_LONG && units * cs * 2 < sms * 3)) return few_launch<8, PUT>(a, how, wide, grid, each, cs);
     return few_launch<4, PUT>(a, how, wide, grid, each, cs);
 }
 int wide_bits(const StoreAttend& a) {
@@ -1356,7 +1365,8 @@ cudaError_t store_attend(const StoreAttend& a, StoreLaunch how) {
     if (a.rw.n_streams == 0 || a.rw.rows == 0) return cudaSuccess;
     const int wide = wide_bits(a);
     const int64_t items = (int64_t)((a.rw.max_rows + SM_ROWS - 1) / SM_ROWS) * a.st.H * a.rw.n_streams;
-    if (a.rw.max_rows > SM_FROM_ROWS && items < INT32_MAX) {
+    const int64_t work = (int64_t)a.rw.n_streams * a.rw.max_rows * a.st.H * (few_blocks(a) + SF_START);
+    if (a.rw.max_rows > SM_FROM_ROWS && work > (int64_t)SF_LITTLE * how.plan->sms && items < INT32_MAX) {
         const int tiles = (a.rw.max_rows + SM_ROWS - 1) / SM_ROWS;
         const size_t smem = many_smem(a.alen);
         // fewer items than half of what the GPU holds: their keys split over clusters, in two tiles a CTA at least, by the

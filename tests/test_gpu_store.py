@@ -39,10 +39,15 @@ def i32(a):
     return dev(a, np.int32)
 
 
+ROOM = 16384       # a context, and a bound on a stream's rows, that lead to the kernel for many rows however few there are
+
+
 def run(T, rng, heads, held, rows, window=0, first=None, size=1.5, layers=1, layer=0):
-    """Streams that hold held[i] positions take rows[i] more: written, read back and attended, all against the reference."""
+    """Streams that hold held[i] positions take rows[i] more: written, read back and attended, all against the reference, in a
+    store and by a bound that just suffice and by ROOM."""
     n = len(held)
     st, pl = make(T, n, max(h + r for h, r in zip(held, rows)), heads, layers)
+    room = make(T, n, ROOM, heads, layers)[0]
     try:
         for lens, pos in ((held, [0] * n), (rows, held)):
             if not sum(lens):
@@ -50,17 +55,23 @@ def run(T, rng, heads, held, rows, window=0, first=None, size=1.5, layers=1, lay
             cu = np.concatenate([[0], np.cumsum(lens)])
             k, v = values(rng, sum(lens), heads, 1.0), values(rng, sum(lens), heads, 0.3)
             st.write(dev(k), dev(v), i32(pos), cu=i32(cu), max_rows=max(lens), layer=layer)
+            room.write(dev(k), dev(v), i32(pos), cu=i32(cu), max_rows=ROOM, layer=layer)
             pl.write(k, v, pos, cu, layer)
         q = values(rng, sum(rows), heads, size)
         got = st.attend(dev(q), i32(held), cu=i32(cu), max_rows=max(rows), window=window, layer=layer,
                         first=None if first is None else i32(first)).cpu().numpy()
+        many = room.attend(dev(q), i32(held), cu=i32(cu), max_rows=ROOM, window=window, layer=layer,
+                           first=None if first is None else i32(first)).cpu().numpy()
         back = [t.cpu().numpy() for t in st.read(i32(held), cu=i32(cu), max_rows=max(rows), rows=sum(rows), layer=layer)]
         st.sync()
         for b, w in zip(back, pl.read(held, cu, layer)):
             assert np.array_equal(b, w)
-        assert np.array_equal(got, pl.attend(q, held, cu, window, first, layer))
+        want = pl.attend(q, held, cu, window, first, layer)
+        assert np.array_equal(got, want) and np.array_equal(many, want)
+        room.sync()
     finally:
         st.close()
+        room.close()
 
 
 @pytest.mark.parametrize("held", [0, 1, 2, 7, 15, 16, 31, 32, 33, 63, 64, 127, 300])
@@ -100,11 +111,12 @@ def test_query_sizes(T, size):
     run(T, np.random.default_rng(5), 1, [40], [33], size=size)
 
 
-def test_extremes(T):
+@pytest.mark.parametrize("ctx", [24, ROOM])
+def test_extremes(T, ctx):
     """The largest magnitudes, +-2^63 and around 2^47 among them, and rows of zeros: nothing wraps."""
     rng = np.random.default_rng(6)
     big = np.array([-2 ** 63, 2 ** 63 - 1, -2 ** 47, 2 ** 47 - 1, 2 ** 47, -2 ** 47 - 1, 2 ** 46, 7, -8, 0, 1, 2 ** 31], dtype=np.int64)
-    st, pl = make(T, 3, 24, 2)
+    st, pl = make(T, 3, ctx, 2)
     n = 24
     pick = lambda rows, p: np.where(rng.random((rows, 2, 64)) < p, rng.choice(big, (rows, 2, 64)), rng.integers(-9, 9, (rows, 2, 64)))  # noqa: E731
     k, v = pick(3 * n, 0.1), pick(3 * n, 0.05)
@@ -116,7 +128,7 @@ def test_extremes(T):
         assert np.array_equal(b.cpu().numpy(), w)
     for p in (0.0, 0.02, 0.5, 1.0):
         q = pick(3 * n, p)
-        assert np.array_equal(st.attend(dev(q), i32(pos), cu=i32(cu), max_rows=n).cpu().numpy(), pl.attend(q, pos, cu))
+        assert np.array_equal(st.attend(dev(q), i32(pos), cu=i32(cu), max_rows=ctx).cpu().numpy(), pl.attend(q, pos, cu))
         # single rows at the last position too
         q1, p1 = q[:3], [n - 1] * 3
         assert np.array_equal(st.attend(dev(q1), i32(p1)).cpu().numpy(), pl.attend(q1, p1))
@@ -154,26 +166,27 @@ def test_layers_and_slots_are_apart(T):
     st.close()
 
 
+@pytest.mark.parametrize("ctx,most", [(50, 6), (ROOM, ROOM)])
 @pytest.mark.parametrize("off", [0, 1])
-def test_strided_rows_and_rows_left_alone(T, off):
+def test_strided_rows_and_rows_left_alone(T, off, ctx, most):
     """Keys, values and queries as slices of a qkv row (also at an odd element), outputs with rows that no stream has: those
     stay as they were, in the call's outputs and in the store."""
     import torch
     rng = np.random.default_rng(9)
     H, d = 2, 128
-    st, pl = make(T, 3, 50, H)
+    st, pl = make(T, 3, ctx, H)
     cu, pos, rows = [0, 4, 4, 9], [2, 0, 0], 12
     qkv = torch.zeros(rows, 3 * d + 5 + off, dtype=torch.int64, device="cuda")
     x = values(rng, rows, 3 * H, 1.0).reshape(rows, 3 * d)
     qkv[:, off:off + 3 * d] = dev(x)
     part = [qkv[:, off + i * d:off + (i + 1) * d] for i in range(3)]
-    st.write(part[1], part[2], i32(pos), cu=i32(cu), max_rows=6)
+    st.write(part[1], part[2], i32(pos), cu=i32(cu), max_rows=most)
     host = [x[:, i * d:(i + 1) * d].reshape(rows, H, 64) for i in range(3)]
     pl.write(host[1], host[2], pos, cu)
     outs = [torch.full((rows, H, 64), -77, dtype=torch.int64, device="cuda") for _ in range(3)]
-    got = st.attend(part[0], i32(pos), cu=i32(cu), max_rows=6, out=outs[0])
+    got = st.attend(part[0], i32(pos), cu=i32(cu), max_rows=most, out=outs[0])
     assert got is outs[0]
-    st.read(i32(pos), cu=i32(cu), max_rows=6, rows=rows, out=outs[1:])
+    st.read(i32(pos), cu=i32(cu), max_rows=most, rows=rows, out=outs[1:])
     want = [pl.attend(host[0], pos, cu), *pl.read(pos, cu)]
     for o, w in zip(outs, want):
         o = o.cpu().numpy()
@@ -185,12 +198,13 @@ def test_strided_rows_and_rows_left_alone(T, off):
     st.close()
 
 
-def test_bad_rows_are_flagged_and_skipped(T):
+@pytest.mark.parametrize("ctx,most", [(16, 2), (ROOM, ROOM)])
+def test_bad_rows_are_flagged_and_skipped(T, ctx, most):
     """Each device check by itself: the stream concerned is left out, the others are done, and sync() reports it once."""
     import torch
     from streaming_machine_b200 import engine
     rng = np.random.default_rng(10)
-    st, pl = make(T, 3, 16, 1)
+    st, pl = make(T, 3, ctx, 1)
     k, v, q = (values(rng, 6, 1, 1.0) for _ in range(3))
     good = [0, 2, 4, 6]
     st.write(dev(k), dev(v), i32([0, 0, 0]), cu=i32(good), max_rows=2)
@@ -199,11 +213,11 @@ def test_bad_rows_are_flagged_and_skipped(T):
     k2, v2 = values(rng, 6, 1, 1.0), values(rng, 6, 1, 1.0)
     #       cu, pos, the code, the streams left out
     bad = [([0, 2, 1, 6], [0, 0, 0], 1, (1, 2)), ([0, 2, 4, 7], [0, 0, 0], 1, (2,)), ([-1, 2, 4, 6], [0, 0, 0], 1, (0,)),
-           ([0, 2, 4, 6], [15, 0, 0], 4, (0,)), ([0, 2, 4, 6], [0, -1, 0], 4, (1,)), ([0, 2, 4, 6], [0, 0, 2 ** 31 - 1], 4, (2,)),
+           ([0, 2, 4, 6], [ctx - 1, 0, 0], 4, (0,)), ([0, 2, 4, 6], [0, -1, 0], 4, (1,)), ([0, 2, 4, 6], [0, 0, 2 ** 31 - 1], 4, (2,)),
            ([0, 2, 4, 2 ** 31 - 1], [0, 0, 0], 1, (2,)), ([-2 ** 31, 2, 4, 6], [0, 0, 0], 1, (0,))]
-    for cu, pos, code, left in bad:
+    for cu, pos, code, left in bad if most == 2 else bad[1:]:      # (the first is told by the bound)
         out = torch.full((6, 1, 64), -5, dtype=torch.int64, device="cuda")
-        st.attend(dev(q), i32(pos), cu=i32(cu), max_rows=2, out=out)
+        st.attend(dev(q), i32(pos), cu=i32(cu), max_rows=most, out=out)
         with pytest.raises(engine.B2Error) as ex:
             st.sync()
         assert ex.value.code == code
@@ -216,7 +230,7 @@ def test_bad_rows_are_flagged_and_skipped(T):
         kk, vv = k.copy(), v.copy()
         for s in left:
             kk[2 * s:2 * s + 2], vv[2 * s:2 * s + 2] = k2[2 * s:2 * s + 2], v2[2 * s:2 * s + 2]
-        st.write(dev(kk), dev(vv), i32(pos), cu=i32(cu), max_rows=2)
+        st.write(dev(kk), dev(vv), i32(pos), cu=i32(cu), max_rows=most)
         with pytest.raises(engine.B2Error):
             st.sync()
         for b, w in zip(st.read(i32([0, 0, 0]), cu=i32(good), max_rows=2, rows=6), pl.read([0, 0, 0], good)):
@@ -334,14 +348,16 @@ def run_long(T, rng, heads, held, rows, window=0, first=None, max_rows=None):
     (1, [2100, 40], [1, 1]), (12, [1030] * 5 + [3] * 11, [1] * 16), (1, [20000], [1]), (12, [60, 99, 7] * 50, [1] * 150),
     (2, [40000, 33000, 5], [1, 2, 1]), (5, [4100], [20]),
     (12, [199, 60] * 75, [1] * 150), (1, [900, 77] * 50, [1] * 100), (2, [1630, 9] * 25, [1] * 50), (6, [13000] * 3 + [40] * 5, [1] * 8),
-    (1, [60001], [1]), (2, [700, 3], [40, 64]), (1, [3000], [130]), (3, [6000, 50], [64, 1]), (12, [0] * 8, [200, 130, 64, 65, 127, 128, 1, 30])])
+    (1, [60001], [1]), (2, [700, 3], [40, 64]), (1, [3000], [130]), (3, [6000, 50], [64, 1]), (12, [2000], [130]),
+    (2, [9000], [200]), (1, [30000], [64]), (5, [1500, 700], [100, 40]), (12, [4100, 9], [64, 50]),
+    (1, [3] * 1100, ([24, 1, 70] + [2] * 8) * 100), (12, [0] * 8, [200, 130, 64, 65, 127, 128, 1, 30])])
 def test_long_and_many(T, heads, held, rows):
     """Every shape of launch: a warp, 4, 8 and 16 warps a row and head, keys split over clusters of 2 to 8 CTAs, for few
     rows and for many; streams much shorter than the longest beside it."""
     run_long(T, np.random.default_rng(len(held) + heads), heads, held, rows)
 
 
-@pytest.mark.parametrize("rows", [[1, 1], [18, 3], [90, 22]])
+@pytest.mark.parametrize("rows", [[1, 1], [18, 3], [90, 22], [700, 22]])
 def test_long_windows(T, rows):
     run_long(T, np.random.default_rng(16), 2, [3000, 1500], rows, window=1111, first=[0, 1490])
 
