@@ -179,11 +179,14 @@ __global__ void __launch_bounds__(SW_WARPS * 32) k_store_read(Store4 st, StoreRo
 //           shared memory, the largest score and value shift by warp maxima
 //   pass 2  a = ARR[start - score], Z += a, the weight's three bytes into three planes of shared memory
 //   pass 3  num: the planes as the A rows, the values' codes as B (4 keys x 8 dims of nibbles turned by byte permutes)
-// PUT (store_step): the warp into whose block the row's own position falls holds its key and value first.
-// Bound by the chain of dependent steps where there are few units (3.4 us for 17 keys in a graph, 7.5 for 16 x 1,024), by
-// instruction issue where there are many (512 x 192: 23 us, 2.6 TB/s; about 240 instructions a warp and block of 32 keys,
-// 1.6 an SM and clock) and by both on long contexts (4 x 32,768: 32 us, 3.2 TB/s). Copies of the next blocks into L2 ahead
-// of their loads, and two blocks in flight a warp below 16 warps, gave nothing or cost occupancy.
+// PUT (store_step): the warp into whose block the row's own position falls holds its key and value first. RING: the codes come
+// by asynchronous copies into a ring in shared memory, three blocks ahead, in place of loads one block ahead (two at 16 warps).
+// What shared memory a CTA does not take the table's entries use as L1 (71 KB: with 8 bytes a key and the ring 4 x 32,768 took
+// 41 us), so the weights' planes lie where the scores were.
+// Bound by the chain of dependent steps where there are few units (3.1 us for 17 keys in a graph, 7.1 for 16 x 1,024), by
+// instruction issue where there are many (512 x 192: 21 us, 2.8 TB/s; about 240 instructions a warp and block of 32 keys) and by
+// both on long contexts (4 x 32,768: 29 us, 3.5 TB/s; 256 x 2,000: 92 us, 4.4 TB/s). Copies of the next blocks into L2 ahead
+// of their loads, and two blocks of registers ahead below 16 warps, gave nothing or cost occupancy.
 // ---------------------------------------------------------------------------------------------------------------------
 constexpr int SF_BYTES = 5;      // shared memory a key: 4 its score, later 3 of them its weight's planes; 1 its value's shift
 // a warp's ring of blocks of 32 keys (or values) on their way
@@ -656,11 +659,12 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, NW == 1 ? 7 : (NW == 
 //           swap those through shared memory and each adds w c for half of the 64 dims: 48 registers of sums a lane in
 //           place of 96, which lets 16 warps share an SM
 // CTAs are persistent so that the table is copied twice an SM, the longest rows first.
-// Bound by the integer work of a (row, key) pair, about 21 operations over both passes (the score's two byte planes, its
-// shift, the table's index, the weight's rounding and bytes), and by the latency of an item's start and end: 195 us for
-// 32 prompts of 300 to 512 (84 of them the items' queries, sums and outputs, 43 pass 1), 182 us for 2 x 256 rows on 8,000
-// positions. IPC 1.7; the tensor cores' share of the time is a sixth. Of 128 rows on 16 warps a CTA it took 246 us (one CTA
-// an SM: nothing runs while it waits), with the sums of all 64 dims in one warp (8 warps an SM) 288.
+// Bound by the latency of dependent integer steps (16 warps an SM; a tile of 64 x 64 pairs takes an SM 1.4 us, 6,200 warp
+// instructions at 2.3 a clock; fewer of them, the table's place in two steps less and the weights by a product in place of
+// shifts, gained nothing) and of an item's start and end (5 us for each of the 18 items that an SM takes): 194 us for 32 prompts of 300
+// to 512 rows, 183 us for 2 x 256 rows on 8,000 positions. The tensor cores' share of the time is a sixth. Slower: 128 rows on 16
+// warps a CTA (one CTA an SM: nothing runs while it waits), the sums of all 64 dims in one warp (8 warps an SM), two items a
+// CTA side by side that share a table (192 us and 5% more on long contexts), an item's queries and first tiles copied ahead.
 // ---------------------------------------------------------------------------------------------------------------------
 constexpr int SM_WARPS = 8, SM_THREADS = SM_WARPS * 32, SM_ROWS = 64, SM_KEYS = 64;
 constexpr int SM_STREAMS = 1024;         // up to so many streams the items are listed
@@ -1246,7 +1250,8 @@ constexpr int SM_SMEM_MOST = 200 * 1024;
 constexpr int SF_MOST_KEYS = 8192;   // of a CTA: 40 KB of shared memory
 // a warp a unit where units are many and short: from SF_WARP_UNITS an SM on up to 1,024 keys (20 KB a CTA; 200 x 160, 16 an SM:
 // 10.1 us against 13.6), below that where their blocks of 32 keys are at most twice the units an SM less five (64 x 160, 5 an SM
-// of 5 blocks: 5.8 against 6.1, 64 x 256 7.7 against 6.9; 140 x 256, 11 an SM of 8: 9.5 against 13.3, 100 x 900 30 against 23)
+// of 5 blocks: 5.8 against 6.1, 64 x 256 7.7 against 6.9; 140 x 256, 11 an SM of 8: 9.5 against 13.3, 100 x 900 30 against 23;
+// a step's one warp would put the row's own key and value first: 64 x 160 in the engine 0.605 ms a step against 0.581)
 constexpr int SF_WARP_UNITS = 12, SF_WARP_BLOCKS = 32;
 // blocks of 32 keys a warp from which they come through the ring, three on their way: 100 x 900 (8 blocks) 26.6 us straight into
 // registers, 22.8 through the ring, 512 x 192 (6) 22.3 and 21.1, 4 x 32,768 (16) 30.8 and 29.3; but 200 x 160 (5) 10.1 and 11.0,
@@ -1336,7 +1341,7 @@ cudaError_t attend_few(const StoreAttend& a, StoreLaunch how, int wide) {
     const int blocks = few_blocks(a);
     const int64_t units = (int64_t)a.rw.n_streams * a.rw.max_rows * a.st.H;
     const int sms = how.plan->sms;
-    if (blocks <= SF_WARP_BLOCKS && (units >= (int64_t)SF_WARP_UNITS * sms || (int64_t)(blocks + 5) * sms <= 2 * units))
+    if (blocks <= SF_WARP_BLOCKS && (units >= (int64_t)SF_WARP_UNITS * sms || (!PUT && (int64_t)(blocks + 5) * sms <= 2 * units)))
         return few_launch<1, PUT>(a, how, wide, dim3((unsigned)(((int64_t)a.rw.max_rows * a.st.H + 3) / 4), a.rw.n_streams), blocks, 1);
     // a cluster costs about 1.3 us (its barriers), a warp's block of 32 keys 0.5 (from L2) to 1.2 us (from HBM): the keys are
     // split where that leaves half the SMs idle, and while there is a long run of keys for every CTA of two an SM

@@ -26,7 +26,8 @@ INT32_MIN, INT32_MAX = -2 ** 31, 2 ** 31 - 1
 
 
 def _i32(x: int) -> int:
-    """A number as the C ABI's int32 takes it: one outside stands for the nearest (ctypes would drop its upper bits)."""
+    """A number as the C ABI's int32 takes it: one outside stands for the nearest (ctypes would drop its upper bits). The
+    calls come here where x >> 31 is not 0."""
     return x if INT32_MIN <= x <= INT32_MAX else (INT32_MIN if x < 0 else INT32_MAX)
 
 
@@ -62,6 +63,7 @@ class Store:
         self.n_streams, self.max_ctx, self.n_head, self.n_layer = n_streams, max_ctx, n_head, n_layer
         self._tensor, self._i64, self._i32 = torch.Tensor, torch.int64, torch.int32
         self._row, self._flat, self._unit = (n_head, HEAD), (n_head * HEAD,), (HEAD, 1)
+        self._width = n_head * HEAD
         self._stream, self._index = (torch._C._cuda_getCurrentRawStream, device) if cuda else (lambda i: None, -1)
         L = lib()
         self._f_write, self._f_read, self._f_attend, self._f_step = L.b2_store_write, L.b2_store_read, L.b2_store_attend, L.b2_store_step
@@ -72,7 +74,11 @@ class Store:
     def _rows(self, x, name: str):
         """(pointer, row stride) of int64 rows [rows, n_head, 64] or [rows, n_head * 64]; only the rows may be strided."""
         if isinstance(x, self._tensor) and x.dtype is self._i64 and x.get_device() == self._index:
-            shape, st, d = x.shape, x.stride(), self.n_head * HEAD
+            if x.ndim == 3 and x.is_contiguous():
+                _, h, d = x.shape
+                if h == self.n_head and d == HEAD:
+                    return x.data_ptr(), self._width
+            shape, st, d = x.shape, x.stride(), self._width
             if (shape[1:] == self._row and (st[1:] == self._unit or (self.n_head == 1 and st[2] == 1))) or \
                     (shape[1:] == self._flat and st[1] == 1):
                 if st[0] >= d:
@@ -89,20 +95,23 @@ class Store:
         return f"{x.dtype} on {x.device}" if isinstance(x, self._tensor) else type(x).__name__
 
     def _ints(self, x, name: str, n: int):
-        if isinstance(x, self._tensor) and x.dtype is self._i32 and x.get_device() == self._index and x.shape == (n,) and \
-                x.is_contiguous():
+        if isinstance(x, self._tensor) and x.dtype is self._i32 and x.get_device() == self._index and x.ndim == 1 and \
+                x.numel() == n and x.is_contiguous():
             return x.data_ptr()
         what = f"shape {tuple(x.shape)}, strides {x.stride()}, " if isinstance(x, self._tensor) else ""
         raise ValueError(f"{name}: {n} torch.int32 values in a row on {self.device}, got {what}{self._what(x)}")
 
     def _table(self, pos, cu, rows: int, max_rows):
         """The row table's arguments: cu, pos, n_streams, rows, max_rows."""
-        n = pos.shape[0] if isinstance(pos, self._tensor) and pos.dim() == 1 else -1
+        n = pos.numel() if isinstance(pos, self._tensor) else -1
         p = self._ints(pos, "pos", n)
         if cu is not None:
             if max_rows is None:
                 raise ValueError("max_rows (the most rows a stream gives) goes with cu")
-            return self._ints(cu, "cu", n + 1), p, _i32(n), rows, _i32(max_rows)
+            c = self._ints(cu, "cu", n + 1)
+            if (n | max_rows) >> 31:
+                n, max_rows = _i32(n), _i32(max_rows)
+            return c, p, n, rows, max_rows
         if rows != n or max_rows not in (None, 1):
             raise ValueError(f"without cu every stream gives one row: {rows} rows, {n} positions, max_rows {max_rows}")
         return None, p, n, rows, 1
@@ -129,11 +138,13 @@ class Store:
         """Hold rows k, v (int64 [rows, n_head, 64], or rows of n_head * 64; rows may be strided, as slices of a qkv row
         are) at their streams' positions."""
         h = self._open()
+        if layer >> 31:
+            layer = _i32(layer)
         (pk, ldk), (pv, ldv), rows = self._rows(k, "k"), self._rows(v, "v"), k.shape[0]
         if rows != v.shape[0]:
             raise ValueError(f"{rows} rows of keys, {v.shape[0]} of values")
         cu, pos, n, rows, most = self._table(pos, cu, rows, max_rows)
-        rc = self._f_write(h, _i32(layer), pk, ldk, pv, ldv, cu, pos, n, rows, most, self._stream(self._index))
+        rc = self._f_write(h, layer, pk, ldk, pv, ldv, cu, pos, n, rows, most, self._stream(self._index))
         if rc:
             self._done(rc)
 
@@ -142,6 +153,8 @@ class Store:
         are (with cu; its last entry). out: two tensors to fill instead of new ones. Rows that no stream has keep what
         `out` held."""
         h = self._open()
+        if layer >> 31:
+            layer = _i32(layer)
         if rows is None:
             if cu is not None:
                 raise ValueError("rows (cu's last entry) goes with cu")
@@ -151,7 +164,7 @@ class Store:
         else:
             k, v = self._out(out[0], rows, "out k"), self._out(out[1], rows, "out v")
         cu, pos, n, rows, most = self._table(pos, cu, rows, max_rows)
-        rc = self._f_read(h, _i32(layer), cu, pos, n, rows, most, k.data_ptr(), v.data_ptr(), self._stream(self._index))
+        rc = self._f_read(h, layer, cu, pos, n, rows, most, k.data_ptr(), v.data_ptr(), self._stream(self._index))
         if rc:
             self._done(rc)
         return k, v
@@ -161,6 +174,8 @@ class Store:
         values: int64 [rows, n_head, 64]. A row at position p sees the positions from the largest of 0, first[stream] (if
         given) and p - window + 1 (if window > 0) to p; one that sees none gets zeros."""
         h = self._open()
+        if (layer | window) >> 31:
+            layer, window = _i32(layer), _i32(window)
         pq, ldq = self._rows(q, "q")
         rows = q.shape[0]
         if out is not None:
@@ -171,7 +186,7 @@ class Store:
             out = q.new_empty((rows, *self._row))
         cu, pos, n, rows, most = self._table(pos, cu, rows, max_rows)
         f = None if first is None else self._ints(first, "first", n)
-        rc = self._f_attend(h, _i32(layer), pq, ldq, cu, pos, f, n, rows, most, _i32(window), out.data_ptr(), self._stream(self._index))
+        rc = self._f_attend(h, layer, pq, ldq, cu, pos, f, n, rows, most, window, out.data_ptr(), self._stream(self._index))
         if rc:
             self._done(rc)
         return out
@@ -179,6 +194,8 @@ class Store:
     def step(self, q, k, v, pos, window: int = 0, first=None, layer: int = 0, out=None):
         """A decode step, write() and attend() of one row a stream in one launch: row i is stream i's, at position pos[i]."""
         h = self._open()
+        if (layer | window) >> 31:
+            layer, window = _i32(layer), _i32(window)
         (pq, ldq), (pk, ldk), (pv, ldv), n = self._rows(q, "q"), self._rows(k, "k"), self._rows(v, "v"), q.shape[0]
         if k.shape[0] != n or v.shape[0] != n:
             raise ValueError(f"{n} rows of queries, {k.shape[0]} of keys, {v.shape[0]} of values")
@@ -190,7 +207,7 @@ class Store:
             out = q.new_empty((n, *self._row))
         p = self._ints(pos, "pos", n)
         f = None if first is None else self._ints(first, "first", n)
-        rc = self._f_step(h, _i32(layer), pq, ldq, pk, ldk, pv, ldv, p, f, n, _i32(window), out.data_ptr(), self._stream(self._index))
+        rc = self._f_step(h, layer, pq, ldq, pk, ldk, pv, ldv, p, f, n, window, out.data_ptr(), self._stream(self._index))
         if rc:
             self._done(rc)
         return out
