@@ -64,6 +64,7 @@ class Store:
         self._tensor, self._i64, self._i32 = torch.Tensor, torch.int64, torch.int32
         self._row, self._flat, self._unit = (n_head, HEAD), (n_head * HEAD,), (HEAD, 1)
         self._width = n_head * HEAD
+        self._none = torch.empty(0, dtype=torch.int64, device=self.device)
         self._stream, self._index = (torch._C._cuda_getCurrentRawStream, device) if cuda else (lambda i: None, -1)
         L = lib()
         self._f_write, self._f_read, self._f_attend, self._f_step = L.b2_store_write, L.b2_store_read, L.b2_store_attend, L.b2_store_step
@@ -158,9 +159,10 @@ class Store:
         if rows is None:
             if cu is not None:
                 raise ValueError("rows (cu's last entry) goes with cu")
-            rows = len(pos)
+            rows = pos.numel() if isinstance(pos, self._tensor) else len(pos)
         if out is None:
-            k, v = self.torch.empty((2, rows, *self._row), dtype=self._i64, device=self.device).unbind(0)
+            k = self._none.new_empty((rows, *self._row))     # (quicker than torch.empty, or one tensor taken apart)
+            v = self.torch.empty_like(k)
         else:
             k, v = self._out(out[0], rows, "out k"), self._out(out[1], rows, "out v")
         cu, pos, n, rows, most = self._table(pos, cu, rows, max_rows)
