@@ -442,7 +442,7 @@ int run_attend(b2_handle* h, int rows, int l, uint64_t* or_out, cudaStream_t st,
 
 // "store_bits" 4, after layer l's qkv bank (q, k, v in QKV's rows): (Pythia's turn,) the rows' keys and values into the
 // 4-bit store and the arrival over it; a decode step's in one launch
-int run_store4(b2_handle* h, int rows, int l, uint64_t* or_out, cudaStream_t st) {
+int run_store4(b2_handle* h, int rows, int l, uint64_t* or_out, cudaStream_t st, bool decode = false) {
     const int d = h->cfg.d_model;
     const bool py = h->cfg.kind == B2_PYTHIA, step = !h->rows4.cu;
     const int hs = py ? 192 : 64;                       // Pythia's columns are per head q, k, v
@@ -465,6 +465,7 @@ int run_store4(b2_handle* h, int rows, int l, uint64_t* or_out, cudaStream_t st)
         a.COS = h->COS;
         a.SIN = h->SIN;
     }
+    a.early = decode && h->early_keys;                  // the launch before is the qkv bank
     a.stamp = stamp_slot(h, B2_PROF_ATTEND);
     prof_begin(h, B2_PROF_ATTEND, st);
     e = step ? store_step(a, how) : store_attend(a, how);
@@ -681,7 +682,7 @@ int run_decode_wq(b2_handle* h, int n, cudaStream_t st) {
             return rc;
         }
         if (h->store_bits == 4) {
-            if ((rc = run_store4(h, n, l, o0 + FUSED_ROWS, st))) return rc;
+            if ((rc = run_store4(h, n, l, o0 + FUSED_ROWS, st, true))) return rc;
         } else {
             if (!heads_done) return fail(h, B2_ERR_STATE, "qkv bank %d: heads16 not done in its epilogue", l);
             if ((rc = run_attend(h, n, l, o0 + FUSED_ROWS, st, 0, true))) return rc;
@@ -744,7 +745,7 @@ int run_decode_wq_pythia(b2_handle* h, int n, cudaStream_t st) {
                          (int)h->rot, (const int32_t*)h->COS, (const int32_t*)h->SIN, h->q16, h->qexp, h->d_err,
                          (const double*)nullptr, (const double*)nullptr, (int64_t*)nullptr, stamp_slot(h, B2_PROF_HEADS))))
             return rc;
-        if ((rc = four ? run_store4(h, n, l, o0 + FUSED_ROWS, st) : run_attend(h, n, l, o0 + FUSED_ROWS, st, 0, true))) return rc;
+        if ((rc = four ? run_store4(h, n, l, o0 + FUSED_ROWS, st, true) : run_attend(h, n, l, o0 + FUSED_ROWS, st, 0, true))) return rc;
         // MLP branch from the same R: fc + bend -> mproj; then both branches into R (mproj, proj)
         q = wq_args(h, 4 * l + 2, h->G2, d, o0 + 2 * FUSED_ROWS);
         if ((rc = run_bank(h, 4 * l + 2, EPI_PLAIN_EDGE, n, h->HID, F, nullptr, st, nullptr, nullptr, &q,

@@ -179,7 +179,8 @@ __global__ void __launch_bounds__(SW_WARPS * 32) k_store_read(Store4 st, StoreRo
 //           shared memory, the largest score and value shift by warp maxima
 //   pass 2  a = ARR[start - score], Z += a, the weight's three bytes into three planes of shared memory
 //   pass 3  num: the planes as the A rows, the values' codes as B (4 keys x 8 dims of nibbles turned by byte permutes)
-// PUT (store_step): the warp into whose block the row's own position falls holds its key and value first. RING: the codes come
+// PUT (store_step): the warp into whose block the row's own position falls holds its key and value first; early: what earlier
+// steps wrote is asked for into L2 before the dependency wait (the engine's steps: 0.586 -> 0.572 ms at 64 x 160). RING: the codes come
 // by asynchronous copies into a ring in shared memory, three blocks ahead, in place of loads one block ahead (two at 16 warps).
 // What shared memory a CTA does not take the table's entries use as L1 (71 KB: with 8 bytes a key and the ring 4 x 32,768 took
 // 41 us), so the weights' planes lie where the scores were.
@@ -198,6 +199,7 @@ constexpr int SF_RING = 4;
 B2_DEV void copy16(void* to, const void* from) {      // 16 bytes, asynchronously, past L1
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(saddr(to)), "l"(from) : "memory");
 }
+B2_DEV void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 B2_DEV void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 B2_DEV void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -340,13 +342,23 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, NW == 1 ? 7 : (NW == 
     uint8_t* const mem = sm + (RING ? (NW == 1 ? 4 : NW) * D * sizeof(SfBlock) : 0) + (size_t)un * chunk * SF_BYTES;
     int32_t* const SC = reinterpret_cast<int32_t*>(mem);             // [chunk]; then of four keys each the three planes' words
     int8_t* const VS = reinterpret_cast<int8_t*>(mem + (size_t)chunk * 4);   // [chunk]
-    griddep_wait();
-    stamp_begin(a.stamp);
-    griddep_launch();
+    auto begin = [&]() {
+        griddep_wait();
+        stamp_begin(a.stamp);
+        griddep_launch();
+    };
+    const bool early = PUT && a.early;
+    if (!early) begin();
     const int H = a.st.H, s = blockIdx.y, rank = cs > 1 ? (int)cluster_rank() : 0;
     const int unit = NW == 1 ? blockIdx.x * UN + un : blockIdx.x / cs, i = unit / H, h = unit - i * H;
     StoreRun run;
-    if (!store_run(a.rw, s, a.st.lim, run, a.err) || i >= run.n) return;   // the same for a whole cluster
+    // (early: a read from L2, since only the wait makes sure of L1; a step has no cu)
+    const bool some = early ? store_run(a.rw, s, s + 1, __ldcg(a.rw.pos + s), a.st.lim, run, a.err)
+                            : store_run(a.rw, s, a.st.lim, run, a.err);
+    if (!some || i >= run.n) {                                       // the same for a whole cluster
+        if (early) begin();
+        return;
+    }
     const int row = run.r0 + i, p = run.p0 + i;
     int lo = a.window > 0 ? max(0, p - a.window + 1) : 0;
     if (a.first) lo = max(lo, a.first[s]);
@@ -363,19 +375,29 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, NW == 1 ? 7 : (NW == 
         __syncwarp();                                                // the warp's own loads come after it
     };
     if (lo > p) {
+        if (early) begin();
         if (PUT && rank == 0 && wid == 0) put();
         if (PUT) unit_sync<NW>();                                    // out may be k or v
         for (int t = ut; t < 64 && rank == 0; t += NW * 32) out[t] = 0;
         return;
     }
-    int64_t x[1][2];
-    load_pair(a.q.x + (size_t)row * a.q.ld + h * a.q.hs + 2 * lane, wide & 1, x[0][0], x[0][1]);
     // blocks of 32 positions; this CTA's are b0 .. b0 + nb - 1
     const int first_block = lo >> 5, blocks = (p >> 5) - first_block + 1;
     const int per = cs > 1 ? (blocks + cs - 1) / cs : blocks;
     const int b0 = first_block + rank * per, nb = max(0, min(per, blocks - rank * per));
     const size_t base = kv_index(a.rw.slot0 + s, a.layer, h, 0, a.st.L, H, a.st.ctx) + (size_t)b0 * 32;
     const int from = lo - b0 * 32, to = p - b0 * 32;                 // visible: from <= local key <= to
+    if (early) {                                                     // what earlier steps wrote: into L2 while the launch before ends
+        const uint8_t* const line = lane < 8 ? a.st.k + base * 32 + lane * 128 : a.st.v + base * 32 + (lane - 8) * 128;
+        for (int b = wid; b < nb; b += NW) {
+            if (lane < 16) prefetch_l2(line + (size_t)b * 1024);
+            else if (lane == 16) prefetch_l2(a.st.ks + (base + (size_t)b * 32) * 2);
+            else if (lane == 17) prefetch_l2(a.st.vs + base + (size_t)b * 32);
+        }
+        begin();
+    }
+    int64_t x[1][2];
+    load_pair(a.q.x + (size_t)row * a.q.ld + h * a.q.hs + 2 * lane, wide & 1, x[0][0], x[0][1]);
     // of a block's keys the one whose score this lane finishes, and its place: a block's scores, shifts and planes are kept in
     // the order of the values' operands, key 4m + x at 8x + m
     const int mine = 16 * (j >> 1) + 8 * (j & 1) + g, place = 8 * (mine & 3) + (mine >> 2);

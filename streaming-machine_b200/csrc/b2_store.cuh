@@ -62,6 +62,7 @@ struct StoreAttend {
     // COS is given ([positions][8] at 2^-30)
     StoreVec k{nullptr, 0, 0}, v{nullptr, 0, 0};
     const int32_t *COS = nullptr, *SIN = nullptr;
+    bool early = false;    // store_step: the row table and the positions before the rows' own were written two launches before or more
 };
 
 // what the launches are sized by, once per device (the current one) and arrival table; to be called before the first launch
