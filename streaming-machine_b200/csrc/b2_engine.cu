@@ -1085,6 +1085,7 @@ int finalize_pythia(b2_handle* h) {
 int b2_finalize(b2_handle* h) {
     if (!h) return B2_ERR_ARG;
     CK(cudaSetDevice(h->device));
+    drop_graph(h);                    // a captured step holds the old banks' and tables' addresses
     dfree(h, h->entry_w);             // stored rows of the old weights
     dfree(h, h->entry_p);
     h->entry_w = h->entry_p = nullptr;
