@@ -191,11 +191,14 @@ int dalloc(b2_handle* h, T** p, size_t n) {
     return B2_OK;
 }
 
-void dfree(b2_handle* h, void* p) {
+// (the pointer is cleared: a call that fails half-way leaves none behind that a later one would free again, when the address
+// may be another allocation's)
+template <class T>
+void dfree(b2_handle* h, T*& p) {
     if (!p) return;
-    for (size_t i = 0; i < h->allocs.size(); i++)
-        if (h->allocs[i] == p) { h->allocs.erase(h->allocs.begin() + i); break; }
+    h->allocs.erase(std::find(h->allocs.begin(), h->allocs.end(), (void*)p));
     cudaFree(p);
+    p = nullptr;
 }
 
 void drop_graph(b2_handle* h) {
@@ -234,7 +237,7 @@ int upload_table32(b2_handle* h, int32_t** dst, const int64_t* src, int64_t n, c
         if (src[i] < INT32_MIN || src[i] > INT32_MAX) return fail(h, B2_ERR_VALUE, "table %s[%lld] does not fit int32", name, (long long)i);
         t[i] = (int32_t)src[i];
     }
-    if (*dst) dfree(h, *dst);
+    dfree(h, *dst);
     int rc = dalloc(h, dst, (size_t)n);
     if (rc) return rc;
     CK(cudaMemcpy(*dst, t.data(), sizeof(int32_t) * n, cudaMemcpyHostToDevice));
@@ -886,7 +889,7 @@ int b2_set_bank(b2_handle* h, const char* name, const int16_t* w, const int64_t*
     if (nin != want_in[k] || nout != want_out[k])
         return fail(h, B2_ERR_ARG, "b2_set_bank %s: shape [%d][%d], want [%d][%d]", name, nin, nout, want_in[k], want_out[k]);
     DevBank& bk = h->banks[bi];
-    if (bk.w) { dfree(h, bk.w); dfree(h, bk.e); dfree(h, bk.b); bk.w = nullptr; }
+    if (bk.w) { dfree(h, bk.w); dfree(h, bk.e); dfree(h, bk.b); }
     tc_bank_free(bk.tc);
     bk.nin = nin;
     bk.nout = nout;
@@ -949,7 +952,7 @@ int b2_set_array(b2_handle* h, const char* name, const int64_t* data, int64_t n)
         int64_t want = (int64_t)(name[1] == 't' ? c.vocab : c.n_ctx) * c.d_model;
         if (n != want) return fail(h, B2_ERR_ARG, "%s: %lld values, want %lld", name, (long long)n, (long long)want);
         int64_t** dst = name[1] == 't' ? &h->wte : &h->wpe;
-        if (*dst) dfree(h, *dst);
+        dfree(h, *dst);
         if ((rc = dalloc(h, dst, (size_t)n))) return rc;
         CK(cudaMemcpy(*dst, data, sizeof(int64_t) * n, cudaMemcpyHostToDevice));
     } else if (!strcmp(name, "phi") || !strcmp(name, "log2") || !strcmp(name, "exp2")) {
@@ -973,7 +976,7 @@ int b2_set_array(b2_handle* h, const char* name, const int64_t* data, int64_t n)
         if (n != c.d_model) return fail(h, B2_ERR_ARG, "%s: %lld values, want %d", name, (long long)n, c.d_model);
         b2_handle::Norm& nm = h->norms[norm_index(h, name, &part)];
         int64_t** dst = part[0] == 'g' ? &nm.g : &nm.b;
-        if (*dst) dfree(h, *dst);
+        dfree(h, *dst);
         if ((rc = dalloc(h, dst, (size_t)n))) return rc;
         CK(cudaMemcpy(*dst, data, sizeof(int64_t) * n, cudaMemcpyHostToDevice));
     } else {
@@ -1008,7 +1011,6 @@ int b2_set_scalar(b2_handle* h, const char* name, int64_t v) {
         if (!v) {
             dfree(h, h->entry_w);
             dfree(h, h->entry_p);
-            h->entry_w = h->entry_p = nullptr;
         }
         drop_graph(h);
         return B2_OK;
@@ -1072,7 +1074,7 @@ int finalize_pythia(b2_handle* h) {
             t[(size_t)v * d + i] = y;
         }
     }
-    if (h->wte) dfree(h, h->wte);
+    dfree(h, h->wte);
     int rc = dalloc(h, &h->wte, t.size());
     if (rc) return rc;
     CK(cudaMemcpy(h->wte, t.data(), sizeof(int64_t) * t.size(), cudaMemcpyHostToDevice));
@@ -1088,7 +1090,6 @@ int b2_finalize(b2_handle* h) {
     drop_graph(h);                    // a captured step holds the old banks' and tables' addresses
     dfree(h, h->entry_w);             // stored rows of the old weights
     dfree(h, h->entry_p);
-    h->entry_w = h->entry_p = nullptr;
     for (size_t i = 0; i < h->banks.size(); i++)
         if (!h->banks[i].w) return fail(h, B2_ERR_STATE, "bank %zu not set", i);
     if (h->cfg.kind == B2_PYTHIA) {
@@ -1207,27 +1208,15 @@ int b2_alloc_streams(b2_handle* h, int32_t n_streams, int32_t max_ctx) {
                         "in [0, 65536], exp2's in [65536, 131071] (bits 0x%x)", STORE_MAX_ALEN, STORE_MAX_ARR, h->tables4_bad);
     }
     // drop old stream/row buffers
-    void* old[] = {h->pf_blocks, h->sigf, h->qraw, h->kv.kraw, h->row_or, h->wq_acc, h->wq_nsat, h->wq_ctr, h->fr_C, h->fr_HIS,
-                   h->fr_p5v, h->fr_p5i, h->fr_list, h->fr_cnt, h->fr_sv, h->fr_si, h->G2, h->race_v,
-                   h->race_i, h->kv.k, h->kv.kmask, h->kv.kexp, h->kv.v, h->slot_len, h->slot_tok, h->row_slot, h->row_pos,
-                   h->row_tok, h->R, h->QKV, h->ATT, h->HID, h->x16, h->ex, h->q16, h->qexp, h->LS, h->head_rows,
-                   h->race_out, h->logits, h->mem4, h->cu4, h->pos4};
-    for (void* p : old) dfree(h, p);
+    auto drop = [&](auto*&... p) { (dfree(h, p), ...); };
+    drop(h->pf_blocks, h->sigf, h->qraw, h->kv.kraw, h->row_or, h->wq_acc, h->wq_nsat, h->wq_ctr, h->fr_C, h->fr_HIS,
+         h->fr_p5v, h->fr_p5i, h->fr_list, h->fr_cnt, h->fr_sv, h->fr_si, h->G2, h->race_v, h->race_i, h->kv.k, h->kv.kmask,
+         h->kv.kexp, h->kv.v, h->slot_len, h->slot_tok, h->row_slot, h->row_pos, h->row_tok, h->R, h->QKV, h->ATT, h->HID,
+         h->x16, h->ex, h->q16, h->qexp, h->LS, h->head_rows, h->race_out, h->logits, h->mem4, h->cu4, h->pos4, h->gen_desc,
+         h->gen_base);
     tc_rows_free(h->tcr);
     drop_graph(h);
-    dfree(h, h->gen_desc);
-    dfree(h, h->gen_base);
     h->n_slots = 0;
-    h->sigf = nullptr;
-    h->qraw = nullptr;
-    h->kv.kraw = nullptr;
-    h->pf_blocks = nullptr;
-    h->mem4 = nullptr;
-    h->cu4 = h->pos4 = nullptr;
-    h->kv.k = nullptr;
-    h->kv.kmask = nullptr;
-    h->kv.kexp = nullptr;
-    h->kv.v = nullptr;
     h->st4 = Store4{};
     h->store_bits = h->store_want;
     const int L = c.n_layer, H = c.n_head, d = c.d_model, F = c.d_ff;

@@ -51,3 +51,34 @@ def test_a_captured_step_takes_new_tables(small, bits):
     finally:
         e.close()
         fresh.close()
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_a_failed_allocation_frees_nothing_twice(M, small, bits):
+    """Streams that do not fit, after streams that did: the old buffers are gone with the failed call, and the next one does
+    not free their addresses again, which belong to whoever allocated since (torch and another engine here)."""
+    import torch
+    from streaming_machine_b200 import engine
+    ids = np.random.default_rng(34).integers(0, V, (2, 20))
+    m = small if bits == 16 else layers(M, 4)
+    e = engine.Engine(m, n_streams=2, max_ctx=32, store_bits=bits)
+    other = None
+    try:
+        want = scores(e, ids)
+        with pytest.raises(engine.B2Error) as ex:
+            e.alloc_streams(65535, 1024)                           # 16 bits: the keys fit, the values do not; 4: 216 GB
+        assert ex.value.code == 3
+        with pytest.raises(engine.B2Error) as ex:
+            e.prefill(ids)
+        assert ex.value.code == 6
+        torch.cuda.empty_cache()
+        sizes = [k for k in range(12, 29) for _ in range(3)]
+        held = [torch.full((2 ** k,), k, dtype=torch.uint8, device="cuda") for k in sizes]
+        other = engine.Engine(m, n_streams=2, max_ctx=32, store_bits=bits)
+        e.alloc_streams(2, 32)
+        assert np.array_equal(scores(e, ids), want) and np.array_equal(scores(other, ids), want)
+        assert all(bool((t == k).all()) for t, k in zip(held, sizes))
+    finally:
+        e.close()
+        if other:
+            other.close()
