@@ -185,7 +185,10 @@ int dalloc(b2_handle* h, T** p, size_t n) {
     void* q = nullptr;
     if (n == 0) n = 1;
     cudaError_t e = cudaMalloc(&q, n * sizeof(T));
-    if (e != cudaSuccess) return fail(h, B2_ERR_NOMEM, "cudaMalloc(%zu bytes): %s", n * sizeof(T), cudaGetErrorString(e));
+    if (e != cudaSuccess) {
+        cudaGetLastError();           // told here: the next call that looks for errors is not to find it
+        return fail(h, B2_ERR_NOMEM, "cudaMalloc(%zu bytes): %s", n * sizeof(T), cudaGetErrorString(e));
+    }
     h->allocs.push_back(q);
     *p = (T*)q;
     return B2_OK;
@@ -1283,7 +1286,10 @@ int b2_alloc_streams(b2_handle* h, int32_t n_streams, int32_t max_ctx) {
         return rc;
     if (h->tc_min_rows < (1 << 30)) {
         rc = tc_rows_alloc(h->tcr, mr, F > d ? F : d, h->d_err);
-        if (rc) return fail(h, B2_ERR_NOMEM, "tensor-core row buffers: %s", cudaGetErrorString((cudaError_t)rc));
+        if (rc) {
+            cudaGetLastError();
+            return fail(h, B2_ERR_NOMEM, "tensor-core row buffers: %s", cudaGetErrorString((cudaError_t)rc));
+        }
     }
     h->n_slots = n_streams;
     h->max_ctx = max_ctx;

@@ -82,3 +82,20 @@ def test_a_failed_allocation_frees_nothing_twice(M, small, bits):
         e.close()
         if other:
             other.close()
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_a_failed_allocation_is_told_once(M, small, bits):
+    """Streams that do not fit: B2_ERR_NOMEM, and a smaller allocation right after it is not refused for that error."""
+    from streaming_machine_b200 import engine
+    e = engine.Engine(small if bits == 16 else layers(M, 4), n_streams=1, max_ctx=32, store_bits=bits)
+    try:
+        want = scores(e, [[1, 2, 3]])
+        for _ in range(2):
+            with pytest.raises(engine.B2Error) as ex:
+                e.alloc_streams(65535, 1024)                       # 319 GB; in 4 bits and 4 layers 216
+            assert ex.value.code == 3
+            e.alloc_streams(1, 32)
+            assert np.array_equal(scores(e, [[1, 2, 3]]), want)
+    finally:
+        e.close()
