@@ -240,6 +240,7 @@ int upload_table32(b2_handle* h, int32_t** dst, const int64_t* src, int64_t n, c
         if (src[i] < INT32_MIN || src[i] > INT32_MAX) return fail(h, B2_ERR_VALUE, "table %s[%lld] does not fit int32", name, (long long)i);
         t[i] = (int32_t)src[i];
     }
+    h->finalized = false;
     dfree(h, *dst);
     int rc = dalloc(h, dst, (size_t)n);
     if (rc) return rc;
@@ -891,25 +892,26 @@ int b2_set_bank(b2_handle* h, const char* name, const int16_t* w, const int64_t*
     int want_out[5] = {3 * c.d_model, c.d_model, c.d_ff, c.d_model, c.vocab};
     if (nin != want_in[k] || nout != want_out[k])
         return fail(h, B2_ERR_ARG, "b2_set_bank %s: shape [%d][%d], want [%d][%d]", name, nin, nout, want_in[k], want_out[k]);
-    DevBank& bk = h->banks[bi];
-    if (bk.w) { dfree(h, bk.w); dfree(h, bk.e); dfree(h, bk.b); }
-    tc_bank_free(bk.tc);
-    bk.nin = nin;
-    bk.nout = nout;
-    int rc;
-    if ((rc = dalloc(h, &bk.w, (size_t)nin * nout))) return rc;
-    if ((rc = dalloc(h, &bk.e, (size_t)nout))) return rc;
-    if ((rc = dalloc(h, &bk.b, (size_t)nout))) return rc;
     std::vector<int32_t> e32(nout);
     for (int j = 0; j < nout; j++) {
         if (e[j] < -200 || e[j] > 200) return fail(h, B2_ERR_VALUE, "bank %s: exponent %lld out of range", name, (long long)e[j]);
         e32[j] = (int32_t)e[j];
     }
+    DevBank& bk = h->banks[bi];
+    h->finalized = false;                // from here on the old bank is gone, whatever becomes of the new one
+    dfree(h, bk.w);
+    dfree(h, bk.e);
+    dfree(h, bk.b);
+    tc_bank_free(bk.tc);
+    bk.nin = nin;
+    bk.nout = nout;
+    int rc;
+    if ((rc = dalloc(h, &bk.e, (size_t)nout)) || (rc = dalloc(h, &bk.b, (size_t)nout)) || (rc = dalloc(h, &bk.w, (size_t)nin * nout)))
+        return rc;
     CK(cudaMemcpy(bk.w, w, sizeof(int16_t) * (size_t)nin * nout, cudaMemcpyHostToDevice));
     CK(cudaMemcpy(bk.e, e32.data(), sizeof(int32_t) * nout, cudaMemcpyHostToDevice));
     if (b) CK(cudaMemcpy(bk.b, b, sizeof(int64_t) * nout, cudaMemcpyHostToDevice));
     else CK(cudaMemset(bk.b, 0, sizeof(int64_t) * nout));   // no bias (Pythia's head, pythia_base2.py:56)
-    h->finalized = false;
     return B2_OK;
 }
 
@@ -955,6 +957,7 @@ int b2_set_array(b2_handle* h, const char* name, const int64_t* data, int64_t n)
         int64_t want = (int64_t)(name[1] == 't' ? c.vocab : c.n_ctx) * c.d_model;
         if (n != want) return fail(h, B2_ERR_ARG, "%s: %lld values, want %lld", name, (long long)n, (long long)want);
         int64_t** dst = name[1] == 't' ? &h->wte : &h->wpe;
+        h->finalized = false;
         dfree(h, *dst);
         if ((rc = dalloc(h, dst, (size_t)n))) return rc;
         CK(cudaMemcpy(*dst, data, sizeof(int64_t) * n, cudaMemcpyHostToDevice));
@@ -979,6 +982,7 @@ int b2_set_array(b2_handle* h, const char* name, const int64_t* data, int64_t n)
         if (n != c.d_model) return fail(h, B2_ERR_ARG, "%s: %lld values, want %d", name, (long long)n, c.d_model);
         b2_handle::Norm& nm = h->norms[norm_index(h, name, &part)];
         int64_t** dst = part[0] == 'g' ? &nm.g : &nm.b;
+        h->finalized = false;
         dfree(h, *dst);
         if ((rc = dalloc(h, dst, (size_t)n))) return rc;
         CK(cudaMemcpy(*dst, data, sizeof(int64_t) * n, cudaMemcpyHostToDevice));

@@ -99,3 +99,19 @@ def test_a_failed_allocation_is_told_once(M, small, bits):
             assert np.array_equal(scores(e, [[1, 2, 3]]), want)
     finally:
         e.close()
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_a_refused_bank_leaves_the_old_one(small, bits):
+    """A bank that b2_set_bank refuses for an exponent, in an engine that runs: the old one stays, its captured step too."""
+    from streaming_machine_b200 import engine
+    ids = np.random.default_rng(35).integers(0, V, (2, 20))
+    e = engine.Engine(small, n_streams=2, max_ctx=32, store_bits=bits)
+    try:
+        want = scores(e, ids)
+        with pytest.raises(engine.B2Error) as ex:
+            set_bank(e, dict(small, **{"fc.0.e": np.r_[300, small["fc.0.e"][1:]]}), "fc.0")
+        assert ex.value.code == 5
+        assert np.array_equal(scores(e, ids), want)
+    finally:
+        e.close()
