@@ -96,7 +96,8 @@ int b2_set_array(b2_handle* h, const char* name, const int64_t* data, int64_t n)
  * where to16 would round the row; 0 (default) drops them. "store_bits": 4 makes the next b2_alloc_streams hold the
  * streams' keys and values in 4 bits (67 bytes a position and head in place of 396; b2_store_* below says what is held and
  * how the arrival reads it; Pythia's turn comes before it), 16 (default) as the reference does; 4 is refused with a float
- * arrival or turn, with "entry_tables", and for tables that b2_store_create would refuse. */
+ * arrival or turn, with "entry_tables", and for tables that b2_store_create would refuse: b2_alloc_streams, or, where such a
+ * table is given afterwards, every call that runs over the streams reports B2_ERR_VALUE. */
 int b2_set_scalar(b2_handle* h, const char* name, int64_t v);
 
 /* All arrays given: build the device layouts. */

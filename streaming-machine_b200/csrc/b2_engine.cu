@@ -802,6 +802,19 @@ int ensure_ready(b2_handle* h) {
     return B2_OK;
 }
 
+// whether the tables are those that streams held in `bits` bits take
+int check_tables(b2_handle* h, int bits) {
+    if (bits != 4 || !h->tables4_bad) return B2_OK;
+    return fail(h, B2_ERR_VALUE, "store_bits 4: the arrival table has 1 .. %d entries in [0, %d], the first at least 1, log2's are "
+                "in [0, 65536], exp2's in [65536, 131071] (bits 0x%x)", STORE_MAX_ALEN, STORE_MAX_ARR, h->tables4_bad);
+}
+
+// for the calls that run over the streams: a table may have been given after they were allocated
+int ensure_streams(b2_handle* h) {
+    const int rc = ensure_ready(h);
+    return rc ? rc : check_tables(h, h->store_bits);
+}
+
 int read_device_error(b2_handle* h) {
     uint32_t e = 0;
     CK(cudaMemcpy(&e, h->d_err, sizeof e, cudaMemcpyDeviceToHost));
@@ -1147,6 +1160,7 @@ int b2_finalize(b2_handle* h) {
     }
     const char* env = getenv("B2_TC_MIN_ROWS");
     if (env && tc_ok) h->tc_min_rows = atoi(env);
+    if (h->n_slots && h->store_bits == 4 && !h->tables4_bad) CK(store_init(h->alen, h->plan4));   // the arrival table's length
     h->finalized = true;
     return B2_OK;
 }
@@ -1210,9 +1224,8 @@ int b2_alloc_streams(b2_handle* h, int32_t n_streams, int32_t max_ctx) {
     if (h->store_want == 4) {
         if (max_ctx > STORE_MAX_CTX) return fail(h, B2_ERR_ARG, "store_bits 4: max_ctx %d (at most %d)", max_ctx, STORE_MAX_CTX);
         if (n_streams > 65535) return fail(h, B2_ERR_ARG, "store_bits 4: n_streams %d (at most 65535)", n_streams);
-        if (h->tables4_bad)
-            return fail(h, B2_ERR_VALUE, "store_bits 4: the arrival table has 1 .. %d entries in [0, %d], the first at least 1, log2's are "
-                        "in [0, 65536], exp2's in [65536, 131071] (bits 0x%x)", STORE_MAX_ALEN, STORE_MAX_ARR, h->tables4_bad);
+        const int rc = check_tables(h, 4);
+        if (rc) return rc;
     }
     // drop old stream/row buffers
     auto drop = [&](auto*&... p) { (dfree(h, p), ...); };
@@ -1308,7 +1321,7 @@ int b2_alloc_streams(b2_handle* h, int32_t n_streams, int32_t max_ctx) {
 
 int b2_prefill(b2_handle* h, const int32_t* ids, const int32_t* lens, int32_t n_streams, int32_t* next_tok,
                int64_t* logits, void* stream) {
-    int rc = ensure_ready(h);
+    int rc = ensure_streams(h);
     if (rc) return rc;
     if (!ids || !lens || !next_tok || n_streams < 1 || n_streams > h->n_slots)
         return fail(h, B2_ERR_ARG, "b2_prefill: bad argument (n_streams %d of %d slots)", n_streams, h->n_slots);
@@ -1481,7 +1494,7 @@ int run_steps(b2_handle* h, int n, int n_steps, int32_t* out, int ld, int64_t* l
 }  // namespace
 
 int b2_step(b2_handle* h, const int32_t* tok_in, int32_t n_streams, int32_t* tok_out, int64_t* logits, void* stream) {
-    int rc = ensure_ready(h);
+    int rc = ensure_streams(h);
     if (rc) return rc;
     if (n_streams < 1 || n_streams > h->n_slots || !tok_out) return fail(h, B2_ERR_ARG, "b2_step: bad argument");
     if (!tok_in && !h->primed) return fail(h, B2_ERR_STATE, "b2_step without tok_in before any b2_prefill");
@@ -1491,7 +1504,7 @@ int b2_step(b2_handle* h, const int32_t* tok_in, int32_t n_streams, int32_t* tok
 }
 
 int b2_generate(b2_handle* h, int32_t n_streams, int32_t n_steps, int32_t* tokens_out, void* stream) {
-    int rc = ensure_ready(h);
+    int rc = ensure_streams(h);
     if (rc) return rc;
     if (n_streams < 1 || n_streams > h->n_slots || n_steps < 0 || !tokens_out) return fail(h, B2_ERR_ARG, "b2_generate: bad argument");
     if (!h->primed) return fail(h, B2_ERR_STATE, "b2_generate before b2_prefill");
@@ -1499,7 +1512,7 @@ int b2_generate(b2_handle* h, int32_t n_streams, int32_t n_steps, int32_t* token
 }
 
 int b2_step_host(b2_handle* h, const int32_t* tok_in, int32_t n_streams, int32_t* tok_out) {
-    int rc = ensure_ready(h);
+    int rc = ensure_streams(h);
     if (rc) return rc;
     if (!tok_in || !tok_out || n_streams < 1 || n_streams > h->n_slots) return fail(h, B2_ERR_ARG, "b2_step_host: bad argument");
     cudaStream_t st = 0;

@@ -115,3 +115,56 @@ def test_a_refused_bank_leaves_the_old_one(small, bits):
         assert np.array_equal(scores(e, ids), want)
     finally:
         e.close()
+
+
+def test_refused_tables_stay_refused(small):
+    """A table that 4-bit streams cannot take, given when they exist already: every call that would run over them is refused
+    (the banks by themselves are not), until the table is a good one or the streams are allocated with 16 bits."""
+    from streaming_machine_b200 import engine
+    ids = np.random.default_rng(32).integers(0, V, (2, 20))
+    big = np.minimum(small["arrival"] * 4, 1 << 25)
+    e, fresh = (engine.Engine(m, n_streams=2, max_ctx=32, store_bits=b) for m, b in ((small, 4), (dict(small, arrival=big), 16)))
+    try:
+        want = scores(e, ids)
+        row = np.arange(768)[None] * 100
+        bank = e.bank("proj.0", row, 2)
+        for name, bad in (("arrival", big), ("arrival", np.r_[0, small["arrival"]]), ("arrival", np.ones(32769)), ("log2", small["log2"] - 1),
+                          ("exp2", small["exp2"] - 1)):
+            set_array(e, name, bad)
+            e._call("b2_finalize", e.h)
+            for call in (lambda: e.prefill(ids), lambda: e.step(n=2), lambda: e.generate_device(2, 2), lambda: e.step_host(ids[:, 0])):
+                with pytest.raises(engine.B2Error) as ex:
+                    call()
+                assert ex.value.code == 5
+            assert e.bank("proj.0", row, 2).shape == bank.shape    # (by the table given, where the bank reads it)
+            set_array(e, name, small[name])
+            e._call("b2_finalize", e.h)
+            assert np.array_equal(scores(e, ids), want)
+        set_array(e, "arrival", big)
+        e._call("b2_set_scalar", e.h, b"store_bits", 16)
+        e._call("b2_finalize", e.h)
+        with pytest.raises(engine.B2Error) as ex:
+            e.prefill(ids)                                         # the streams are those in 4 bits still
+        assert ex.value.code == 5
+        e.alloc_streams(2, 32)
+        assert np.array_equal(scores(e, ids), scores(fresh, ids))
+    finally:
+        e.close()
+        fresh.close()
+
+
+@pytest.mark.parametrize("n", [100, 32768])
+def test_a_table_of_another_length(small, n):
+    """4-bit streams that exist already take a shorter or longer arrival table: the launches are sized by the new one."""
+    from streaming_machine_b200 import engine
+    ids = np.random.default_rng(33).integers(0, V, (2, 500))
+    table = np.r_[small["arrival"], np.ones(n, np.int64)][:n]
+    e, fresh = (engine.Engine(m, n_streams=2, max_ctx=600, store_bits=4) for m in (small, dict(small, arrival=table)))
+    try:
+        e.prefill(ids)
+        set_array(e, "arrival", table)
+        e._call("b2_finalize", e.h)
+        assert np.array_equal(scores(e, ids), scores(fresh, ids))
+    finally:
+        e.close()
+        fresh.close()
