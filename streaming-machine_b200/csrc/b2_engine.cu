@@ -959,13 +959,6 @@ int b2_set_array(b2_handle* h, const char* name, const int64_t* data, int64_t n)
     CK(cudaSetDevice(h->device));
     const b2_config& c = h->cfg;
     int rc;
-    const int t4 = !strcmp(name, "arrival") ? 1 : (!strcmp(name, "log2") ? 2 : (!strcmp(name, "exp2") ? 4 : 0));
-    if (t4) {
-        const int64_t lo = t4 == 4 ? 65536 : 0, hi = t4 == 1 ? STORE_MAX_ARR : (t4 == 2 ? 65536 : 131071);
-        bool ok = t4 != 1 || (n <= STORE_MAX_ALEN && data[0] >= 1);
-        for (int64_t i = 0; i < n && ok; i++) ok = data[i] >= lo && data[i] <= hi;
-        h->tables4_bad = (h->tables4_bad & ~t4) | (ok ? 0 : t4);
-    }
     if (!strcmp(name, "wte") || !strcmp(name, "wpe")) {
         int64_t want = (int64_t)(name[1] == 't' ? c.vocab : c.n_ctx) * c.d_model;
         if (n != want) return fail(h, B2_ERR_ARG, "%s: %lld values, want %lld", name, (long long)n, (long long)want);
@@ -1003,6 +996,14 @@ int b2_set_array(b2_handle* h, const char* name, const int64_t* data, int64_t n)
         return fail(h, B2_ERR_ARG, "b2_set_array: unknown array '%s'", name);
     }
     h->finalized = false;
+    // the table now in place: whether 4-bit streams take it
+    const int t4 = !strcmp(name, "arrival") ? 1 : (!strcmp(name, "log2") ? 2 : (!strcmp(name, "exp2") ? 4 : 0));
+    if (t4) {
+        const int64_t lo = t4 == 4 ? 65536 : 0, hi = t4 == 1 ? STORE_MAX_ARR : (t4 == 2 ? 65536 : 131071);
+        bool ok = t4 != 1 || (n <= STORE_MAX_ALEN && data[0] >= 1);
+        for (int64_t i = 0; i < n && ok; i++) ok = data[i] >= lo && data[i] <= hi;
+        h->tables4_bad = (h->tables4_bad & ~t4) | (ok ? 0 : t4);
+    }
     return B2_OK;
 }
 

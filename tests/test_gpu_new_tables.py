@@ -168,3 +168,23 @@ def test_a_table_of_another_length(small, n):
     finally:
         e.close()
         fresh.close()
+
+
+def test_a_refused_array_leaves_the_verdict(small):
+    """What b2_set_array refuses does not replace the table, and does not decide whether the table in place suits 4 bits."""
+    from streaming_machine_b200 import engine
+    e = engine.Engine(small, n_streams=1, max_ctx=32, store_bits=4)
+    try:
+        for name, bad in (("log2", np.full(10, -1)), ("exp2", np.zeros(65537)), ("log2", np.full(65536, 2 ** 40))):
+            with pytest.raises(engine.B2Error):
+                set_array(e, name, bad)
+            e.alloc_streams(1, 32)                                 # the good table is there still
+        set_array(e, "log2", small["log2"] + 65536)
+        with pytest.raises(engine.B2Error):
+            set_array(e, "log2", np.ones(10))
+        e._call("b2_finalize", e.h)
+        with pytest.raises(engine.B2Error) as ex:
+            e.alloc_streams(1, 32)                                 # and the bad one
+        assert ex.value.code == 5
+    finally:
+        e.close()
