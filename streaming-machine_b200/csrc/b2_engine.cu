@@ -1309,6 +1309,8 @@ int b2_alloc_streams(b2_handle* h, int32_t n_streams, int32_t max_ctx) {
             return fail(h, B2_ERR_NOMEM, "tensor-core row buffers: %s", cudaGetErrorString((cudaError_t)rc));
         }
     }
+    // what was cleared above is queued on the legacy stream, which the calls' streams need not wait for
+    CK(cudaDeviceSynchronize());
     h->n_slots = n_streams;
     h->max_ctx = max_ctx;
     h->primed = false;

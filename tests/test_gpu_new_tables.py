@@ -188,3 +188,23 @@ def test_a_refused_array_leaves_the_verdict(small):
         assert ex.value.code == 5
     finally:
         e.close()
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_streams_are_ready_when_alloc_returns(small, bits):
+    """b2_alloc_streams clears what it allocates on the legacy stream, which a caller's stream need not wait for: that is done
+    when it returns, however long the legacy stream was busy before."""
+    import torch
+    from streaming_machine_b200 import engine
+
+    class Busy(engine.Engine):
+        def alloc_streams(self, n_streams, max_ctx):
+            torch.cuda._sleep(400_000_000)                         # a fifth of a second
+            super().alloc_streams(n_streams, max_ctx)
+            self.done = torch.cuda.default_stream().query()
+
+    e = Busy(small, n_streams=64, max_ctx=1024, store_bits=bits)
+    try:
+        assert e.done
+    finally:
+        e.close()
