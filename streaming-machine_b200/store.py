@@ -23,6 +23,15 @@ from .engine import B2Error, StoreConfig, _torch, lib
 
 HEAD = 64
 INT32_MIN, INT32_MAX = -2 ** 31, 2 ** 31 - 1
+_ended = []      # (handle, memory) of stores that ended while a graph was captured: freeing one waits for the device
+
+
+def _free_ended(torch):
+    """Free what has ended, unless a capture is under way on this thread's stream (the wait would break it)."""
+    while _ended and not torch.cuda.is_current_stream_capturing():
+        h, memory = _ended.pop()
+        lib().b2_store_destroy(h)                        # (waits for the device: the memory may be used again)
+        del memory
 
 
 def _i32(x: int) -> int:
@@ -39,6 +48,7 @@ class Store:
     def __init__(self, M: dict, n_streams: int, max_ctx: int, n_head: int, n_layer: int = 1, device: int = 0):
         self.h = None
         self._host(_torch(), "cuda", device, n_streams, max_ctx, n_head, n_layer)
+        _free_ended(self.torch)
         t = [np.ascontiguousarray(M[k], dtype=np.int64) for k in ("arrival", "log2", "exp2")]
         if t[1].size != 65536 or t[2].size != 65536:
             raise ValueError("the log2 and exp2 tables have 65,536 entries")
@@ -220,9 +230,12 @@ class Store:
         self._done(lib().b2_store_sync(self._open()))
 
     def close(self):
+        """Free the store once the device is done with it. During a capture on this thread's stream that is put off until a
+        store is made or closed outside of one (a capture in another thread is not seen: end no store meanwhile)."""
         if getattr(self, "h", None):
-            lib().b2_store_destroy(self.h)               # (waits for the device)
+            _ended.append((self.h, self._memory))
             self.h = self._memory = None
+            _free_ended(self.torch)
 
     def __del__(self):
         try:
