@@ -661,7 +661,7 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, NW == 1 ? 7 : (NW == 
             out[ut + 32 * x] = y;
             any |= mag(y);
         }
-        if (a.or_out) {
+        if (PUT && a.or_out) {
             any = warp_or64(any);
             if (lane == 0) atomicOr((unsigned long long*)&a.or_out[row], (unsigned long long)any);
         }
@@ -1191,15 +1191,6 @@ __global__ void __launch_bounds__(SM_THREADS, 2) k_store_attend_many(StoreAttend
                         to[1] = o[x + 1];
                     }
                 }
-            }
-            if (a.or_out) {
-                uint64_t any = 0;
-#pragma unroll
-                for (int x = 0; x < 8; x++)
-                    if (cs == 1 || (x >> 1) % cs == rank) any |= mag(o[x]);
-                any |= __shfl_xor_sync(0xffffffffu, any, 1);
-                any |= __shfl_xor_sync(0xffffffffu, any, 2);
-                if (j == 0 && r < nr) atomicOr((unsigned long long*)&a.or_out[run.r0 + i0 + r], (unsigned long long)any);
             }
             if (cs > 1) cluster_sync();                                // the others have read this CTA's sums
         }

@@ -55,7 +55,7 @@ struct StoreAttend {
     const int32_t* LOG2;
     const int32_t* EXP2;
     int64_t* out;          // [rows][H][64]
-    uint64_t* or_out;      // optional [rows]: OR of |out| per row (the next bank's to16 shift)
+    uint64_t* or_out;      // store_step, optional [rows]: OR of |out| per row (the next bank's to16 shift)
     uint32_t* err;
     uint64_t* stamp = nullptr;   // b2_profile mode 2
     // store_step: the rows' own keys and values, held first (one row a stream); Pythia's turn of q and k before it, where
