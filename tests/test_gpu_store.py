@@ -615,3 +615,40 @@ def test_first_calls_captured_and_forked():
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     r = subprocess.run([sys.executable, "-c", FIRST_CALLS], cwd=root, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "same" in r.stdout, r.stdout + r.stderr
+
+
+def test_a_writer_beside_readers(T):
+    """Readers of the positions 0 .. 599 on two streams of work while a third writes the positions from 600 on, other values
+    every time: the readers' results do not move, and what was written last is what the store holds and attends over."""
+    import torch
+    rng = np.random.default_rng(22)
+    st, quiet = make(T, 4, 700, 4)[0], make(T, 4, 700, 4)[0]
+    hist = [dev(values(rng, 4 * 600, 4, s)) for s in (1.0, 0.3)]
+    cu = i32([0, 600, 1200, 1800, 2400])
+    for s in (st, quiet):
+        s.write(*hist, i32([0] * 4), cu=cu, max_rows=600)
+    q1, q2, q3 = dev(values(rng, 4, 4, 1.5)), dev(values(rng, 100, 4, 1.5)), dev(values(rng, 200, 4, 1.5))
+    p1, p2, cu2 = i32([599, 400, 599, 31]), i32([550, 550]), i32([0, 50, 100])
+    want1, want2 = st.attend(q1, p1), st.attend(q2, p2, cu=cu2, max_rows=50)
+    new = [[dev(values(rng, 200, 4, s)) for s in (1.0, 0.3)] for _ in range(31)]
+    cuw, posw = i32([0, 50, 100, 150, 200]), i32([600] * 4)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    got = []
+    for kv in new:
+        with torch.cuda.stream(streams[0]):
+            got.append((want1, st.attend(q1, p1)))
+        with torch.cuda.stream(streams[1]):
+            got.append((want2, st.attend(q2, p2, cu=cu2, max_rows=50)))
+        with torch.cuda.stream(streams[2]):
+            st.write(*kv, posw, cu=cuw, max_rows=50)
+    torch.cuda.synchronize()
+    assert all(torch.equal(w, g) for w, g in got)
+    quiet.write(*new[-1], posw, cu=cuw, max_rows=50)
+    every = dict(cu=i32(np.arange(5) * 650), max_rows=650, rows=2600)
+    for a, b in zip(st.read(i32([0] * 4), **every), quiet.read(i32([0] * 4), **every)):
+        assert torch.equal(a, b)
+    assert torch.equal(st.attend(q3, posw, cu=cuw, max_rows=50), quiet.attend(q3, posw, cu=cuw, max_rows=50))
+    for s in (st, quiet):
+        s.sync()
+        s.close()

@@ -228,3 +228,29 @@ def test_launch_shapes_of_the_decode_paths(M):
         got.append(e.generate(ids, 6))
         e.close()
     assert all(np.array_equal(g, got[0]) for g in got)
+
+
+@pytest.mark.parametrize("early", ["1", "0"])
+@pytest.mark.parametrize("kind,n,ctx", [("gpt2", 1, 1024), ("gpt2", 3, 1024), ("gpt2", 16, 1024), ("gpt2", 64, 1024), ("pythia", 1, 2048),
+                                        ("pythia", 16, 2048), ("pythia", 64, 2048)])
+def test_long_steps_equal_the_prompt_pass(kind, n, ctx, early, M, PM, monkeypatch):
+    """Captured decode steps near a long context's end, with what is held asked for ahead of the dependency wait and without
+    (B2_EARLY_KEYS): keys split over clusters of 8, 4 and 2 CTAs, 4 and 8 warps a CTA, registers and ring. The same scores as
+    a prompt pass over the same words, over the edges of blocks of 32 positions, and again after a rewind."""
+    from streaming_machine_b200 import engine
+    monkeypatch.setenv("B2_EARLY_KEYS", early)
+    e = engine.Engine(layers(M if kind == "gpt2" else PM, 2), n_streams=n, max_ctx=ctx, store_bits=4)
+    try:
+        rng = np.random.default_rng(n + ctx)
+        ids = rng.integers(0, V, (n, ctx))
+        lens = ctx - rng.integers(0, 40, n)
+        lens[0] = ctx                                              # the last position
+        _, want = e.prefill([ids[s, :lens[s]] for s in range(n)], logits=True)
+        e.prefill([ids[s, :lens[s] - 5] for s in range(n)])
+        for again in range(2):
+            for t in range(5, 0, -1):
+                _, got = e.step([ids[s, lens[s] - t] for s in range(n)], logits=True)
+            assert np.array_equal(got, want)
+            e.rewind(lens - 5, [ids[s, lens[s] - 5] for s in range(n)])
+    finally:
+        e.close()

@@ -145,3 +145,30 @@ def test_the_two_references_agree():
     fast.write(0, k, v)
     for window, first in ((0, 0), (7, 0), (0, 12), (9, 25)):
         assert np.array_equal(fast.attend(0, q, 0, window, first), slow.attend(q, [0], [0, 30], window, [first]))
+
+
+@pytest.mark.parametrize("spread", [0, 1, 3, 4, 7, 20])
+def test_the_error_in_bits_of_the_largest(spread):
+    """What four bits lose, by bit lengths: with t that of the largest magnitude of a value's 64 dims or a key's half, values
+    lose at most 2^(t - 4), and less than 2^(t - 3) where the code is 7 (an eighth of 2^t); a key's half next to a larger one, of bit length
+    T, at most 2^(T - 7) where that is more (all of it, 7 bits below)."""
+    rng = np.random.default_rng(spread)
+    for T in (20, 33, 47):
+        for _ in range(20):
+            x = np.zeros(64, np.int64)
+            for half, t in ((slice(0, 32), T), (slice(32, 64), T - spread)):
+                x[half] = rng.integers(-(1 << t) + 1, 1 << t, 32)
+                x[half][3] = (1 << t) - 1 - rng.integers(0, 2)               # held as 7
+            k, v = ref.hold_key(x), ref.hold_value(x)
+            for held, got, parts in ((k, ref.read_key(k), (slice(0, 32), slice(32, 64))), (v, ref.read_value(v), (slice(0, 64),))):
+                for part in parts:
+                    t = int(np.abs(x[part]).max()).bit_length()
+                    seven = np.array(held[0])[part] == 7
+                    off = np.abs(x[part] - got[part])
+                    most = max(t - 4, T - 7)
+                    assert (off[~seven] <= 1 << most).all()
+                    assert (off[seven] < 2 << most).all()
+                    if spread == 0:
+                        assert off.max() > (1 << t) // 16                # a sixteenth does not hold
+                    if spread >= 7 and part == slice(32, 64):
+                        assert (got[part] == 0).all() or spread == 7
