@@ -1278,14 +1278,21 @@ size_t few_smem(int warps, int keys, bool ring) { return (ring ? warps * SF_RING
 size_t many_smem(int alen) { return sizeof(SmShared) + (size_t)(alen + 1) * 4; }
 
 namespace {
+// the most shared memory that a launch of these asks for
+template <int NW>
+cudaError_t few_room() {
+    cudaError_t e = cudaSuccess;
+    for (auto f : {k_store_attend_few<NW, false, false>, k_store_attend_few<NW, false, true>, k_store_attend_few<NW, true, false>,
+                   k_store_attend_few<NW, true, true>})
+        if (e == cudaSuccess)
+            e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)few_smem(16, SF_MOST_KEYS, true));
+    return e;
+}
+
 cudaError_t make_plan(int device, int alen, StorePlan& plan) {
     cudaError_t e = cudaDeviceGetAttribute(&plan.sms, cudaDevAttrMultiProcessorCount, device);
-    void (*const few[])(StoreAttend, int, int, int) = {k_store_attend_few<1, false, false>, k_store_attend_few<1, false, true>, k_store_attend_few<1, true, false>, k_store_attend_few<1, true, true>,
-        k_store_attend_few<4, false, false>, k_store_attend_few<4, false, true>, k_store_attend_few<4, true, false>, k_store_attend_few<4, true, true>,
-        k_store_attend_few<8, false, false>, k_store_attend_few<8, false, true>, k_store_attend_few<8, true, false>, k_store_attend_few<8, true, true>,
-        k_store_attend_few<16, false, false>, k_store_attend_few<16, false, true>, k_store_attend_few<16, true, false>, k_store_attend_few<16, true, true>};
-    for (auto f : few)
-        if (e == cudaSuccess) e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)few_smem(16, SF_MOST_KEYS, true));
+    for (auto room : {few_room<1>, few_room<4>, few_room<8>, few_room<16>})
+        if (e == cudaSuccess) e = room();
     if (e == cudaSuccess)
         e = cudaFuncSetAttribute(k_store_attend_many, cudaFuncAttributeMaxDynamicSharedMemorySize, SM_SMEM_MOST);
     if (e != cudaSuccess) return e;
