@@ -208,3 +208,23 @@ def test_streams_are_ready_when_alloc_returns(small, bits):
         assert e.done
     finally:
         e.close()
+
+
+def test_entry_rows_end_with_their_weights(small):
+    """Stored layer-0 rows belong to the weights they were built from: after b2_finalize a captured step does without them until
+    b2_alloc_streams builds them anew."""
+    from streaming_machine_b200 import engine
+    ids = np.random.default_rng(36).integers(0, V, (2, 20))
+    e = engine.Engine(small, n_streams=2, max_ctx=32)
+    try:
+        want = scores(e, ids)
+        e.set_entry_tables(True)
+        e.alloc_streams(2, 32)
+        assert np.array_equal(scores(e, ids), want)
+        set_array(e, "phi", small["phi"])
+        e._call("b2_finalize", e.h)
+        assert np.array_equal(scores(e, ids), want)
+        e.alloc_streams(2, 32)
+        assert np.array_equal(scores(e, ids), want)
+    finally:
+        e.close()
