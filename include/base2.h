@@ -100,7 +100,8 @@ int b2_set_array(b2_handle* h, const char* name, const int64_t* data, int64_t n)
  * table is given afterwards, every call that runs over the streams reports B2_ERR_VALUE. */
 int b2_set_scalar(b2_handle* h, const char* name, int64_t v);
 
-/* All arrays given: build the device layouts. */
+/* All arrays given: build the device layouts. Again after a b2_set_bank or b2_set_array on an engine that runs (calls are refused
+ * in between): the streams stay, a captured step is captured anew, stored entry rows wait for the next b2_alloc_streams. */
 int b2_finalize(b2_handle* h);
 
 /* Reserve `n_streams` independent stream slots with a key/value store of `max_ctx` positions each

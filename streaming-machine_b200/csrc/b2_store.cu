@@ -22,9 +22,9 @@ namespace b2 {
 // write: eight lanes hold a head's key or value (64 int64), lane i of them the pairs of dims i, i + 8, i + 16, i + 24, so
 // that a load of the eight is 128 bytes in a row and the first two pairs are the lower half's; U rows, all asked for before
 // the first is used. The shift is the bit length of the OR of the magnitudes less 3 (the OR has the largest one's bit
-// length). U = 1 where streams give few rows (a decode step, bound by the memory's latency: 1.7 us for 64 rows of 12 heads in
-// a graph), 2 for prompts, bound by its bandwidth: 28 us for 12,600 rows (4.6 TB/s). A row a warp, two dims a lane, took three
-// times the instructions and was bound by them (40 us).
+// length). U = 1 where streams give few rows (a decode step, bound by the memory's latency: 1.9 us for 64 rows of 12 heads in
+// a graph), 2 for prompts, bound by its bandwidth: 25 us for 10,512 rows of 12 heads (5.4 TB/s, call after call). A row a warp,
+// two dims a lane, took three times the instructions and was bound by them (40 us).
 // ---------------------------------------------------------------------------------------------------------------------
 constexpr int SW_WARPS = 8;
 
@@ -180,14 +180,17 @@ __global__ void __launch_bounds__(SW_WARPS * 32) k_store_read(Store4 st, StoreRo
 //   pass 2  a = ARR[start - score], Z += a, the weight's three bytes into three planes of shared memory
 //   pass 3  num: the planes as the A rows, the values' codes as B (4 keys x 8 dims of nibbles turned by byte permutes)
 // PUT (store_step): the warp into whose block the row's own position falls holds its key and value first; early: what earlier
-// steps wrote is asked for into L2 before the dependency wait (the engine's steps: 0.586 -> 0.572 ms at 64 x 160). RING: the codes come
-// by asynchronous copies into a ring in shared memory, three blocks ahead, in place of loads one block ahead (two at 16 warps).
+// steps wrote is asked for into L2 before the dependency wait (the engine's steps: 0.586 -> 0.572 ms at 64 x 160). RING: the
+// codes come by asynchronous copies into a ring in shared memory, three blocks ahead, in place of loads one block ahead (two at
+// 16 warps).
 // What shared memory a CTA does not take the table's entries use as L1 (71 KB: with 8 bytes a key and the ring 4 x 32,768 took
 // 41 us), so the weights' planes lie where the scores were.
-// Bound by the chain of dependent steps where there are few units (3.1 us for 17 keys in a graph, 7.1 for 16 x 1,024), by
-// instruction issue where there are many (512 x 192: 21 us, 2.8 TB/s; about 240 instructions a warp and block of 32 keys) and by
-// both on long contexts (4 x 32,768: 29 us, 3.5 TB/s; 256 x 2,000: 92 us, 4.4 TB/s). Copies of the next blocks into L2 ahead
-// of their loads, and two blocks of registers ahead below 16 warps, gave nothing or cost occupancy.
+// Bound by the chain of dependent steps where there are few units (3.2 us for 17 keys in a graph, 7.1 for 16 x 1,024). Where
+// there are many, by the latency of loads and of dependent steps that too few warps hide (512 x 192: 21 us, 2.8 TB/s; 1,536 CTAs
+// are 1.48 rounds of the 7 an SM that 69 registers and 22 KB allow, the second half empty: 34% of the warp places taken, no
+// warp ready in 43% of the cycles; about 240 instructions a warp and block of 32 keys). On long contexts by that and by the
+// barriers between the passes (4 x 32,768: 30 us, 3.4 TB/s, no warp ready in 51%; 256 x 2,000: 92 us, 4.4 TB/s). Copies of the
+// next blocks into L2 ahead of their loads, and two blocks of registers ahead below 16 warps, gave nothing or cost occupancy.
 // ---------------------------------------------------------------------------------------------------------------------
 constexpr int SF_BYTES = 5;      // shared memory a key: 4 its score, later 3 of them its weight's planes; 1 its value's shift
 // a warp's ring of blocks of 32 keys (or values) on their way
@@ -681,10 +684,13 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, NW == 1 ? 7 : (NW == 
 //           swap those through shared memory and each adds w c for half of the 64 dims: 48 registers of sums a lane in
 //           place of 96, which lets 16 warps share an SM
 // CTAs are persistent so that the table is copied twice an SM, the longest rows first.
-// Bound by the latency of dependent integer steps (16 warps an SM; a tile of 64 x 64 pairs takes an SM 1.4 us, 6,200 warp
-// instructions at 2.3 a clock; fewer of them, the table's place in two steps less and the weights by a product in place of
-// shifts, gained nothing) and of an item's start and end (5 us for each of the 18 items that an SM takes): 194 us for 32 prompts of 300
-// to 512 rows, 183 us for 2 x 256 rows on 8,000 positions. The tensor cores' share of the time is a sixth. Slower: 128 rows on 16
+// 194 us for 32 prompts of 300 to 512 rows, 183 us for 2 x 256 rows on 8,000 positions. Bound by latency that 16 warps an SM do
+// not hide: 1.8 instructions a clock, no warp ready in 55% of the cycles (fixed waits first, then instruction fetches on the
+// prompts, shared and global loads, barriers). The 16 warps are what 128 registers a thread allow, 48 of them sums (112 bytes
+// are spilled at that). A tile of 64 x 64 pairs takes an SM about 1.4 us, the start and end of each of the 18 items that an SM
+// takes of the prompts about 5. Fewer instructions (the table's place in two
+// steps less, the weights by a product in place of shifts) gained nothing. The tensor cores are busy 16% of the time on the
+// prompts, 23% on the long context; with sums in tensor memory more warps would fit, which was not tried. Slower: 128 rows on 16
 // warps a CTA (one CTA an SM: nothing runs while it waits), the sums of all 64 dims in one warp (8 warps an SM), two items a
 // CTA side by side that share a table (192 us and 5% more on long contexts), an item's queries and first tiles copied ahead.
 // ---------------------------------------------------------------------------------------------------------------------
@@ -1255,16 +1261,20 @@ cudaError_t store_read(const Store4& st, const StoreRows& rw, int layer, int64_t
 
 // the few-row kernel is quicker up to so many rows a stream (4 streams on 2,000 positions: 12 rows 21 us, the many-row kernel 38;
 // 32 rows 50 and 40), and of more rows while there is little to do in all: (row, head)s times their blocks of 32 keys and a
-// start of SF_START more, an SM (one prompt of 64 rows 8.8 and 14.3 us, of 256 13.5 and 20.6, 2 x 48 rows on 700 19 and 27; past
-// it 8 x 32 rows on 500 32.6 and 29.7, 16 prompts of 64 19.2 and 16.4)
+// start of SF_START more, an SM (in stores that just hold them: one prompt of 64 rows 8.8 and 14.3 us, of 256 13.5 and 20.6,
+// 2 x 48 rows on 700 19 and 27; past it 8 x 32 rows on 500 32.6 and 29.7, 16 prompts of 64 19.2 and 16.4)
 constexpr int SM_FROM_ROWS = 20, SF_START = 3, SF_LITTLE = 340;
 constexpr int SM_FIXED = 4, SM_SPLIT = 6;
 constexpr int SM_SMEM_MOST = 200 * 1024;
 constexpr int SF_MOST_KEYS = 8192;   // of a CTA: 40 KB of shared memory
-// a warp a unit where units are many and short: from SF_WARP_UNITS an SM on up to 1,024 keys (20 KB a CTA; 200 x 160, 16 an SM:
-// 10.1 us against 13.6), below that where their blocks of 32 keys are at most twice the units an SM less five (64 x 160, 5 an SM
-// of 5 blocks: 5.8 against 6.1, 64 x 256 7.7 against 6.9; 140 x 256, 11 an SM of 8: 9.5 against 13.3, 100 x 900 30 against 23;
-// a step's one warp would put the row's own key and value first: 64 x 160 in the engine 0.605 ms a step against 0.581)
+// The rules from here on go by the positions that a row may see, the store's context (or the window), since what the streams
+// hold is on the device: in a store much larger than its streams they choose for keys that are not there (64 x 160 in a store of
+// 160, 1,024, 2,048 and 32,768 positions, calls in a graph: 5.4, 6.5, 10 and 62 us; 512 x 192: 17, 18, 62 and 487).
+// A warp a unit where units are many and short: from SF_WARP_UNITS an SM on up to 1,024 keys (20 KB a CTA; 200 x 160, 16 an SM:
+// 10.1 us against 13.6); an arrival (not a step) also below that, where the blocks of 32 keys are at most twice the units an SM
+// less five, a line through the crossings measured (64 x 160, 5 an SM of 5 blocks: 5.8 against 6.1, 64 x 256 7.7 against 6.9;
+// 140 x 256, 11 an SM of 8: 9.5 against 13.3, 100 x 900 30 against 23; a step's one warp would put the row's own key and value
+// first: 64 x 160 in the engine 0.605 ms a step against 0.581)
 constexpr int SF_WARP_UNITS = 12, SF_WARP_BLOCKS = 32;
 // blocks of 32 keys a warp from which they come through the ring, three on their way: 100 x 900 (8 blocks) 26.6 us straight into
 // registers, 22.8 through the ring, 512 x 192 (6) 22.3 and 21.1, 4 x 32,768 (16) 30.8 and 29.3; but 200 x 160 (5) 10.1 and 11.0,
