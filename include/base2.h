@@ -238,6 +238,7 @@ int b2_store_step(b2_store* s, int32_t layer, const int64_t* q, int64_t ldq, con
 /* Wait for queued work and report what the device checks flagged since the last call. */
 int b2_store_sync(b2_store* s);
 const char* b2_store_last_error(const b2_store* s);
+/* Waits for the device, as b2_store_create and b2_store_sync do: none of the three while a stream is captured. */
 void b2_store_destroy(b2_store* s);
 
 const char* b2_last_error(const b2_handle* h);

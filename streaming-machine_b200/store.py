@@ -29,7 +29,10 @@ _ended = []      # (handle, memory) of stores that ended while a graph was captu
 def _free_ended(torch):
     """Free what has ended, unless a capture is under way on this thread's stream (the wait would break it)."""
     while _ended and not torch.cuda.is_current_stream_capturing():
-        h, memory = _ended.pop()
+        try:
+            h, memory = _ended.pop()
+        except IndexError:                               # another thread has taken the last
+            return
         lib().b2_store_destroy(h)                        # (waits for the device: the memory may be used again)
         del memory
 

@@ -172,3 +172,25 @@ def test_the_error_in_bits_of_the_largest(spread):
                         assert off.max() > (1 << t) // 16                # a sixteenth does not hold
                     if spread >= 7 and part == slice(32, 64):
                         assert (got[part] == 0).all() or spread == 7
+
+
+def test_ended_stores_are_freed_once(monkeypatch):
+    """Two threads that end stores at once free each of them once, and neither fails because the other took the last."""
+    import types
+    from streaming_machine_b200 import store
+    freed = []
+    monkeypatch.setattr(store, "lib", lambda: types.SimpleNamespace(b2_store_destroy=freed.append))
+
+    def torch_with(capturing):
+        return types.SimpleNamespace(cuda=types.SimpleNamespace(is_current_stream_capturing=capturing))
+
+    def other_thread():                       # between the look at the list and the taking
+        if len(store._ended) == 1:
+            freed.append(store._ended.pop()[0])
+        return False
+    for capturing, left in ((lambda: False, []), (other_thread, []), (lambda: True, [1, 2, 3])):
+        freed.clear()
+        store._ended[:] = [(1, None), (2, None), (3, None)]
+        store._free_ended(torch_with(capturing))
+        assert sorted(freed + [h for h, _ in store._ended]) == [1, 2, 3] and [h for h, _ in store._ended] == left
+    store._ended.clear()
